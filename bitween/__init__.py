@@ -13,7 +13,7 @@ import bitween_amd
 from bitween_amd import *  # noqa: F401,F403
 from bitween_amd import __all__  # noqa: F401
 
-for _name in ("functional", "modules", "quantizer", "quantizer.quantizer", "quantizer.func", "kernels",
+for _name in ("attention", "functional", "modules", "quantizer", "quantizer.quantizer", "quantizer.func", "kernels",
               "kernels.hip_loader"):
     _mod = importlib.import_module("bitween_amd." + _name)
     sys.modules[__name__ + "." + _name] = _mod

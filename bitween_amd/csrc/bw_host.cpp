@@ -17,6 +17,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -38,6 +39,13 @@ struct Library {
     decltype(&bw_qdgrad_tile_rows) qdgrad_tile_rows = nullptr;
     decltype(&bw_quantize_pack_add) quantize = nullptr;
     decltype(&bw_dequantize) dequantize = nullptr;
+    decltype(&bw_rotate_heads) rotate = nullptr;
+    decltype(&bw_rotate_heads_grad) rotate_grad = nullptr;
+    decltype(&bw_rotate_heads_grad_workspace_bytes) rotate_grad_ws_bytes = nullptr;
+    decltype(&bw_cache_write) cache_write = nullptr;
+    decltype(&bw_cache_read) cache_read = nullptr;
+    decltype(&bw_cache_attention) attention = nullptr;
+    decltype(&bw_cache_attention_workspace_bytes) attention_ws_bytes = nullptr;
 } lib;
 
 PyObject* g_check = nullptr;          // Python: check(status, entry point's name) raises for a status other than 0
@@ -487,6 +495,346 @@ PyObject* py_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     });
 }
 
+// ---- rotation, cache and attention of a decode step ----
+
+// A tensor [..., heads, dim] of 16-bit values as rows of tokens: base address, distance of two tokens and of two heads in elements.  A
+// layout that the kernels do not read (leading dimensions that are no single stride, pieces that do not start at 16 bytes) is copied.
+struct Rows {
+    Tensor held;
+    const void* data = nullptr;
+    int64_t row = 0, head = 0;
+    Rows() = default;
+    Rows(const Tensor& t, int64_t tokens) {
+        const int64_t heads = t.size(-2), dim = t.size(-1);
+        held = t.dim() == 3 ? t : t.reshape({tokens, heads, dim});
+        const bool one_token = tokens <= 1, one_head = heads <= 1;
+        if (held.stride(2) != 1 || (!one_token && held.stride(0) % 8) || (!one_head && held.stride(1) % 8) || !aligned16(held.const_data_ptr()))
+            held = held.clone(at::MemoryFormat::Contiguous);
+        data = held.const_data_ptr();
+        row = one_token ? 0 : held.stride(0);                   // (the stride of a single row may be anything)
+        head = one_head ? 0 : held.stride(1);
+    }
+};
+
+inline bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+inline bool on_gpu(const Tensor& t, const Tensor& like) { return t.is_cuda() && t.has_storage() && t.device() == like.device(); }
+
+// [..., heads, dim] with the leading dimensions of `lead`
+bool heads_of(const Tensor& t, at::IntArrayRef lead) {
+    return t.dim() == (int64_t)lead.size() + 2 && t.sizes().slice(0, lead.size()).equals(lead) && t.size(-1) > 0 && t.size(-2) > 0;
+}
+
+struct Rotation {
+    bw_heads heads;
+    int act;
+};
+
+bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions, const Tensor& qw, const Tensor& kw,
+                 double eps, Rotation& r) {
+    if (!lib.rotate || !q.is_cuda() || !q.has_storage() || !half_type(q.scalar_type()) || k.scalar_type() != q.scalar_type()) return false;
+    for (const Tensor* t : {&k, &cos, &sin, &positions})
+        if (!on_gpu(*t, q)) return false;
+    if (positions.scalar_type() != at::kLong || !positions.is_contiguous() || !heads_of(q, positions.sizes()) || !heads_of(k, positions.sizes())) return false;
+    const int64_t dim = q.size(-1);
+    if (k.size(-1) != dim || q.size(-2) > 65535 || k.size(-2) > 65535 || dim > 65535) return false;
+    for (const Tensor* t : {&cos, &sin})
+        if (t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() || !aligned16(t->const_data_ptr())) return false;
+    if (!cos.sizes().equals(sin.sizes()) || cos.size(0) < 1 || cos.size(1) < 1 || 2 * cos.size(1) > dim) return false;
+    at::ScalarType wt = q.scalar_type();
+    for (const Tensor* t : {&qw, &kw})
+        if (t->defined()) {
+            if (!on_gpu(*t, q) || t->dim() != 1 || t->size(0) != dim || !t->is_contiguous() || !aligned16(t->const_data_ptr())) return false;
+            wt = t->scalar_type();
+        }
+    if (wt != q.scalar_type() && wt != at::kFloat) return false;
+    if (qw.defined() && kw.defined() && qw.scalar_type() != kw.scalar_type()) return false;
+    r.act = dtype_code(q.scalar_type());
+    r.heads = {positions.numel(), (int)q.size(-2), (int)k.size(-2), (int)dim, (int)(2 * cos.size(1)), (const float*)cos.const_data_ptr(),
+               (const float*)sin.const_data_ptr(), cos.size(0), (const int64_t*)positions.const_data_ptr(), qw.defined() ? qw.const_data_ptr() : nullptr,
+               kw.defined() ? kw.const_data_ptr() : nullptr, dtype_code(wt), (float)eps};
+    return true;
+}
+
+struct RotateHeadsBackward : public torch::autograd::Node {
+    enum { Q, K, QW, KW, COS, SIN, POSITIONS };
+    torch::autograd::SavedVariable saved[7];
+    c10::SmallVector<int64_t, 5> q_sizes, k_sizes;
+    at::ScalarType type = at::kHalf;
+    double eps = 0;
+    std::string name() const override { return "RotateHeadsBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (auto& v : saved) v.reset_data();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list out(4);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        Tensor t[7];
+        for (int i = 0; i < 7; i++) t[i] = saved[i].unpack();
+        const Tensor gq = grads[0].defined() ? grads[0] : input_metadata(0).zeros_like(), gk = grads[1].defined() ? grads[1] : input_metadata(1).zeros_like();
+        OnDevice on(gq.device());
+        {
+            c10::AutoGradMode off(false);
+            Rotation r;
+            TORCH_CHECK(rotation_of(gq, gk, t[COS], t[SIN], t[POSITIONS], t[QW], t[KW], eps, r), "bw_rotate_heads_grad: the gradients or what the forward saved have changed");
+            const int64_t tokens = r.heads.tokens;
+            const Rows rgq(gq, tokens), rgk(gk, tokens);
+            Rows rq, rk;
+            if (t[QW].defined()) rq = Rows(t[Q], tokens);
+            if (t[KW].defined()) rk = Rows(t[K], tokens);
+            out[0] = empty(q_sizes, type, gq.device());
+            out[1] = empty(k_sizes, type, gq.device());
+            for (int i : {2, 3})
+                if (t[i].defined() && task_should_compute_output(i)) out[i] = empty(t[i].sizes(), t[i].scalar_type(), gq.device());
+            Tensor ws;
+            size_t bytes = 0;
+            if (out[2].defined() || out[3].defined()) bytes = lib.rotate_grad_ws_bytes(&r.heads);
+            if (bytes) ws = empty({(int64_t)bytes}, at::kByte, gq.device());
+            const int st = lib.rotate_grad(&r.heads, r.act, rgq.data, rgq.row, rgq.head, rgk.data, rgk.row, rgk.head, rq.data, rq.row, rq.head, rk.data, rk.row,
+                                           rk.head, out[0].mutable_data_ptr(), out[1].mutable_data_ptr(), out[2].defined() ? out[2].mutable_data_ptr() : nullptr,
+                                           out[3].defined() ? out[3].mutable_data_ptr() : nullptr, bytes ? ws.mutable_data_ptr() : nullptr, bytes,
+                                           stream_of(gq.device().index()));
+            TORCH_CHECK(st == BW_OK, "bw_rotate_heads_grad failed (status ", st, ")");
+        }
+        for (int i : {0, 1})
+            if (!task_should_compute_output(i)) out[i] = Tensor();
+        if (c10::GradMode::is_enabled()) {                      // create_graph: these gradients have no derivative of their own
+            for (auto& v : out)
+                if (v.defined()) {
+                    auto error = std::make_shared<torch::autograd::DelayedError>("rotate_heads has no second derivative", 1);
+                    v = error->apply({v.detach().requires_grad_(true)})[0];
+                }
+        }
+        return out;
+    }
+};
+
+// Autograd runs a leaf's accumulation on the stream where its node was made.  A node that an eager graph keeps alive on another stream would
+// be waited for inside the capture, which a capture cannot do: refused here, while nothing is recorded yet.
+void check_capture(std::initializer_list<const Tensor*> inputs, at::DeviceIndex index) {
+    const auto stream = c10::hip::getCurrentHIPStream(index);
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const auto on = node->stream();
+        TORCH_CHECK(!on || *on == stream.unwrap(), "rotate_heads: a graph recorded on another stream still holds the gradient accumulation of an input of this "
+                    "captured call; drop that graph (its outputs) before the capture");
+    }
+}
+
+// rotate_heads(q, k, cos, sin, positions, q_weight or None, k_weight or None, eps) -> (q, k) or None
+PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 8) return none();
+        for (int i = 0; i < 7; i++)
+            if (!plain(args[i]) && !(i >= 5 && args[i] == Py_None)) return none();
+        const double eps = PyFloat_AsDouble(args[7]);
+        if (PyErr_Occurred()) return nullptr;
+        const Tensor q = unpack(args[0]), k = unpack(args[1]), cos = unpack(args[2]), sin = unpack(args[3]), positions = unpack(args[4]);
+        const Tensor qw = args[5] == Py_None ? Tensor() : unpack(args[5]), kw = args[6] == Py_None ? Tensor() : unpack(args[6]);
+        Rotation r;
+        if (!rotation_of(q, k, cos, sin, positions, qw, kw, eps, r)) return none();
+        bool recorded = false;
+        if (c10::GradMode::is_enabled()) {
+            for (const Tensor* t : {&q, &k, &qw, &kw}) {
+                if (!t->defined()) continue;
+                recorded |= t->requires_grad();
+                TORCH_CHECK(!t->_fw_grad(0).defined(), "rotate_heads has no forward-mode derivative");
+            }
+            if (cos.requires_grad() || sin.requires_grad()) return none();
+        }
+        if (recorded) check_capture({&q, &k, &qw, &kw}, q.device().index());
+        Tensor q_out, k_out;
+        int status = 0;
+        {
+            Unlocked unlocked;
+            c10::AutoGradMode off(false);
+            OnDevice on(q.device());
+            q_out = empty(q.sizes(), q.scalar_type(), q.device());
+            k_out = empty(k.sizes(), q.scalar_type(), q.device());
+            if (r.heads.tokens > 0) {
+                const Rows rq(q, r.heads.tokens), rk(k, r.heads.tokens);
+                status = lib.rotate(&r.heads, r.act, rq.data, rq.row, rq.head, rk.data, rk.row, rk.head, q_out.mutable_data_ptr(), k_out.mutable_data_ptr(),
+                                    stream_of(q.device().index()));
+            }
+        }
+        if (status) return checked({}, status, "bw_rotate_heads");
+        if (recorded) {
+            std::shared_ptr<RotateHeadsBackward> node(new RotateHeadsBackward(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(q, k, qw, kw));
+            const Tensor none_, *keep[7] = {qw.defined() ? &q : &none_, kw.defined() ? &k : &none_, &qw, &kw, &cos, &sin, &positions};
+            for (int i = 0; i < 7; i++) node->saved[i] = torch::autograd::SavedVariable(*keep[i], false);
+            node->q_sizes = q.sizes();
+            node->k_sizes = k.sizes();
+            node->type = q.scalar_type();
+            node->eps = eps;
+            torch::autograd::set_history(torch::autograd::variable_list{q_out, k_out}, node);
+        }
+        PyObject* p = PyTuple_New(2);
+        if (!p) return nullptr;
+        PyTuple_SET_ITEM(p, 0, THPVariable_Wrap(std::move(q_out)));
+        PyTuple_SET_ITEM(p, 1, THPVariable_Wrap(std::move(k_out)));
+        return p;
+    });
+}
+
+// The cache that six arguments name: keys, values, key_meta or None, value_meta or None, bits, group size.
+struct Cache {
+    Tensor keys, values, key_meta, value_meta;
+    bw_cache c = {};
+};
+
+bool cache_of(PyObject* const* args, Cache& h) {
+    if (!lib.attention || !plain(args[0]) || !plain(args[1]) || !PyLong_Check(args[4]) || !PyLong_Check(args[5])) return false;
+    const int64_t bits = PyLong_AsLong(args[4]), group = PyLong_AsLong(args[5]);
+    if (PyErr_Occurred() || (bits != 16 && bits != 8 && bits != 4)) return false;
+    h.keys = unpack(args[0]);
+    h.values = unpack(args[1]);
+    if (!h.keys.is_cuda() || !h.keys.has_storage() || h.keys.dim() != 4 || !on_gpu(h.values, h.keys) || !h.values.sizes().equals(h.keys.sizes()) ||
+        h.values.scalar_type() != h.keys.scalar_type() || !h.keys.is_contiguous() || !h.values.is_contiguous())
+        return false;
+    for (int i = 0; i < 4; i++)
+        if (h.keys.size(i) < 1 || h.keys.size(i) >= (int64_t)1 << 31) return false;
+    int64_t dim = h.keys.size(3);
+    if (bits == 16) {
+        if (!half_type(h.keys.scalar_type()) || args[2] != Py_None || args[3] != Py_None) return false;
+    } else {
+        dim = dim * 32 / bits;
+        if (h.keys.scalar_type() != at::kInt || !plain(args[2]) || !plain(args[3]) || group < 1 || group > dim || dim % group) return false;
+        h.key_meta = unpack(args[2]);
+        h.value_meta = unpack(args[3]);
+        const int64_t want[5] = {h.keys.size(0), h.keys.size(1), dim / group, h.keys.size(2), 2};
+        for (const Tensor* t : {&h.key_meta, &h.value_meta})
+            if (!on_gpu(*t, h.keys) || t->scalar_type() != at::kHalf || !t->sizes().equals(want) || !t->is_contiguous()) return false;
+    }
+    h.c = {h.keys.data_ptr(), h.values.data_ptr(), bits == 16 ? nullptr : h.key_meta.data_ptr(), bits == 16 ? nullptr : h.value_meta.data_ptr(),
+           h.keys.size(0), (int)h.keys.size(1), (int)h.keys.size(2), (int)dim, (int)bits, (int)group, bits == 16 ? dtype_code(h.keys.scalar_type()) : BW_F16};
+    return true;
+}
+
+bool slots_of(PyObject* o, const Tensor& like, Tensor& slots) {
+    if (!plain(o)) return false;
+    slots = unpack(o);
+    return on_gpu(slots, like) && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous();
+}
+
+inline bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
+// cache_write(k, v, slots, keys, values, key_meta, value_meta, bits, group_size) -> True or None
+PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        Cache h;
+        Tensor slots;
+        if (nargs != 9 || !plain(args[0]) || !plain(args[1]) || !cache_of(args + 3, h) || !slots_of(args[2], h.keys, slots)) {
+            if (PyErr_Occurred()) return nullptr;
+            return none();
+        }
+        const Tensor k = unpack(args[0]), v = unpack(args[1]);
+        for (const Tensor* t : {&k, &v})
+            if (!on_gpu(*t, h.keys) || !half_type(t->scalar_type()) || t->dim() != 3 || t->size(0) != slots.size(0) || t->size(1) != h.c.kv_heads ||
+                t->size(2) != h.c.dim || wants_grad(*t))
+                return none();
+        if (k.scalar_type() != v.scalar_type() || (h.c.bits == 16 && k.scalar_type() != h.keys.scalar_type())) return none();
+        if (wants_grad(h.keys) || wants_grad(h.values)) return none();
+        int status = 0;
+        {
+            Unlocked unlocked;
+            c10::AutoGradMode off(false);
+            for (const Tensor* t : {&h.keys, &h.values, &h.key_meta, &h.value_meta})       // written in place: what autograd saved of them is stale
+                if (t->defined()) torch::autograd::impl::bump_version(*t);
+            const int64_t tokens = slots.size(0);
+            if (tokens > 0) {
+                OnDevice on(k.device());
+                const Rows rk(k, tokens), rv(v, tokens);
+                status = lib.cache_write(&h.c, dtype_code(k.scalar_type()), tokens, rk.data, rk.row, rk.head, rv.data, rv.row, rv.head,
+                                         (const int64_t*)slots.const_data_ptr(), stream_of(k.device().index()));
+            }
+        }
+        if (status) return checked({}, status, "bw_cache_write");
+        Py_RETURN_TRUE;
+    });
+}
+
+// cache_read(slots, keys, values, key_meta, value_meta, bits, group_size, output code) -> (k, v) or None
+PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        Cache h;
+        Tensor slots;
+        if (nargs != 8 || !cache_of(args + 1, h) || !slots_of(args[0], h.keys, slots)) {
+            if (PyErr_Occurred()) return nullptr;
+            return none();
+        }
+        const int code = (int)PyLong_AsLong(args[7]);
+        if (PyErr_Occurred()) return nullptr;
+        if ((code != BW_F16 && code != BW_BF16) || (h.c.bits == 16 && code != h.c.dtype)) return none();
+        Tensor k, v;
+        int status = 0;
+        {
+            Unlocked unlocked;
+            c10::AutoGradMode off(false);
+            OnDevice on(slots.device());
+            const int64_t tokens = slots.size(0);
+            k = empty({tokens, h.c.kv_heads, h.c.dim}, dtype_of(code), slots.device());
+            v = empty({tokens, h.c.kv_heads, h.c.dim}, dtype_of(code), slots.device());
+            if (tokens > 0)
+                status = lib.cache_read(&h.c, code, tokens, (const int64_t*)slots.const_data_ptr(), k.mutable_data_ptr(), v.mutable_data_ptr(),
+                                        stream_of(slots.device().index()));
+        }
+        if (status) return checked({}, status, "bw_cache_read");
+        PyObject* p = PyTuple_New(2);
+        if (!p) return nullptr;
+        PyTuple_SET_ITEM(p, 0, THPVariable_Wrap(std::move(k)));
+        PyTuple_SET_ITEM(p, 1, THPVariable_Wrap(std::move(v)));
+        return p;
+    });
+}
+
+// cache_attention(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale) -> out or None
+PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        Cache h;
+        if (nargs != 10 || !plain(args[0]) || !plain(args[1]) || !plain(args[2]) || !cache_of(args + 3, h)) {
+            if (PyErr_Occurred()) return nullptr;
+            return none();
+        }
+        const Tensor q = unpack(args[0]), table = unpack(args[1]), lengths = unpack(args[2]);
+        const double scale = PyFloat_AsDouble(args[9]);
+        if (PyErr_Occurred()) return nullptr;
+        for (const Tensor* t : {&q, &table, &lengths})
+            if (!on_gpu(*t, h.keys)) return none();
+        if (!half_type(q.scalar_type()) || (h.c.bits == 16 && q.scalar_type() != h.keys.scalar_type()) || q.dim() != 3 || q.size(2) != h.c.dim ||
+            q.size(1) < 1 || q.size(1) > 65535 || q.size(1) % h.c.kv_heads || wants_grad(q))
+            return none();
+        const int64_t batch = q.size(0);
+        if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch || table.size(1) < 1 || (table.size(1) > 1 && table.stride(1) != 1) ||
+            lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != batch || !lengths.is_contiguous())
+            return none();
+        Tensor out;
+        int status = 0;
+        {
+            Unlocked unlocked;
+            c10::AutoGradMode off(false);
+            OnDevice on(q.device());
+            out = empty({batch, q.size(1), q.size(2)}, q.scalar_type(), q.device());
+            if (batch > 0) {
+                const Rows rq(q, batch);
+                const size_t bytes = lib.attention_ws_bytes(&h.c, batch, (int)q.size(1), table.size(1));
+                Tensor ws;
+                if (bytes) ws = empty({(int64_t)bytes}, at::kByte, q.device());
+                status = lib.attention(&h.c, dtype_code(q.scalar_type()), rq.data, batch, (int)q.size(1), rq.row, rq.head,
+                                       (const int32_t*)table.const_data_ptr(), table.size(1), batch > 1 ? table.stride(0) : table.size(1),
+                                       (const int32_t*)lengths.const_data_ptr(), (float)scale, out.mutable_data_ptr(), bytes ? ws.mutable_data_ptr() : nullptr,
+                                       bytes, stream_of(q.device().index()));
+            }
+        }
+        return checked(std::move(out), status, "bw_cache_attention");
+    });
+}
+
 // bind({entry point name: address}, check, dict with the fused gradient's row limits): once, after the kernel library is loaded
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject *table, *check, *limits;
@@ -507,6 +855,13 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(l.qdgrad_tile_rows, "bw_qdgrad_tile_rows");
     get(l.quantize, "bw_quantize_pack_add");
     get(l.dequantize, "bw_dequantize");
+    get(l.rotate, "bw_rotate_heads");
+    get(l.rotate_grad, "bw_rotate_heads_grad");
+    get(l.rotate_grad_ws_bytes, "bw_rotate_heads_grad_workspace_bytes");
+    get(l.cache_write, "bw_cache_write");
+    get(l.cache_read, "bw_cache_read");
+    get(l.attention, "bw_cache_attention");
+    get(l.attention_ws_bytes, "bw_cache_attention_workspace_bytes");
     if (PyErr_Occurred()) return nullptr;
     if (!ok) {
         PyErr_SetString(PyExc_RuntimeError, "bind: an entry point is missing");
@@ -527,6 +882,10 @@ PyMethodDef methods[] = {
     {"input_grad", (PyCFunction)(void*)py_input_grad, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void*)py_quantize, METH_FASTCALL, nullptr},
     {"dequantize", (PyCFunction)(void*)py_dequantize, METH_FASTCALL, nullptr},
+    {"rotate_heads", (PyCFunction)(void*)py_rotate_heads, METH_FASTCALL, nullptr},
+    {"cache_write", (PyCFunction)(void*)py_cache_write, METH_FASTCALL, nullptr},
+    {"cache_read", (PyCFunction)(void*)py_cache_read, METH_FASTCALL, nullptr},
+    {"cache_attention", (PyCFunction)(void*)py_cache_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_bw_host", "Native host path of bitween_amd", -1, methods};

@@ -23,11 +23,26 @@ _DTYPE_CODE = {torch.float16: BW_F16, torch.bfloat16: BW_BF16, torch.float32: BW
 
 ABI_VERSION = 10           # what bw_abi_version() of a matching library returns
 ENTRY_POINTS = ("bw_abi_version", "bw_strerror", "bw_quantize_pack", "bw_quantize_pack_add", "bw_dequantize", "bw_qgemv", "bw_qgemm",
-                "bw_qgemm_ws", "bw_qgemm_static", "bw_qgemm_workspace_bytes", "bw_qgemm_tile_rows", "bw_qgemm_tile_cols", "bw_qlinear", "bw_qlinear_ws", "bw_qlinear_workspace_bytes", "bw_qdgrad", "bw_qdgrad_workspace_bytes", "bw_qdgrad_tile_rows", "bw_qdgrad_rows_slices", "bw_cast_bf16_f16", "bw_qlinear_decode_rows", "bw_qgemv_last_kernel")
+                "bw_qgemm_ws", "bw_qgemm_static", "bw_qgemm_workspace_bytes", "bw_qgemm_tile_rows", "bw_qgemm_tile_cols", "bw_qlinear", "bw_qlinear_ws", "bw_qlinear_workspace_bytes", "bw_qdgrad", "bw_qdgrad_workspace_bytes", "bw_qdgrad_tile_rows", "bw_qdgrad_rows_slices", "bw_cast_bf16_f16", "bw_qlinear_decode_rows", "bw_qgemv_last_kernel",
+                "bw_rotate_heads", "bw_rotate_heads_grad", "bw_rotate_heads_grad_workspace_bytes", "bw_cache_write", "bw_cache_read", "bw_cache_attention", "bw_cache_attention_workspace_bytes")
 
 
 class BitweenHipError(RuntimeError):
     pass
+
+
+class Heads(ctypes.Structure):
+    """bw_heads"""
+    _fields_ = [("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int), ("k_heads", ctypes.c_int), ("dim", ctypes.c_int), ("rotary", ctypes.c_int),
+                ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
+class Cache(ctypes.Structure):
+    """bw_cache"""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("key_meta", ctypes.c_void_p), ("value_meta", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int), ("page_size", ctypes.c_int), ("dim", ctypes.c_int), ("bits", ctypes.c_int),
+                ("group", ctypes.c_int), ("dtype", ctypes.c_int)]
 
 
 def library_path():
@@ -85,6 +100,18 @@ def load():
     lib.bw_qlinear_decode_rows.restype = i32
     lib.bw_qgemv_last_kernel.argtypes = []
     lib.bw_qgemv_last_kernel.restype = ctypes.c_char_p
+    heads, cache, size = ctypes.POINTER(Heads), ctypes.POINTER(Cache), ctypes.c_size_t
+    lib.bw_rotate_heads.argtypes = [heads, i32, vp, i64, i64, vp, i64, i64, vp, vp, vp]
+    lib.bw_rotate_heads_grad.argtypes = [heads, i32] + [vp, i64, i64] * 4 + [vp, vp, vp, vp, vp, size, vp]
+    lib.bw_rotate_heads_grad_workspace_bytes.argtypes = [heads]
+    lib.bw_cache_write.argtypes = [cache, i32, i64, vp, i64, i64, vp, i64, i64, vp, vp]
+    lib.bw_cache_read.argtypes = [cache, i32, i64, vp, vp, vp, vp]
+    lib.bw_cache_attention.argtypes = [cache, i32, vp, i64, i32, i64, i64, vp, i64, i64, vp, ctypes.c_float, vp, vp, size, vp]
+    lib.bw_cache_attention_workspace_bytes.argtypes = [cache, i64, i32, i64]
+    for name in ("bw_rotate_heads_grad_workspace_bytes", "bw_cache_attention_workspace_bytes"):
+        getattr(lib, name).restype = size
+    for name in ("bw_rotate_heads", "bw_rotate_heads_grad", "bw_cache_write", "bw_cache_read", "bw_cache_attention"):
+        getattr(lib, name).restype = i32
     for name in ("bw_quantize_pack", "bw_quantize_pack_add", "bw_dequantize", "bw_qgemv", "bw_qgemm", "bw_qgemm_ws", "bw_qgemm_static", "bw_qlinear"):
         getattr(lib, name).restype = i32
     _lib = lib

@@ -220,6 +220,85 @@ int bw_qdgrad(const void* grad_y, int act_dtype, int64_t M, int64_t N, int64_t l
               int64_t K, int bits, int group, void* grad_x, int64_t ldx,
               void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Between the quantized linears of a decoder layer: rotation of queries and keys, key-value cache, attention of one new token ----
+ * No counterpart in the reference, whose models bring these as eager torch operations. */
+
+/* One rotation for the queries [T][Hq][D] and keys [T][Hk][D] of T tokens, with the norm of each head in the same pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight        (y = x where the weight is NULL)
+ *   out_i = y_i c_i - y_{i+h} s_i,  out_{i+h} = y_{i+h} c_i + y_i s_i  for i < h = rotary / 2;  out_i = y_i for i >= rotary
+ * c, s = cos[p], sin[p] (float32, [table_rows][h]) at the token's position p.  A token whose position lies outside the table is padding:
+ * its outputs are zero and it adds nothing to gradients.  float32 arithmetic, one rounding at the end.
+ *   q, k           act_dtype (BW_F16 | BW_BF16); a token's row `*_row` elements apart, a head `*_head` apart, a head's values adjacent
+ *   q_weight, k_weight  [D] of weight_dtype (act_dtype or BW_F32) or NULL, each for itself
+ *   q_out, k_out   act_dtype, contiguous
+ * D a multiple of 8 up to 256, rotary a multiple of 8 up to D, rows, heads and pointers aligned to 16 bytes (positions to 8). */
+typedef struct bw_heads {
+    int64_t tokens;
+    int q_heads, k_heads, dim, rotary;
+    const float *cos, *sin;
+    int64_t table_rows;
+    const int64_t* positions;
+    const void *q_weight, *k_weight;
+    int weight_dtype;
+    float eps;
+} bw_heads;
+
+int bw_rotate_heads(const bw_heads* heads, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                    int64_t k_head, void* q_out, void* k_out, void* stream);
+
+/* Its gradients: q_grad, k_grad [T][H][D] contiguous from the gradients of the outputs (gq, gk: strided as q and k above) and, where a
+ * weight is given, its gradient [D] in weight_dtype.  q and k (the inputs of the forward) are read only where their weight is given.
+ * The sums over tokens and heads are taken in a fixed order through a workspace of bw_rotate_heads_grad_workspace_bytes(...) bytes
+ * (16-byte aligned; 0 = none needed): the same inputs give the same bits. */
+size_t bw_rotate_heads_grad_workspace_bytes(const bw_heads* heads);
+
+int bw_rotate_heads_grad(const bw_heads* heads, int act_dtype, const void* gq, int64_t gq_row, int64_t gq_head, const void* gk, int64_t gk_row,
+                         int64_t gk_head, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                         void* q_grad, void* k_grad, void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* A paged key-value cache: `pages` pages of page_size token rows for each of kv_heads heads.
+ *   bits 16   keys, values [pages][kv_heads][page_size][dim] of dtype (BW_F16 | BW_BF16); key_meta, value_meta unused
+ *   bits 8|4  keys, values int32 [pages][kv_heads][page_size][dim * bits / 32], packed like qweight; key_meta, value_meta float16 pairs
+ *             (scale, zero point) [pages][kv_heads][dim / group][page_size][2], group 32, 64 or 128; dtype unused
+ * dim a multiple of 8 up to 256 (of group), page_size a power of two from 16 to 1024; pointers aligned to 16 bytes.
+ * Slot n is row n % page_size of page n / page_size. */
+typedef struct bw_cache {
+    void *keys, *values, *key_meta, *value_meta;
+    int64_t pages;
+    int kv_heads, page_size, dim, bits, group, dtype;
+} bw_cache;
+
+/* Keys and values of T tokens into their slots.  A slot outside the cache is left out (padding); the slots of one call differ - of two
+ * tokens with the same slot either may be kept, in parts.  8 and 4 bits, for every group of a head's values:
+ *   lo = min(0, values), hi = max(0, values), r = (hi - lo) / (2^bits - 1), difference and quotient rounded to float32
+ *   scale = r rounded up to float16, from 2^-24 to 65504;  zero point = rint(-lo / scale), code = rint(x / scale) + zero point, both
+ *   clipped to 0 ... 2^bits - 1
+ * so that scale * (code - zero point) is within half a scale of x (of a finite x within 65504 scales).  A group that holds an infinity or
+ * a NaN gets a NaN scale: it reads back as NaN.
+ *   k, v  act_dtype (BW_F16 | BW_BF16, the cache's dtype at 16 bits), strided like q of bw_rotate_heads */
+int bw_cache_write(const bw_cache* cache, int act_dtype, int64_t T, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                   int64_t v_head, const int64_t* slots, void* stream);
+
+/* The rows of T slots as k_out, v_out [T][kv_heads][dim] of out_dtype (BW_F16 | BW_BF16; the cache's dtype at 16 bits): scale * (code -
+ * zero point) rounded once (a finite value beyond float16's range to its largest).  Zeros for a slot outside the cache. */
+int bw_cache_read(const bw_cache* cache, int out_dtype, int64_t T, const int64_t* slots, void* k_out, void* v_out, void* stream);
+
+/* Attention of one new token of each of B sequences over its cached tokens:
+ *   out = sum_t softmax_t(scale q . k_t) v_t,  t < lengths[b],  token t in row t % page_size of page page_table[b][t / page_size]
+ * Query head h reads key-value head h / (q_heads / kv_heads).  Codes enter with their exact values scale * (code - zero point), sums and
+ * softmax are float32, out is rounded once.  A sequence without tokens (length 0 or less) gets zeros.  A length beyond
+ * max_pages * page_size is taken as that; a page number outside the cache is a page without tokens.  Rows behind a sequence's last token
+ * are not looked at, whatever they hold; an infinity or a NaN among the cached values leaves nothing finite where it enters.
+ *   q [B][q_heads][dim] act_dtype, strided as above; page_table int32, `table_row` elements from sequence to sequence; out contiguous
+ * The cache is cut into equal pieces of work over all sequences; the parts of a sequence that lie in several of them are joined by a second
+ * kernel in a fixed order, through a workspace of bw_cache_attention_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed). */
+size_t bw_cache_attention_workspace_bytes(const bw_cache* cache, int64_t B, int q_heads, int64_t max_pages);
+
+int bw_cache_attention(const bw_cache* cache, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head,
+                       const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, void* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
