@@ -1,0 +1,603 @@
+// bw_attention_kernel.h - attention of one new token over a paged cache: the kernel template, its arguments and the split of its work.
+//
+// Work is counted in tiles of 32 tokens of one segment: one sequence, one key-value head, up to 16 of the query heads that read it.  The
+// tiles of all segments, in order, are cut into equal pieces, one for each workgroup, so that sequences of very different length load the
+// chip evenly; lengths are read on the GPU, so the cut follows them.  A segment that lies in one piece is finished by its workgroup; the parts
+// of one that lies in several go to the workspace and are joined by attention_join_kernel.
+//
+// The four waves of a workgroup take tiles in turn, each with a running reference r and sum l of its own.  One wave, one tile, everything in
+// registers:
+//   S^T[token][query] = K Q^T        A = 16 tokens of K (a lane: token lane % 16, 8 values of the head at a time), B = 16 queries
+//   P^T = exp2(S^T c - r)            a lane holds query lane % 16, tokens 4 (lane / 16) + i of each half of the tile
+//   O^T[d][query] += V^T P^T         B = P^T as it lies there; A = V^T: a lane loads a piece of the rows of just those 8 tokens and pairs
+//                                    the tokens with byte permutes
+// The order of the head's values in an MFMA is free as long as K and Q agree, and that of the tokens as long as P and V agree, so nothing
+// crosses lanes: no LDS, no shuffles until the waves are joined.  r is only raised when a score passes it by 2^8 (one vote a tile).
+//
+// Fewer than 16 queries leave columns of the MFMAs empty: the matrix cores have room (16 KB of a 16-bit tile take 32 MFMAs, some 500 cycles
+// of one SIMD, and about 8000 cycles of a SIMD's share of HBM).
+//
+// Codes enter as exact integers in float16, and the scales are applied in float32:
+//   K: S = s (Q . (q - mid) + (mid - z) sum Q) for each group, mid = 2^(bits-1): a lane's codes are one token's, its products four others'
+//   V: O += (P s) (q - z): a pair of codes is two tokens', whose scales and zero points the lane has anyway
+// so no value is rounded on its way in.  P s can be anything from 2^-24 to 2^16 times P: r then follows score + log2 of the token's scale
+// (a power of two 2^e), P is held relative to that and l adds P 2^-e.  P goes in as two 16-bit numbers whose sum it is (to 2^-16 and better):
+// one alone would err as much as the result's own rounding.
+#pragma once
+#include "bw_cache.h"
+
+constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
+constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
+
+struct AttentionArgs {
+    const uint16_t* q;
+    int64_t q_row, q_head;
+    const int32_t *table, *lengths;
+    int64_t table_row;
+    const uint8_t *keys, *values;
+    const uint32_t *key_meta, *value_meta;
+    uint16_t* out;
+    float* partial;                              // 2 slots for each workgroup: r [16], l [16], O [queries][dim]
+    int64_t page_bytes, meta_words;              // of one head in one page: row bytes * page_size; pairs
+    uint32_t pages;
+    int B, q_heads, kv_heads, share, queries, q_groups;   // queries: of a segment, at most 16; q_groups: segments of a key-value head
+    int dim, row_bytes, page_shift, max_tokens, q_bf16, min_tiles, whole;
+    float scale;                                 // times log2 e
+};
+
+// What a workgroup (or the join of a segment) has to know of the split.
+struct Split {
+    uint32_t tiles;                              // of all sequences, for one head
+    uint64_t total;                              // tiles of all segments
+    uint32_t pieces;
+    BW_DEV uint64_t start(uint32_t w) const { return (total >> 32) == 0 && total * pieces >> 32 == 0 ? (uint32_t)total * w / pieces : total * w / pieces; }
+    BW_DEV uint32_t piece_of(uint64_t tile) const { return (uint32_t)(((tile + 1) * pieces - 1) / total); }
+};
+
+BW_DEV int tokens_of(const AttentionArgs& a, int b) {
+    const int n = a.lengths[b];
+    return n < 0 ? 0 : n < a.max_tokens ? n : a.max_tokens;
+}
+BW_DEV uint32_t tiles_of(int tokens) { return ((uint32_t)tokens + kTile - 1) >> kTileShift; }
+
+// Sums of tiles over the sequences by one workgroup of 256 threads: thread i sums a run of sequences, the runs are added up over the lanes and
+// then the waves.  `found(b, before)` is called by one thread, for the sequence that `wanted` asks for: wanted(before, tiles) -> bool.
+template <class Wanted, class Found>
+BW_DEV void scan_sequences(const AttentionArgs& a, uint32_t* lds, uint32_t& all, Wanted&& wanted, Found&& found) {
+    const int run = (a.B + 255) >> 8, first = (int)threadIdx.x * run, lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    uint32_t mine = 0;
+    for (int b = first; b < first + run && b < a.B; b++) mine += tiles_of(tokens_of(a, b));
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t other = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += other;
+    }
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    uint32_t before = sum - mine;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        if (w < wave) before += lds[w];
+        all += lds[w];
+    }
+    for (int b = first; b < first + run && b < a.B; b++) {
+        const uint32_t t = run == 1 ? mine : tiles_of(tokens_of(a, b));
+        if (wanted(all, before, t)) found(b, before);
+        before += t;
+    }
+    __syncthreads();
+}
+
+BW_DEV Split split_of(const AttentionArgs& a, uint32_t tiles, uint32_t grid) {
+    Split s;
+    s.tiles = tiles;
+    s.total = (uint64_t)tiles * (uint32_t)(a.kv_heads * a.q_groups);
+    const uint64_t pieces = (s.total + a.min_tiles - 1) / (uint32_t)a.min_tiles;
+    s.pieces = pieces < grid ? (uint32_t)pieces : grid;
+    return s;
+}
+
+BW_DEV void store_out(const AttentionArgs& a, int64_t row, int d, f4 o) {
+    uint2 w;
+    if (a.q_bf16) w = uint2{f32_to_bf16(o[0]) | (uint32_t)f32_to_bf16(o[1]) << 16, f32_to_bf16(o[2]) | (uint32_t)f32_to_bf16(o[3]) << 16};
+    else w = uint2{as_u32(h2{(_Float16)o[0], (_Float16)o[1]}), as_u32(h2{(_Float16)o[2], (_Float16)o[3]})};
+    *reinterpret_cast<uint2*>(a.out + row * a.dim + d) = w;
+}
+
+// ---- formats ----
+// How the values of a head lie in MFMAs: NK operand blocks of 32 values for K and Q, NV output blocks of 16 values for V.
+//   K, Q: lane group kg = lane / 16 holds values k_at(block, kg) .. + 7      V: lane m = lane % 16 holds value v_at(m, j) for block j
+
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+// 16 bits, DT = BW_F16 | BW_BF16; DP: the head dimension filled up to 64, 128 or 256.  Lanes behind the head's end read its beginning again:
+// against zeros of Q, and into outputs that nobody stores.
+template <int DT, int DP> struct Format16 {
+    static constexpr bool kCodes = false, kBf16 = DT == BW_BF16;
+    static constexpr int kDim = DP, NK = DP / 32, NV = DP / 16, kGroups = 1, kKeyWords = NK * 4, kValueWords = NV / 2;
+    static BW_DEV int k_at(int block, int kg) { return 32 * block + 8 * kg; }
+    // 64: 4 neighbouring values (8 bytes) of a lane; 128: 8 (16 bytes); 256: 8 of each half
+    static BW_DEV int v_at(int m, int j) { return DP == 64 ? 4 * m + j : (j >> 3) * 128 + 8 * m + (j & 7); }
+};
+// BITS-bit codes in GROUPS groups of GS values: every MFMA, of K and of V, keeps to one group.
+template <int BITS, int GROUPS, int GS> struct FormatQ {
+    static constexpr bool kCodes = true, kBf16 = false;
+    static constexpr int kBits = BITS, kGroup = GS, kGroups = GROUPS, kDim = GROUPS * GS, NK = kDim / 32, NV = kDim / 16;
+    static constexpr int kPerK = GS / 32, kPerV = GS / 16;                  // operand blocks and output blocks of a group
+    static constexpr int kKeyGroupWords = GS * BITS / 128, kKeyWords = GROUPS * kKeyGroupWords;
+    static constexpr int kValueBytes = kPerV * BITS / 8, kValueGroupWords = kValueBytes > 4 ? kValueBytes / 4 : 1, kValueWords = GROUPS * kValueGroupWords;
+    static BW_DEV int k_at(int block, int kg) { return (block / kPerK) * GS + kg * (GS / 4) + (block % kPerK) * 8; }
+    static BW_DEV int v_at(int m, int j) { return (j / kPerV) * GS + m * kPerV + j % kPerV; }
+};
+
+template <bool BF16> BW_DEV f4 mfma(u4 a, u4 b, f4 c) {
+    if constexpr (BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// Two float32 as 16-bit numbers, towards zero; split_pair leaves in x and y what is missing.
+template <bool BF16> BW_DEV uint32_t pair_of(float x, float y) {
+    if constexpr (BF16) return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+}
+template <bool BF16> BW_DEV uint32_t split_pair(float& x, float& y) {
+    const uint32_t p = pair_of<BF16>(x, y);
+    if constexpr (BF16) {
+        x -= __builtin_bit_cast(float, p << 16);
+        y -= __builtin_bit_cast(float, p & 0xFFFF0000u);
+    } else {
+        x -= (float)as_h2(p)[0];
+        y -= (float)as_h2(p)[1];
+    }
+    return p;
+}
+
+// Codes of one word (8 bits: 4, 4 bits: 8) as float16 q - mid, in the order that Q is laid out in (query_order).
+template <int BITS> BW_DEV void key_codes(uint32_t w, uint32_t* out) {
+    if constexpr (BITS == 8) {
+        const h2 mid = splat((_Float16)-1152.f);
+        out[0] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + mid);
+        out[1] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + mid);
+    } else {
+        const h2 mid = splat((_Float16)-1032.f), mid16 = splat((_Float16)-72.f), k16 = splat((_Float16)0.0625f);
+        const uint32_t w8 = w >> 8;
+        out[0] = as_u32(as_h2(and_or(w, 0x000F000Fu, kMagic)) + mid);
+        out[1] = as_u32(__builtin_elementwise_fma(as_h2(and_or(w, 0x00F000F0u, kMagic)), k16, mid16));
+        out[2] = as_u32(as_h2(and_or(w8, 0x000F000Fu, kMagic)) + mid);
+        out[3] = as_u32(__builtin_elementwise_fma(as_h2(and_or(w8, 0x00F000F0u, kMagic)), k16, mid16));
+    }
+}
+template <int BITS> BW_DEV int query_order(int e) { return BITS == 4 ? (e >> 1) + 4 * (e & 1) : e; }
+
+// Codes j of two tokens as a float16 pair of q - z: `a` holds 16 bits of each (token_pair), zz and zz16 are -(1024 + z) and -(64 + z) of both.
+template <bool HIGH> BW_DEV uint32_t token_pair(uint32_t second, uint32_t first) { return __builtin_amdgcn_perm(second, first, HIGH ? 0x07060302u : 0x05040100u); }
+template <int BITS, int J> BW_DEV uint32_t value_codes(uint32_t a, h2 zz, h2 zz16) {
+    if constexpr (BITS == 8) return as_u32(as_h2(and_or(J ? a >> 8 : a, 0x00FF00FFu, kMagic)) + zz);
+    else if constexpr (J % 2 == 0) return as_u32(as_h2(and_or(J ? a >> 8 : a, 0x000F000Fu, kMagic)) + zz);
+    else return as_u32(__builtin_elementwise_fma(as_h2(and_or(J > 1 ? a >> 8 : a, 0x00F000F0u, kMagic)), splat((_Float16)0.0625f), zz16));
+}
+
+// One tile's rows and pairs as they come from memory.
+template <class F> struct KeyTile {
+    uint32_t raw[2][F::kKeyWords];
+    u4 meta[2][F::kGroups];                      // of tokens 4 kg .. + 3 of each half
+};
+template <class F> struct ValueTile {
+    uint32_t raw[8][F::kValueWords];             // token 4 kg + i of half h: 4 h + i
+    u4 meta[2][F::kGroups];
+};
+
+template <int WORDS> BW_DEV void load_words(const uint8_t* p, uint32_t* out) {
+    if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; i++) {
+            const u4 v = reinterpret_cast<const u4*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) out[4 * i + j] = v[j];
+        }
+    } else if constexpr (WORDS == 2) {
+        const u2 v = *reinterpret_cast<const u2*>(p);
+        out[0] = v[0];
+        out[1] = v[1];
+    } else {
+        static_assert(WORDS == 1, "words of a lane");
+        out[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+
+// Where a tile's two halves lie: pages as the table names them, and whether a half has tokens at all.
+struct Halves { uint32_t page[2]; };
+
+template <class F>
+__global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
+    constexpr int kChunk = F::kDim < 128 ? F::kDim : 128, kPitch = kChunk + 4, kChunkBlocks = kChunk / 16;
+    __shared__ float outs[kWaves][kQueries][kPitch];
+    __shared__ float stats[kWaves][2][kQueries];
+    __shared__ uint32_t lds[8];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), m = lane & 15, kg = lane >> 4;
+    const uint32_t per_seq = (uint32_t)(a.kv_heads * a.q_groups);
+
+    // the piece of this workgroup: segment (b, hq) from tile `from` on, `left` tiles in all
+    uint32_t b, hq, from;
+    uint64_t left;
+    if (a.whole) {
+        b = blockIdx.x / per_seq;
+        hq = blockIdx.x - b * per_seq;
+        from = 0;
+        left = tiles_of(tokens_of(a, (int)b));
+    } else {
+        uint32_t all;
+        if (threadIdx.x < 4) lds[4 + threadIdx.x] = 0;
+        scan_sequences(a, lds, all,
+                       [&](uint32_t all_, uint32_t before, uint32_t t) {
+                           const Split s = split_of(a, all_, gridDim.x);
+                           if (blockIdx.x >= s.pieces) return false;
+                           const uint64_t at = s.start(blockIdx.x);
+                           return (uint64_t)before * per_seq <= at && at < (uint64_t)(before + t) * per_seq;
+                       },
+                       [&](int b_, uint32_t before) { lds[4] = (uint32_t)b_; lds[5] = before; });
+        for (uint32_t e = blockIdx.x; e < (uint32_t)a.B; e += gridDim.x) {      // sequences without tokens
+            if (tokens_of(a, (int)e) > 0) continue;
+            uint2* out = reinterpret_cast<uint2*>(a.out + (int64_t)e * a.q_heads * a.dim);
+            for (int i = (int)threadIdx.x; i < a.q_heads * a.dim / 4; i += 256) out[i] = uint2{0, 0};
+        }
+        const Split s = split_of(a, all, gridDim.x);
+        if (blockIdx.x >= s.pieces) return;
+        const uint64_t at = s.start(blockIdx.x);
+        left = s.start(blockIdx.x + 1) - at;
+        b = __builtin_amdgcn_readfirstlane(lds[4]);
+        const uint64_t rest = at - (uint64_t)__builtin_amdgcn_readfirstlane(lds[5]) * per_seq;
+        const uint32_t t = tiles_of(tokens_of(a, (int)b));
+        hq = (uint32_t)(rest / t);
+        from = (uint32_t)(rest - (uint64_t)hq * t);
+    }
+    do {
+        const int n = tokens_of(a, (int)b);
+        const uint32_t tiles = tiles_of(n);
+        const uint32_t to = left < tiles - from ? from + (uint32_t)left : tiles;
+        const int head = (int)(hq / (uint32_t)a.q_groups), first_query = (int)(hq - (uint32_t)head * a.q_groups) * kQueries;
+        const int queries = a.share - first_query < kQueries ? a.share - first_query : kQueries;
+        const int q_head = head * a.share + first_query;
+        const int32_t* table = a.table + (int64_t)b * a.table_row;
+        const int page_mask = (1 << a.page_shift) - 1;
+
+        // ---- Q: operand blocks, and for codes the sum of every group and a power of two that brings bfloat16 into float16 ----
+        u4 q[F::NK];
+        float q_sum[F::kGroups], score_scale = a.scale;
+        {
+            const uint16_t* src = a.q + b * a.q_row + (q_head + (m < queries ? m : 0)) * a.q_head;
+#pragma unroll
+            for (int k = 0; k < F::NK; k++) {
+                const int d = F::k_at(k, kg);
+                q[k] = m < queries && d < a.dim ? *reinterpret_cast<const u4*>(src + d) : u4{0, 0, 0, 0};
+            }
+            if constexpr (F::kCodes) {
+                float x[F::NK][8], top = 0.f;
+#pragma unroll
+                for (int k = 0; k < F::NK; k++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const uint16_t u = (uint16_t)(q[k][e / 2] >> (16 * (e & 1)));
+                        x[k][e] = a.q_bf16 ? bf16_to_f32(u) : f16_bits(u);
+                        top = fmaxf(top, __builtin_fabsf(x[k][e]));
+                    }
+                if (a.q_bf16) {                                   // exact but for values 2^38 and more below the largest
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const int e = top > 0.f && top <= 3.4e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+                    score_scale = __builtin_ldexpf(a.scale, e);
+#pragma unroll
+                    for (int k = 0; k < F::NK; k++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[k][i] = __builtin_ldexpf(x[k][i], -e);
+                }
+#pragma unroll
+                for (int g = 0; g < F::kGroups; g++) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int k = g * F::kPerK; k < (g + 1) * F::kPerK; k++) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) s += x[k][e];
+#pragma unroll
+                        for (int p = 0; p < 4; p++) {
+                            const h2 v = {(_Float16)x[k][query_order<F::kBits>(2 * p)], (_Float16)x[k][query_order<F::kBits>(2 * p + 1)]};
+                            q[k][p] = as_u32(v);
+                        }
+                    }
+                    s += __shfl_xor(s, 16, 64);
+                    q_sum[g] = s + __shfl_xor(s, 32, 64);
+                }
+            }
+        }
+
+        // ---- addresses ----
+        uint32_t key_off[F::kCodes ? F::kGroups : F::NK], value_off[F::kCodes ? F::kGroups : (F::kDim + 127) / 128];
+        if constexpr (F::kCodes) {
+#pragma unroll
+            for (int g = 0; g < F::kGroups; g++) {
+                key_off[g] = (uint32_t)(m * a.row_bytes + (g * F::kGroup + kg * (F::kGroup / 4)) * F::kBits / 8);
+                value_off[g] = (uint32_t)(4 * kg * a.row_bytes + g * F::kGroup * F::kBits / 8 + m * F::kValueBytes);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < F::NK; k++) key_off[k] = (uint32_t)(m * a.row_bytes + (F::k_at(k, kg) < a.dim ? 2 * F::k_at(k, kg) : 0));
+#pragma unroll
+            for (int h = 0; h < (F::kDim + 127) / 128; h++) value_off[h] = (uint32_t)(4 * kg * a.row_bytes + (F::v_at(m, 8 * h) < a.dim ? 2 * F::v_at(m, 8 * h) : 0));
+        }
+        auto halves_of = [&](uint32_t t) {
+            const int at = (int)t * kTile;
+            Halves h;
+            h.page[0] = __builtin_amdgcn_readfirstlane((uint32_t)table[at >> a.page_shift]);
+            h.page[1] = at + 16 < n ? __builtin_amdgcn_readfirstlane((uint32_t)table[(at + 16) >> a.page_shift]) : 0xFFFFFFFFu;
+            return h;
+        };
+        auto row_of = [&](const Halves& h, uint32_t t, int half) {  // row of the half's first token, in rows of this head's pages
+            const uint32_t page = h.page[half] < a.pages ? h.page[half] : 0;
+            return ((int64_t)page * a.kv_heads + head << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
+        };
+        auto load_meta = [&](const uint32_t* base, const Halves& h, uint32_t t, int half, u4* out) {
+            const uint32_t page = h.page[half] < a.pages ? h.page[half] : 0;
+            const uint32_t* p = base + (((int64_t)page * a.kv_heads + head) * F::kGroups << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
+#pragma unroll
+            for (int g = 0; g < F::kGroups; g++) out[g] = *reinterpret_cast<const u4*>(p + (g << a.page_shift) + 4 * kg);
+        };
+        KeyTile<F> keys;
+        ValueTile<F> values;
+        auto load_keys = [&](const Halves& h, uint32_t t) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const uint8_t* base = a.keys + row_of(h, t, half) * a.row_bytes;
+                if constexpr (F::kCodes) {
+#pragma unroll
+                    for (int g = 0; g < F::kGroups; g++) load_words<F::kKeyGroupWords>(base + key_off[g], keys.raw[half] + g * F::kKeyGroupWords);
+                    load_meta(a.key_meta, h, t, half, keys.meta[half]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < F::NK; k++) load_words<4>(base + key_off[k], keys.raw[half] + 4 * k);
+                }
+            }
+        };
+        auto load_values = [&](const Halves& h, uint32_t t) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const uint8_t* base = a.values + row_of(h, t, half) * a.row_bytes;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint8_t* row = base + i * a.row_bytes;
+                    uint32_t* out = values.raw[4 * half + i];
+                    if constexpr (F::kCodes) {
+#pragma unroll
+                        for (int g = 0; g < F::kGroups; g++) {
+                            const uint8_t* p = row + value_off[g];
+                            if constexpr (F::kValueBytes >= 4) load_words<F::kValueBytes / 4>(p, out + g * F::kValueGroupWords);
+                            else if constexpr (F::kValueBytes == 2) out[g] = *reinterpret_cast<const uint16_t*>(p);
+                            else out[g] = *p;
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < (F::kDim + 127) / 128; k++) load_words<F::kDim == 64 ? 2 : 4>(row + value_off[k], out + 4 * k);
+                    }
+                }
+                if constexpr (F::kCodes) load_meta(a.value_meta, h, t, half, values.meta[half]);
+            }
+        };
+
+        // ---- tiles ----
+        f4 acc[F::NV];
+        float r = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+        uint32_t t = from + wave;
+        if (t < to) {
+            Halves h = halves_of(t);
+            load_keys(h, t);
+            load_values(h, t);
+            for (;;) {
+                const uint32_t next = t + kWaves;
+                const bool more = next < to;
+                Halves hn = h;
+                if (more) hn = halves_of(next);
+                const int at = (int)t * kTile;
+                const bool full = at + kTile <= n && h.page[0] < a.pages && h.page[1] < a.pages;
+                bool seen[8];
+                if (!full) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) seen[e] = at + 16 * (e >> 2) + 4 * kg + (e & 3) < n && h.page[e >> 2] < a.pages;
+                }
+                // scores, in units of log 2
+                float x[8];
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    f4 s = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (F::kCodes) {
+#pragma unroll
+                        for (int g = 0; g < F::kGroups; g++) {
+                            f4 dot = {0.f, 0.f, 0.f, 0.f};
+                            uint32_t codes[4 * F::kPerK];
+#pragma unroll
+                            for (int w = 0; w < F::kKeyGroupWords; w++) key_codes<F::kBits>(keys.raw[half][g * F::kKeyGroupWords + w], codes + w * (16 / F::kBits));
+#pragma unroll
+                            for (int k = 0; k < F::kPerK; k++)
+                                dot = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[g * F::kPerK + k], dot);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const uint32_t pair = keys.meta[half][g][i];
+                                const float sc = f16_bits(pair), off = (float)(1 << (F::kBits - 1)) - f16_bits(pair >> 16);
+                                s[i] = __builtin_fmaf(sc, __builtin_fmaf(off, q_sum[g], dot[i]), s[i]);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < F::NK; k++) {
+                            const uint32_t* w = keys.raw[half] + 4 * k;
+                            s = mfma<F::kBf16>(u4{w[0], w[1], w[2], w[3]}, q[k], s);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[4 * half + i] = s[i] * score_scale;
+                }
+                if (more) load_keys(hn, next);
+                // reference: for codes the scores are raised by the exponent of the token's largest value scale
+                float unit[8];                                    // 2^-e
+                if constexpr (F::kCodes) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        if (!full) {
+#pragma unroll
+                            for (int g = 0; g < F::kGroups; g++) values.meta[e >> 2][g][e & 3] = seen[e] ? values.meta[e >> 2][g][e & 3] : 0u;
+                        }
+                        float top = f16_bits(values.meta[e >> 2][0][e & 3]);
+#pragma unroll
+                        for (int g = 1; g < F::kGroups; g++) top = fmaxf(top, f16_bits(values.meta[e >> 2][g][e & 3]));
+                        const int ex = __builtin_amdgcn_frexp_expf(top);
+                        x[e] += (float)ex;
+                        unit[e] = __builtin_ldexpf(1.f, -ex);
+                    }
+                }
+                if (!full) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = seen[e] ? x[e] : -INFINITY;
+                }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                if (__builtin_amdgcn_ballot_w64(top > r + kSlack)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), r);
+                    const float keep = top == r ? 1.f : __builtin_amdgcn_exp2f(r - top);
+                    r = top;
+                    l *= keep;
+#pragma unroll
+                    for (int j = 0; j < F::NV; j++) acc[j] *= keep;
+                }
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    p[e] = __builtin_amdgcn_exp2f(x[e] - r);
+                    if (!full) p[e] = seen[e] ? p[e] : 0.f;
+                    l = F::kCodes ? __builtin_fmaf(p[e], unit[e], l) : l + p[e];
+                }
+                // weighted values
+                if constexpr (F::kCodes) {
+#pragma unroll
+                    for (int g = 0; g < F::kGroups; g++) {
+                        float pg[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) pg[e] = p[e] * (f16_bits(values.meta[e >> 2][g][e & 3]) * unit[e]);
+                        u4 hi, lo;
+                        h2 zz[4], zz16[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const h2 z = as_h2(token_pair<true>(values.meta[i >> 1][g][2 * (i & 1) + 1], values.meta[i >> 1][g][2 * (i & 1)]));
+                            zz[i] = splat((_Float16)-1024.f) - z;
+                            zz16[i] = splat((_Float16)-64.f) - z;
+                            hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
+                            lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
+                        }
+                        static_for<0, F::kPerV>([&](auto jc) {
+                            constexpr int j = decltype(jc)::value, per = 16 / F::kBits;       // codes in 16 bits of a token
+                            u4 v;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                constexpr int w = j / (2 * per);
+                                const uint32_t pair = token_pair<(j / per) & 1>(values.raw[2 * i + 1][g * F::kValueGroupWords + w], values.raw[2 * i][g * F::kValueGroupWords + w]);
+                                v[i] = value_codes<F::kBits, j % per>(pair, zz[i], zz16[i]);
+                            }
+                            acc[g * F::kPerV + j] = mfma<false>(v, hi, acc[g * F::kPerV + j]);
+                            acc[g * F::kPerV + j] = mfma<false>(v, lo, acc[g * F::kPerV + j]);
+                        });
+                    }
+                } else {
+                    if (!full) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+#pragma unroll
+                            for (int w = 0; w < F::kValueWords; w++) values.raw[e][w] = seen[e] ? values.raw[e][w] : 0u;
+                    }
+                    u4 hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        hi[i] = split_pair<F::kBf16>(p[2 * i], p[2 * i + 1]);
+                        lo[i] = pair_of<F::kBf16>(p[2 * i], p[2 * i + 1]);
+                    }
+                    static_for<0, F::NV>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        u4 v;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[i] = token_pair<(j & 1) != 0>(values.raw[2 * i + 1][j / 2], values.raw[2 * i][j / 2]);
+                        acc[j] = mfma<F::kBf16>(v, hi, acc[j]);
+                        acc[j] = mfma<F::kBf16>(v, lo, acc[j]);
+                    });
+                }
+                if (!more) break;
+                load_values(hn, next);
+                h = hn;
+                t = next;
+            }
+        }
+
+        // ---- the four waves of the workgroup joined ----
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (kg == 0) {
+            stats[wave][0][m] = r;
+            stats[wave][1][m] = l;
+        }
+        __syncthreads();
+        const float r_all = fmaxf(fmaxf(stats[0][0][m], stats[1][0][m]), fmaxf(stats[2][0][m], stats[3][0][m]));
+        const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - r_all);
+        const bool complete = from == 0 && to == tiles;
+        float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (from == 0)) * (2 * kQueries + a.queries * a.dim);
+        auto joined = [&](int query, float& top) {                // sum of the waves' l, relative to the largest r
+            top = fmaxf(fmaxf(stats[0][0][query], stats[1][0][query]), fmaxf(stats[2][0][query], stats[3][0][query]));
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float rw = stats[w][0][query];
+                sum += (rw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rw - top)) * stats[w][1][query];
+            }
+            return sum;
+        };
+        if (!complete && threadIdx.x < (uint32_t)queries) {
+            float top;
+            slot[kQueries + threadIdx.x] = joined((int)threadIdx.x, top);
+            slot[threadIdx.x] = top;
+        }
+#pragma unroll
+        for (int c = 0; c < (F::NV + kChunkBlocks - 1) / kChunkBlocks; c++) {
+            if (c) __syncthreads();
+            if (m < queries) {
+#pragma unroll
+                for (int j = c * kChunkBlocks; j < (c + 1) * kChunkBlocks && j < F::NV; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) outs[wave][m][F::v_at(4 * kg + i, j) - c * kChunk] = acc[j][i] * f;
+            }
+            __syncthreads();
+            for (int e = (int)threadIdx.x; e < queries * (kChunk / 4); e += 256) {
+                const int query = e / (kChunk / 4), d = (e - query * (kChunk / 4)) * 4;
+                if (c * kChunk + d >= a.dim) continue;
+                f4 o = *reinterpret_cast<const f4*>(&outs[0][query][d]);
+#pragma unroll
+                for (int w = 1; w < kWaves; w++) o += *reinterpret_cast<const f4*>(&outs[w][query][d]);
+                if (complete) {
+                    float top;
+                    const float sum = joined(query, top), inv = sum == 0.f ? 0.f : 1.f / sum;
+                    store_out(a, (int64_t)b * a.q_heads + q_head + query, c * kChunk + d, o * inv);
+                } else {
+                    *reinterpret_cast<f4*>(slot + 2 * kQueries + query * a.dim + c * kChunk + d) = o;
+                }
+            }
+        }
+        __syncthreads();                                          // (the next segment writes stats and outs again)
+        left -= to - from;
+        from = 0;
+        if (left) {
+            if (++hq == per_seq) {
+                hq = 0;
+                do
+                    if (++b >= (uint32_t)a.B) return;             // (never, while nobody writes the lengths)
+                while (tokens_of(a, (int)b) == 0);
+            }
+        }
+    } while (left);
+}
