@@ -6,54 +6,67 @@
 
 namespace {
 
-// One workgroup for 128 values of a segment's output [queries][dim]: 32 threads of 4 values each, eight such rows that share the pieces.
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, uint32_t grid, int chunks) {
-    __shared__ uint32_t lds[8];
-    __shared__ float tops[8][32];
-    __shared__ f4 outs[8][32];
-    __shared__ float sums[8][32];
-    const uint32_t segment = blockIdx.x / (uint32_t)chunks, chunk = blockIdx.x - segment * chunks, per_seq = (uint32_t)(a.kv_heads * a.q_groups);
-    const uint32_t b = segment / per_seq, hq = segment - b * per_seq;
-    uint32_t all;
-    scan_sequences(a, lds, all, [&](uint32_t, uint32_t, uint32_t) { return true; },
-                   [&](int b_, uint32_t before) { if ((uint32_t)b_ == b) lds[4] = before; });
-    const uint32_t tiles = tiles_of(tokens_of(a, (int)b));
-    if (tiles == 0) return;
-    const Split s = split_of(a, all, grid);
-    const uint64_t first = (uint64_t)lds[4] * per_seq + (uint64_t)hq * tiles;
-    const uint32_t w0 = s.piece_of(first), w1 = s.piece_of(first + tiles - 1);
-    if (w0 == w1) return;
+// One workgroup for 128 values of the output [queries][dim] of the segment that piece blockIdx.x / chunks began and left unfinished, if it did: 32
+// threads of 4 values each, 8 such rows that share the parts, four parts of a thread under way at a time.  What bounds it is the way to
+// memory and back twice (the joint, the parts), not its work.
+constexpr int kJoinValues = 128, kJoinRows = 8, kJoinAhead = 4;
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, int chunks) {
+    __shared__ float tops[kJoinRows][32], sums[kJoinRows][32];
+    __shared__ f4 outs[kJoinRows][32];
+    const uint32_t w0 = blockIdx.x / (uint32_t)chunks, chunk = blockIdx.x - w0 * chunks;
+    const Joint joint = a.joints[w0];
+    if (joint.parts == 0) return;
+    const uint32_t b = joint.b, hq = joint.hq, w1 = w0 + joint.parts - 1;
     const int head = (int)(hq / (uint32_t)a.q_groups), first_query = (int)(hq - (uint32_t)head * a.q_groups) * kQueries;
     const int queries = a.share - first_query < kQueries ? a.share - first_query : kQueries;
     const int x = (int)threadIdx.x & 31, y = (int)threadIdx.x >> 5;
     const int e = ((int)chunk * 32 + x) * 4, query = e / a.dim;
     const bool live = query < queries;
     const int64_t pitch = 2 * kQueries + a.queries * a.dim;
-    auto slot = [&](uint32_t w) { return a.partial + (2 * (int64_t)w + (w == w0)) * pitch; };
-    float top = -INFINITY;
-    if (live)
-        for (uint32_t w = w0 + y; w <= w1; w += 8) top = fmaxf(top, slot(w)[query]);
-    tops[y][x] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = fmaxf(top, tops[i][x]);
+    float top = -INFINITY, sum = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    if (live)
-        for (uint32_t w = w0 + y; w <= w1; w += 8) {
-            const float* p = slot(w);
-            const float r = p[query], f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - top);
-            sum += f * p[kQueries + query];
-            o += f * *reinterpret_cast<const f4*>(p + 2 * kQueries + e);
+    if (live) {
+        for (uint32_t w = w0 + y; w <= w1; w += kJoinAhead * kJoinRows) {
+            float r[kJoinAhead], l[kJoinAhead];
+            f4 v[kJoinAhead];
+#pragma unroll
+            for (int i = 0; i < kJoinAhead; i++) {
+                const uint32_t part = w + i * kJoinRows;
+                const float* p = a.partial + (2 * (int64_t)(part <= w1 ? part : w) + (part == w0)) * pitch;
+                r[i] = part <= w1 ? p[query] : -INFINITY;
+                l[i] = p[kQueries + query];
+                v[i] = *reinterpret_cast<const f4*>(p + 2 * kQueries + e);
+            }
+            float now = top;
+#pragma unroll
+            for (int i = 0; i < kJoinAhead; i++) now = fmaxf(now, r[i]);
+            const float keep = top == now ? 1.f : __builtin_amdgcn_exp2f(top - now);
+            top = now;
+            sum *= keep;
+            o *= keep;
+#pragma unroll
+            for (int i = 0; i < kJoinAhead; i++) {
+                if (w + i * kJoinRows > w1) break;
+                const float f = r[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[i] - top);
+                sum += f * l[i];
+                o += f * v[i];
+            }
         }
-    outs[y][x] = o;
+    }
+    tops[y][x] = top;
     sums[y][x] = sum;
+    outs[y][x] = o;
     __syncthreads();
     if (y || !live) return;
 #pragma unroll
-    for (int i = 1; i < 8; i++) {
-        o += outs[i][x];
-        sum += sums[i][x];
+    for (int i = 1; i < kJoinRows; i++) top = fmaxf(top, tops[i][x]);
+    o = f4{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinRows; i++) {
+        const float f = tops[i][x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(tops[i][x] - top);
+        sum += f * sums[i][x];
+        o += f * outs[i][x];
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     store_out(a, (int64_t)b * a.q_heads + head * a.share + first_query + query, e - query * a.dim, o * inv);
@@ -62,14 +75,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, ui
 int attention_check(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     if (int st = bw_cache_check(c)) return st;
     if (B < 0 || q_heads < 1 || q_heads % c->kv_heads || max_pages < 1) return BW_EINVAL;
-    if (B > 1 << 20 || q_heads > 65535 || B * q_heads >= (int64_t)1 << 31 || max_pages * c->page_size >= (int64_t)1 << 25) return BW_EUNSUPPORTED;
-    if (B * ((max_pages * c->page_size + kTile - 1) / kTile) >= (int64_t)1 << 31 || B * q_heads * ((c->dim + 127) / 128 + 1) >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    if (B > 1 << 20 || q_heads > 65535 || max_pages * c->page_size >= (int64_t)1 << 25) return BW_EUNSUPPORTED;
+    if (B * ((max_pages * c->page_size + kTile - 1) / kTile + kSegmentCost) >= ((int64_t)1 << 31) / q_heads || B * q_heads >= (int64_t)1 << 29) return BW_EUNSUPPORTED;
     return BW_OK;
 }
 
 // Workgroups, and whether every segment gets one of its own.
 struct Plan { uint32_t grid; bool whole; };
-constexpr int kMinTiles = 8, kWholeTokens = 512;
+constexpr int kMinUnits = 8, kWholeTokens = 512;
 Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
     Plan p;
@@ -88,7 +101,7 @@ extern "C" size_t bw_cache_attention_workspace_bytes(const bw_cache* c, int64_t 
     if (attention_check(c, B, q_heads, max_pages) != BW_OK || B == 0) return 0;
     const Plan p = plan_of(c, B, q_heads, max_pages);
     const int share = q_heads / c->kv_heads, queries = share < kQueries ? share : kQueries;
-    return p.whole ? 0 : (size_t)p.grid * 2 * (2 * kQueries + queries * c->dim) * sizeof(float);
+    return p.whole ? 0 : (size_t)p.grid * (sizeof(Joint) + 2 * (2 * kQueries + queries * c->dim) * sizeof(float));
 }
 
 extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head,
@@ -112,7 +125,8 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     a.keys = (const uint8_t*)c->keys; a.values = (const uint8_t*)c->values;
     a.key_meta = (const uint32_t*)c->key_meta; a.value_meta = (const uint32_t*)c->value_meta;
     a.out = (uint16_t*)out;
-    a.partial = (float*)workspace;
+    a.joints = (Joint*)workspace;
+    a.partial = (float*)(a.joints + plan.grid);
     a.pages = (uint32_t)c->pages;
     a.B = (int)B;
     a.q_heads = q_heads; a.kv_heads = c->kv_heads; a.share = q_heads / c->kv_heads;
@@ -122,7 +136,7 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     a.page_shift = bw_log2(c->page_size);
     a.max_tokens = (int)(max_pages * c->page_size);
     a.q_bf16 = act_dtype == BW_BF16;
-    a.min_tiles = kMinTiles;
+    a.min_units = kMinUnits;
     a.whole = plan.whole;
     a.scale = scale * 1.44269504088896340736f;
     const hipStream_t st = (hipStream_t)stream;
@@ -139,8 +153,8 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     }
     if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     if (!plan.whole) {
-        const int chunks = (a.queries * a.dim + 127) / 128;
-        hipLaunchKernelGGL(attention_join_kernel, dim3((unsigned)(B * a.kv_heads * a.q_groups * chunks)), dim3(256), 0, st, a, plan.grid, chunks);
+        const int chunks = (a.queries * a.dim + kJoinValues - 1) / kJoinValues;
+        hipLaunchKernelGGL(attention_join_kernel, dim3(plan.grid * chunks), dim3(256), 0, st, a, chunks);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;

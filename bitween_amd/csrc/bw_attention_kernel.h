@@ -1,9 +1,10 @@
 // bw_attention_kernel.h - attention of one new token over a paged cache: the kernel template, its arguments and the split of its work.
 //
-// Work is counted in tiles of 32 tokens of one segment: one sequence, one key-value head, up to 16 of the query heads that read it.  The
-// tiles of all segments, in order, are cut into equal pieces, one for each workgroup, so that sequences of very different length load the
-// chip evenly; lengths are read on the GPU, so the cut follows them.  A segment that lies in one piece is finished by its workgroup; the parts
-// of one that lies in several go to the workspace and are joined by attention_join_kernel.
+// Work is counted in tiles of 32 tokens of one segment: one sequence, one key-value head, up to 16 of the query heads that read it.  A segment
+// counts as its tiles and kSegmentCost more, what beginning and joining it takes.  The segments, one after the other, are cut into equal pieces,
+// one for each workgroup, so that sequences of very different length load the chip evenly; lengths are read on the GPU, so the cut
+// follows them.  A segment that lies in one piece is finished by its workgroup; the parts of one that lies in several go to the workspace
+// and are joined by attention_join_kernel.
 //
 // The four waves of a workgroup take tiles in turn, each with a running reference r and sum l of its own.  One wave, one tile, everything in
 // registers:
@@ -27,7 +28,11 @@
 #include "bw_cache.h"
 
 constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
+constexpr uint32_t kSegmentCost = 5;             // tiles
 constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
+
+// A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
+struct Joint { uint32_t b, hq, parts, unused; };
 
 struct AttentionArgs {
     const uint16_t* q;
@@ -37,66 +42,90 @@ struct AttentionArgs {
     const uint8_t *keys, *values;
     const uint32_t *key_meta, *value_meta;
     uint16_t* out;
+    Joint* joints;                               // what each workgroup leaves to join
     float* partial;                              // 2 slots for each workgroup: r [16], l [16], O [queries][dim]
     int64_t page_bytes, meta_words;              // of one head in one page: row bytes * page_size; pairs
     uint32_t pages;
     int B, q_heads, kv_heads, share, queries, q_groups;   // queries: of a segment, at most 16; q_groups: segments of a key-value head
-    int dim, row_bytes, page_shift, max_tokens, q_bf16, min_tiles, whole;
+    int dim, row_bytes, page_shift, max_tokens, q_bf16, min_units, whole;
     float scale;                                 // times log2 e
 };
 
-// What a workgroup (or the join of a segment) has to know of the split.
-struct Split {
-    uint32_t tiles;                              // of all sequences, for one head
-    uint64_t total;                              // tiles of all segments
-    uint32_t pieces;
-    BW_DEV uint64_t start(uint32_t w) const { return (total >> 32) == 0 && total * pieces >> 32 == 0 ? (uint32_t)total * w / pieces : total * w / pieces; }
-    BW_DEV uint32_t piece_of(uint64_t tile) const { return (uint32_t)(((tile + 1) * pieces - 1) / total); }
-};
+// A value that all lanes read at one address, through the scalar cache: lengths and table, which nothing writes while the kernel runs.
+BW_DEV int32_t uniform_load(const int32_t* p, int64_t i) { return ((const __attribute__((address_space(4))) int32_t*)p)[i]; }
 
-BW_DEV int tokens_of(const AttentionArgs& a, int b) {
-    const int n = a.lengths[b];
-    return n < 0 ? 0 : n < a.max_tokens ? n : a.max_tokens;
-}
+BW_DEV int clipped(const AttentionArgs& a, int n) { return n < 0 ? 0 : n < a.max_tokens ? n : a.max_tokens; }
+BW_DEV int tokens_of(const AttentionArgs& a, uint32_t b) { return clipped(a, uniform_load(a.lengths, b)); }
 BW_DEV uint32_t tiles_of(int tokens) { return ((uint32_t)tokens + kTile - 1) >> kTileShift; }
+BW_DEV uint32_t units_of(int tokens) { return tokens ? tiles_of(tokens) + kSegmentCost : 0; }
 
-// Sums of tiles over the sequences by one workgroup of 256 threads: thread i sums a run of sequences, the runs are added up over the lanes and
-// then the waves.  `found(b, before)` is called by one thread, for the sequence that `wanted` asks for: wanted(before, tiles) -> bool.
-template <class Wanted, class Found>
-BW_DEV void scan_sequences(const AttentionArgs& a, uint32_t* lds, uint32_t& all, Wanted&& wanted, Found&& found) {
-    const int run = (a.B + 255) >> 8, first = (int)threadIdx.x * run, lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+// The pieces, in units: `longer` of them have one more than the others.  Tile i of a segment is its unit kSegmentCost + i.
+struct Split {
+    uint32_t pieces, size, longer;
+    BW_DEV uint32_t start(uint32_t w) const { return w * size + (w < longer ? w : longer); }
+    BW_DEV uint32_t piece_of(uint32_t unit) const {
+        const uint32_t head = longer * (size + 1);
+        return unit < head ? unit / (size + 1) : longer + (unit - head) / size;
+    }
+};
+BW_DEV Split split_of(const AttentionArgs& a, uint32_t units, uint32_t grid) {
+    const uint32_t total = units * (uint32_t)(a.kv_heads * a.q_groups), pieces = (total + a.min_units - 1) / (uint32_t)a.min_units;
+    Split s;
+    s.pieces = pieces < grid ? pieces : grid;
+    s.size = s.pieces ? total / s.pieces : 0;
+    s.longer = total - s.pieces * s.size;
+    return s;
+}
+
+// A sequence, the units (for one head) of the sequences before it, and of all.
+struct Place { uint32_t b, before, all; };
+
+// The sequence that wanted(all, before, units) picks, by sums over the sequences.  Up to 64 sequences every wave does it for itself, a lane for
+// each sequence; more: thread i sums a run of them, the runs are added up over the lanes and then the four waves.
+template <class Wanted>
+BW_DEV Place find_sequence(const AttentionArgs& a, uint32_t* lds, Wanted&& wanted) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const bool wide = a.B > 64;
+    const int run = wide ? (a.B + 255) >> 8 : 1, first = wide ? (int)threadIdx.x * run : lane;
     uint32_t mine = 0;
-    for (int b = first; b < first + run && b < a.B; b++) mine += tiles_of(tokens_of(a, b));
+    for (int b = first; b < first + run && b < a.B; b++) mine += units_of(clipped(a, a.lengths[b]));
     uint32_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t other = __shfl_up(sum, o, 64);
         if (lane >= o) sum += other;
     }
+    Place p = {0, 0, 0};
+    if (!wide) {
+        p.all = __builtin_amdgcn_readlane(sum, 63);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < a.B && wanted(p.all, sum - mine, mine));
+        if (hit) {
+            p.b = (uint32_t)__builtin_ctzll(hit);
+            p.before = __builtin_amdgcn_readlane(sum - mine, p.b);
+        }
+        return p;
+    }
     if (lane == 63) lds[wave] = sum;
     __syncthreads();
     uint32_t before = sum - mine;
-    all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
-        if (w < wave) before += lds[w];
-        all += lds[w];
+        const uint32_t part = __builtin_amdgcn_readfirstlane(lds[w]);
+        if (w < wave) before += part;
+        p.all += part;
     }
     for (int b = first; b < first + run && b < a.B; b++) {
-        const uint32_t t = run == 1 ? mine : tiles_of(tokens_of(a, b));
-        if (wanted(all, before, t)) found(b, before);
+        const uint32_t t = run == 1 ? mine : units_of(clipped(a, a.lengths[b]));
+        if (wanted(p.all, before, t)) {
+            lds[4] = (uint32_t)b;
+            lds[5] = before;
+        }
         before += t;
     }
     __syncthreads();
-}
-
-BW_DEV Split split_of(const AttentionArgs& a, uint32_t tiles, uint32_t grid) {
-    Split s;
-    s.tiles = tiles;
-    s.total = (uint64_t)tiles * (uint32_t)(a.kv_heads * a.q_groups);
-    const uint64_t pieces = (s.total + a.min_tiles - 1) / (uint32_t)a.min_tiles;
-    s.pieces = pieces < grid ? (uint32_t)pieces : grid;
-    return s;
+    p.b = __builtin_amdgcn_readfirstlane(lds[4]);
+    p.before = __builtin_amdgcn_readfirstlane(lds[5]);
+    return p;
 }
 
 BW_DEV void store_out(const AttentionArgs& a, int64_t row, int d, f4 o) {
@@ -219,44 +248,42 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), m = lane & 15, kg = lane >> 4;
     const uint32_t per_seq = (uint32_t)(a.kv_heads * a.q_groups);
 
-    // the piece of this workgroup: segment (b, hq) from tile `from` on, `left` tiles in all
-    uint32_t b, hq, from;
-    uint64_t left;
+    // the piece of this workgroup: from unit `at` of segment (b, hq) on, `left` units in all
+    uint32_t b, hq, at, left;
+    Split s;
     if (a.whole) {
         b = blockIdx.x / per_seq;
         hq = blockIdx.x - b * per_seq;
-        from = 0;
-        left = tiles_of(tokens_of(a, (int)b));
+        at = 0;
+        left = tiles_of(tokens_of(a, b)) + kSegmentCost;
     } else {
-        uint32_t all;
-        if (threadIdx.x < 4) lds[4 + threadIdx.x] = 0;
-        scan_sequences(a, lds, all,
-                       [&](uint32_t all_, uint32_t before, uint32_t t) {
-                           const Split s = split_of(a, all_, gridDim.x);
-                           if (blockIdx.x >= s.pieces) return false;
-                           const uint64_t at = s.start(blockIdx.x);
-                           return (uint64_t)before * per_seq <= at && at < (uint64_t)(before + t) * per_seq;
-                       },
-                       [&](int b_, uint32_t before) { lds[4] = (uint32_t)b_; lds[5] = before; });
+        const Place place = find_sequence(a, lds, [&](uint32_t all, uint32_t before, uint32_t units) {
+            s = split_of(a, all, gridDim.x);
+            const uint32_t start = s.start(blockIdx.x);
+            return blockIdx.x < s.pieces && before * per_seq <= start && start < (before + units) * per_seq;
+        });
+        if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
         for (uint32_t e = blockIdx.x; e < (uint32_t)a.B; e += gridDim.x) {      // sequences without tokens
-            if (tokens_of(a, (int)e) > 0) continue;
+            if (tokens_of(a, e) > 0) continue;
             uint2* out = reinterpret_cast<uint2*>(a.out + (int64_t)e * a.q_heads * a.dim);
             for (int i = (int)threadIdx.x; i < a.q_heads * a.dim / 4; i += 256) out[i] = uint2{0, 0};
         }
-        const Split s = split_of(a, all, gridDim.x);
+        s = split_of(a, place.all, gridDim.x);
         if (blockIdx.x >= s.pieces) return;
-        const uint64_t at = s.start(blockIdx.x);
-        left = s.start(blockIdx.x + 1) - at;
-        b = __builtin_amdgcn_readfirstlane(lds[4]);
-        const uint64_t rest = at - (uint64_t)__builtin_amdgcn_readfirstlane(lds[5]) * per_seq;
-        const uint32_t t = tiles_of(tokens_of(a, (int)b));
-        hq = (uint32_t)(rest / t);
-        from = (uint32_t)(rest - (uint64_t)hq * t);
+        const uint32_t start = s.start(blockIdx.x), rest = start - place.before * per_seq;
+        left = s.start(blockIdx.x + 1) - start;
+        b = place.b;
+        const uint32_t units = units_of(tokens_of(a, b));
+        hq = rest / units;
+        at = rest - hq * units;
     }
+    const uint32_t first_left = left;
     do {
-        const int n = tokens_of(a, (int)b);
-        const uint32_t tiles = tiles_of(n);
-        const uint32_t to = left < tiles - from ? from + (uint32_t)left : tiles;
+        const int n = tokens_of(a, b);
+        const uint32_t tiles = tiles_of(n), units = tiles + kSegmentCost, end = left < units - at ? at + left : units;
+        const uint32_t from = at > kSegmentCost ? at - kSegmentCost : 0, to = end > kSegmentCost ? end - kSegmentCost : 0;
+        const uint32_t taken = end - at;
+        if (from < to || a.whole) {
         const int head = (int)(hq / (uint32_t)a.q_groups), first_query = (int)(hq - (uint32_t)head * a.q_groups) * kQueries;
         const int queries = a.share - first_query < kQueries ? a.share - first_query : kQueries;
         const int q_head = head * a.share + first_query;
@@ -329,8 +356,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
         auto halves_of = [&](uint32_t t) {
             const int at = (int)t * kTile;
             Halves h;
-            h.page[0] = __builtin_amdgcn_readfirstlane((uint32_t)table[at >> a.page_shift]);
-            h.page[1] = at + 16 < n ? __builtin_amdgcn_readfirstlane((uint32_t)table[(at + 16) >> a.page_shift]) : 0xFFFFFFFFu;
+            h.page[0] = (uint32_t)uniform_load(table, at >> a.page_shift);
+            h.page[1] = at + 16 < n ? (uint32_t)uniform_load(table, (at + 16) >> a.page_shift) : 0xFFFFFFFFu;
             return h;
         };
         auto row_of = [&](const Halves& h, uint32_t t, int half) {  // row of the half's first token, in rows of this head's pages
@@ -390,150 +417,153 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 #pragma unroll
         for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
         uint32_t t = from + wave;
+        Halves h = {}, hn = {};
         if (t < to) {
-            Halves h = halves_of(t);
+            h = halves_of(t);
             load_keys(h, t);
             load_values(h, t);
-            for (;;) {
-                const uint32_t next = t + kWaves;
-                const bool more = next < to;
-                Halves hn = h;
-                if (more) hn = halves_of(next);
-                const int at = (int)t * kTile;
-                const bool full = at + kTile <= n && h.page[0] < a.pages && h.page[1] < a.pages;
-                bool seen[8];
-                if (!full) {
+        }
+        while (t < to) {
+            const uint32_t next = t + kWaves;
+            const bool more = next < to;
+            if (more) hn = halves_of(next);
+            // Tokens that do not count: behind the end, or on a page outside the cache.
+            const bool full = (int)t * kTile + kTile <= n && h.page[0] < a.pages && h.page[1] < a.pages;
+            bool seen[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) seen[e] = at + 16 * (e >> 2) + 4 * kg + (e & 3) < n && h.page[e >> 2] < a.pages;
-                }
-                // scores, in units of log 2
-                float x[8];
+            for (int e = 0; e < 8; e++) seen[e] = (int)t * kTile + 16 * (e >> 2) + 4 * kg + (e & 3) < n && h.page[e >> 2] < a.pages;
+            // scores, in units of log 2
+            float x[8];
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    f4 s = {0.f, 0.f, 0.f, 0.f};
-                    if constexpr (F::kCodes) {
-#pragma unroll
-                        for (int g = 0; g < F::kGroups; g++) {
-                            f4 dot = {0.f, 0.f, 0.f, 0.f};
-                            uint32_t codes[4 * F::kPerK];
-#pragma unroll
-                            for (int w = 0; w < F::kKeyGroupWords; w++) key_codes<F::kBits>(keys.raw[half][g * F::kKeyGroupWords + w], codes + w * (16 / F::kBits));
-#pragma unroll
-                            for (int k = 0; k < F::kPerK; k++)
-                                dot = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[g * F::kPerK + k], dot);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const uint32_t pair = keys.meta[half][g][i];
-                                const float sc = f16_bits(pair), off = (float)(1 << (F::kBits - 1)) - f16_bits(pair >> 16);
-                                s[i] = __builtin_fmaf(sc, __builtin_fmaf(off, q_sum[g], dot[i]), s[i]);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < F::NK; k++) {
-                            const uint32_t* w = keys.raw[half] + 4 * k;
-                            s = mfma<F::kBf16>(u4{w[0], w[1], w[2], w[3]}, q[k], s);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[4 * half + i] = s[i] * score_scale;
-                }
-                if (more) load_keys(hn, next);
-                // reference: for codes the scores are raised by the exponent of the token's largest value scale
-                float unit[8];                                    // 2^-e
-                if constexpr (F::kCodes) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        if (!full) {
-#pragma unroll
-                            for (int g = 0; g < F::kGroups; g++) values.meta[e >> 2][g][e & 3] = seen[e] ? values.meta[e >> 2][g][e & 3] : 0u;
-                        }
-                        float top = f16_bits(values.meta[e >> 2][0][e & 3]);
-#pragma unroll
-                        for (int g = 1; g < F::kGroups; g++) top = fmaxf(top, f16_bits(values.meta[e >> 2][g][e & 3]));
-                        const int ex = __builtin_amdgcn_frexp_expf(top);
-                        x[e] += (float)ex;
-                        unit[e] = __builtin_ldexpf(1.f, -ex);
-                    }
-                }
-                if (!full) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = seen[e] ? x[e] : -INFINITY;
-                }
-                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                if (__builtin_amdgcn_ballot_w64(top > r + kSlack)) {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), r);
-                    const float keep = top == r ? 1.f : __builtin_amdgcn_exp2f(r - top);
-                    r = top;
-                    l *= keep;
-#pragma unroll
-                    for (int j = 0; j < F::NV; j++) acc[j] *= keep;
-                }
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    p[e] = __builtin_amdgcn_exp2f(x[e] - r);
-                    if (!full) p[e] = seen[e] ? p[e] : 0.f;
-                    l = F::kCodes ? __builtin_fmaf(p[e], unit[e], l) : l + p[e];
-                }
-                // weighted values
+            for (int half = 0; half < 2; half++) {
+                f4 s = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (F::kCodes) {
 #pragma unroll
                     for (int g = 0; g < F::kGroups; g++) {
-                        float pg[8];
+                        f4 dot = {0.f, 0.f, 0.f, 0.f};
+                        uint32_t codes[4 * F::kPerK];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) pg[e] = p[e] * (f16_bits(values.meta[e >> 2][g][e & 3]) * unit[e]);
-                        u4 hi, lo;
-                        h2 zz[4], zz16[4];
+                        for (int w = 0; w < F::kKeyGroupWords; w++) key_codes<F::kBits>(keys.raw[half][g * F::kKeyGroupWords + w], codes + w * (16 / F::kBits));
+#pragma unroll
+                        for (int k = 0; k < F::kPerK; k++)
+                            dot = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[g * F::kPerK + k], dot);
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const h2 z = as_h2(token_pair<true>(values.meta[i >> 1][g][2 * (i & 1) + 1], values.meta[i >> 1][g][2 * (i & 1)]));
-                            zz[i] = splat((_Float16)-1024.f) - z;
-                            zz16[i] = splat((_Float16)-64.f) - z;
-                            hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
-                            lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
+                            const uint32_t pair = keys.meta[half][g][i];
+                            const float sc = f16_bits(pair), off = (float)(1 << (F::kBits - 1)) - f16_bits(pair >> 16);
+                            s[i] = __builtin_fmaf(sc, __builtin_fmaf(off, q_sum[g], dot[i]), s[i]);
                         }
-                        static_for<0, F::kPerV>([&](auto jc) {
-                            constexpr int j = decltype(jc)::value, per = 16 / F::kBits;       // codes in 16 bits of a token
-                            u4 v;
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                constexpr int w = j / (2 * per);
-                                const uint32_t pair = token_pair<(j / per) & 1>(values.raw[2 * i + 1][g * F::kValueGroupWords + w], values.raw[2 * i][g * F::kValueGroupWords + w]);
-                                v[i] = value_codes<F::kBits, j % per>(pair, zz[i], zz16[i]);
-                            }
-                            acc[g * F::kPerV + j] = mfma<false>(v, hi, acc[g * F::kPerV + j]);
-                            acc[g * F::kPerV + j] = mfma<false>(v, lo, acc[g * F::kPerV + j]);
-                        });
                     }
                 } else {
-                    if (!full) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-#pragma unroll
-                            for (int w = 0; w < F::kValueWords; w++) values.raw[e][w] = seen[e] ? values.raw[e][w] : 0u;
+                    for (int k = 0; k < F::NK; k++) {
+                        const uint32_t* w = keys.raw[half] + 4 * k;
+                        s = mfma<F::kBf16>(u4{w[0], w[1], w[2], w[3]}, q[k], s);
                     }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[4 * half + i] = s[i] * score_scale;
+            }
+            if (more) load_keys(hn, next);
+            // reference: for codes the scores are raised by the exponent of the token's largest value scale
+            float unit[8];                                    // 2^-e
+            if constexpr (F::kCodes) {
+                if (!full) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+#pragma unroll
+                        for (int g = 0; g < F::kGroups; g++) values.meta[e >> 2][g][e & 3] = seen[e] ? values.meta[e >> 2][g][e & 3] : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float top = f16_bits(values.meta[e >> 2][0][e & 3]);
+#pragma unroll
+                    for (int g = 1; g < F::kGroups; g++) top = fmaxf(top, f16_bits(values.meta[e >> 2][g][e & 3]));
+                    const int ex = __builtin_amdgcn_frexp_expf(top);
+                    x[e] += (float)ex;
+                    unit[e] = __builtin_ldexpf(1.f, -ex);
+                }
+            }
+            if (!full) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = seen[e] ? x[e] : -INFINITY;
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            if (__builtin_amdgcn_ballot_w64(top > r + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), r);
+                const float keep = top == r ? 1.f : __builtin_amdgcn_exp2f(r - top);
+                r = top;
+                l *= keep;
+#pragma unroll
+                for (int j = 0; j < F::NV; j++) acc[j] *= keep;
+            }
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e] - r);
+            if (!full) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) p[e] = seen[e] ? p[e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                l = F::kCodes ? __builtin_fmaf(p[e], unit[e], l) : l + p[e];
+            }
+            // weighted values
+            if constexpr (F::kCodes) {
+#pragma unroll
+                for (int g = 0; g < F::kGroups; g++) {
+                    float pg[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) pg[e] = p[e] * (f16_bits(values.meta[e >> 2][g][e & 3]) * unit[e]);
                     u4 hi, lo;
+                    h2 zz[4], zz16[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        hi[i] = split_pair<F::kBf16>(p[2 * i], p[2 * i + 1]);
-                        lo[i] = pair_of<F::kBf16>(p[2 * i], p[2 * i + 1]);
+                        const h2 z = as_h2(token_pair<true>(values.meta[i >> 1][g][2 * (i & 1) + 1], values.meta[i >> 1][g][2 * (i & 1)]));
+                        zz[i] = splat((_Float16)-1024.f) - z;
+                        zz16[i] = splat((_Float16)-64.f) - z;
+                        hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
+                        lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
                     }
-                    static_for<0, F::NV>([&](auto jc) {
-                        constexpr int j = decltype(jc)::value;
+                    static_for<0, F::kPerV>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value, per = 16 / F::kBits;       // codes in 16 bits of a token
                         u4 v;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) v[i] = token_pair<(j & 1) != 0>(values.raw[2 * i + 1][j / 2], values.raw[2 * i][j / 2]);
-                        acc[j] = mfma<F::kBf16>(v, hi, acc[j]);
-                        acc[j] = mfma<F::kBf16>(v, lo, acc[j]);
+                        for (int i = 0; i < 4; i++) {
+                            constexpr int w = j / (2 * per);
+                            const uint32_t pair = token_pair<(j / per) & 1>(values.raw[2 * i + 1][g * F::kValueGroupWords + w], values.raw[2 * i][g * F::kValueGroupWords + w]);
+                            v[i] = value_codes<F::kBits, j % per>(pair, zz[i], zz16[i]);
+                        }
+                        acc[g * F::kPerV + j] = mfma<false>(v, hi, acc[g * F::kPerV + j]);
+                        acc[g * F::kPerV + j] = mfma<false>(v, lo, acc[g * F::kPerV + j]);
                     });
                 }
-                if (!more) break;
-                load_values(hn, next);
-                h = hn;
-                t = next;
+            } else {
+                if (!full) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+#pragma unroll
+                        for (int w = 0; w < F::kValueWords; w++) values.raw[e][w] = seen[e] ? values.raw[e][w] : 0u;
+                }
+                u4 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    hi[i] = split_pair<F::kBf16>(p[2 * i], p[2 * i + 1]);
+                    lo[i] = pair_of<F::kBf16>(p[2 * i], p[2 * i + 1]);
+                }
+                static_for<0, F::NV>([&](auto jc) {
+                    constexpr int j = decltype(jc)::value;
+                    u4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = token_pair<(j & 1) != 0>(values.raw[2 * i + 1][j / 2], values.raw[2 * i][j / 2]);
+                    acc[j] = mfma<F::kBf16>(v, hi, acc[j]);
+                    acc[j] = mfma<F::kBf16>(v, lo, acc[j]);
+                });
             }
+            if (more) load_values(hn, next);
+            h = hn;
+            t = next;
         }
 
         // ---- the four waves of the workgroup joined ----
@@ -548,6 +578,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
         const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - r_all);
         const bool complete = from == 0 && to == tiles;
         float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (from == 0)) * (2 * kQueries + a.queries * a.dim);
+        if (!complete && from == 0 && threadIdx.x == 0)
+            a.joints[blockIdx.x] = Joint{b, hq, s.piece_of(s.start(blockIdx.x) + (first_left - left) + units - at - 1) - blockIdx.x + 1, 0};
         auto joined = [&](int query, float& top) {                // sum of the waves' l, relative to the largest r
             top = fmaxf(fmaxf(stats[0][0][query], stats[1][0][query]), fmaxf(stats[2][0][query], stats[3][0][query]));
             float sum = 0.f;
@@ -589,14 +621,15 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
             }
         }
         __syncthreads();                                          // (the next segment writes stats and outs again)
-        left -= to - from;
-        from = 0;
+        }
+        left -= taken;
+        at = 0;
         if (left) {
             if (++hq == per_seq) {
                 hq = 0;
                 do
                     if (++b >= (uint32_t)a.B) return;             // (never, while nobody writes the lengths)
-                while (tokens_of(a, (int)b) == 0);
+                while (tokens_of(a, b) == 0);
             }
         }
     } while (left);
