@@ -82,7 +82,7 @@ int attention_check(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages
 
 // Workgroups, and whether every segment gets one of its own.
 struct Plan { uint32_t grid; bool whole; };
-constexpr int kMinUnits = 8, kWholeTokens = 512;
+constexpr int kMinUnits = 4, kWholeTokens = 512;
 Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
     Plan p;

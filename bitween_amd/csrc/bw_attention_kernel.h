@@ -129,9 +129,7 @@ BW_DEV Place find_sequence(const AttentionArgs& a, uint32_t* lds, Wanted&& wante
 }
 
 BW_DEV void store_out(const AttentionArgs& a, int64_t row, int d, f4 o) {
-    uint2 w;
-    if (a.q_bf16) w = uint2{f32_to_bf16(o[0]) | (uint32_t)f32_to_bf16(o[1]) << 16, f32_to_bf16(o[2]) | (uint32_t)f32_to_bf16(o[3]) << 16};
-    else w = uint2{as_u32(h2{(_Float16)o[0], (_Float16)o[1]}), as_u32(h2{(_Float16)o[2], (_Float16)o[3]})};
+    const uint2 w = a.q_bf16 ? uint2{narrow_pair<BW_BF16>(o[0], o[1]), narrow_pair<BW_BF16>(o[2], o[3])} : uint2{narrow_pair<BW_F16>(o[0], o[1]), narrow_pair<BW_F16>(o[2], o[3])};
     *reinterpret_cast<uint2*>(a.out + row * a.dim + d) = w;
 }
 

@@ -19,6 +19,24 @@ static inline int bw_cache_check(const bw_cache* c) {
     return BW_OK;
 }
 
+// n / d and what is left for n < 2^31, by one multiplication.
+struct FastDiv {
+    uint32_t d, mul;
+    int shift;
+    FastDiv(uint32_t divisor = 1) : d(divisor), mul(0), shift(0) {
+        if (d == 1) return;                                   // mul 0: n itself
+        int bits = 1;
+        while ((1ull << bits) < d) bits++;
+        mul = (uint32_t)((1ull << (31 + bits)) / d + 1);
+        shift = bits - 1;
+    }
+    BW_DEV uint32_t div(uint32_t n, uint32_t& rest) const {
+        const uint32_t q = mul ? __umulhi(n, mul) >> shift : n;
+        rest = n - q * d;
+        return q;
+    }
+};
+
 static inline int bw_log2(int v) {
     int s = 0;
     while ((1 << s) < v) s++;
@@ -30,8 +48,12 @@ template <int DT> BW_DEV float widen16(uint16_t u) {
     if constexpr (DT == BW_F16) return (float)__builtin_bit_cast(_Float16, u);
     else return bf16_to_f32(u);
 }
-template <int DT> BW_DEV uint16_t narrow16(float f) {
-    if constexpr (DT == BW_F16) return __builtin_bit_cast(uint16_t, (_Float16)f);
-    else return f32_to_bf16(f);
+template <int DT> BW_DEV uint32_t narrow_pair(float x, float y) {
+    if constexpr (DT == BW_F16) return as_u32(h2{(_Float16)x, (_Float16)y});
+    else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});        // (one instruction)
+    }
 }
+template <int DT> BW_DEV uint16_t narrow16(float f) { return (uint16_t)narrow_pair<DT>(f, f); }
 BW_DEV float f16_bits(uint32_t u) { return (float)__builtin_bit_cast(_Float16, (uint16_t)u); }

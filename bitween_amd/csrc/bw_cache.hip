@@ -4,12 +4,18 @@
 // The group / 8 neighbouring threads of a group agree on its extrema with cross-lane shuffles (group / 8 divides 64 and every row starts at
 // a multiple of it, so a group never leaves its wave), and the first of them stores the group's pair.
 //
-// The code of x is rint(x / s) of the exact quotient: with r = fl(1 / s), t = fl(x r) and one step t + (x - t s) r the result is the
-// correctly rounded quotient wherever rint could tell a difference - x has at most 11 significant bits and s 11, so a quotient up to 256
-// that is not exactly half way between two whole numbers lies at least 2^-13 from half way, and one that is half way has at most 10 bits, which
-// the step returns exactly (the residual of a representable quotient is exact in the fused operation).
+// The code of x is rint(x / s) of the exact quotient: with r = 1 / s to within a unit of its last place, t = x r and one step t + (x - t s) r the
+// result is the correctly rounded quotient wherever rint could tell a difference - x has at most 11 significant bits and s 11, so a
+// quotient up to 256 that is not exactly half way between two whole numbers lies at least 2^-13 from half way, and one that is half way has at
+// most 10 bits, which the step returns exactly (the residual is exact in the fused operation).  The range over 15 or 255 is that step too, with the
+// correctly rounded reciprocal: the correctly rounded quotient (checked over a whole binade and samples of all others).
 //
-// Both are one pass over memory: what bounds them is HBM beyond a few hundred tokens and the launch below.
+// Extrema of 16-bit floats are whole-number maxima of their bits: a positive value's bits grow with it, a negative one's are negative, so
+// max(0, bits) over a group is its largest value (or 0), max(0, bits ^ sign) its most negative one, and an infinity or a NaN shows as bits from the
+// infinity's on.  Both fit one register on the way over the lanes.
+//
+// Both kernels are one pass over memory: what bounds them is HBM beyond a few hundred tokens and the launch below.  32768 tokens of 8 heads of 128
+// at 8 bits: DOC_WRITE to write, DOC_READ to read back.
 #include "bw_cache.h"
 
 namespace {
@@ -22,7 +28,8 @@ struct CacheArgs {
     uint32_t *key_meta, *value_meta;
     uint16_t *k_out, *v_out;
     int64_t rows;                                // pages * page_size
-    int T, units, chunks, heads, groups, dim;    // units: threads of a token (2 * heads * chunks); chunks: dim / 8
+    int T, heads, groups, dim;
+    FastDiv units, chunks;                       // threads of a token (2 * heads * chunks); dim / 8
     int page_shift, group_shift;                 // group / 8 = 1 << group_shift
 };
 
@@ -39,19 +46,24 @@ BW_DEV int64_t pair_index(const CacheArgs& a, int64_t slot, int head, int g) {
 struct Unit { int token, head, chunk; bool value; };
 BW_DEV Unit unit_of(const CacheArgs& a, uint32_t i) {
     Unit u;
-    u.token = (int)(i / (uint32_t)a.units);
-    uint32_t at = i - (uint32_t)u.token * a.units;
-    u.value = at >= (uint32_t)a.units / 2;
-    if (u.value) at -= a.units / 2;
-    u.head = (int)(at / (uint32_t)a.chunks);
-    u.chunk = (int)(at - (uint32_t)u.head * a.chunks);
+    uint32_t at, chunk;
+    u.token = (int)a.units.div(i, at);
+    const uint32_t head = a.chunks.div(at, chunk);             // keys' heads, then values'
+    u.value = head >= (uint32_t)a.heads;
+    u.head = (int)head - (u.value ? a.heads : 0);
+    u.chunk = (int)chunk;
     return u;
 }
+
+// Larger of the two 16-bit whole numbers of each half.
+typedef short s2 __attribute__((ext_vector_type(2)));
+BW_DEV uint32_t max16(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s2, a), __builtin_bit_cast(s2, b))); }
+template <int CTRL> BW_DEV uint32_t max16_over(uint32_t v) { return max16(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false)); }
 
 template <int DT, int BITS>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    const bool live = i < (uint32_t)a.T * (uint32_t)a.units;
+    const bool live = i < (uint32_t)a.T * a.units.d;
     const Unit u = unit_of(a, live ? i : 0);
     const int64_t slot = a.slots[u.token];
     const bool kept = live && slot >= 0 && slot < a.rows;
@@ -61,46 +73,52 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
     if constexpr (BITS == 16) {
         if (kept) *reinterpret_cast<u4*>(out + (row_index(a, slot, u.head) * a.dim + u.chunk * 8) * 2) = w;
     } else {
-        constexpr float top = (float)((1 << BITS) - 1);
-        float x[8];
-        float lo = 0.f, hi = 0.f, bad = 0.f;
+        constexpr float top = (float)((1 << BITS) - 1), inv_top = 1.f / top;
+        uint32_t hi = 0, lo = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[j] = widen16<DT>((uint16_t)(w[j / 2] >> (16 * (j & 1))));
-            lo = fminf(lo, x[j]);
-            hi = fmaxf(hi, x[j]);
-            bad = fmaxf(bad, __builtin_fabsf(x[j]) <= 3.402823466e38f ? 0.f : 1.f);
+        for (int j = 0; j < 4; j++) {
+            hi = max16(hi, w[j]);
+            lo = max16(lo, w[j] ^ 0x80008000u);
         }
-        for (int o = 1; o < 1 << a.group_shift; o <<= 1) {
-            lo = fminf(lo, __shfl_xor(lo, o, 64));
-            hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-            bad = fmaxf(bad, __shfl_xor(bad, o, 64));
-        }
+        // low half: the largest value, high half: the size of the most negative one
+        uint32_t both = max16(__builtin_amdgcn_perm(lo, hi, 0x05040100u), __builtin_amdgcn_perm(lo, hi, 0x07060302u));
+        both = max16_over<0xB1>(both);                          // quad_perm: the neighbour
+        both = max16_over<0x4E>(both);                          // ... and the other two of four
+        if (a.group_shift > 2) both = max16_over<0x141>(both);  // row_half_mirror: the other four of eight
+        if (a.group_shift > 3) both = max16_over<0x140>(both);  // row_mirror: the other eight of sixteen
+        constexpr uint32_t inf = DT == BW_F16 ? 0x7C00u : 0x7F80u;
+        const bool bad = (both & 0xFFFFu) >= inf || (both >> 16) >= inf;
+        const float largest = widen16<DT>((uint16_t)both), smallest = -widen16<DT>((uint16_t)(both >> 16));
         // the scale rounds up, so that no code has to be clipped for its rounding; never 0
-        const float step = fminf(__fdiv_rn(__fsub_rn(hi, lo), top), 65504.f);
-        uint16_t sb = __builtin_bit_cast(uint16_t, (_Float16)step);
-        if ((float)__builtin_bit_cast(_Float16, sb) < step) sb++;
-        if (sb == 0) sb = 1;
-        const float s = (float)__builtin_bit_cast(_Float16, sb), r = __fdiv_rn(1.f, s);
+        const float range = largest - smallest, t0 = range * inv_top;
+        const float step = fminf(__builtin_fmaf(__builtin_fmaf(-t0, top, range), inv_top, t0), 65504.f);
+        uint32_t sb = __builtin_bit_cast(uint16_t, (_Float16)step);
+        sb += f16_bits(sb) < step ? 1 : 0;
+        sb = sb ? sb : 1;
+        const float s = f16_bits(sb), r = __builtin_amdgcn_rcpf(s);
+        // 1.5 2^23 added: the nearest whole number (ties to even) in the low bits, and whole numbers may be added to it
+        constexpr float kWhole = 12582912.f;
         auto whole = [&](float v) {
             const float t = v * r;
-            return rintf(__builtin_fmaf(__builtin_fmaf(-t, s, v), r, t));
+            return __builtin_fmaf(__builtin_fmaf(-t, s, v), r, t) + kWhole;
         };
-        const float z = fminf(whole(-lo), top);
-        uint32_t words[BITS / 4] = {};
+        const float z = fminf(whole(-smallest) - kWhole, top);
+        uint32_t q[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float q = fminf(fmaxf(whole(x[j]) + z, 0.f), top);        // (a NaN: 0)
-            words[j * BITS / 32] |= (uint32_t)q << (j * BITS % 32);
+            const float x = whole(widen16<DT>((uint16_t)(w[j / 2] >> (16 * (j & 1))))) + z;
+            q[j] = __builtin_bit_cast(uint32_t, fminf(fmaxf(x, kWhole), kWhole + top));        // (a NaN: 0)
         }
-        if (bad > 0.f) sb = 0x7E00;
         if (kept) {
+            auto bytes = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+                return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0C0C0400u), __builtin_amdgcn_perm(b1, b0, 0x0C0C0400u), 0x05040100u);
+            };
             uint8_t* dst = out + row_index(a, slot, u.head) * (a.dim * BITS / 8) + u.chunk * BITS;
-            if constexpr (BITS == 8) *reinterpret_cast<u2*>(dst) = u2{words[0], words[1]};
-            else *reinterpret_cast<uint32_t*>(dst) = words[0];
+            if constexpr (BITS == 8) *reinterpret_cast<u2*>(dst) = u2{bytes(q[0], q[1], q[2], q[3]), bytes(q[4], q[5], q[6], q[7])};
+            else *reinterpret_cast<uint32_t*>(dst) = bytes(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4);
             if ((u.chunk & ((1 << a.group_shift) - 1)) == 0)
                 (u.value ? a.value_meta : a.key_meta)[pair_index(a, slot, u.head, u.chunk >> a.group_shift)] =
-                    sb | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)z) << 16;
+                    (bad ? 0x7E00u : sb) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)z) << 16;
         }
     }
 }
@@ -108,7 +126,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
 template <int DT, int BITS>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= (uint32_t)a.T * (uint32_t)a.units) return;
+    if (i >= (uint32_t)a.T * a.units.d) return;
     const Unit u = unit_of(a, i);
     const int64_t slot = a.slots[u.token];
     const uint8_t* in = u.value ? a.values : a.keys;
@@ -119,16 +137,26 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
         } else {
             const uint8_t* src = in + row_index(a, slot, u.head) * (a.dim * BITS / 8) + u.chunk * BITS;
             const uint32_t pair = (u.value ? a.value_meta : a.key_meta)[pair_index(a, slot, u.head, u.chunk >> a.group_shift)];
-            const float s = f16_bits(pair), z = f16_bits(pair >> 16);
             uint32_t words[BITS / 4];
             if constexpr (BITS == 8) { const u2 t = *reinterpret_cast<const u2*>(src); words[0] = t[0]; words[1] = t[1]; }
             else words[0] = *reinterpret_cast<const uint32_t*>(src);
+            h2 v[4];                                             // q - z, exact
+            GroupConstNat<BITS> g;
+            g.set(as_h2(pair)[0], as_h2(pair)[1]);
+            if constexpr (BITS == 8) {
+                dequant_word8_nat<false>(words[0], g, v);
+                dequant_word8_nat<false>(words[1], g, v + 2);
+            } else {
+                dequant_word4_nat<false>(words[0], g, v);
+            }
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float q = (float)((words[j * BITS / 32] >> (j * BITS % 32)) & ((1u << BITS) - 1));
-                float x = s * (q - z);                                       // exact in float32: 11 bits times 9
-                if (DT == BW_F16 && __builtin_fabsf(x) > 65504.f) x = __builtin_copysignf(65504.f, x);
-                w[j / 2] |= (uint32_t)narrow16<DT>(x) << (16 * (j & 1));
+            for (int j = 0; j < 4; j++) {
+                if constexpr (DT == BW_F16) {                    // one rounding; beyond the largest number: that number; a NaN scale: NaN
+                    const h2 most = splat((_Float16)65504.f);
+                    w[j] = as_u32(__builtin_elementwise_max(__builtin_elementwise_min(v[j] * g.s, most), -most) + (g.s - g.s));
+                } else {
+                    w[j] = narrow_pair<DT>((float)v[j][0] * (float)g.s[0], (float)v[j][1] * (float)g.s[0]);
+                }
             }
         }
     }
@@ -137,7 +165,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
 }
 
 CacheArgs args_of(const bw_cache* c) {
-    CacheArgs a = {};
+    CacheArgs a{};
     a.keys = (uint8_t*)c->keys;
     a.values = (uint8_t*)c->values;
     a.key_meta = (uint32_t*)c->key_meta;
@@ -145,8 +173,8 @@ CacheArgs args_of(const bw_cache* c) {
     a.rows = c->pages * c->page_size;
     a.heads = c->kv_heads;
     a.dim = c->dim;
-    a.chunks = c->dim / 8;
-    a.units = 2 * c->kv_heads * a.chunks;
+    a.chunks = FastDiv(c->dim / 8);
+    a.units = FastDiv(2 * c->kv_heads * (c->dim / 8));
     a.page_shift = bw_log2(c->page_size);
     if (c->bits != 16) {
         a.groups = c->dim / c->group;
@@ -158,14 +186,14 @@ CacheArgs args_of(const bw_cache* c) {
 // Runs `launch(args, blocks)` over the tokens, in several launches where a thread's number would pass 31 bits.
 template <class F>
 int over_tokens(CacheArgs a, int64_t T, F&& launch) {
-    const int64_t most = ((int64_t)1 << 31) / a.units - 1;
+    const int64_t most = ((int64_t)1 << 31) / a.units.d - 1;
     for (int64_t at = 0; at < T; at += most) {
         CacheArgs b = a;
         b.T = (int)(T - at < most ? T - at : most);
         b.slots += at;
         if (b.k) { b.k += at * a.k_row; b.v += at * a.v_row; }
         if (b.k_out) { b.k_out += at * a.heads * a.dim; b.v_out += at * a.heads * a.dim; }
-        launch(b, dim3((unsigned)(((int64_t)b.T * a.units + 255) / 256)));
+        launch(b, dim3((unsigned)(((int64_t)b.T * a.units.d + 255) / 256)));
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;
