@@ -1,8 +1,8 @@
 // Writing tokens into the paged key-value cache, quantised as they are written, and reading them back.
 //
-// A thread owns 8 consecutive values of one token's key or value head: 16 bytes of 16-bit input, and 16, 8 or 4 bytes of the cache.
-// The group / 8 neighbouring threads of a group agree on its extrema with cross-lane shuffles (group / 8 divides 64 and every row starts at
-// a multiple of it, so a group never leaves its wave), and the first of them stores the group's pair.
+// A thread owns 8 or 16 consecutive values of one token's key or value head.  The 2 ... 8 neighbouring threads of a group agree on its extrema with
+// cross-lane moves (their number divides 64 and every row starts at a multiple of it, so a group never leaves its wave), and the first of
+// them stores the group's pair.
 //
 // The code of x is rint(x / s) of the exact quotient: with r = 1 / s to within a unit of its last place, t = x r and one step t + (x - t s) r the
 // result is the correctly rounded quotient wherever rint could tell a difference - x has at most 11 significant bits and s 11, so a
@@ -29,8 +29,8 @@ struct CacheArgs {
     uint16_t *k_out, *v_out;
     int64_t rows;                                // pages * page_size
     int T, heads, groups, dim;
-    FastDiv units, chunks;                       // threads of a token (2 * heads * chunks); dim / 8
-    int page_shift, group_shift;                 // group / 8 = 1 << group_shift
+    FastDiv units, chunks;                       // threads of a token (2 * heads * chunks) and of a head
+    int page_shift, group_shift;                 // 1 << group_shift threads for a group
 };
 
 // Row `row` of page `page` of a head: in rows, and in pairs of group g.
@@ -60,32 +60,50 @@ typedef short s2 __attribute__((ext_vector_type(2)));
 BW_DEV uint32_t max16(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s2, a), __builtin_bit_cast(s2, b))); }
 template <int CTRL> BW_DEV uint32_t max16_over(uint32_t v) { return max16(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false)); }
 
+// Workgroups go to the eight dies in turn: here each die gets kRun neighbouring ones of every 8 kRun, so that the pairs of neighbouring tokens,
+// which share lines, are put together in one die's cache.
+constexpr uint32_t kRun = 32;
+BW_DEV uint32_t block_of(uint32_t b, uint32_t n) {
+    const uint32_t at = b & (8 * kRun - 1), base = b - at;
+    return base + 8 * kRun <= n ? base + (at & 7) * kRun + (at >> 3) : b;
+}
+
+// Values of a thread: for codes 16, so that the two thirds of the work that are a group's and an address's are shared by more of them (with 8: 49 us
+// for the case below, 380 operations for 16 values against 230).
+template <int BITS> constexpr int kWriteValues = BITS == 16 ? 8 : 16;
+
 template <int DT, int BITS>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    constexpr int V = kWriteValues<BITS>;
+    const uint32_t i = block_of(blockIdx.x, gridDim.x) * 256u + threadIdx.x;
     const bool live = i < (uint32_t)a.T * a.units.d;
     const Unit u = unit_of(a, live ? i : 0);
     const int64_t slot = a.slots[u.token];
     const bool kept = live && slot >= 0 && slot < a.rows;
-    const uint16_t* src = u.value ? a.v + u.token * a.v_row + u.head * a.v_head : a.k + u.token * a.k_row + u.head * a.k_head;
-    const u4 w = *reinterpret_cast<const u4*>(src + u.chunk * 8);
+    const uint16_t* src = (u.value ? a.v + u.token * a.v_row + u.head * a.v_head : a.k + u.token * a.k_row + u.head * a.k_head) + u.chunk * V;
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int n = 0; n < V / 8; n++) {
+        const u4 t = reinterpret_cast<const u4*>(src)[n];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[4 * n + j] = t[j];
+    }
     uint8_t* out = u.value ? a.values : a.keys;
     if constexpr (BITS == 16) {
-        if (kept) *reinterpret_cast<u4*>(out + (row_index(a, slot, u.head) * a.dim + u.chunk * 8) * 2) = w;
+        if (kept) *reinterpret_cast<u4*>(out + (row_index(a, slot, u.head) * a.dim + u.chunk * 8) * 2) = u4{w[0], w[1], w[2], w[3]};
     } else {
         constexpr float top = (float)((1 << BITS) - 1), inv_top = 1.f / top;
         uint32_t hi = 0, lo = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < V / 2; j++) {
             hi = max16(hi, w[j]);
             lo = max16(lo, w[j] ^ 0x80008000u);
         }
         // low half: the largest value, high half: the size of the most negative one
         uint32_t both = max16(__builtin_amdgcn_perm(lo, hi, 0x05040100u), __builtin_amdgcn_perm(lo, hi, 0x07060302u));
         both = max16_over<0xB1>(both);                          // quad_perm: the neighbour
-        both = max16_over<0x4E>(both);                          // ... and the other two of four
+        if (a.group_shift > 1) both = max16_over<0x4E>(both);   // ... and the other two of four
         if (a.group_shift > 2) both = max16_over<0x141>(both);  // row_half_mirror: the other four of eight
-        if (a.group_shift > 3) both = max16_over<0x140>(both);  // row_mirror: the other eight of sixteen
         constexpr uint32_t inf = DT == BW_F16 ? 0x7C00u : 0x7F80u;
         const bool bad = (both & 0xFFFFu) >= inf || (both >> 16) >= inf;
         const float largest = widen16<DT>((uint16_t)both), smallest = -widen16<DT>((uint16_t)(both >> 16));
@@ -103,19 +121,23 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
             return __builtin_fmaf(__builtin_fmaf(-t, s, v), r, t) + kWhole;
         };
         const float z = fminf(whole(-smallest) - kWhole, top);
-        uint32_t q[8];
+        uint32_t q[V];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < V; j++) {
             const float x = whole(widen16<DT>((uint16_t)(w[j / 2] >> (16 * (j & 1))))) + z;
-            q[j] = __builtin_bit_cast(uint32_t, fminf(fmaxf(x, kWhole), kWhole + top));        // (a NaN: 0)
+            q[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_fmed3f(x, kWhole, kWhole + top));   // (a group with a NaN is marked by its scale)
         }
         if (kept) {
             auto bytes = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
                 return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0C0C0400u), __builtin_amdgcn_perm(b1, b0, 0x0C0C0400u), 0x05040100u);
             };
-            uint8_t* dst = out + row_index(a, slot, u.head) * (a.dim * BITS / 8) + u.chunk * BITS;
-            if constexpr (BITS == 8) *reinterpret_cast<u2*>(dst) = u2{bytes(q[0], q[1], q[2], q[3]), bytes(q[4], q[5], q[6], q[7])};
-            else *reinterpret_cast<uint32_t*>(dst) = bytes(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4);
+            uint8_t* dst = out + row_index(a, slot, u.head) * (a.dim * BITS / 8) + u.chunk * (V * BITS / 8);
+            if constexpr (BITS == 8) {
+                *reinterpret_cast<u4*>(dst) = u4{bytes(q[0], q[1], q[2], q[3]), bytes(q[4], q[5], q[6], q[7]), bytes(q[8], q[9], q[10], q[11]), bytes(q[12], q[13], q[14], q[15])};
+            } else {
+                *reinterpret_cast<u2*>(dst) = u2{bytes(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4),
+                                                 bytes(q[8] | q[9] << 4, q[10] | q[11] << 4, q[12] | q[13] << 4, q[14] | q[15] << 4)};
+            }
             if ((u.chunk & ((1 << a.group_shift) - 1)) == 0)
                 (u.value ? a.value_meta : a.key_meta)[pair_index(a, slot, u.head, u.chunk >> a.group_shift)] =
                     (bad ? 0x7E00u : sb) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)z) << 16;
@@ -124,11 +146,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
 }
 
 template <int DT, int BITS>
-__global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= (uint32_t)a.T * a.units.d) return;
-    const Unit u = unit_of(a, i);
-    const int64_t slot = a.slots[u.token];
+BW_DEV u4 read_unit(const CacheArgs& a, const Unit& u, int64_t slot) {
     const uint8_t* in = u.value ? a.values : a.keys;
     u4 w = {0, 0, 0, 0};
     if (slot >= 0 && slot < a.rows) {
@@ -160,11 +178,32 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
             }
         }
     }
-    uint16_t* out = (u.value ? a.v_out : a.k_out) + ((int64_t)u.token * a.heads + u.head) * a.dim + u.chunk * 8;
-    *reinterpret_cast<u4*>(out) = w;
+    return w;
 }
 
-CacheArgs args_of(const bw_cache* c) {
+// UN chunks of a thread, 256 chunks apart, all under way at a time.
+template <int DT, int BITS, int UN>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
+    const uint32_t first = block_of(blockIdx.x, gridDim.x) * (256u * UN) + threadIdx.x, all = (uint32_t)a.T * a.units.d;
+    Unit u[UN];
+    int64_t slot[UN];
+    u4 w[UN];
+#pragma unroll
+    for (int n = 0; n < UN; n++) {
+        const uint32_t i = first + 256 * n;
+        u[n] = unit_of(a, i < all ? i : 0);
+        slot[n] = a.slots[u[n].token];
+    }
+#pragma unroll
+    for (int n = 0; n < UN; n++) w[n] = read_unit<DT, BITS>(a, u[n], slot[n]);
+#pragma unroll
+    for (int n = 0; n < UN; n++) {
+        uint16_t* out = (u[n].value ? a.v_out : a.k_out) + ((int64_t)u[n].token * a.heads + u[n].head) * a.dim + u[n].chunk * 8;
+        if (first + 256 * n < all) *reinterpret_cast<u4*>(out) = w[n];
+    }
+}
+
+CacheArgs args_of(const bw_cache* c, int values) {
     CacheArgs a{};
     a.keys = (uint8_t*)c->keys;
     a.values = (uint8_t*)c->values;
@@ -173,17 +212,21 @@ CacheArgs args_of(const bw_cache* c) {
     a.rows = c->pages * c->page_size;
     a.heads = c->kv_heads;
     a.dim = c->dim;
-    a.chunks = FastDiv(c->dim / 8);
-    a.units = FastDiv(2 * c->kv_heads * (c->dim / 8));
+    a.chunks = FastDiv(c->dim / values);
+    a.units = FastDiv(2 * c->kv_heads * (c->dim / values));
     a.page_shift = bw_log2(c->page_size);
     if (c->bits != 16) {
         a.groups = c->dim / c->group;
-        a.group_shift = bw_log2(c->group / 8);
+        a.group_shift = bw_log2(c->group / values);
     }
     return a;
 }
 
-// Runs `launch(args, blocks)` over the tokens, in several launches where a thread's number would pass 31 bits.
+// Chunks from which on a thread of the read-back takes kAhead of them (36 -> 33 us for the case above; four: no further).
+constexpr int kAhead = 2;
+constexpr int64_t kManyChunks = (int64_t)kAhead * 256 * 2048;
+
+// Runs `launch(args, chunks)` over the tokens, in several launches where a thread's number would pass 31 bits.
 template <class F>
 int over_tokens(CacheArgs a, int64_t T, F&& launch) {
     const int64_t most = ((int64_t)1 << 31) / a.units.d - 1;
@@ -193,19 +236,27 @@ int over_tokens(CacheArgs a, int64_t T, F&& launch) {
         b.slots += at;
         if (b.k) { b.k += at * a.k_row; b.v += at * a.v_row; }
         if (b.k_out) { b.k_out += at * a.heads * a.dim; b.v_out += at * a.heads * a.dim; }
-        launch(b, dim3((unsigned)(((int64_t)b.T * a.units.d + 255) / 256)));
+        launch(b, (int64_t)b.T * a.units.d);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;
 }
 
+template <int DT, int BITS> void launch_write(const CacheArgs& a, int64_t chunks, hipStream_t stream) {
+    hipLaunchKernelGGL((cache_write_kernel<DT, BITS>), dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, stream, a);
+}
+template <int DT, int BITS> void launch_read(const CacheArgs& a, int64_t chunks, hipStream_t stream) {
+    if (chunks < kManyChunks) hipLaunchKernelGGL((cache_read_kernel<DT, BITS, 1>), dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((cache_read_kernel<DT, BITS, kAhead>), dim3((unsigned)((chunks + 256 * kAhead - 1) / (256 * kAhead))), dim3(256), 0, stream, a);
+}
+
 }  // namespace
 
-#define BW_BY_FORMAT(KERNEL, DT)                                                                                          \
-    over_tokens(a, T, [&](const CacheArgs& b, dim3 grid) {                                                                \
-        if (c->bits == 16) hipLaunchKernelGGL((KERNEL<DT, 16>), grid, dim3(256), 0, (hipStream_t)stream, b);              \
-        else if (c->bits == 8) hipLaunchKernelGGL((KERNEL<DT, 8>), grid, dim3(256), 0, (hipStream_t)stream, b);           \
-        else hipLaunchKernelGGL((KERNEL<DT, 4>), grid, dim3(256), 0, (hipStream_t)stream, b);                             \
+#define BW_BY_FORMAT(LAUNCH, DT)                                       \
+    over_tokens(a, T, [&](const CacheArgs& b, int64_t chunks) {        \
+        if (c->bits == 16) LAUNCH<DT, 16>(b, chunks, (hipStream_t)stream);     \
+        else if (c->bits == 8) LAUNCH<DT, 8>(b, chunks, (hipStream_t)stream);  \
+        else LAUNCH<DT, 4>(b, chunks, (hipStream_t)stream);            \
     })
 
 extern "C" int bw_cache_write(const bw_cache* c, int act_dtype, int64_t T, const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -215,11 +266,11 @@ extern "C" int bw_cache_write(const bw_cache* c, int act_dtype, int64_t T, const
     if ((act_dtype != BW_F16 && act_dtype != BW_BF16) || (c->bits == 16 && act_dtype != c->dtype)) return BW_EUNSUPPORTED;
     if (T == 0) return BW_OK;
     if (!bw_aligned(k, 16) || !bw_aligned(v, 16) || !bw_aligned(slots, 8) || (k_row | k_head | v_row | v_head) % 8) return BW_EALIGN;
-    CacheArgs a = args_of(c);
+    CacheArgs a = args_of(c, c->bits == 16 ? kWriteValues<16> : kWriteValues<8>);
     a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
     a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
     a.slots = slots;
-    return act_dtype == BW_F16 ? BW_BY_FORMAT(cache_write_kernel, BW_F16) : BW_BY_FORMAT(cache_write_kernel, BW_BF16);
+    return act_dtype == BW_F16 ? BW_BY_FORMAT(launch_write, BW_F16) : BW_BY_FORMAT(launch_write, BW_BF16);
 }
 
 extern "C" int bw_cache_read(const bw_cache* c, int out_dtype, int64_t T, const int64_t* slots, void* k_out, void* v_out, void* stream) {
@@ -228,8 +279,8 @@ extern "C" int bw_cache_read(const bw_cache* c, int out_dtype, int64_t T, const 
     if ((out_dtype != BW_F16 && out_dtype != BW_BF16) || (c->bits == 16 && out_dtype != c->dtype)) return BW_EUNSUPPORTED;
     if (T == 0) return BW_OK;
     if (!bw_aligned(k_out, 16) || !bw_aligned(v_out, 16) || !bw_aligned(slots, 8)) return BW_EALIGN;
-    CacheArgs a = args_of(c);
+    CacheArgs a = args_of(c, 8);
     a.slots = slots;
     a.k_out = (uint16_t*)k_out; a.v_out = (uint16_t*)v_out;
-    return out_dtype == BW_F16 ? BW_BY_FORMAT(cache_read_kernel, BW_F16) : BW_BY_FORMAT(cache_read_kernel, BW_BF16);
+    return out_dtype == BW_F16 ? BW_BY_FORMAT(launch_read, BW_F16) : BW_BY_FORMAT(launch_read, BW_BF16);
 }
