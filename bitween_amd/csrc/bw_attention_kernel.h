@@ -18,9 +18,13 @@
 // Fewer than 16 queries leave columns of the MFMAs empty: the matrix cores have room (16 KB of a 16-bit tile take 32 MFMAs, some 500 cycles
 // of one SIMD, and about 8000 cycles of a SIMD's share of HBM).
 //
-// Codes enter as exact integers in float16, and the scales are applied in float32:
-//   K: S = s (Q . (q - mid) + (mid - z) sum Q) for each group, mid = 2^(bits-1): a lane's codes are one token's, its products four others'
-//   V: O += (P s) (q - z): a pair of codes is two tokens', whose scales and zero points the lane has anyway
+// Codes enter the MFMAs as they are: a whole number in the low bits of a 16-bit float is that number times 2^-24, a subnormal, which the matrix cores
+// take, so that unpacking is a byte permute or a shift and an AND for two codes.  They line products up as if a subnormal were 2^-14 and cut them
+// 24 bits below the largest: 2^-16 of a code's unit (measured: sums of 32 within 5e-4 units of the largest factor), nothing beside 255
+// units, but too much beside 15, so 4-bit codes go in four bits higher, where it is 2^-20.
+// Scales and zero points are applied in float32:
+//   K: S = s (Q . c - z sum Q) for each group
+//   V: O += (P s) c, and another MFMA whose rows are the zero points sums (P s) z, which is taken off at the end
 // so no value is rounded on its way in.  P s can be anything from 2^-24 to 2^16 times P: r then follows score + log2 of the token's scale
 // (a power of two 2^e), P is held relative to that and l adds P 2^-e.  P goes in as two 16-bit numbers whose sum it is (to 2^-16 and better):
 // one alone would err as much as the result's own rounding.
@@ -143,6 +147,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 // against zeros of Q, and into outputs that nobody stores.
 template <int DT, int DP> struct Format16 {
     static constexpr bool kCodes = false, kBf16 = DT == BW_BF16;
+    static constexpr int kBits = 16, kPerV = DP / 16;
     static constexpr int kDim = DP, NK = DP / 32, NV = DP / 16, kGroups = 1, kKeyWords = NK * 4, kValueWords = NV / 2;
     static BW_DEV int k_at(int block, int kg) { return 32 * block + 8 * kg; }
     // 64: 4 neighbouring values (8 bytes) of a lane; 128: 8 (16 bytes); 256: 8 of each half
@@ -181,29 +186,30 @@ template <bool BF16> BW_DEV uint32_t split_pair(float& x, float& y) {
     return p;
 }
 
-// Codes of one word (8 bits: 4, 4 bits: 8) as float16 q - mid, in the order that Q is laid out in (query_order).
+// Codes of one word as operand pairs, in units of 2^-kUnit.  8 bits: (0, 1) (2, 3); 4 bits: (0, 4) (1, 5) (2, 6) (3, 7), the order of Q too.
+template <int BITS> constexpr int kUnit = BITS == 8 ? 24 : 20;
 template <int BITS> BW_DEV void key_codes(uint32_t w, uint32_t* out) {
     if constexpr (BITS == 8) {
-        const h2 mid = splat((_Float16)-1152.f);
-        out[0] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + mid);
-        out[1] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + mid);
+        out[0] = __builtin_amdgcn_perm(0u, w, 0x0C010C00u);
+        out[1] = __builtin_amdgcn_perm(0u, w, 0x0C030C02u);
     } else {
-        const h2 mid = splat((_Float16)-1032.f), mid16 = splat((_Float16)-72.f), k16 = splat((_Float16)0.0625f);
-        const uint32_t w8 = w >> 8;
-        out[0] = as_u32(as_h2(and_or(w, 0x000F000Fu, kMagic)) + mid);
-        out[1] = as_u32(__builtin_elementwise_fma(as_h2(and_or(w, 0x00F000F0u, kMagic)), k16, mid16));
-        out[2] = as_u32(as_h2(and_or(w8, 0x000F000Fu, kMagic)) + mid);
-        out[3] = as_u32(__builtin_elementwise_fma(as_h2(and_or(w8, 0x00F000F0u, kMagic)), k16, mid16));
+        out[0] = w << 4 & 0x00F000F0u;
+        out[1] = w & 0x00F000F0u;
+        out[2] = w >> 4 & 0x00F000F0u;
+        out[3] = w >> 8 & 0x00F000F0u;
     }
 }
 template <int BITS> BW_DEV int query_order(int e) { return BITS == 4 ? (e >> 1) + 4 * (e & 1) : e; }
 
-// Codes j of two tokens as a float16 pair of q - z: `a` holds 16 bits of each (token_pair), zz and zz16 are -(1024 + z) and -(64 + z) of both.
+// 16 bits of each of two tokens' words, and code J of both as an operand pair.
 template <bool HIGH> BW_DEV uint32_t token_pair(uint32_t second, uint32_t first) { return __builtin_amdgcn_perm(second, first, HIGH ? 0x07060302u : 0x05040100u); }
-template <int BITS, int J> BW_DEV uint32_t value_codes(uint32_t a, h2 zz, h2 zz16) {
-    if constexpr (BITS == 8) return as_u32(as_h2(and_or(J ? a >> 8 : a, 0x00FF00FFu, kMagic)) + zz);
-    else if constexpr (J % 2 == 0) return as_u32(as_h2(and_or(J ? a >> 8 : a, 0x000F000Fu, kMagic)) + zz);
-    else return as_u32(__builtin_elementwise_fma(as_h2(and_or(J > 1 ? a >> 8 : a, 0x00F000F0u, kMagic)), splat((_Float16)0.0625f), zz16));
+template <int BITS, int J> BW_DEV uint32_t value_codes(uint32_t second, uint32_t first) {
+    if constexpr (BITS == 8) {
+        return __builtin_amdgcn_perm(second, first, 0x0C040C00u + 0x00010001u * (J % 4));
+    } else {
+        const uint32_t a = token_pair<(J / 4) % 2 != 0>(second, first);
+        return (J % 4 == 0 ? a << 4 : a >> 4 * (J % 4 - 1)) & 0x00F000F0u;
+    }
 }
 
 // One tile's rows and pairs as they come from memory.
@@ -288,7 +294,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
         const int32_t* table = a.table + (int64_t)b * a.table_row;
         const int page_mask = (1 << a.page_shift) - 1;
 
-        // ---- Q: operand blocks, and for codes the sum of every group and a power of two that brings bfloat16 into float16 ----
+        // ---- Q: operand blocks; over codes brought near 2^14 by a power of two, with the sum of every group in the codes' unit ----
         u4 q[F::NK];
         float q_sum[F::kGroups], score_scale = a.scale;
         {
@@ -308,31 +314,27 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                         x[k][e] = a.q_bf16 ? bf16_to_f32(u) : f16_bits(u);
                         top = fmaxf(top, __builtin_fabsf(x[k][e]));
                     }
-                if (a.q_bf16) {                                   // exact but for values 2^38 and more below the largest
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const int e = top > 0.f && top <= 3.4e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
-                    score_scale = __builtin_ldexpf(a.scale, e);
-#pragma unroll
-                    for (int k = 0; k < F::NK; k++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[k][i] = __builtin_ldexpf(x[k][i], -e);
-                }
+                // exact but for values 2^28 and more below the largest
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const int ex = top > 0.f && top <= 3.4e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+                score_scale = __builtin_ldexpf(a.scale, ex + kUnit<F::kBits>);
 #pragma unroll
                 for (int g = 0; g < F::kGroups; g++) {
-                    float s = 0.f;
+                    float sum = 0.f;
 #pragma unroll
                     for (int k = g * F::kPerK; k < (g + 1) * F::kPerK; k++) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) s += x[k][e];
-#pragma unroll
-                        for (int p = 0; p < 4; p++) {
-                            const h2 v = {(_Float16)x[k][query_order<F::kBits>(2 * p)], (_Float16)x[k][query_order<F::kBits>(2 * p + 1)]};
-                            q[k][p] = as_u32(v);
+                        for (int e = 0; e < 8; e++) {
+                            x[k][e] = __builtin_ldexpf(x[k][e], -ex);
+                            sum += x[k][e];
                         }
+#pragma unroll
+                        for (int p = 0; p < 4; p++)
+                            q[k][p] = as_u32(h2{(_Float16)x[k][query_order<F::kBits>(2 * p)], (_Float16)x[k][query_order<F::kBits>(2 * p + 1)]});
                     }
-                    s += __shfl_xor(s, 16, 64);
-                    q_sum[g] = s + __shfl_xor(s, 32, 64);
+                    sum += __shfl_xor(sum, 16, 64);
+                    q_sum[g] = __builtin_ldexpf(sum + __shfl_xor(sum, 32, 64), -kUnit<F::kBits>);
                 }
             }
         }
@@ -410,10 +412,12 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
         };
 
         // ---- tiles ----
-        f4 acc[F::NV];
+        f4 acc[F::NV], zeros[F::kGroups];                         // zeros: sums of (P s) z, the same in every row
         float r = -INFINITY, l = 0.f;
 #pragma unroll
         for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < F::kGroups; g++) zeros[g] = f4{0.f, 0.f, 0.f, 0.f};
         uint32_t t = from + wave;
         Halves h = {}, hn = {};
         if (t < to) {
@@ -427,9 +431,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
             if (more) hn = halves_of(next);
             // Tokens that do not count: behind the end, or on a page outside the cache.
             const bool full = (int)t * kTile + kTile <= n && h.page[0] < a.pages && h.page[1] < a.pages;
-            bool seen[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) seen[e] = (int)t * kTile + 16 * (e >> 2) + 4 * kg + (e & 3) < n && h.page[e >> 2] < a.pages;
+            auto seen = [&](int e) { return (int)t * kTile + 16 * (e >> 2) + 4 * kg + (e & 3) < n && h.page[e >> 2] < a.pages; };
             // scores, in units of log 2
             float x[8];
 #pragma unroll
@@ -448,8 +450,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const uint32_t pair = keys.meta[half][g][i];
-                            const float sc = f16_bits(pair), off = (float)(1 << (F::kBits - 1)) - f16_bits(pair >> 16);
-                            s[i] = __builtin_fmaf(sc, __builtin_fmaf(off, q_sum[g], dot[i]), s[i]);
+                            const float part = __builtin_fmaf(-f16_bits(pair >> 16), q_sum[g], dot[i]);
+                            s[i] = g ? __builtin_fmaf(f16_bits(pair), part, s[i]) : f16_bits(pair) * part;
                         }
                     }
                 } else {
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[4 * half + i] = s[i] * score_scale;
+                for (int i = 0; i < 4; i++) x[4 * half + i] = F::kCodes ? s[i] : s[i] * score_scale;
             }
             if (more) load_keys(hn, next);
             // reference: for codes the scores are raised by the exponent of the token's largest value scale
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 #pragma unroll
                     for (int e = 0; e < 8; e++)
 #pragma unroll
-                        for (int g = 0; g < F::kGroups; g++) values.meta[e >> 2][g][e & 3] = seen[e] ? values.meta[e >> 2][g][e & 3] : 0u;
+                        for (int g = 0; g < F::kGroups; g++) values.meta[e >> 2][g][e & 3] = seen(e) ? values.meta[e >> 2][g][e & 3] : 0u;
                 }
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -478,13 +480,13 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 #pragma unroll
                     for (int g = 1; g < F::kGroups; g++) top = fmaxf(top, f16_bits(values.meta[e >> 2][g][e & 3]));
                     const int ex = __builtin_amdgcn_frexp_expf(top);
-                    x[e] += (float)ex;
+                    x[e] = __builtin_fmaf(x[e], score_scale, (float)ex);
                     unit[e] = __builtin_ldexpf(1.f, -ex);
                 }
             }
             if (!full) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = seen[e] ? x[e] : -INFINITY;
+                for (int e = 0; e < 8; e++) x[e] = seen(e) ? x[e] : -INFINITY;
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             if (__builtin_amdgcn_ballot_w64(top > r + kSlack)) {
@@ -495,13 +497,17 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                 l *= keep;
 #pragma unroll
                 for (int j = 0; j < F::NV; j++) acc[j] *= keep;
+                if constexpr (F::kCodes) {
+#pragma unroll
+                    for (int g = 0; g < F::kGroups; g++) zeros[g] *= keep;
+                }
             }
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e] - r);
             if (!full) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = seen[e] ? p[e] : 0.f;
+                for (int e = 0; e < 8; e++) p[e] = seen(e) ? p[e] : 0.f;
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -514,35 +520,32 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                     float pg[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) pg[e] = p[e] * (f16_bits(values.meta[e >> 2][g][e & 3]) * unit[e]);
-                    u4 hi, lo;
-                    h2 zz[4], zz16[4];
+                    u4 hi, lo, z;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const h2 z = as_h2(token_pair<true>(values.meta[i >> 1][g][2 * (i & 1) + 1], values.meta[i >> 1][g][2 * (i & 1)]));
-                        zz[i] = splat((_Float16)-1024.f) - z;
-                        zz16[i] = splat((_Float16)-64.f) - z;
+                        z[i] = token_pair<true>(values.meta[i >> 1][g][2 * (i & 1) + 1], values.meta[i >> 1][g][2 * (i & 1)]);
                         hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
                         lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
                     }
+                    u4 v[F::kPerV];
                     static_for<0, F::kPerV>([&](auto jc) {
-                        constexpr int j = decltype(jc)::value, per = 16 / F::kBits;       // codes in 16 bits of a token
-                        u4 v;
+                        constexpr int j = decltype(jc)::value, w = j * F::kBits / 32;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            constexpr int w = j / (2 * per);
-                            const uint32_t pair = token_pair<(j / per) & 1>(values.raw[2 * i + 1][g * F::kValueGroupWords + w], values.raw[2 * i][g * F::kValueGroupWords + w]);
-                            v[i] = value_codes<F::kBits, j % per>(pair, zz[i], zz16[i]);
-                        }
-                        acc[g * F::kPerV + j] = mfma<false>(v, hi, acc[g * F::kPerV + j]);
-                        acc[g * F::kPerV + j] = mfma<false>(v, lo, acc[g * F::kPerV + j]);
+                        for (int i = 0; i < 4; i++)
+                            v[j][i] = value_codes<F::kBits, j % (32 / F::kBits)>(values.raw[2 * i + 1][g * F::kValueGroupWords + w], values.raw[2 * i][g * F::kValueGroupWords + w]);
+                        acc[g * F::kPerV + j] = mfma<false>(v[j], hi, acc[g * F::kPerV + j]);
                     });
+                    zeros[g] = mfma<false>(z, hi, zeros[g]);
+#pragma unroll
+                    for (int j = 0; j < F::kPerV; j++) acc[g * F::kPerV + j] = mfma<false>(v[j], lo, acc[g * F::kPerV + j]);
+                    zeros[g] = mfma<false>(z, lo, zeros[g]);
                 }
             } else {
                 if (!full) {
 #pragma unroll
                     for (int e = 0; e < 8; e++)
 #pragma unroll
-                        for (int w = 0; w < F::kValueWords; w++) values.raw[e][w] = seen[e] ? values.raw[e][w] : 0u;
+                        for (int w = 0; w < F::kValueWords; w++) values.raw[e][w] = seen(e) ? values.raw[e][w] : 0u;
                 }
                 u4 hi, lo;
 #pragma unroll
@@ -600,7 +603,11 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 #pragma unroll
                 for (int j = c * kChunkBlocks; j < (c + 1) * kChunkBlocks && j < F::NV; j++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) outs[wave][m][F::v_at(4 * kg + i, j) - c * kChunk] = acc[j][i] * f;
+                    for (int i = 0; i < 4; i++) {
+                        float o = acc[j][i];
+                        if constexpr (F::kCodes) o = __builtin_fmaf(o, (float)(1 << kUnit<F::kBits>), -zeros[j / F::kPerV][i]);
+                        outs[wave][m][F::v_at(4 * kg + i, j) - c * kChunk] = o * f;
+                    }
             }
             __syncthreads();
             for (int e = (int)threadIdx.x; e < queries * (kChunk / 4); e += 256) {

@@ -104,7 +104,11 @@ class Batch:
     def check(self, out, scale=None, lengths=None):
         """out against 64 bits.  One rounding of the result; weights of the softmax held to 16 bits or better (2^-16 of their sum times the largest
         value); scores in float32: a sum of dim products, the scaling and the exponential's argument, together at most (dim + 16) 2^-24 of the sum of
-        the products' magnitudes, which changes a weight by that much relative to itself."""
+        the products' magnitudes, which changes a weight by that much relative to itself.  Over codes a value is the difference scale * code -
+        scale * zero point, and it is these two that the weights multiply: an error of 2^-20 of a weight (two float16 numbers, each cut to 11 bits) is
+        2^-20 of a group's whole range (2^bits - 1) scale, however near to each other code and zero point are, and sums of 32 products of codes
+        are cut by at most 32 * 2^-16 of a unit of 8 bits or 32 * 2^-20 of a unit of 4 bits, 2^-18.9 and 2^-18.9 of the range.  So the largest
+        value is the group's largest range there."""
         c = self.cache
         dim, kv = self.q.shape[2], c.keys.shape[1]
         share = self.q.shape[1] // kv
@@ -121,7 +125,12 @@ class Batch:
             weights = torch.softmax(scores, 1).transpose(1, 2).contiguous()
             want = torch.matmul(weights, v.contiguous()).reshape(-1, dim)
             reach = (torch.matmul(k.abs(), q.abs().transpose(1, 2).contiguous()) * abs(scale)).amax(1).reshape(-1, 1)      # of a query head
-            top = v.abs().amax(1).repeat_interleave(share, 0)
+            top = v.abs().amax(1)
+            if self.bits != 16:
+                at = self.slots[b][:n]
+                pairs = c.value_meta[at // c.page_size, :, :, at % c.page_size].double()
+                top = (pairs[..., 0].amax(0) * (2 ** self.bits - 1)).repeat_interleave(self.group, -1)
+            top = top.repeat_interleave(share, 0)
             bound = half_step(self.dtype) * want.abs() + (2.0 ** -16 + 2 * (dim + 16) * 2.0 ** -24 * reach) * top + 2.0 ** -25
             worst = ((got - want).abs() / bound).max().item()
             assert worst <= 1, f"sequence {b} of {n} tokens: {worst:.3f} times the bound"
