@@ -87,7 +87,7 @@ Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
     Plan p;
     p.whole = max_pages * c->page_size <= kWholeTokens && segments < (int64_t)1 << 31;
-    p.grid = p.whole ? (uint32_t)segments : (uint32_t)bw_device_cus() * 2;
+    p.grid = p.whole ? (uint32_t)segments : (uint32_t)bw_device_cus() * (c->dim > 128 ? 1 : 2);        // (kResident)
     return p;
 }
 

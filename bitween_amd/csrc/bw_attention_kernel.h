@@ -32,7 +32,7 @@
 #include "bw_cache.h"
 
 constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
-constexpr uint32_t kSegmentCost = 5;             // tiles
+constexpr uint32_t kSegmentCost = 8;             // tiles
 constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
 
 // A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
@@ -74,7 +74,7 @@ struct Split {
 };
 BW_DEV Split split_of(const AttentionArgs& a, uint32_t units, uint32_t grid) {
     const uint32_t total = units * (uint32_t)(a.kv_heads * a.q_groups), pieces = (total + a.min_units - 1) / (uint32_t)a.min_units;
-    Split s;
+    Split s = {};
     s.pieces = pieces < grid ? pieces : grid;
     s.size = s.pieces ? total / s.pieces : 0;
     s.longer = total - s.pieces * s.size;
@@ -212,15 +212,18 @@ template <int BITS, int J> BW_DEV uint32_t value_codes(uint32_t second, uint32_t
     }
 }
 
+// Where a tile's two halves lie: pages as the table names them.
+struct Halves { uint32_t page[2]; };
+
 // One tile's rows and pairs as they come from memory.
-template <class F> struct KeyTile {
-    uint32_t raw[2][F::kKeyWords];
-    u4 meta[2][F::kGroups];                      // of tokens 4 kg .. + 3 of each half
+template <class F> struct Tile {
+    Halves h;
+    uint32_t key[2][F::kKeyWords];
+    uint32_t value[8][F::kValueWords];           // token 4 kg + i of half h: 4 h + i
+    uint32_t pairs[F::kGroups];                  // of a group, in lane m of 16: keys' (m < 8) or values' token 4 kg + m % 4 of half m / 4 % 2
 };
-template <class F> struct ValueTile {
-    uint32_t raw[8][F::kValueWords];             // token 4 kg + i of half h: 4 h + i
-    u4 meta[2][F::kGroups];
-};
+// What lane L of the 16 has.
+template <int L> BW_DEV uint32_t row_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + L, 0xF, 0xF, true); }
 
 template <int WORDS> BW_DEV void load_words(const uint8_t* p, uint32_t* out) {
     if constexpr (WORDS % 4 == 0) {
@@ -240,11 +243,35 @@ template <int WORDS> BW_DEV void load_words(const uint8_t* p, uint32_t* out) {
     }
 }
 
-// Where a tile's two halves lie: pages as the table names them, and whether a half has tokens at all.
-struct Halves { uint32_t page[2]; };
+// Workgroups of a CU at a time: heads of more than 128 values fill the registers with one.
+template <class F> constexpr int kResident = F::kDim > 128 ? 1 : 2;
+
+// What a workgroup has of a segment: tiles from ... to - 1 of `tiles`.
+struct Segment {
+    uint32_t b, hq, from, to, tiles, units;      // units: of the piece that it takes
+    int n, head, q_head, queries;
+    const int32_t* table;
+};
+BW_DEV Segment segment_of(const AttentionArgs& a, uint32_t b, uint32_t hq, uint32_t at, uint32_t left) {
+    Segment g;
+    g.b = b;
+    g.hq = hq;
+    g.n = tokens_of(a, b);
+    g.tiles = tiles_of(g.n);
+    const uint32_t all = g.tiles + kSegmentCost, end = left < all - at ? at + left : all;
+    g.from = at > kSegmentCost ? at - kSegmentCost : 0;
+    g.to = end > kSegmentCost ? end - kSegmentCost : 0;
+    g.units = end - at;
+    g.head = (int)(hq / (uint32_t)a.q_groups);
+    const int first_query = (int)(hq - (uint32_t)g.head * a.q_groups) * kQueries;
+    g.queries = a.share - first_query < kQueries ? a.share - first_query : kQueries;
+    g.q_head = g.head * a.share + first_query;
+    g.table = a.table + (int64_t)b * a.table_row;
+    return g;
+}
 
 template <class F>
-__global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionArgs a) {
     constexpr int kChunk = F::kDim < 128 ? F::kDim : 128, kPitch = kChunk + 4, kChunkBlocks = kChunk / 16;
     __shared__ float outs[kWaves][kQueries][kPitch];
     __shared__ float stats[kWaves][2][kQueries];
@@ -254,7 +281,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 
     // the piece of this workgroup: from unit `at` of segment (b, hq) on, `left` units in all
     uint32_t b, hq, at, left;
-    Split s;
+    Split s = {};
     if (a.whole) {
         b = blockIdx.x / per_seq;
         hq = blockIdx.x - b * per_seq;
@@ -281,135 +308,156 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
         hq = rest / units;
         at = rest - hq * units;
     }
-    const uint32_t first_left = left;
-    do {
-        const int n = tokens_of(a, b);
-        const uint32_t tiles = tiles_of(n), units = tiles + kSegmentCost, end = left < units - at ? at + left : units;
-        const uint32_t from = at > kSegmentCost ? at - kSegmentCost : 0, to = end > kSegmentCost ? end - kSegmentCost : 0;
-        const uint32_t taken = end - at;
-        if (from < to || a.whole) {
-        const int head = (int)(hq / (uint32_t)a.q_groups), first_query = (int)(hq - (uint32_t)head * a.q_groups) * kQueries;
-        const int queries = a.share - first_query < kQueries ? a.share - first_query : kQueries;
-        const int q_head = head * a.share + first_query;
-        const int32_t* table = a.table + (int64_t)b * a.table_row;
-        const int page_mask = (1 << a.page_shift) - 1;
+    Segment g = segment_of(a, b, hq, at, left);
+    if (g.from >= g.to && !a.whole) return;
+    uint32_t position = s.start(blockIdx.x);                      // of the segment's units of this piece, among all (not of whole segments)
+    const int page_mask = (1 << a.page_shift) - 1;
 
-        // ---- Q: operand blocks; over codes brought near 2^14 by a power of two, with the sum of every group in the codes' unit ----
-        u4 q[F::NK];
-        float q_sum[F::kGroups], score_scale = a.scale;
-        {
-            const uint16_t* src = a.q + b * a.q_row + (q_head + (m < queries ? m : 0)) * a.q_head;
+    // ---- addresses ----
+    uint32_t key_off[F::kCodes ? F::kGroups : F::NK], value_off[F::kCodes ? F::kGroups : (F::kDim + 127) / 128];
+    if constexpr (F::kCodes) {
 #pragma unroll
-            for (int k = 0; k < F::NK; k++) {
-                const int d = F::k_at(k, kg);
-                q[k] = m < queries && d < a.dim ? *reinterpret_cast<const u4*>(src + d) : u4{0, 0, 0, 0};
-            }
+        for (int g = 0; g < F::kGroups; g++) {
+            key_off[g] = (uint32_t)(m * a.row_bytes + (g * F::kGroup + kg * (F::kGroup / 4)) * F::kBits / 8);
+            value_off[g] = (uint32_t)(4 * kg * a.row_bytes + g * F::kGroup * F::kBits / 8 + m * F::kValueBytes);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < F::NK; k++) key_off[k] = (uint32_t)(m * a.row_bytes + (F::k_at(k, kg) < a.dim ? 2 * F::k_at(k, kg) : 0));
+#pragma unroll
+        for (int h = 0; h < (F::kDim + 127) / 128; h++) value_off[h] = (uint32_t)(4 * kg * a.row_bytes + (F::v_at(m, 8 * h) < a.dim ? 2 * F::v_at(m, 8 * h) : 0));
+    }
+    Tile<F> tile;                                                 // the one under way
+    u4 q_raw[F::NK];
+    auto halves_of = [&](const Segment& g, uint32_t t) {
+        const int at = (int)t * kTile;
+        Halves h;
+        h.page[0] = (uint32_t)uniform_load(g.table, at >> a.page_shift);
+        h.page[1] = at + 16 < g.n ? (uint32_t)uniform_load(g.table, (at + 16) >> a.page_shift) : 0xFFFFFFFFu;
+        return h;
+    };
+    auto row_of = [&](const Segment& g, const Halves& h, uint32_t t, int half) {  // row of the half's first token, in rows of this head's pages
+        const uint32_t page = h.page[half] < a.pages ? h.page[half] : 0;
+        return (((int64_t)page * a.kv_heads + g.head) << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
+    };
+    const uint32_t* pair_base = (m < 8 ? a.key_meta : a.value_meta) + 4 * kg + (m & 3);
+    auto load_keys = [&](const Segment& g, uint32_t t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint8_t* base = a.keys + row_of(g, tile.h, t, half) * a.row_bytes;
             if constexpr (F::kCodes) {
-                float x[F::NK][8], top = 0.f;
 #pragma unroll
-                for (int k = 0; k < F::NK; k++)
+                for (int c = 0; c < F::kGroups; c++) load_words<F::kKeyGroupWords>(base + key_off[c], tile.key[half] + c * F::kKeyGroupWords);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint16_t u = (uint16_t)(q[k][e / 2] >> (16 * (e & 1)));
-                        x[k][e] = a.q_bf16 ? bf16_to_f32(u) : f16_bits(u);
-                        top = fmaxf(top, __builtin_fabsf(x[k][e]));
-                    }
-                // exact but for values 2^28 and more below the largest
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const int ex = top > 0.f && top <= 3.4e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
-                score_scale = __builtin_ldexpf(a.scale, ex + kUnit<F::kBits>);
-#pragma unroll
-                for (int g = 0; g < F::kGroups; g++) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int k = g * F::kPerK; k < (g + 1) * F::kPerK; k++) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            x[k][e] = __builtin_ldexpf(x[k][e], -ex);
-                            sum += x[k][e];
-                        }
-#pragma unroll
-                        for (int p = 0; p < 4; p++)
-                            q[k][p] = as_u32(h2{(_Float16)x[k][query_order<F::kBits>(2 * p)], (_Float16)x[k][query_order<F::kBits>(2 * p + 1)]});
-                    }
-                    sum += __shfl_xor(sum, 16, 64);
-                    q_sum[g] = __builtin_ldexpf(sum + __shfl_xor(sum, 32, 64), -kUnit<F::kBits>);
-                }
+                for (int k = 0; k < F::NK; k++) load_words<4>(base + key_off[k], tile.key[half] + 4 * k);
             }
         }
-
-        // ---- addresses ----
-        uint32_t key_off[F::kCodes ? F::kGroups : F::NK], value_off[F::kCodes ? F::kGroups : (F::kDim + 127) / 128];
         if constexpr (F::kCodes) {
-#pragma unroll
-            for (int g = 0; g < F::kGroups; g++) {
-                key_off[g] = (uint32_t)(m * a.row_bytes + (g * F::kGroup + kg * (F::kGroup / 4)) * F::kBits / 8);
-                value_off[g] = (uint32_t)(4 * kg * a.row_bytes + g * F::kGroup * F::kBits / 8 + m * F::kValueBytes);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < F::NK; k++) key_off[k] = (uint32_t)(m * a.row_bytes + (F::k_at(k, kg) < a.dim ? 2 * F::k_at(k, kg) : 0));
-#pragma unroll
-            for (int h = 0; h < (F::kDim + 127) / 128; h++) value_off[h] = (uint32_t)(4 * kg * a.row_bytes + (F::v_at(m, 8 * h) < a.dim ? 2 * F::v_at(m, 8 * h) : 0));
-        }
-        auto halves_of = [&](uint32_t t) {
-            const int at = (int)t * kTile;
-            Halves h;
-            h.page[0] = (uint32_t)uniform_load(table, at >> a.page_shift);
-            h.page[1] = at + 16 < n ? (uint32_t)uniform_load(table, (at + 16) >> a.page_shift) : 0xFFFFFFFFu;
-            return h;
-        };
-        auto row_of = [&](const Halves& h, uint32_t t, int half) {  // row of the half's first token, in rows of this head's pages
-            const uint32_t page = h.page[half] < a.pages ? h.page[half] : 0;
-            return ((int64_t)page * a.kv_heads + head << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
-        };
-        auto load_meta = [&](const uint32_t* base, const Halves& h, uint32_t t, int half, u4* out) {
-            const uint32_t page = h.page[half] < a.pages ? h.page[half] : 0;
-            const uint32_t* p = base + (((int64_t)page * a.kv_heads + head) * F::kGroups << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
-#pragma unroll
-            for (int g = 0; g < F::kGroups; g++) out[g] = *reinterpret_cast<const u4*>(p + (g << a.page_shift) + 4 * kg);
-        };
-        KeyTile<F> keys;
-        ValueTile<F> values;
-        auto load_keys = [&](const Halves& h, uint32_t t) {
+            int64_t at[2];
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                const uint8_t* base = a.keys + row_of(h, t, half) * a.row_bytes;
+                const uint32_t page = tile.h.page[half] < a.pages ? tile.h.page[half] : 0;
+                at[half] = ((((int64_t)page * a.kv_heads + g.head) * F::kGroups) << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
+            }
+            const uint32_t* p = pair_base + (m & 4 ? at[1] : at[0]);
+#pragma unroll
+            for (int c = 0; c < F::kGroups; c++) tile.pairs[c] = p[c << a.page_shift];
+        }
+    };
+    auto load_values = [&](const Segment& g, uint32_t t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint8_t* base = a.values + row_of(g, tile.h, t, half) * a.row_bytes;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint8_t* row = base + i * a.row_bytes;
+                uint32_t* out = tile.value[4 * half + i];
                 if constexpr (F::kCodes) {
 #pragma unroll
-                    for (int g = 0; g < F::kGroups; g++) load_words<F::kKeyGroupWords>(base + key_off[g], keys.raw[half] + g * F::kKeyGroupWords);
-                    load_meta(a.key_meta, h, t, half, keys.meta[half]);
+                    for (int c = 0; c < F::kGroups; c++) {
+                        const uint8_t* p = row + value_off[c];
+                        if constexpr (F::kValueBytes >= 4) load_words<F::kValueBytes / 4>(p, out + c * F::kValueGroupWords);
+                        else if constexpr (F::kValueBytes == 2) out[c] = *reinterpret_cast<const uint16_t*>(p);
+                        else out[c] = *p;
+                    }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < F::NK; k++) load_words<4>(base + key_off[k], keys.raw[half] + 4 * k);
+                    for (int k = 0; k < (F::kDim + 127) / 128; k++) load_words<F::kDim == 64 ? 2 : 4>(row + value_off[k], out + 4 * k);
                 }
             }
-        };
-        auto load_values = [&](const Halves& h, uint32_t t) {
+        }
+    };
+    // A segment's queries and first tile: asked for while the segment before it is put together.
+    auto begin = [&](const Segment& g) __attribute__((always_inline)) {
+        const uint16_t* src = a.q + g.b * a.q_row + (g.q_head + (m < g.queries ? m : 0)) * a.q_head;
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const uint8_t* base = a.values + row_of(h, t, half) * a.row_bytes;
+        for (int k = 0; k < F::NK; k++) {
+            const int d = F::k_at(k, kg);
+            q_raw[k] = m < g.queries && d < a.dim ? *reinterpret_cast<const u4*>(src + d) : u4{0, 0, 0, 0};
+        }
+        if (g.from + wave < g.to) {
+            tile.h = halves_of(g, g.from + wave);
+            load_keys(g, g.from + wave);
+            load_values(g, g.from + wave);
+        }
+    };
+    begin(g);
+    for (;;) {
+        left -= g.units;
+        Segment after = g;
+        bool more_segments = false;
+        if (left) {
+            if (++hq == per_seq) {
+                hq = 0;
+                do
+                    if (++b >= (uint32_t)a.B) return;             // (never, while nobody writes the lengths)
+                while (tokens_of(a, b) == 0);
+            }
+            after = segment_of(a, b, hq, 0, left);
+            more_segments = after.from < after.to;
+        }
+        const int n = g.n;
+        const uint32_t to = g.to;
+
+        // ---- Q: over codes brought near 2^14 by a power of two, with the sum of every group in the codes' unit ----
+        float q_sum[F::kGroups], score_scale = a.scale;
+        u4 q[F::NK];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint8_t* row = base + i * a.row_bytes;
-                    uint32_t* out = values.raw[4 * half + i];
-                    if constexpr (F::kCodes) {
+        for (int k = 0; k < F::NK; k++) q[k] = q_raw[k];
+        if constexpr (F::kCodes) {
+            float x[F::NK][8], top = 0.f;
 #pragma unroll
-                        for (int g = 0; g < F::kGroups; g++) {
-                            const uint8_t* p = row + value_off[g];
-                            if constexpr (F::kValueBytes >= 4) load_words<F::kValueBytes / 4>(p, out + g * F::kValueGroupWords);
-                            else if constexpr (F::kValueBytes == 2) out[g] = *reinterpret_cast<const uint16_t*>(p);
-                            else out[g] = *p;
-                        }
-                    } else {
+            for (int k = 0; k < F::NK; k++)
 #pragma unroll
-                        for (int k = 0; k < (F::kDim + 127) / 128; k++) load_words<F::kDim == 64 ? 2 : 4>(row + value_off[k], out + 4 * k);
+                for (int e = 0; e < 8; e++) {
+                    const uint16_t u = (uint16_t)(q[k][e / 2] >> (16 * (e & 1)));
+                    x[k][e] = a.q_bf16 ? bf16_to_f32(u) : f16_bits(u);
+                    top = fmaxf(top, __builtin_fabsf(x[k][e]));
+                }
+            // exact but for values 2^28 and more below the largest
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const int ex = top > 0.f && top <= 3.4e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+            score_scale = __builtin_ldexpf(a.scale, ex + kUnit<F::kBits>);
+#pragma unroll
+            for (int c = 0; c < F::kGroups; c++) {
+                float sum = 0.f;
+#pragma unroll
+                for (int k = c * F::kPerK; k < (c + 1) * F::kPerK; k++) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[k][e] = __builtin_ldexpf(x[k][e], -ex);
+                        sum += x[k][e];
                     }
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+                        q[k][p] = as_u32(h2{(_Float16)x[k][query_order<F::kBits>(2 * p)], (_Float16)x[k][query_order<F::kBits>(2 * p + 1)]});
                 }
-                if constexpr (F::kCodes) load_meta(a.value_meta, h, t, half, values.meta[half]);
+                sum += __shfl_xor(sum, 16, 64);
+                q_sum[c] = __builtin_ldexpf(sum + __shfl_xor(sum, 32, 64), -kUnit<F::kBits>);
             }
-        };
+        }
 
         // ---- tiles ----
         f4 acc[F::NV], zeros[F::kGroups];                         // zeros: sums of (P s) z, the same in every row
@@ -417,72 +465,84 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
 #pragma unroll
         for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int g = 0; g < F::kGroups; g++) zeros[g] = f4{0.f, 0.f, 0.f, 0.f};
-        uint32_t t = from + wave;
-        Halves h = {}, hn = {};
-        if (t < to) {
-            h = halves_of(t);
-            load_keys(h, t);
-            load_values(h, t);
-        }
-        while (t < to) {
+        for (int c = 0; c < F::kGroups; c++) zeros[c] = f4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t t = g.from + wave; t < to; t += kWaves) {
+            // The second half of the workgroups shares its CUs with the first, whose waves, being older, go before: 17 against 21 us of a launch's 24.
+            // Going first every other tile evens it out (3 % of it).
+            __builtin_amdgcn_s_setprio(0);
+            if (blockIdx.x >= gridDim.x / 2 && (t / kWaves & 1)) __builtin_amdgcn_s_setprio(1);
             const uint32_t next = t + kWaves;
             const bool more = next < to;
-            if (more) hn = halves_of(next);
+            Halves hn = {};
+            if (more) hn = halves_of(g, next);
             // Tokens that do not count: behind the end, or on a page outside the cache.
-            const bool full = (int)t * kTile + kTile <= n && h.page[0] < a.pages && h.page[1] < a.pages;
-            auto seen = [&](int e) { return (int)t * kTile + 16 * (e >> 2) + 4 * kg + (e & 3) < n && h.page[e >> 2] < a.pages; };
+            const bool full = (int)t * kTile + kTile <= n && tile.h.page[0] < a.pages && tile.h.page[1] < a.pages;
+            const Halves h = tile.h;
+            auto counts = [&](int half, int i) { return (int)t * kTile + 16 * half + 4 * kg + i < n && h.page[half] < a.pages; };
+            auto seen = [&](int e) { return counts(e >> 2, e & 3); };
+            uint32_t pairs[F::kGroups];
+            if constexpr (F::kCodes) {
+#pragma unroll
+                for (int c = 0; c < F::kGroups; c++) pairs[c] = tile.pairs[c];
+                if (!full) {
+                    const bool own = m & 4 ? counts(1, m & 3) : counts(0, m & 3);
+#pragma unroll
+                    for (int c = 0; c < F::kGroups; c++) pairs[c] = own ? pairs[c] : 0u;
+                }
+            }
             // scores, in units of log 2
             float x[8];
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
+            static_for<0, 2>([&](auto hc) {
+                constexpr int half = decltype(hc)::value;
                 f4 s = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (F::kCodes) {
 #pragma unroll
-                    for (int g = 0; g < F::kGroups; g++) {
+                    for (int c = 0; c < F::kGroups; c++) {
                         f4 dot = {0.f, 0.f, 0.f, 0.f};
                         uint32_t codes[4 * F::kPerK];
 #pragma unroll
-                        for (int w = 0; w < F::kKeyGroupWords; w++) key_codes<F::kBits>(keys.raw[half][g * F::kKeyGroupWords + w], codes + w * (16 / F::kBits));
+                        for (int w = 0; w < F::kKeyGroupWords; w++) key_codes<F::kBits>(tile.key[half][c * F::kKeyGroupWords + w], codes + w * (16 / F::kBits));
 #pragma unroll
                         for (int k = 0; k < F::kPerK; k++)
-                            dot = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[g * F::kPerK + k], dot);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t pair = keys.meta[half][g][i];
-                            const float part = __builtin_fmaf(-f16_bits(pair >> 16), q_sum[g], dot[i]);
-                            s[i] = g ? __builtin_fmaf(f16_bits(pair), part, s[i]) : f16_bits(pair) * part;
-                        }
+                            dot = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[c * F::kPerK + k], dot);
+                        const uint32_t zero = pairs[c] >> 16;
+                        static_for<0, 4>([&](auto ic) {
+                            constexpr int i = decltype(ic)::value, lane_of = 4 * half + i;
+                            const float part = __builtin_fmaf(-f16_bits(row_lane<lane_of>(zero)), q_sum[c], dot[i]);
+                            s[i] = c ? __builtin_fmaf(f16_bits(row_lane<lane_of>(pairs[c])), part, s[i]) : f16_bits(row_lane<lane_of>(pairs[c])) * part;
+                        });
                     }
                 } else {
 #pragma unroll
                     for (int k = 0; k < F::NK; k++) {
-                        const uint32_t* w = keys.raw[half] + 4 * k;
+                        const uint32_t* w = tile.key[half] + 4 * k;
                         s = mfma<F::kBf16>(u4{w[0], w[1], w[2], w[3]}, q[k], s);
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[4 * half + i] = F::kCodes ? s[i] : s[i] * score_scale;
+            });
+            if (more) {
+                tile.h = hn;
+                load_keys(g, next);
             }
-            if (more) load_keys(hn, next);
             // reference: for codes the scores are raised by the exponent of the token's largest value scale
-            float unit[8];                                    // 2^-e
+            float unit[8], value_scale[F::kGroups][8];        // 2^-e; scales times that
             if constexpr (F::kCodes) {
-                if (!full) {
+                static_for<0, 8>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    float top = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-#pragma unroll
-                        for (int g = 0; g < F::kGroups; g++) values.meta[e >> 2][g][e & 3] = seen(e) ? values.meta[e >> 2][g][e & 3] : 0u;
-                }
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float top = f16_bits(values.meta[e >> 2][0][e & 3]);
-#pragma unroll
-                    for (int g = 1; g < F::kGroups; g++) top = fmaxf(top, f16_bits(values.meta[e >> 2][g][e & 3]));
+                    for (int c = 0; c < F::kGroups; c++) {
+                        value_scale[c][e] = f16_bits(row_lane<8 + e>(pairs[c]));
+                        top = c ? fmaxf(top, value_scale[c][e]) : value_scale[c][e];
+                    }
                     const int ex = __builtin_amdgcn_frexp_expf(top);
                     x[e] = __builtin_fmaf(x[e], score_scale, (float)ex);
                     unit[e] = __builtin_ldexpf(1.f, -ex);
-                }
+#pragma unroll
+                    for (int c = 0; c < F::kGroups; c++) value_scale[c][e] *= unit[e];
+                });
             }
             if (!full) {
 #pragma unroll
@@ -499,7 +559,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                 for (int j = 0; j < F::NV; j++) acc[j] *= keep;
                 if constexpr (F::kCodes) {
 #pragma unroll
-                    for (int g = 0; g < F::kGroups; g++) zeros[g] *= keep;
+                    for (int c = 0; c < F::kGroups; c++) zeros[c] *= keep;
                 }
             }
             float p[8];
@@ -510,42 +570,41 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                 for (int e = 0; e < 8; e++) p[e] = seen(e) ? p[e] : 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                l = F::kCodes ? __builtin_fmaf(p[e], unit[e], l) : l + p[e];
-            }
+            for (int e = 0; e < 8; e++) l = F::kCodes ? __builtin_fmaf(p[e], unit[e], l) : l + p[e];
             // weighted values
             if constexpr (F::kCodes) {
 #pragma unroll
-                for (int g = 0; g < F::kGroups; g++) {
+                for (int c = 0; c < F::kGroups; c++) {
                     float pg[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) pg[e] = p[e] * (f16_bits(values.meta[e >> 2][g][e & 3]) * unit[e]);
+                    for (int e = 0; e < 8; e++) pg[e] = p[e] * value_scale[c][e];
                     u4 hi, lo, z;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        z[i] = token_pair<true>(values.meta[i >> 1][g][2 * (i & 1) + 1], values.meta[i >> 1][g][2 * (i & 1)]);
+                    const uint32_t zero_pair = token_pair<true>((uint32_t)__builtin_amdgcn_mov_dpp((int)pairs[c], 0xB1, 0xF, 0xF, true), pairs[c]);
+                    static_for<0, 4>([&](auto ic) {
+                        constexpr int i = decltype(ic)::value;
+                        z[i] = row_lane<8 + 2 * i>(zero_pair);
                         hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
                         lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
-                    }
+                    });
                     u4 v[F::kPerV];
                     static_for<0, F::kPerV>([&](auto jc) {
                         constexpr int j = decltype(jc)::value, w = j * F::kBits / 32;
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            v[j][i] = value_codes<F::kBits, j % (32 / F::kBits)>(values.raw[2 * i + 1][g * F::kValueGroupWords + w], values.raw[2 * i][g * F::kValueGroupWords + w]);
-                        acc[g * F::kPerV + j] = mfma<false>(v[j], hi, acc[g * F::kPerV + j]);
+                            v[j][i] = value_codes<F::kBits, j % (32 / F::kBits)>(tile.value[2 * i + 1][c * F::kValueGroupWords + w], tile.value[2 * i][c * F::kValueGroupWords + w]);
+                        acc[c * F::kPerV + j] = mfma<false>(v[j], hi, acc[c * F::kPerV + j]);
                     });
-                    zeros[g] = mfma<false>(z, hi, zeros[g]);
+                    zeros[c] = mfma<false>(z, hi, zeros[c]);
 #pragma unroll
-                    for (int j = 0; j < F::kPerV; j++) acc[g * F::kPerV + j] = mfma<false>(v[j], lo, acc[g * F::kPerV + j]);
-                    zeros[g] = mfma<false>(z, lo, zeros[g]);
+                    for (int j = 0; j < F::kPerV; j++) acc[c * F::kPerV + j] = mfma<false>(v[j], lo, acc[c * F::kPerV + j]);
+                    zeros[c] = mfma<false>(z, lo, zeros[c]);
                 }
             } else {
                 if (!full) {
 #pragma unroll
                     for (int e = 0; e < 8; e++)
 #pragma unroll
-                        for (int w = 0; w < F::kValueWords; w++) values.raw[e][w] = seen(e) ? values.raw[e][w] : 0u;
+                        for (int w = 0; w < F::kValueWords; w++) tile.value[e][w] = seen(e) ? tile.value[e][w] : 0u;
                 }
                 u4 hi, lo;
 #pragma unroll
@@ -557,15 +616,14 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                     constexpr int j = decltype(jc)::value;
                     u4 v;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = token_pair<(j & 1) != 0>(values.raw[2 * i + 1][j / 2], values.raw[2 * i][j / 2]);
+                    for (int i = 0; i < 4; i++) v[i] = token_pair<(j & 1) != 0>(tile.value[2 * i + 1][j / 2], tile.value[2 * i][j / 2]);
                     acc[j] = mfma<F::kBf16>(v, hi, acc[j]);
                     acc[j] = mfma<F::kBf16>(v, lo, acc[j]);
                 });
             }
-            if (more) load_values(hn, next);
-            h = hn;
-            t = next;
+            if (more) load_values(g, next);
         }
+        if (more_segments) begin(after);
 
         // ---- the four waves of the workgroup joined ----
         l += __shfl_xor(l, 16, 64);
@@ -577,10 +635,10 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
         __syncthreads();
         const float r_all = fmaxf(fmaxf(stats[0][0][m], stats[1][0][m]), fmaxf(stats[2][0][m], stats[3][0][m]));
         const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - r_all);
-        const bool complete = from == 0 && to == tiles;
-        float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (from == 0)) * (2 * kQueries + a.queries * a.dim);
-        if (!complete && from == 0 && threadIdx.x == 0)
-            a.joints[blockIdx.x] = Joint{b, hq, s.piece_of(s.start(blockIdx.x) + (first_left - left) + units - at - 1) - blockIdx.x + 1, 0};
+        const bool complete = g.from == 0 && to == g.tiles;
+        float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (g.from == 0)) * (2 * kQueries + a.queries * a.dim);
+        if (!complete && g.from == 0 && threadIdx.x == 0)         // (the segment ends tiles - to units behind this piece)
+            a.joints[blockIdx.x] = Joint{g.b, g.hq, s.piece_of(position + g.units + g.tiles - to - 1) - blockIdx.x + 1, 0};
         auto joined = [&](int query, float& top) {                // sum of the waves' l, relative to the largest r
             top = fmaxf(fmaxf(stats[0][0][query], stats[1][0][query]), fmaxf(stats[2][0][query], stats[3][0][query]));
             float sum = 0.f;
@@ -591,6 +649,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
             }
             return sum;
         };
+        const int queries = g.queries;
         if (!complete && threadIdx.x < (uint32_t)queries) {
             float top;
             slot[kQueries + threadIdx.x] = joined((int)threadIdx.x, top);
@@ -619,23 +678,15 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(AttentionArgs a) {
                 if (complete) {
                     float top;
                     const float sum = joined(query, top), inv = sum == 0.f ? 0.f : 1.f / sum;
-                    store_out(a, (int64_t)b * a.q_heads + q_head + query, c * kChunk + d, o * inv);
+                    store_out(a, (int64_t)g.b * a.q_heads + g.q_head + query, c * kChunk + d, o * inv);
                 } else {
                     *reinterpret_cast<f4*>(slot + 2 * kQueries + query * a.dim + c * kChunk + d) = o;
                 }
             }
         }
+        if (!more_segments) break;
         __syncthreads();                                          // (the next segment writes stats and outs again)
-        }
-        left -= taken;
-        at = 0;
-        if (left) {
-            if (++hq == per_seq) {
-                hq = 0;
-                do
-                    if (++b >= (uint32_t)a.B) return;             // (never, while nobody writes the lengths)
-                while (tokens_of(a, b) == 0);
-            }
-        }
-    } while (left);
+        position += g.units;
+        g = after;
+    }
 }
