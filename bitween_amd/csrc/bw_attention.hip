@@ -87,14 +87,14 @@ Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
     Plan p;
     p.whole = max_pages * c->page_size <= kWholeTokens && segments < (int64_t)1 << 31;
-    p.grid = p.whole ? (uint32_t)segments : (uint32_t)bw_device_cus() * (c->dim > 128 ? 1 : 2);        // (kResident)
+    p.grid = p.whole ? (uint32_t)segments : (uint32_t)bw_device_cus() * resident_workgroups(c->dim);
     return p;
 }
 
 }  // namespace
 
 template <class F> static void launch(const AttentionArgs& a, uint32_t grid, hipStream_t stream) {
-    hipLaunchKernelGGL(attention_kernel<F>, dim3(grid), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_kernel<F, 1>), dim3(grid), dim3(256), 0, stream, a);
 }
 
 extern "C" size_t bw_cache_attention_workspace_bytes(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {

@@ -220,31 +220,91 @@ template <class F> struct Tile {
     Halves h;
     uint32_t key[2][F::kKeyWords];
     uint32_t value[8][F::kValueWords];           // token 4 kg + i of half h: 4 h + i
-    uint32_t pairs[F::kGroups];                  // of a group, in lane m of 16: keys' (m < 8) or values' token 4 kg + m % 4 of half m / 4 % 2
+    uint32_t pairs[2][F::kGroups];               // of a group: see Fold
 };
-// What lane L of the 16 has.
+// What lane L of the 16, and of the 4, has.
 template <int L> BW_DEV uint32_t row_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x150 + L, 0xF, 0xF, true); }
+template <int L> BW_DEV uint32_t quad_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, L * 0x55, 0xF, 0xF, true); }
+// What the lane N further on (of 16, around) has.
+template <int N> BW_DEV uint32_t lane_after(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x120 + 16 - N, 0xF, 0xF, true); }
 
-template <int WORDS> BW_DEV void load_words(const uint8_t* p, uint32_t* out) {
+// Few queries leave columns of the MFMAs empty, and with them most of what a lane does between the two products: over codes that is more than the
+// unpacking.  With 8 or fewer queries (FOLD 2) or 4 (FOLD 4) they are there 2 or 4 times, and the lanes of each copy ("part" m / (16 / FOLD)) take only
+// their share of the tile's tokens, kTokens = 8 / FOLD instead of 8 each; the weights go back to the first copy's lanes for the second product.
+// 64 sequences of up to 8192 tokens, 8 heads of 128, groups of 32, 4 queries: 119 against 144 us in 4 bits, 125 against 187 us in 8 (fewer registers go
+// to memory, too); groups of 128: 75.5 against 78 and 96 against 98 us.
+//   token j of part p is token 4 h + i of the lane's 8: FOLD 1: j;  2: h = p, i = j;  4: h = p / 2, i = 2 (p % 2) + j
+//   a group's pairs, one load for all: FOLD 1: lanes 0 ... 7 the keys' 8 tokens, 8 ... 15 the values';  2: lanes 4 c + i of part p the keys' and, in a
+//   second register, the values' token j = i;  4: lanes 0, 1 of the four of part p the keys' tokens, 2, 3 the values'
+template <int FOLD> struct Fold {
+    static constexpr int kTokens = 8 / FOLD, kColumns = 16 / FOLD, kRegisters = FOLD == 2 ? 2 : 1;
+    int part;
+    bool odd, high;                              // of part
+    BW_DEV explicit Fold(int m) : part(m / kColumns), odd(part & 1), high(FOLD == 4 ? part & 2 : part & 1) {}
+    BW_DEV int token(int j) const { return FOLD == 1 ? j : FOLD == 2 ? 4 * part + j : 2 * part + j; }          // 4 h + i
+    BW_DEV int pair_token(int m) const { return FOLD == 1 ? m & 7 : FOLD == 2 ? 4 * part + (m & 3) : 2 * part + (m & 1); }
+    static BW_DEV bool pair_is_value(int m) { return FOLD == 1 ? m & 8 : m & 2; }                              // (FOLD 2: by register)
+    template <int J> BW_DEV float pick(const f4* d) const {                                                   // of the products of both halves
+        if constexpr (FOLD == 1) return d[J >> 2][J & 3];
+        else if constexpr (FOLD == 2) return high ? d[1][J] : d[0][J];
+        else return high ? (odd ? d[1][2 + J] : d[1][J]) : (odd ? d[0][2 + J] : d[0][J]);
+    }
+    template <int J> static BW_DEV uint32_t key_pair(uint32_t first) {
+        if constexpr (FOLD == 1) return row_lane<J>(first);
+        else return quad_lane<J>(first);
+    }
+    template <int J> static BW_DEV uint32_t value_pair(uint32_t first, uint32_t second) {
+        if constexpr (FOLD == 1) return row_lane<8 + J>(first);
+        else if constexpr (FOLD == 2) return quad_lane<J>(second);
+        else return quad_lane<2 + J>(first);
+    }
+    // zero points of tokens 2 i and 2 i + 1, side by side
+    template <int I> static BW_DEV uint32_t zero_pair(uint32_t both) { return row_lane<FOLD == 1 ? 8 + 2 * I : FOLD == 2 ? 8 * (I >> 1) + 2 * (I & 1) : 4 * I + 2>(both); }
+    // the lane's weights (pairs of tokens) to those of all 8
+    static BW_DEV u4 all(const uint32_t* own) {
+        if constexpr (FOLD == 1) return u4{own[0], own[1], own[2], own[3]};
+        else if constexpr (FOLD == 2) return u4{own[0], own[1], lane_after<8>(own[0]), lane_after<8>(own[1])};
+        else return u4{own[0], lane_after<4>(own[0]), lane_after<8>(own[0]), lane_after<12>(own[0])};
+    }
+    // over the parts
+    static BW_DEV float max(float v) {
+        if constexpr (FOLD == 4) v = fmaxf(v, __shfl_xor(v, 4, 64));
+        if constexpr (FOLD >= 2) v = fmaxf(v, __shfl_xor(v, 8, 64));
+        return v;
+    }
+    static BW_DEV float sum(float v) {
+        if constexpr (FOLD == 4) v += __shfl_xor(v, 4, 64);
+        if constexpr (FOLD >= 2) v += __shfl_xor(v, 8, 64);
+        return v;
+    }
+};
+
+template <int WORDS, bool NT = false> BW_DEV void load_words(const uint8_t* p, uint32_t* out) {
     if constexpr (WORDS % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < WORDS / 4; i++) {
-            const u4 v = reinterpret_cast<const u4*>(p)[i];
+            const u4 v = NT ? __builtin_nontemporal_load(reinterpret_cast<const u4*>(p) + i) : reinterpret_cast<const u4*>(p)[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) out[4 * i + j] = v[j];
         }
     } else if constexpr (WORDS == 2) {
-        const u2 v = *reinterpret_cast<const u2*>(p);
+        const u2 v = NT ? __builtin_nontemporal_load(reinterpret_cast<const u2*>(p)) : *reinterpret_cast<const u2*>(p);
         out[0] = v[0];
         out[1] = v[1];
     } else {
         static_assert(WORDS == 1, "words of a lane");
-        out[0] = *reinterpret_cast<const uint32_t*>(p);
+        out[0] = NT ? __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p)) : *reinterpret_cast<const uint32_t*>(p);
     }
 }
 
-// Workgroups of a CU at a time: heads of more than 128 values fill the registers with one.
-template <class F> constexpr int kResident = F::kDim > 128 ? 1 : 2;
+// Values are read past the caches, which leaves those to the keys, whose cache lines are taken by more than one load: 165 against 182 us at 64 sequences
+// of 2048 ... 8192 16-bit tokens (8 heads of 128), 96 against 106 us in 8 bits, the keys too no further use.  Not with 64 values to a head, whose loads
+// of values share lines as well: 15.2 against 16.1 us at 128 sequences of 512.
+template <class F> constexpr bool kPast = F::kDim > 64;
+
+// Workgroups of a CU at a time, as the registers allow: 27.7 us with three against 33.6 with two at 64 sequences of 2048 tokens of 12 heads of 64 in 8 bits.
+// Three for heads of 128 leave too few for groups of 32 (175 against 118 us in 4 bits) and won 4 % over groups of 128, nothing in 8 bits.
+constexpr int resident_workgroups(int dim) { return dim > 128 ? 1 : dim > 64 ? 2 : 3; }
 
 // What a workgroup has of a segment: tiles from ... to - 1 of `tiles`.
 struct Segment {
@@ -270,13 +330,16 @@ BW_DEV Segment segment_of(const AttentionArgs& a, uint32_t b, uint32_t hq, uint3
     return g;
 }
 
-template <class F>
-__global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionArgs a) {
+template <class F, int FOLD>
+__global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_kernel(AttentionArgs a) {
     constexpr int kChunk = F::kDim < 128 ? F::kDim : 128, kPitch = kChunk + 4, kChunkBlocks = kChunk / 16;
     __shared__ float outs[kWaves][kQueries][kPitch];
     __shared__ float stats[kWaves][2][kQueries];
     __shared__ uint32_t lds[8];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), m = lane & 15, kg = lane >> 4;
+    using Z = Fold<FOLD>;
+    const Z fold(m);
+    const int column = m & (Z::kColumns - 1);
     const uint32_t per_seq = (uint32_t)(a.kv_heads * a.q_groups);
 
     // the piece of this workgroup: from unit `at` of segment (b, hq) on, `left` units in all
@@ -340,7 +403,9 @@ __global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionA
         const uint32_t page = h.page[half] < a.pages ? h.page[half] : 0;
         return (((int64_t)page * a.kv_heads + g.head) << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
     };
-    const uint32_t* pair_base = (m < 8 ? a.key_meta : a.value_meta) + 4 * kg + (m & 3);
+    // where the lane's pairs lie (FOLD 2: the keys'; the values' lie as far from value_meta)
+    const int pair_token = fold.pair_token(m);
+    const uint32_t* pair_base = (FOLD != 2 && Z::pair_is_value(m) ? a.value_meta : a.key_meta) + 4 * kg + (pair_token & 3);
     auto load_keys = [&](const Segment& g, uint32_t t) __attribute__((always_inline)) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
@@ -360,9 +425,12 @@ __global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionA
                 const uint32_t page = tile.h.page[half] < a.pages ? tile.h.page[half] : 0;
                 at[half] = ((((int64_t)page * a.kv_heads + g.head) * F::kGroups) << a.page_shift) + (((int)t * kTile + 16 * half) & page_mask);
             }
-            const uint32_t* p = pair_base + (m & 4 ? at[1] : at[0]);
+            const uint32_t* p = pair_base + (pair_token & 4 ? at[1] : at[0]);
 #pragma unroll
-            for (int c = 0; c < F::kGroups; c++) tile.pairs[c] = p[c << a.page_shift];
+            for (int c = 0; c < F::kGroups; c++) {
+                tile.pairs[0][c] = p[c << a.page_shift];
+                if constexpr (FOLD == 2) tile.pairs[1][c] = (a.value_meta - a.key_meta + p)[c << a.page_shift];
+            }
         }
     };
     auto load_values = [&](const Segment& g, uint32_t t) __attribute__((always_inline)) {
@@ -377,24 +445,24 @@ __global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionA
 #pragma unroll
                     for (int c = 0; c < F::kGroups; c++) {
                         const uint8_t* p = row + value_off[c];
-                        if constexpr (F::kValueBytes >= 4) load_words<F::kValueBytes / 4>(p, out + c * F::kValueGroupWords);
+                        if constexpr (F::kValueBytes >= 4) load_words<F::kValueBytes / 4, kPast<F>>(p, out + c * F::kValueGroupWords);
                         else if constexpr (F::kValueBytes == 2) out[c] = *reinterpret_cast<const uint16_t*>(p);
                         else out[c] = *p;
                     }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < (F::kDim + 127) / 128; k++) load_words<F::kDim == 64 ? 2 : 4>(row + value_off[k], out + 4 * k);
+                    for (int k = 0; k < (F::kDim + 127) / 128; k++) load_words<F::kDim == 64 ? 2 : 4, kPast<F>>(row + value_off[k], out + 4 * k);
                 }
             }
         }
     };
     // A segment's queries and first tile: asked for while the segment before it is put together.
     auto begin = [&](const Segment& g) __attribute__((always_inline)) {
-        const uint16_t* src = a.q + g.b * a.q_row + (g.q_head + (m < g.queries ? m : 0)) * a.q_head;
+        const uint16_t* src = a.q + g.b * a.q_row + (g.q_head + (column < g.queries ? column : 0)) * a.q_head;
 #pragma unroll
         for (int k = 0; k < F::NK; k++) {
             const int d = F::k_at(k, kg);
-            q_raw[k] = m < g.queries && d < a.dim ? *reinterpret_cast<const u4*>(src + d) : u4{0, 0, 0, 0};
+            q_raw[k] = column < g.queries && d < a.dim ? *reinterpret_cast<const u4*>(src + d) : u4{0, 0, 0, 0};
         }
         if (g.from + wave < g.to) {
             tile.h = halves_of(g, g.from + wave);
@@ -479,77 +547,89 @@ __global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionA
             const bool full = (int)t * kTile + kTile <= n && tile.h.page[0] < a.pages && tile.h.page[1] < a.pages;
             const Halves h = tile.h;
             auto counts = [&](int half, int i) { return (int)t * kTile + 16 * half + 4 * kg + i < n && h.page[half] < a.pages; };
-            auto seen = [&](int e) { return counts(e >> 2, e & 3); };
-            uint32_t pairs[F::kGroups];
+            auto seen = [&](int e) { return counts(e >> 2, e & 3); };               // of the lane's 8 tokens
+            auto own = [&](int j) { const int e = fold.token(j); return e & 4 ? counts(1, e & 3) : counts(0, e & 3); };
+            uint32_t pairs[2][F::kGroups];
             if constexpr (F::kCodes) {
 #pragma unroll
-                for (int c = 0; c < F::kGroups; c++) pairs[c] = tile.pairs[c];
-                if (!full) {
-                    const bool own = m & 4 ? counts(1, m & 3) : counts(0, m & 3);
+                for (int c = 0; c < F::kGroups; c++)
 #pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) pairs[c] = own ? pairs[c] : 0u;
+                    for (int w = 0; w < Z::kRegisters; w++) pairs[w][c] = tile.pairs[w][c];
+                if (!full) {
+                    const bool counted = pair_token & 4 ? counts(1, pair_token & 3) : counts(0, pair_token & 3);
+#pragma unroll
+                    for (int c = 0; c < F::kGroups; c++)
+#pragma unroll
+                        for (int w = 0; w < Z::kRegisters; w++) pairs[w][c] = counted ? pairs[w][c] : 0u;
                 }
             }
             // scores, in units of log 2
-            float x[8];
-            static_for<0, 2>([&](auto hc) {
-                constexpr int half = decltype(hc)::value;
-                f4 s = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (F::kCodes) {
+            float x[Z::kTokens];
+            if constexpr (F::kCodes) {
 #pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) {
-                        f4 dot = {0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < F::kGroups; c++) {
+                    f4 dot[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
                         uint32_t codes[4 * F::kPerK];
 #pragma unroll
                         for (int w = 0; w < F::kKeyGroupWords; w++) key_codes<F::kBits>(tile.key[half][c * F::kKeyGroupWords + w], codes + w * (16 / F::kBits));
 #pragma unroll
                         for (int k = 0; k < F::kPerK; k++)
-                            dot = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[c * F::kPerK + k], dot);
-                        const uint32_t zero = pairs[c] >> 16;
-                        static_for<0, 4>([&](auto ic) {
-                            constexpr int i = decltype(ic)::value, lane_of = 4 * half + i;
-                            const float part = __builtin_fmaf(-f16_bits(row_lane<lane_of>(zero)), q_sum[c], dot[i]);
-                            s[i] = c ? __builtin_fmaf(f16_bits(row_lane<lane_of>(pairs[c])), part, s[i]) : f16_bits(row_lane<lane_of>(pairs[c])) * part;
-                        });
+                            dot[half] = mfma<false>(u4{codes[4 * k], codes[4 * k + 1], codes[4 * k + 2], codes[4 * k + 3]}, q[c * F::kPerK + k], dot[half]);
                     }
-                } else {
+                    const uint32_t zero = pairs[0][c] >> 16;
+                    static_for<0, Z::kTokens>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        const float part = __builtin_fmaf(-f16_bits(Z::template key_pair<j>(zero)), q_sum[c], fold.template pick<j>(dot));
+                        const float scale = f16_bits(Z::template key_pair<j>(pairs[0][c]));
+                        x[j] = c ? __builtin_fmaf(scale, part, x[j]) : scale * part;
+                    });
+                }
+            } else {
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    f4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int k = 0; k < F::NK; k++) {
                         const uint32_t* w = tile.key[half] + 4 * k;
                         s = mfma<F::kBf16>(u4{w[0], w[1], w[2], w[3]}, q[k], s);
                     }
-                }
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[4 * half + i] = F::kCodes ? s[i] : s[i] * score_scale;
-            });
+                    for (int i = 0; i < 4; i++) x[4 * half + i] = s[i] * score_scale;
+                }
+            }
             if (more) {
                 tile.h = hn;
                 load_keys(g, next);
             }
             // reference: for codes the scores are raised by the exponent of the token's largest value scale
-            float unit[8], value_scale[F::kGroups][8];        // 2^-e; scales times that
+            float unit[Z::kTokens], value_scale[F::kGroups][Z::kTokens];        // 2^-e; scales times that
             if constexpr (F::kCodes) {
-                static_for<0, 8>([&](auto ec) {
-                    constexpr int e = decltype(ec)::value;
+                static_for<0, Z::kTokens>([&](auto jc) {
+                    constexpr int j = decltype(jc)::value;
                     float top = 0.f;
 #pragma unroll
                     for (int c = 0; c < F::kGroups; c++) {
-                        value_scale[c][e] = f16_bits(row_lane<8 + e>(pairs[c]));
-                        top = c ? fmaxf(top, value_scale[c][e]) : value_scale[c][e];
+                        value_scale[c][j] = f16_bits(Z::template value_pair<j>(pairs[0][c], pairs[Z::kRegisters - 1][c]));
+                        top = c ? fmaxf(top, value_scale[c][j]) : value_scale[c][j];
                     }
                     const int ex = __builtin_amdgcn_frexp_expf(top);
-                    x[e] = __builtin_fmaf(x[e], score_scale, (float)ex);
-                    unit[e] = __builtin_ldexpf(1.f, -ex);
+                    x[j] = __builtin_fmaf(x[j], score_scale, (float)ex);
+                    unit[j] = __builtin_ldexpf(1.f, -ex);
 #pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) value_scale[c][e] *= unit[e];
+                    for (int c = 0; c < F::kGroups; c++) value_scale[c][j] *= unit[j];
                 });
             }
             if (!full) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = seen(e) ? x[e] : -INFINITY;
+                for (int j = 0; j < Z::kTokens; j++) x[j] = own(j) ? x[j] : -INFINITY;
             }
-            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < Z::kTokens; j++) top = fmaxf(top, x[j]);
             if (__builtin_amdgcn_ballot_w64(top > r + kSlack)) {
+                top = Z::max(top);
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), r);
                 const float keep = top == r ? 1.f : __builtin_amdgcn_exp2f(r - top);
@@ -562,30 +642,32 @@ __global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionA
                     for (int c = 0; c < F::kGroups; c++) zeros[c] *= keep;
                 }
             }
-            float p[8];
+            float p[Z::kTokens];
 #pragma unroll
-            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e] - r);
+            for (int j = 0; j < Z::kTokens; j++) p[j] = __builtin_amdgcn_exp2f(x[j] - r);
             if (!full) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = seen(e) ? p[e] : 0.f;
+                for (int j = 0; j < Z::kTokens; j++) p[j] = own(j) ? p[j] : 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < 8; e++) l = F::kCodes ? __builtin_fmaf(p[e], unit[e], l) : l + p[e];
+            for (int j = 0; j < Z::kTokens; j++) l = F::kCodes ? __builtin_fmaf(p[j], unit[j], l) : l + p[j];
             // weighted values
             if constexpr (F::kCodes) {
 #pragma unroll
                 for (int c = 0; c < F::kGroups; c++) {
-                    float pg[8];
+                    float pg[Z::kTokens];
+                    uint32_t own_hi[Z::kTokens / 2], own_lo[Z::kTokens / 2];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) pg[e] = p[e] * value_scale[c][e];
-                    u4 hi, lo, z;
-                    const uint32_t zero_pair = token_pair<true>((uint32_t)__builtin_amdgcn_mov_dpp((int)pairs[c], 0xB1, 0xF, 0xF, true), pairs[c]);
-                    static_for<0, 4>([&](auto ic) {
-                        constexpr int i = decltype(ic)::value;
-                        z[i] = row_lane<8 + 2 * i>(zero_pair);
-                        hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
-                        lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
-                    });
+                    for (int j = 0; j < Z::kTokens; j++) pg[j] = p[j] * value_scale[c][j];
+#pragma unroll
+                    for (int i = 0; i < Z::kTokens / 2; i++) {
+                        own_hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
+                        own_lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
+                    }
+                    const u4 hi = Z::all(own_hi), lo = Z::all(own_lo);
+                    const uint32_t pair = pairs[Z::kRegisters - 1][c], both = token_pair<true>((uint32_t)__builtin_amdgcn_mov_dpp((int)pair, 0xB1, 0xF, 0xF, true), pair);
+                    u4 z;
+                    static_for<0, 4>([&](auto ic) { z[decltype(ic)::value] = Z::template zero_pair<decltype(ic)::value>(both); });
                     u4 v[F::kPerV];
                     static_for<0, F::kPerV>([&](auto jc) {
                         constexpr int j = decltype(jc)::value, w = j * F::kBits / 32;
@@ -626,14 +708,15 @@ __global__ __launch_bounds__(256, kResident<F>) void attention_kernel(AttentionA
         if (more_segments) begin(after);
 
         // ---- the four waves of the workgroup joined ----
+        l = Z::sum(l);
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        if (kg == 0) {
+        if (lane < Z::kColumns) {
             stats[wave][0][m] = r;
             stats[wave][1][m] = l;
         }
         __syncthreads();
-        const float r_all = fmaxf(fmaxf(stats[0][0][m], stats[1][0][m]), fmaxf(stats[2][0][m], stats[3][0][m]));
+        const float r_all = fmaxf(fmaxf(stats[0][0][column], stats[1][0][column]), fmaxf(stats[2][0][column], stats[3][0][column]));
         const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - r_all);
         const bool complete = g.from == 0 && to == g.tiles;
         float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (g.from == 0)) * (2 * kQueries + a.queries * a.dim);
