@@ -707,6 +707,48 @@ def extras_llama7b_decoder_graph(torch, hip, QuantizedLinear, layers):
     return res
 
 
+def extras_llama7b_decoder_paged(torch, hip, QuantizedLinear, layers):
+    """The decoder of llama7b_decoder_graph (sibling launches fused, HIP glue) with the library's rotation, paged cache and attention
+    of one token in place of the glue's: 512-token prompt and 256 tokens, and the same step again with 3584 tokens cached before it (the glue takes 4096), where the
+    cache is what is read most.  Only on request (--only llama7b_decoder_paged)."""
+    import bitween_amd
+    import bench_decoder as bd
+    nlayers, prompt, new_tokens, cached = 32, 512, 256, 3584
+    with torch.device("cuda"):
+        model = bd.Decoder(layers=nlayers, max_len=cached + new_tokens).half()
+    model.init_weights(seed=0)
+    ids = torch.randint(0, 32000, (prompt,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    qmodel = bitween_amd.Bitween(model, bits=4, group_size=128).quantize(
+        rtn=True, ignore_layers=["lm_head", "embed_tokens"], layer_config=bd.mixed_recipe(nlayers), verbose=False)
+    del model
+    qmodel.alloc_state()
+    bitween_amd.fuse_sibling_linears(qmodel)
+    res = {}
+    for label, bits, glue in (("glue_attention", None, True), ("paged_16_bits", 16, True), ("paged_8_bits", 8, True), ("paged_4_bits", 4, True),
+                              ("paged_16_bits_torch_glue", 16, False)):
+        qmodel.paged = qmodel.glue = None
+        if bits is not None:
+            qmodel.use_paged_cache(bits, 64)
+        if glue:
+            qmodel.use_hip_glue(splits=16)
+        res[label] = {}
+        bd.generate(qmodel, ids, 4)
+        graph = bd.capture_step(qmodel)
+        _, dec_s, toks = bd.generate(qmodel, ids, new_tokens, graph)
+        _, _, toks_eager = bd.generate(qmodel, ids, 32)
+        res[label]["decode_tokens_per_s"] = round((new_tokens - 1) / dec_s, 1)
+        res[label]["graph_tokens_equal_eager_tokens"] = bool(torch.equal(toks[:32], toks_eager))
+        qmodel.pos.fill_(cached)                                      # the cache holds what it held; the time does not depend on it
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(64):
+            graph.replay()
+        torch.cuda.synchronize()
+        res[label]["decode_tokens_per_s_at_3584"] = round(64 / (time.perf_counter() - t0), 1)
+        del graph
+    return res
+
+
 def build_probes():
     """hipcc bench_probes.hip for gfx950 into bench_probes.so next to this file (works without a GPU)."""
     import subprocess
@@ -845,6 +887,7 @@ EXTRAS = {"opt125m_fc1": extras_opt125m_fc1, "decode": extras_decode, "decode_in
           # the heavy sections last: the GEMMs and the 7B model leave the board warm, which shows in the decode timings
           "backward": extras_backward, "llama7b_decoder_graph": extras_llama7b_decoder_graph,
           "transformers_drop_in_check": extras_llama7b_end_to_end}
+ON_REQUEST = {"llama7b_decoder_paged": extras_llama7b_decoder_paged}      # sections that only --only runs
 
 
 def main():
@@ -857,7 +900,7 @@ def main():
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--no-extras", action="store_true")
     ap.add_argument("--no-cpu", action="store_true")
-    ap.add_argument("--only", choices=sorted(EXTRAS), default=None,
+    ap.add_argument("--only", choices=sorted({**EXTRAS, **ON_REQUEST}), default=None,
                     help="run just this section of the extras and print it (used for profiling one kernel)")
     ap.add_argument("--probe", default=None, metavar="K,N,M,BITS,GROUP",
                     help="run only eager decode launches of this one shape over 12 rotating layer copies (one dispatch per "
@@ -919,7 +962,7 @@ def main():
     layers = [[make_layer(torch, QuantizedLinear, k, n, bits, g, seed=100 * li + i)
                for i, (_, k, n) in enumerate(LLAMA7B_LINEARS)] for li in range(args.layers)]
     if args.only:
-        print(json.dumps({args.only: EXTRAS[args.only](torch, hip, QuantizedLinear, layers)}))
+        print(json.dumps({args.only: {**EXTRAS, **ON_REQUEST}[args.only](torch, hip, QuantizedLinear, layers)}))
         return
     xs = {k: torch.randn(m, k, device="cuda", dtype=torch.float16) for k in (4096, 11008)}
     passes = max(1, MODEL_LAYERS // args.layers)           # a step = one token through MODEL_LAYERS decoder layers

@@ -16,6 +16,9 @@ With use_hip_glue() the decode step runs the same arithmetic through five small 
 (bench_decoder_glue.hip: residual add + RMSNorm, rotary + cache write, split attention + combine, SwiGLU) instead
 of about seventeen torch kernels per layer; the prompt always goes through the torch ops.
 
+With use_paged_cache(bits) queries and keys are rotated, cached and attended to by the library's own operators (bitween_amd.rotate_heads and a
+PagedCache of 16, 8 or 4 bits per layer), with or without the glue kernels around them.
+
 Random weights N(0, 0.02) from a seed (no checkpoint can be fetched); the numbers say how fast the path runs,
 not what it generates.
 """
@@ -149,10 +152,22 @@ class Decoder(nn.Module):
         self.norm = nn.Parameter(torch.ones(hidden))
         self.lm_head = nn.Linear(hidden, vocab, bias=False)
         self.glue = None
+        self.paged = None
 
     def use_hip_glue(self, splits=12):
         """Run step() through the HIP glue kernels (head dimension 128, float16 parameters; call after alloc_state)."""
         self.glue = HipGlue(self, splits)
+
+    def use_paged_cache(self, bits=16, group_size=64, page_size=64):
+        """Keep keys and values in a PagedCache per layer instead of self.kv (call after alloc_state; self.paged = None goes back).  The cache
+        lies in pages in an order of its own, the rotary table is float32."""
+        from bitween_amd import PagedCache
+        dev = self.lm_head.weight.device
+        pages = -(-self.max_len // page_size)
+        self.paged = [PagedCache(pages, self.heads, self.head_dim, page_size, bits, group_size, device=dev) for _ in self.layers]
+        self.page_table = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)[None]
+        ang = self._angles()
+        self.cos32, self.sin32 = ang.cos(), ang.sin()
 
     @torch.no_grad()
     def init_weights(self, seed):
@@ -165,14 +180,36 @@ class Decoder(nn.Module):
         """KV cache [layer][k|v][1, heads, max_len, head_dim], rotary table, and the device-side counters."""
         dev = self.lm_head.weight.device
         self.kv = torch.zeros(len(self.layers), 2, 1, self.heads, self.max_len, self.head_dim, dtype=torch.float16, device=dev)
-        half = self.head_dim // 2
-        inv = 1.0 / (10000.0 ** (torch.arange(0, half, device=dev, dtype=torch.float32) / half))
-        ang = torch.arange(self.max_len, device=dev, dtype=torch.float32)[:, None] * inv[None, :]
+        ang = self._angles()
         self.cos, self.sin = ang.cos().to(torch.float16), ang.sin().to(torch.float16)   # [max_len, head_dim / 2]
         self.pos = torch.zeros(1, dtype=torch.int64, device=dev)          # position of the token being fed
         self.tok = torch.zeros(1, 1, dtype=torch.int64, device=dev)       # the token being fed
         self.out = torch.zeros(self.max_len, dtype=torch.int64, device=dev)   # out[p] = token chosen after position p
         self.key_index = torch.arange(self.max_len, device=dev)
+
+    def _angles(self):
+        dev, half = self.lm_head.weight.device, self.head_dim // 2
+        inv = 1.0 / (10000.0 ** (torch.arange(0, half, device=dev, dtype=torch.float32) / half))
+        return torch.arange(self.max_len, device=dev, dtype=torch.float32)[:, None] * inv[None, :]
+
+    def _place(self, pos_index):
+        """Where the tokens at pos_index go in every layer's pages, and how long the sequence is with them."""
+        if self.paged is not None:
+            self._slots = self.paged[0].slots(self.page_table, pos_index, torch.zeros_like(pos_index))
+            self._lengths = (pos_index[-1:] + 1).to(torch.int32)
+
+    def _rotate_and_cache(self, i, q, k, v, pos_index):
+        """q, k, v [T, hidden] -> rotated q, k and v [T, heads, head_dim], the latter two in layer i's pages as well."""
+        from bitween_amd import rotate_heads
+        q, k, v = (x.view(x.shape[0], self.heads, self.head_dim) for x in (q, k, v))
+        q, k = rotate_heads(q, k, self.cos32, self.sin32, pos_index)
+        self.paged[i].write(k, v, self._slots)
+        return q, k, v
+
+    def _attend_paged(self, q, k, v, i):
+        """The attention of a decode step: rotation, cache write and attention, [1, hidden]."""
+        q, _, _ = self._rotate_and_cache(i, q, k, v, self.pos)
+        return self.paged[i].attend(q, self.page_table, self._lengths).view(1, self.hidden)
 
     def _rope(self, qk):
         """qk [T, 2 * heads, head_dim] float16 -> the same with pairs (x_i, x_{i + d/2}) rotated by the angle of the
@@ -192,6 +229,12 @@ class Decoder(nn.Module):
         att = layer.self_attn
         h = F.rms_norm(x, (self.hidden,), layer.input_layernorm, self.eps)
         q, k, v = att.q_proj(h), att.k_proj(h), att.v_proj(h)
+        if self.paged is not None:
+            if causal:
+                o = self._attend_prompt(*self._rotate_and_cache(i, q, k, v, pos_index))
+            else:
+                o = self._attend_paged(q, k, v, i)
+            return self._mlp(layer, x + att.o_proj(o.reshape(t, self.hidden)))
         if (q.untyped_storage().data_ptr() == k.untyped_storage().data_ptr() and q.data_ptr() + 2 * q.shape[-1] == k.data_ptr()
                 and q.stride(0) == k.stride(0)):
             qk = torch.as_strided(q, (t, 2 * self.hidden), (q.stride(0), 1))     # q and k came out of one fused launch
@@ -204,14 +247,20 @@ class Decoder(nn.Module):
         kc.index_copy_(2, pos_index, k.transpose(0, 1)[None])
         vc.index_copy_(2, pos_index, v.transpose(0, 1)[None])
         if causal:                                                       # prefill from an empty cache
-            o = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None],
-                                               is_causal=True)[0].transpose(0, 1)
+            o = self._attend_prompt(q, k, v)
         else:
             # one query row against the whole cache (bias hides the unwritten tail): two small batched products and
             # a softmax - the fused attention kernel takes 45 us for this, these three together about 15
             scores = torch.baddbmm(bias, q.transpose(0, 1), kc[0].transpose(1, 2), alpha=self.head_dim ** -0.5)
             o = torch.bmm(torch.softmax(scores, dim=-1, dtype=torch.float32).to(torch.float16), vc[0]).transpose(0, 1)
-        x = x + att.o_proj(o.reshape(t, self.hidden))
+        return self._mlp(layer, x + att.o_proj(o.reshape(t, self.hidden)))
+
+    @staticmethod
+    def _attend_prompt(q, k, v):
+        return F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None],
+                                              is_causal=True)[0].transpose(0, 1)
+
+    def _mlp(self, layer, x):
         h = F.rms_norm(x, (self.hidden,), layer.post_attention_layernorm, self.eps)
         return x + layer.mlp.down_proj(F.silu(layer.mlp.gate_proj(h)) * layer.mlp.up_proj(h))
 
@@ -221,6 +270,7 @@ class Decoder(nn.Module):
         t = ids.shape[0]
         x = self.embed_tokens(ids)
         pos_index = torch.arange(t, device=ids.device)
+        self._place(pos_index)
         self._cos, self._sin = self.cos[:t, None, :], self.sin[:t, None, :]
         for i, layer in enumerate(self.layers):
             x = self._layer(i, layer, x, pos_index, None, True)
@@ -234,12 +284,13 @@ class Decoder(nn.Module):
         """step() with the glue of a layer in five launches: the residual add of a block is folded into the RMSNorm
         that follows it, the rotary embedding and the cache write into the attention."""
         g = self.glue
+        attend = g.rope_attention if self.paged is None else self._attend_paged
         x = self.embed_tokens(self.tok[0])
         delta = None
         for i, layer in enumerate(self.layers):
             att, mlp = layer.self_attn, layer.mlp
             x, h = g.add_rmsnorm(x, delta, layer.input_layernorm)
-            delta = att.o_proj(g.rope_attention(att.q_proj(h), att.k_proj(h), att.v_proj(h), i))
+            delta = att.o_proj(attend(att.q_proj(h), att.k_proj(h), att.v_proj(h), i))
             x, h = g.add_rmsnorm(x, delta, layer.post_attention_layernorm)
             delta = mlp.down_proj(g.silu_mul(mlp.gate_proj(h), mlp.up_proj(h)))
         _, h = g.add_rmsnorm(x, delta, self.norm)
@@ -249,6 +300,7 @@ class Decoder(nn.Module):
     def step(self):
         """Feed tok at position pos, choose the next token greedily, advance: every tensor it touches is static, so
         the call can be captured once and replayed."""
+        self._place(self.pos)
         if self.glue is not None:
             logits = self._step_hip()
             self.tok.copy_(logits.argmax(-1, keepdim=True))

@@ -261,8 +261,16 @@ class PagedCache:
         return cache_attention(q, page_table, lengths, self.keys, self.values, self.key_meta, self.value_meta, self.bits, self.group_size, scale)
 
     def slots(self, page_table, positions, sequences=None):
-        """The slots (int64) of the tokens at `positions` (int64 [tokens]): of the sequences 0, 1, ... one each, or of `sequences` (int64 [tokens])."""
+        """The slots (int64) of the tokens at `positions` (int64 [tokens]): of the sequences 0, 1, ... one each, or of `sequences` (int64 [tokens]).
+        A position that the table has no page for - a negative one of a padded batch, one behind the last page - has the slot -1: padding."""
         size = self.keys.shape[2]
         if sequences is None:
-            sequences = torch.arange(len(positions), device=positions.device)
-        return page_table[sequences, positions // size].long() * size + positions % size
+            if len(positions) != len(page_table):
+                raise ValueError(f"positions must be [{len(page_table)}], one for each sequence, where no sequences are given")
+            pages = page_table
+        else:
+            pages = page_table[sequences]
+        column = positions // size
+        kept = (column >= 0) & (column < pages.shape[1])
+        page = pages.gather(1, column.clamp(0, pages.shape[1] - 1).long()[:, None])[:, 0].long()
+        return torch.where(kept & (page >= 0) & (page < self.keys.shape[0]), page * size + positions % size, -1)

@@ -190,3 +190,12 @@ def test_errors_on_the_gpu():
             call()
     with torch.no_grad():
         c.attend(q.clone().requires_grad_(True), table, lengths)
+
+
+def test_slots_of_positions_without_a_page_are_padding():
+    c = bw.PagedCache(3, 2, 128, 16, device="cpu")
+    table = torch.tensor([[2, 0], [-1, 3], [1, 1]], dtype=torch.int32)
+    assert c.slots(table, torch.tensor([-1, 3, 32])).tolist() == [-1, -1, -1]
+    assert c.slots(table, torch.tensor([31, 16, 5, 17, 31], dtype=torch.int32), torch.tensor([0, 1, 2, 2, 0])).tolist() == [15, -1, 21, 17, 15]
+    with pytest.raises(ValueError):
+        c.slots(table, torch.tensor([1]))
