@@ -148,7 +148,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 template <int DT, int DP> struct Format16 {
     static constexpr bool kCodes = false, kBf16 = DT == BW_BF16;
     static constexpr int kBits = 16, kPerV = DP / 16;
-    static constexpr int kDim = DP, NK = DP / 32, NV = DP / 16, kGroups = 1, kKeyWords = NK * 4, kValueWords = NV / 2;
+    static constexpr int kDim = DP, NK = DP / 32, NV = DP / 16, kGroups = 1, kKeyWords = NK * 4, kValueWords = NV / 2, kValueLoads = (DP + 127) / 128, kMerge = 1;
     static BW_DEV int k_at(int block, int kg) { return 32 * block + 8 * kg; }
     // 64: 4 neighbouring values (8 bytes) of a lane; 128: 8 (16 bytes); 256: 8 of each half
     static BW_DEV int v_at(int m, int j) { return DP == 64 ? 4 * m + j : (j >> 3) * 128 + 8 * m + (j & 7); }
@@ -159,7 +159,11 @@ template <int BITS, int GROUPS, int GS> struct FormatQ {
     static constexpr int kBits = BITS, kGroup = GS, kGroups = GROUPS, kDim = GROUPS * GS, NK = kDim / 32, NV = kDim / 16;
     static constexpr int kPerK = GS / 32, kPerV = GS / 16;                  // operand blocks and output blocks of a group
     static constexpr int kKeyGroupWords = GS * BITS / 128, kKeyWords = GROUPS * kKeyGroupWords;
-    static constexpr int kValueBytes = kPerV * BITS / 8, kValueGroupWords = kValueBytes > 4 ? kValueBytes / 4 : 1, kValueWords = GROUPS * kValueGroupWords;
+    // A lane's part of a group in a row of V is kValueBytes; parts of less than a word are loaded kMerge groups at a time (see exchanged)
+    static constexpr int kGroupBytes = GS * BITS / 8, kValueBytes = kPerV * BITS / 8, kMerge = kValueBytes < 4 ? 4 / kValueBytes : 1;
+    static constexpr int kValueGroupWords = kValueBytes > 4 ? kValueBytes / 4 : 1, kMerged = GROUPS / kMerge, kValueLoads = kMerged + GROUPS % kMerge, kValueWords = kValueGroupWords * kValueLoads;
+    static constexpr int value_word(int c, int j) { return kMerge == 1 ? c * kValueGroupWords + j * BITS / 32 : c < kMerged * kMerge ? c / kMerge : c - kMerged * (kMerge - 1); }
+    static constexpr int value_code(int c, int j) { return kMerge == 1 ? j % (32 / BITS) : (c < kMerged * kMerge ? c % kMerge * kPerV : 0) + j; }
     static BW_DEV int k_at(int block, int kg) { return (block / kPerK) * GS + kg * (GS / 4) + (block % kPerK) * 8; }
     static BW_DEV int v_at(int m, int j) { return (j / kPerV) * GS + m * kPerV + j % kPerV; }
 };
@@ -228,6 +232,19 @@ template <int L> BW_DEV uint32_t quad_lane(uint32_t v) { return (uint32_t)__buil
 // What the lane N further on (of 16, around) has.
 template <int N> BW_DEV uint32_t lane_after(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x120 + 16 - N, 0xF, 0xF, true); }
 
+// Groups whose part for a lane is 1 or 2 bytes of a row of V: instead of that from each, lane m loads word m / MERGE of group m % MERGE, and the MERGE lanes of
+// one word index exchange their bytes or halves, so that each has its part of every group in one register.
+// 4 bits in groups of 32, 8 heads of 128: 104 against 118 us with 4 queries each (64 sequences of up to 8192 tokens), 67 against 80 with 16 (32 sequences);
+// 8 bits 125 against 122 and 84 against 89.
+template <int MERGE> struct Exchange {
+    uint32_t pairs, quads;                       // byte selectors
+    BW_DEV explicit Exchange(int m) : pairs(m & 1 ? 0x03070105u : 0x06020400u), quads(m & (MERGE / 2) ? 0x03020706u : 0x05040100u) {}
+    BW_DEV uint32_t operator()(uint32_t v) const {
+        if constexpr (MERGE == 4) v = __builtin_amdgcn_perm((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true), v, pairs);
+        return __builtin_amdgcn_perm((uint32_t)__builtin_amdgcn_mov_dpp((int)v, MERGE == 4 ? 0x4E : 0xB1, 0xF, 0xF, true), v, quads);
+    }
+};
+
 // Few queries leave columns of the MFMAs empty, and with them most of what a lane does between the two products: over codes that is more than the
 // unpacking.  With 8 or fewer queries (FOLD 2) or 4 (FOLD 4) they are there 2 or 4 times, and the lanes of each copy ("part" m / (16 / FOLD)) take only
 // their share of the tile's tokens, kTokens = 8 / FOLD instead of 8 each; the weights go back to the first copy's lanes for the second product.
@@ -244,10 +261,11 @@ template <int FOLD> struct Fold {
     BW_DEV int token(int j) const { return FOLD == 1 ? j : FOLD == 2 ? 4 * part + j : 2 * part + j; }          // 4 h + i
     BW_DEV int pair_token(int m) const { return FOLD == 1 ? m & 7 : FOLD == 2 ? 4 * part + (m & 3) : 2 * part + (m & 1); }
     static BW_DEV bool pair_is_value(int m) { return FOLD == 1 ? m & 8 : m & 2; }                              // (FOLD 2: by register)
+    static BW_DEV float select(bool which, float yes, float no) { return which ? yes : no; }      // (its operands are there: no branch)
     template <int J> BW_DEV float pick(const f4* d) const {                                                   // of the products of both halves
         if constexpr (FOLD == 1) return d[J >> 2][J & 3];
-        else if constexpr (FOLD == 2) return high ? d[1][J] : d[0][J];
-        else return high ? (odd ? d[1][2 + J] : d[1][J]) : (odd ? d[0][2 + J] : d[0][J]);
+        if constexpr (FOLD == 2) return select(high, d[1][J], d[0][J]);
+        return select(high, select(odd, d[1][(2 + J) & 3], d[1][J & 3]), select(odd, d[0][(2 + J) & 3], d[0][J & 3]));
     }
     template <int J> static BW_DEV uint32_t key_pair(uint32_t first) {
         if constexpr (FOLD == 1) return row_lane<J>(first);
@@ -306,6 +324,11 @@ template <class F> constexpr bool kPast = F::kDim > 64;
 // Three for heads of 128 leave too few for groups of 32 (175 against 118 us in 4 bits) and won 4 % over groups of 128, nothing in 8 bits.
 constexpr int resident_workgroups(int dim) { return dim > 128 ? 1 : dim > 64 ? 2 : 3; }
 
+// Tiles that a wave has asked for.  Two where the registers hold them: 70 us against 74.5 at 64 sequences of up to 8192 tokens, 8 heads of 128, 4 bits in
+// groups of 128, 100 against 104 in groups of 32; with more of them in registers (8 or more queries) 67 us became 74, and 8 and 16 bits, whose
+// tiles are larger, gain nothing or lose.
+template <class F, int FOLD> constexpr int tiles_ahead = F::kBits == 4 && F::kDim <= 128 && (F::kGroups <= 2 || FOLD == 4) ? 2 : 1;
+
 // What a workgroup has of a segment: tiles from ... to - 1 of `tiles`.
 struct Segment {
     uint32_t b, hq, from, to, tiles, units;      // units: of the piece that it takes
@@ -340,6 +363,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
     using Z = Fold<FOLD>;
     const Z fold(m);
     const int column = m & (Z::kColumns - 1);
+    const Exchange<F::kMerge> exchanged(m);
     const uint32_t per_seq = (uint32_t)(a.kv_heads * a.q_groups);
 
     // the piece of this workgroup: from unit `at` of segment (b, hq) on, `left` units in all
@@ -377,20 +401,24 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
     const int page_mask = (1 << a.page_shift) - 1;
 
     // ---- addresses ----
-    uint32_t key_off[F::kCodes ? F::kGroups : F::NK], value_off[F::kCodes ? F::kGroups : (F::kDim + 127) / 128];
+    uint32_t key_off[F::kCodes ? F::kGroups : F::NK], value_off[F::kValueLoads];
     if constexpr (F::kCodes) {
 #pragma unroll
-        for (int g = 0; g < F::kGroups; g++) {
-            key_off[g] = (uint32_t)(m * a.row_bytes + (g * F::kGroup + kg * (F::kGroup / 4)) * F::kBits / 8);
-            value_off[g] = (uint32_t)(4 * kg * a.row_bytes + g * F::kGroup * F::kBits / 8 + m * F::kValueBytes);
-        }
+        for (int c = 0; c < F::kGroups; c++) key_off[c] = (uint32_t)(m * a.row_bytes + (c * F::kGroup + kg * (F::kGroup / 4)) * F::kBits / 8);
+#pragma unroll
+        for (int w = 0; w < F::kMerged; w++)
+            value_off[w] = (uint32_t)(4 * kg * a.row_bytes + (w * F::kMerge + m % F::kMerge) * F::kGroupBytes + m / F::kMerge * (F::kMerge * F::kValueBytes));
+#pragma unroll
+        for (int w = F::kMerged; w < F::kValueLoads; w++)
+            value_off[w] = (uint32_t)(4 * kg * a.row_bytes + (F::kMerged * (F::kMerge - 1) + w) * F::kGroupBytes + m * F::kValueBytes);
     } else {
 #pragma unroll
         for (int k = 0; k < F::NK; k++) key_off[k] = (uint32_t)(m * a.row_bytes + (F::k_at(k, kg) < a.dim ? 2 * F::k_at(k, kg) : 0));
 #pragma unroll
-        for (int h = 0; h < (F::kDim + 127) / 128; h++) value_off[h] = (uint32_t)(4 * kg * a.row_bytes + (F::v_at(m, 8 * h) < a.dim ? 2 * F::v_at(m, 8 * h) : 0));
+        for (int h = 0; h < F::kValueLoads; h++) value_off[h] = (uint32_t)(4 * kg * a.row_bytes + (F::v_at(m, 8 * h) < a.dim ? 2 * F::v_at(m, 8 * h) : 0));
     }
-    Tile<F> tile;                                                 // the one under way
+    constexpr int kAhead = tiles_ahead<F, FOLD>;
+    Tile<F> ring[kAhead];                                         // the ones under way: asked for, or worked on
     u4 q_raw[F::NK];
     auto halves_of = [&](const Segment& g, uint32_t t) {
         const int at = (int)t * kTile;
@@ -406,7 +434,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
     // where the lane's pairs lie (FOLD 2: the keys'; the values' lie as far from value_meta)
     const int pair_token = fold.pair_token(m);
     const uint32_t* pair_base = (FOLD != 2 && Z::pair_is_value(m) ? a.value_meta : a.key_meta) + 4 * kg + (pair_token & 3);
-    auto load_keys = [&](const Segment& g, uint32_t t) __attribute__((always_inline)) {
+    auto load_keys = [&](Tile<F>& tile, const Segment& g, uint32_t t) __attribute__((always_inline)) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint8_t* base = a.keys + row_of(g, tile.h, t, half) * a.row_bytes;
@@ -433,7 +461,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             }
         }
     };
-    auto load_values = [&](const Segment& g, uint32_t t) __attribute__((always_inline)) {
+    auto load_values = [&](Tile<F>& tile, const Segment& g, uint32_t t) __attribute__((always_inline)) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint8_t* base = a.values + row_of(g, tile.h, t, half) * a.row_bytes;
@@ -443,20 +471,21 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                 uint32_t* out = tile.value[4 * half + i];
                 if constexpr (F::kCodes) {
 #pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) {
-                        const uint8_t* p = row + value_off[c];
-                        if constexpr (F::kValueBytes >= 4) load_words<F::kValueBytes / 4, kPast<F>>(p, out + c * F::kValueGroupWords);
-                        else if constexpr (F::kValueBytes == 2) out[c] = *reinterpret_cast<const uint16_t*>(p);
-                        else out[c] = *p;
+                    for (int w = 0; w < F::kMerged; w++)
+                        load_words<F::kValueGroupWords, kPast<F>>(row + value_off[w], out + w * F::kValueGroupWords);
+#pragma unroll
+                    for (int w = F::kMerged; w < F::kValueLoads; w++) {
+                        if constexpr (F::kValueBytes == 2) out[w] = *reinterpret_cast<const uint16_t*>(row + value_off[w]);
+                        else out[w] = row[value_off[w]];
                     }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < (F::kDim + 127) / 128; k++) load_words<F::kDim == 64 ? 2 : 4, kPast<F>>(row + value_off[k], out + 4 * k);
+                    for (int k = 0; k < F::kValueLoads; k++) load_words<F::kDim == 64 ? 2 : 4, kPast<F>>(row + value_off[k], out + 4 * k);
                 }
             }
         }
     };
-    // A segment's queries and first tile: asked for while the segment before it is put together.
+    // A segment's queries and first tiles: asked for while the segment before it is put together.
     auto begin = [&](const Segment& g) __attribute__((always_inline)) {
         const uint16_t* src = a.q + g.b * a.q_row + (g.q_head + (column < g.queries ? column : 0)) * a.q_head;
 #pragma unroll
@@ -464,10 +493,13 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             const int d = F::k_at(k, kg);
             q_raw[k] = column < g.queries && d < a.dim ? *reinterpret_cast<const u4*>(src + d) : u4{0, 0, 0, 0};
         }
-        if (g.from + wave < g.to) {
-            tile.h = halves_of(g, g.from + wave);
-            load_keys(g, g.from + wave);
-            load_values(g, g.from + wave);
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const uint32_t t = g.from + wave + i * kWaves;
+            if (t >= g.to) break;
+            ring[i].h = halves_of(g, t);
+            load_keys(ring[i], g, t);
+            load_values(ring[i], g, t);
         }
     };
     begin(g);
@@ -534,12 +566,12 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
         for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < F::kGroups; c++) zeros[c] = f4{0.f, 0.f, 0.f, 0.f};
-        for (uint32_t t = g.from + wave; t < to; t += kWaves) {
+        auto step = [&](Tile<F>& tile, const uint32_t t) __attribute__((always_inline)) {
             // The second half of the workgroups shares its CUs with the first, whose waves, being older, go before: 17 against 21 us of a launch's 24.
             // Going first every other tile evens it out (3 % of it).
             __builtin_amdgcn_s_setprio(0);
             if (blockIdx.x >= gridDim.x / 2 && (t / kWaves & 1)) __builtin_amdgcn_s_setprio(1);
-            const uint32_t next = t + kWaves;
+            const uint32_t next = t + kAhead * kWaves;
             const bool more = next < to;
             Halves hn = {};
             if (more) hn = halves_of(g, next);
@@ -601,7 +633,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             }
             if (more) {
                 tile.h = hn;
-                load_keys(g, next);
+                load_keys(tile, g, next);
             }
             // reference: for codes the scores are raised by the exponent of the token's largest value scale
             float unit[Z::kTokens], value_scale[F::kGroups][Z::kTokens];        // 2^-e; scales times that
@@ -653,8 +685,14 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             for (int j = 0; j < Z::kTokens; j++) l = F::kCodes ? __builtin_fmaf(p[j], unit[j], l) : l + p[j];
             // weighted values
             if constexpr (F::kCodes) {
+                if constexpr (F::kMerge > 1) {
 #pragma unroll
-                for (int c = 0; c < F::kGroups; c++) {
+                    for (int w = 0; w < F::kMerged; w++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) tile.value[e][w] = exchanged(tile.value[e][w]);
+                }
+                static_for<0, F::kGroups>([&](auto cc) {
+                    constexpr int c = decltype(cc)::value;
                     float pg[Z::kTokens];
                     uint32_t own_hi[Z::kTokens / 2], own_lo[Z::kTokens / 2];
 #pragma unroll
@@ -670,17 +708,16 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                     static_for<0, 4>([&](auto ic) { z[decltype(ic)::value] = Z::template zero_pair<decltype(ic)::value>(both); });
                     u4 v[F::kPerV];
                     static_for<0, F::kPerV>([&](auto jc) {
-                        constexpr int j = decltype(jc)::value, w = j * F::kBits / 32;
+                        constexpr int j = decltype(jc)::value, w = F::value_word(c, j);
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            v[j][i] = value_codes<F::kBits, j % (32 / F::kBits)>(tile.value[2 * i + 1][c * F::kValueGroupWords + w], tile.value[2 * i][c * F::kValueGroupWords + w]);
+                        for (int i = 0; i < 4; i++) v[j][i] = value_codes<F::kBits, F::value_code(c, j)>(tile.value[2 * i + 1][w], tile.value[2 * i][w]);
                         acc[c * F::kPerV + j] = mfma<false>(v[j], hi, acc[c * F::kPerV + j]);
                     });
                     zeros[c] = mfma<false>(z, hi, zeros[c]);
 #pragma unroll
                     for (int j = 0; j < F::kPerV; j++) acc[c * F::kPerV + j] = mfma<false>(v[j], lo, acc[c * F::kPerV + j]);
                     zeros[c] = mfma<false>(z, lo, zeros[c]);
-                }
+                });
             } else {
                 if (!full) {
 #pragma unroll
@@ -703,7 +740,12 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                     acc[j] = mfma<F::kBf16>(v, lo, acc[j]);
                 });
             }
-            if (more) load_values(g, next);
+            if (more) load_values(tile, g, next);
+        };
+        for (uint32_t t = g.from + wave; t < to; t += kAhead * kWaves) {
+            step(ring[0], t);
+            if constexpr (kAhead == 2)
+                if (t + kWaves < to) step(ring[1], t + kWaves);
         }
         if (more_segments) begin(after);
 
