@@ -139,6 +139,7 @@ def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=
                   [pages, kv_heads, dim / group_size, page_size, 2]: (scale, zero point) of every group of a head's values
 
     Slot n is row n % page_size of page n // page_size; a slot outside the cache is left out (padding).  The slots of one call must differ.
+    k and v may be rows of the cache itself (they are copied first); keys and values must not share memory.
     A group's range includes zero, its scale is rounded up to float16, so that scale * (code - zero point) is within half a scale of the
     value; a group with an infinity or a NaN reads back as NaN.  dim is a multiple of 8 up to 256, page_size a power of two from 16 to 1024,
     group_size 32, 64 or 128."""
@@ -156,6 +157,9 @@ def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=
         raise ValueError("slots must be [tokens], one for every row of k and v")
     _one_gpu(what, keys, k, v, slots)
     _no_grad(what, k, v, keys, values)
+    for a, b in ((keys, values), (key_meta, value_meta)):
+        if a is not None and a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes:
+            raise ValueError(f"{what}: keys and values of a cache that is written must not share memory")
     _taken(what, _native("cache_write")(_hip._plain(k), _hip._plain(v), _whole(slots, "slots", torch.int64),
                                         *_cache_args(keys, values, key_meta, value_meta, bits, group_size)))
 

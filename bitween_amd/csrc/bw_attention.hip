@@ -86,7 +86,7 @@ constexpr int kMinUnits = 4, kWholeTokens = 512;
 Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
     Plan p;
-    p.whole = max_pages * c->page_size <= kWholeTokens && segments < (int64_t)1 << 31;
+    p.whole = max_pages * c->page_size <= kWholeTokens && segments < (int64_t)1 << 24;          // (2^32 threads of a launch)
     p.grid = p.whole ? (uint32_t)segments : (uint32_t)bw_device_cus() * resident_workgroups(c->dim);
     return p;
 }

@@ -540,6 +540,8 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const int ex = top > 0.f && top <= 3.4e38f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
             score_scale = __builtin_ldexpf(a.scale, ex + kUnit<F::kBits>);
+            // (queries beyond 2^120: the largest number keeps scores finite that are, and they are 2^100 apart either way)
+            if (__builtin_isinf(score_scale)) score_scale = __builtin_copysignf(3.4028235e38f, score_scale);
 #pragma unroll
             for (int c = 0; c < F::kGroups; c++) {
                 float sum = 0.f;
@@ -763,7 +765,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
         const bool complete = g.from == 0 && to == g.tiles;
         float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (g.from == 0)) * (2 * kQueries + a.queries * a.dim);
         if (!complete && g.from == 0 && threadIdx.x == 0)         // (the segment ends tiles - to units behind this piece)
-            a.joints[blockIdx.x] = Joint{g.b, g.hq, s.piece_of(position + g.units + g.tiles - to - 1) - blockIdx.x + 1, 0};
+            a.joints[blockIdx.x] = Joint{g.b, g.hq, min(s.piece_of(position + g.units + g.tiles - to - 1), s.pieces - 1) - blockIdx.x + 1, 0};
         auto joined = [&](int query, float& top) {                // sum of the waves' l, relative to the largest r
             top = fmaxf(fmaxf(stats[0][0][query], stats[1][0][query]), fmaxf(stats[2][0][query], stats[3][0][query]));
             float sum = 0.f;

@@ -205,6 +205,12 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
     }
 }
 
+// Two pieces of memory of `bytes` that share some.
+bool overlap(const void* a, const void* b, int64_t bytes) {
+    const int64_t apart = (int64_t)((const char*)a - (const char*)b);
+    return apart < bytes && apart > -bytes;
+}
+
 CacheArgs args_of(const bw_cache* c, int values) {
     CacheArgs a{};
     a.keys = (uint8_t*)c->keys;
@@ -270,6 +276,8 @@ extern "C" int bw_cache_write(const bw_cache* c, int act_dtype, int64_t T, const
     if ((act_dtype != BW_F16 && act_dtype != BW_BF16) || (c->bits == 16 && act_dtype != c->dtype)) return BW_EUNSUPPORTED;
     if (T == 0) return BW_OK;
     if (!bw_aligned(k, 16) || !bw_aligned(v, 16) || !bw_aligned(slots, 8) || (k_row | k_head | v_row | v_head) % 8) return BW_EALIGN;
+    const int64_t values = c->pages * c->page_size * c->kv_heads * c->dim;
+    if (overlap(c->keys, c->values, values / 8 * c->bits) || (c->bits != 16 && overlap(c->key_meta, c->value_meta, values / c->group * 4))) return BW_EINVAL;
     CacheArgs a = args_of(c, c->bits == 16 ? kWriteValues<16> : kWriteValues<8>);
     a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
     a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;

@@ -639,12 +639,13 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         Rotation r;
         if (!rotation_of(q, k, cos, sin, positions, qw, kw, eps, r)) return none();
         bool recorded = false;
+        for (const Tensor* t : {&q, &k, &qw, &kw}) {
+            if (!t->defined()) continue;
+            recorded |= t->requires_grad();
+            TORCH_CHECK(!t->_fw_grad(0).defined(), "rotate_heads has no forward-mode derivative");
+        }
+        recorded &= c10::GradMode::is_enabled();
         if (c10::GradMode::is_enabled()) {
-            for (const Tensor* t : {&q, &k, &qw, &kw}) {
-                if (!t->defined()) continue;
-                recorded |= t->requires_grad();
-                TORCH_CHECK(!t->_fw_grad(0).defined(), "rotate_heads has no forward-mode derivative");
-            }
             if (cos.requires_grad() || sin.requires_grad()) return none();
         }
         if (recorded) check_capture({&q, &k, &qw, &kw}, q.device().index());
@@ -722,6 +723,12 @@ bool slots_of(PyObject* o, const Tensor& like, Tensor& slots) {
     return on_gpu(slots, like) && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous();
 }
 
+// Two contiguous tensors of one size that share memory.
+inline bool overlap(const Tensor& a, const Tensor& b) {
+    const auto *x = (const char*)a.const_data_ptr(), *y = (const char*)b.const_data_ptr();
+    return x < y + b.nbytes() && y < x + a.nbytes();
+}
+
 inline bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 
 // cache_write(k, v, slots, keys, values, key_meta, value_meta, bits, group_size) -> True or None
@@ -733,13 +740,13 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (PyErr_Occurred()) return nullptr;
             return none();
         }
-        const Tensor k = unpack(args[0]), v = unpack(args[1]);
+        Tensor k = unpack(args[0]), v = unpack(args[1]);
         for (const Tensor* t : {&k, &v})
             if (!on_gpu(*t, h.keys) || !half_type(t->scalar_type()) || t->dim() != 3 || t->size(0) != slots.size(0) || t->size(1) != h.c.kv_heads ||
                 t->size(2) != h.c.dim || wants_grad(*t))
                 return none();
         if (k.scalar_type() != v.scalar_type() || (h.c.bits == 16 && k.scalar_type() != h.keys.scalar_type())) return none();
-        if (wants_grad(h.keys) || wants_grad(h.values)) return none();
+        if (wants_grad(h.keys) || wants_grad(h.values) || overlap(h.keys, h.values) || (h.key_meta.defined() && overlap(h.key_meta, h.value_meta))) return none();
         int status = 0;
         {
             Unlocked unlocked;
@@ -749,6 +756,8 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             const int64_t tokens = slots.size(0);
             if (tokens > 0) {
                 OnDevice on(k.device());
+                for (Tensor* t : {&k, &v})                      // rows of this very cache: they may be written before they are read
+                    if (t->is_alias_of(h.keys) || t->is_alias_of(h.values)) *t = t->clone();
                 const Rows rk(k, tokens), rv(v, tokens);
                 status = lib.cache_write(&h.c, dtype_code(k.scalar_type()), tokens, rk.data, rk.row, rk.head, rv.data, rv.row, rv.head,
                                          (const int64_t*)slots.const_data_ptr(), stream_of(k.device().index()));

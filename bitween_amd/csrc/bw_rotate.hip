@@ -278,20 +278,22 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(const float* partial, 
     }
 }
 
+// Values of a chunk: 8, where whole 16-byte chunks fill the rotated halves and what lies behind them.
+int chunk_of(const bw_heads* h) { return h->dim % 16 == 0 && h->rotary % 16 == 0 ? 8 : 4; }
+
 int heads_check(const bw_heads* h, int act_dtype) {
     if (!h || h->tokens < 0 || h->q_heads < 1 || h->k_heads < 1 || h->dim < 1 || h->rotary < 1 || h->rotary > h->dim || h->table_rows < 1) return BW_EINVAL;
     if (h->tokens > 0 && (!h->cos || !h->sin || !h->positions)) return BW_EINVAL;
     if (act_dtype != BW_F16 && act_dtype != BW_BF16) return BW_EUNSUPPORTED;
     if ((h->q_weight || h->k_weight) && h->weight_dtype != act_dtype && h->weight_dtype != BW_F32) return BW_EUNSUPPORTED;
     if (h->dim % 8 || h->rotary % 8 || h->dim > kMaxDim) return BW_EUNSUPPORTED;
-    if (h->tokens * ((int64_t)h->q_heads + h->k_heads) >= (int64_t)1 << 31 || h->q_heads > 65535 || h->k_heads > 65535) return BW_EUNSUPPORTED;
+    if (h->q_heads > 65535 || h->k_heads > 65535 || h->tokens >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    const int64_t items = h->tokens * ((int64_t)h->q_heads + h->k_heads);
+    if (items >= (int64_t)1 << 31 || items << bw_log2(h->dim / (2 * chunk_of(h))) >= (int64_t)1 << 32) return BW_EUNSUPPORTED;   // threads of a launch
     if (!bw_aligned(h->cos, 16) || !bw_aligned(h->sin, 16) || !bw_aligned(h->positions, 8) || !bw_aligned(h->q_weight, 16) || !bw_aligned(h->k_weight, 16))
         return BW_EALIGN;
     return BW_OK;
 }
-
-// Values of a chunk: 8, where whole 16-byte chunks fill the rotated halves and what lies behind them.
-int chunk_of(const bw_heads* h) { return h->dim % 16 == 0 && h->rotary % 16 == 0 ? 8 : 4; }
 
 RotateArgs args_of(const bw_heads* h) {
     RotateArgs a = {};

@@ -231,7 +231,8 @@ int bw_qdgrad(const void* grad_y, int act_dtype, int64_t M, int64_t N, int64_t l
  *   q, k           act_dtype (BW_F16 | BW_BF16); a token's row `*_row` elements apart, a head `*_head` apart, a head's values adjacent
  *   q_weight, k_weight  [D] of weight_dtype (act_dtype or BW_F32) or NULL, each for itself
  *   q_out, k_out   act_dtype, contiguous
- * D a multiple of 8 up to 256, rotary a multiple of 8 up to D, rows, heads and pointers aligned to 16 bytes (positions to 8). */
+ * D a multiple of 8 up to 256, rotary a multiple of 8 up to D, rows, heads and pointers aligned to 16 bytes (positions to 8); fewer than
+ * 2^31 heads in all, and of 2^36 values. */
 typedef struct bw_heads {
     int64_t tokens;
     int q_heads, k_heads, dim, rotary;
@@ -276,7 +277,8 @@ typedef struct bw_cache {
  *   clipped to 0 ... 2^bits - 1
  * so that scale * (code - zero point) is within half a scale of x (of a finite x within 65504 scales).  A group that holds an infinity or
  * a NaN gets a NaN scale: it reads back as NaN.
- *   k, v  act_dtype (BW_F16 | BW_BF16, the cache's dtype at 16 bits), strided like q of bw_rotate_heads */
+ *   k, v  act_dtype (BW_F16 | BW_BF16, the cache's dtype at 16 bits), strided like q of bw_rotate_heads, no part of the cache
+ * Keys and values that share memory (or their pairs) are refused with BW_EINVAL. */
 int bw_cache_write(const bw_cache* cache, int act_dtype, int64_t T, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                    int64_t v_head, const int64_t* slots, void* stream);
 

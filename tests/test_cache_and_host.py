@@ -55,6 +55,14 @@ def test_cache_entry_points_check_their_arguments():
     assert lib.bw_cache_read(c, 0, 1, P, P + 2, P, None) == EALIGN
 
 
+def test_keys_and_values_that_share_memory_are_not_written():
+    lib = hip_loader.load()
+    size = 4 * 2 * 16 * 64                                       # bytes of keys or values at 8 bits
+    for fields in (dict(), dict(values=P + size), dict(values=P + size - 16, value_meta=P + size), dict(values=P - size + 16, value_meta=P + size),
+                   dict(values=P + size, value_meta=P + size // 32 * 4 - 16), dict(bits=16, values=P + 2 * size - 16)):
+        assert lib.bw_cache_write(_cache(**fields), 0, 1, P, 128, 64, P, 128, 64, P, None) == EINVAL
+
+
 def test_attention_entry_point_checks_its_arguments():
     lib, c, c16 = hip_loader.load(), _cache(), _cache(bits=16, dtype=1)
     ok = [c, 0, P, 1, 2, 128, 64, P, 4, 4, P, 1.0, P, P, 1 << 30, None]
@@ -97,7 +105,8 @@ def test_rotation_entry_points_check_their_arguments():
             assert call(heads(**{field: None})) == EINVAL
         assert call(heads(rotary=72)) == EINVAL
         assert call(heads(), act=2) == EUNSUPPORTED and call(heads(weight_dtype=1)) == EUNSUPPORTED
-        for fields in (dict(dim=68, rotary=64), dict(rotary=60), dict(dim=264), dict(tokens=1 << 40), dict(q_heads=70000)):
+        for fields in (dict(dim=68, rotary=64), dict(rotary=60), dict(dim=264), dict(tokens=1 << 40), dict(q_heads=70000), dict(tokens=1 << 29),
+                       dict(tokens=1 << 31)):
             assert call(heads(**fields)) == EUNSUPPORTED
         assert call(heads(cos=P + 4)) == EALIGN and call(heads(positions=P + 4)) == EALIGN and call(heads(q_weight=P + 2)) == EALIGN
         assert call(heads(), out=None) == EINVAL and call(heads(), out=P + 2) == EALIGN and call(heads(), row=100) == EALIGN

@@ -27,6 +27,16 @@ def test_odd_heads_at_16_bits(dim, dtype):
     b.check(b.attend())
 
 
+@pytest.mark.parametrize("bits,dtype", [(8, torch.bfloat16), (4, torch.float16)])
+@pytest.mark.parametrize("share", [3, 7, 12])
+@pytest.mark.parametrize("group,groups", [(32, n) for n in range(1, 9)] + [(64, n) for n in range(1, 5)] + [(128, 1), (128, 2)])
+def test_every_number_of_groups_with_few_and_many_queries(group, groups, share, bits, dtype):
+    b = Batch([1, 20, 33, 0, 450, 1300], 2 * share, 2, group * groups, 32, bits, group, dtype, seed=group + groups)
+    b.check(b.attend())
+    b = Batch([70, 511], 2 * share, 2, group * groups, 64, bits, group, dtype, seed=groups)
+    b.check(b.attend())
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 512, 1024])
 @pytest.mark.parametrize("bits,group,dtype", [(16, 0, torch.float16), (8, 64, torch.float16), (4, 32, torch.bfloat16)])
 def test_pages(page, bits, group, dtype):
@@ -215,3 +225,55 @@ def test_a_decode_loop(bits, group, dtype):
         holder.q = q
         holder.slots = [cache.slots(table, torch.arange(int(n), device="cuda"), torch.full((int(n),), b, device="cuda")) for b, n in enumerate(lengths)]
         holder.check(out)
+
+
+@pytest.mark.parametrize("bits,group", [(8, 64), (4, 128)])
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** 118, 2.0 ** 121, 2.0 ** -100, 2.0 ** -130])
+def test_queries_at_the_ends_of_bfloat16(size, bits, group):
+    """Over codes the queries' exponent is taken out and put back into the scores: at the upper end one token has all the weight (scores 2^90 and
+    more apart), at the lower end every token has the same."""
+    b = Batch([70, 700], 4, 2, 128, 32, bits, group, torch.bfloat16, seed=3)
+    b.q = (b.q.float() * size).to(torch.bfloat16)
+    b.check(b.attend())
+
+
+@pytest.mark.parametrize("bits,group,dtype", [(16, 0, torch.float16), (8, 64, torch.bfloat16), (4, 32, torch.float16)])
+def test_a_padded_step_is_the_step_of_its_sequences(bits, group, dtype):
+    """Rotation, write and attention of a batch whose idle rows have position -1, length 0 and a table of anything, captured once and replayed: the
+    sequences get what they get alone, idle rows zeros, and the cache nothing of theirs."""
+    heads, kv, dim, page = 8, 2, 128, 32
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    caches = [bw.PagedCache(12, kv, dim, page, bits, group or 64, dtype) for _ in range(2)]
+    angle = torch.arange(100, device="cuda", dtype=torch.float32)[:, None] / 10000.0 ** (torch.arange(64, device="cuda", dtype=torch.float32) / 64)
+    cos, sin = angle.cos(), angle.sin()
+    table = torch.tensor([[3, 1, 9], [0, 0, 0], [7, 4, 2], [-5, 2 ** 30, 3]], dtype=torch.int32, device="cuda")
+    active = torch.tensor([0, 2], device="cuda")
+    lengths, positions = torch.tensor([31, 0, 64, 0], dtype=torch.int32, device="cuda"), torch.tensor([30, -1, 63, -1], device="cuda")
+    for b in (0, 2):
+        n = int(positions[b])
+        x = torch.randn(n, 2 * kv, dim, device="cuda", generator=gen).to(dtype)
+        for cache in caches:
+            cache.write(x[:, :kv], x[:, kv:], cache.slots(table, torch.arange(n, device="cuda"), torch.full((n,), b, device="cuda")))
+    qkv = torch.zeros(4, heads + 2 * kv, dim, device="cuda", dtype=dtype)
+
+    def step(cache, qkv, positions, table, lengths):
+        q, k = bw.rotate_heads(qkv[:, :heads], qkv[:, heads:heads + kv], cos, sin, positions)
+        cache.write(k, qkv[:, heads + kv:], cache.slots(table, positions))
+        return cache.attend(q, table, lengths)
+
+    step(caches[0], qkv, positions, table, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(caches[0], qkv, positions, table, lengths)
+    for _ in range(4):
+        qkv.copy_(torch.randn(qkv.shape, device="cuda", generator=gen))
+        qkv[1::2] = float("nan")
+        graph.replay()
+        want = step(caches[1], qkv[active], positions[active], table[active], lengths[active])
+        assert torch.equal(out[active], want) and not out[1::2].any()
+        for a, b in zip((getattr(c, name) for c in caches[:1] for name in ("keys", "values", "key_meta", "value_meta")),
+                        (getattr(c, name) for c in caches[1:] for name in ("keys", "values", "key_meta", "value_meta"))):
+            assert a is None and b is None or torch.equal(a, b)
+        positions += (positions >= 0).long()
+        lengths += (lengths > 0).int()

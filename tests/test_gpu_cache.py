@@ -215,3 +215,28 @@ def test_rows_behind_four_gibibytes(bits, group):
     if bits != 16:
         at = torch.arange(20, device="cuda")
         _check_read(c, at, bw.read_cache(at, c.keys, c.values, c.key_meta, c.value_meta, bits, group)[0], c.keys, c.key_meta)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rows_of_the_cache_itself_may_be_written(dtype):
+    """Every row of a page one row further on, and pages the other way round: what is read is what was there before the call."""
+    c = _cache(4, 2, 64, 1024, 16, 0, dtype)
+    c.keys.copy_(torch.randn(c.keys.shape, device="cuda"))
+    c.values.copy_(torch.randn(c.values.shape, device="cuda"))
+    k, v = c.keys.clone(), c.values.clone()
+    c.write(c.keys[1].transpose(0, 1)[:1023], c.values[1].transpose(0, 1)[:1023], torch.arange(1025, 2048, device="cuda"))
+    for got, was in ((c.keys, k), (c.values, v)):
+        assert torch.equal(got[1, :, 1:], was[1, :, :1023]) and torch.equal(got[1, :, 0], was[1, :, 0])
+        assert torch.equal(got[[0, 2, 3]], was[[0, 2, 3]])
+
+
+def test_keys_and_values_in_one_place_are_refused():
+    c = _cache(2, 2, 64, 16, 8, 64, torch.float16)
+    x, slots = torch.randn(3, 2, 64, device="cuda").half(), torch.arange(3, device="cuda")
+    before = c.keys.clone()
+    with pytest.raises(ValueError):
+        bw.write_cache(x, x, slots, c.keys, c.keys, c.key_meta, c.value_meta, 8, 64)
+    with pytest.raises(ValueError):
+        bw.write_cache(x, x, slots, c.keys, c.values, c.key_meta, c.key_meta, 8, 64)
+    assert torch.equal(c.keys, before)
+    bw.read_cache(slots, c.keys, c.keys, c.key_meta, c.key_meta, 8, 64)                 # reading is as good

@@ -243,3 +243,14 @@ def test_another_stream():
         got = bw.rotate_heads(q, k, cos, sin, pos, *w)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+    q, k, cos, sin, pos, _ = _inputs(5, 2, 1, 64, 64, torch.float16, [(0, 0), (0, 0)])
+    with fwad.dual_level():
+        dual = fwad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(RuntimeError):
+            bw.rotate_heads(dual, k, cos, sin, pos)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            bw.rotate_heads(dual, k, cos, sin, pos)
