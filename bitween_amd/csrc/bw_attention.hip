@@ -7,12 +7,14 @@
 namespace {
 
 // One workgroup for 128 values of the output [queries][dim] of the segment that piece blockIdx.x / chunks began and left unfinished, if it did: 32
-// threads of 4 values each, 8 such rows that share the parts, four parts of a thread under way at a time.  What bounds it is the way to
-// memory and back twice (the joint, the parts), not its work.
-constexpr int kJoinValues = 128, kJoinRows = 8, kJoinAhead = 4;
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, int chunks) {
-    __shared__ float tops[kJoinRows][32], sums[kJoinRows][32];
-    __shared__ f4 outs[kJoinRows][32];
+// threads of 4 values each, ROWS such rows that share the parts, four parts of a thread under way at a time.  What bounds it is the way to
+// memory and back twice (the joint, the parts) and the number of threads that are launched to find nothing: two rows unless segments are so few that
+// each has 8 pieces and more (16 sequences of 1024, 8 heads of 128: 24.0 us with two, 24.8 with 8, 27 with 16; one sequence of 65537: 31.6, 26.6, 26.2).
+constexpr int kJoinValues = 128, kJoinAhead = 4, kManyParts = 8;
+template <int ROWS>
+__global__ __launch_bounds__(32 * ROWS) void attention_join_kernel(AttentionArgs a, int chunks) {
+    __shared__ float tops[ROWS][32], sums[ROWS][32];
+    __shared__ f4 outs[ROWS][32];
     const uint32_t w0 = blockIdx.x / (uint32_t)chunks, chunk = blockIdx.x - w0 * chunks;
     const Joint joint = a.joints[w0];
     if (joint.parts == 0) return;
@@ -26,12 +28,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
     float top = -INFINITY, sum = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
     if (live) {
-        for (uint32_t w = w0 + y; w <= w1; w += kJoinAhead * kJoinRows) {
+        for (uint32_t w = w0 + y; w <= w1; w += kJoinAhead * ROWS) {
             float r[kJoinAhead], l[kJoinAhead];
             f4 v[kJoinAhead];
 #pragma unroll
             for (int i = 0; i < kJoinAhead; i++) {
-                const uint32_t part = w + i * kJoinRows;
+                const uint32_t part = w + i * ROWS;
                 const float* p = a.partial + (2 * (int64_t)(part <= w1 ? part : w) + (part == w0)) * pitch;
                 r[i] = part <= w1 ? p[query] : -INFINITY;
                 l[i] = p[kQueries + query];
@@ -46,7 +48,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
             o *= keep;
 #pragma unroll
             for (int i = 0; i < kJoinAhead; i++) {
-                if (w + i * kJoinRows > w1) break;
+                if (w + i * ROWS > w1) break;
                 const float f = r[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[i] - top);
                 sum += f * l[i];
                 o += f * v[i];
@@ -59,11 +61,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a, in
     __syncthreads();
     if (y || !live) return;
 #pragma unroll
-    for (int i = 1; i < kJoinRows; i++) top = fmaxf(top, tops[i][x]);
+    for (int i = 1; i < ROWS; i++) top = fmaxf(top, tops[i][x]);
     o = f4{0.f, 0.f, 0.f, 0.f};
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoinRows; i++) {
+    for (int i = 0; i < ROWS; i++) {
         const float f = tops[i][x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(tops[i][x] - top);
         sum += f * sums[i][x];
         o += f * outs[i][x];
@@ -154,7 +156,8 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     if (!plan.whole) {
         const int chunks = (a.queries * a.dim + kJoinValues - 1) / kJoinValues;
-        hipLaunchKernelGGL(attention_join_kernel, dim3(plan.grid * chunks), dim3(256), 0, st, a, chunks);
+        if ((int64_t)plan.grid >= kManyParts * B * c->kv_heads * a.q_groups) hipLaunchKernelGGL(attention_join_kernel<8>, dim3(plan.grid * chunks), dim3(256), 0, st, a, chunks);
+        else hipLaunchKernelGGL(attention_join_kernel<2>, dim3(plan.grid * chunks), dim3(64), 0, st, a, chunks);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;
