@@ -84,12 +84,15 @@ int attention_check(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages
 
 // Workgroups, and whether every segment gets one of its own.
 struct Plan { uint32_t grid; bool whole; };
-constexpr int kMinUnits = 4, kWholeTokens = 512;
+constexpr int kWholeTokens = 512;
 Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
     Plan p;
     p.whole = max_pages * c->page_size <= kWholeTokens && segments < (int64_t)1 << 24;          // (2^32 threads of a launch)
-    p.grid = p.whole ? (uint32_t)segments : (uint32_t)bw_device_cus() * resident_workgroups(c->dim);
+    // (no more than there can be pieces: workgroups that find nothing cost their launch)
+    const int64_t resident = (int64_t)bw_device_cus() * resident_workgroups(c->dim);
+    const int64_t pieces = (segments * ((max_pages * c->page_size + kTile - 1) / kTile + kSegmentCost) + kWaves - 1) / kWaves;
+    p.grid = (uint32_t)(p.whole ? segments : resident < pieces ? resident : pieces);
     return p;
 }
 
@@ -138,7 +141,7 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     a.page_shift = bw_log2(c->page_size);
     a.max_tokens = (int)(max_pages * c->page_size);
     a.q_bf16 = act_dtype == BW_BF16;
-    a.min_units = kMinUnits;
+    a.cus = bw_device_cus();
     a.whole = plan.whole;
     a.scale = scale * 1.44269504088896340736f;
     const hipStream_t st = (hipStream_t)stream;

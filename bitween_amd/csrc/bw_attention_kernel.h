@@ -33,6 +33,7 @@
 
 constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
 constexpr uint32_t kSegmentCost = 8;             // tiles
+constexpr uint32_t kManyUnits = 16;              // see split_of
 constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
 
 // A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
@@ -51,7 +52,7 @@ struct AttentionArgs {
     int64_t page_bytes, meta_words;              // of one head in one page: row bytes * page_size; pairs
     uint32_t pages;
     int B, q_heads, kv_heads, share, queries, q_groups;   // queries: of a segment, at most 16; q_groups: segments of a key-value head
-    int dim, row_bytes, page_shift, max_tokens, q_bf16, min_units, whole;
+    int dim, row_bytes, page_shift, max_tokens, q_bf16, cus, whole;
     float scale;                                 // times log2 e
 };
 
@@ -72,8 +73,13 @@ struct Split {
         return unit < head ? unit / (size + 1) : longer + (unit - head) / size;
     }
 };
+// Less than kManyUnits for every workgroup that can be resident: one piece for a CU at most, of so many units that its waves have equally many.
+// Smaller ones cost more in parts to join, and a second piece on some of the CUs is waited for by all.  8 sequences of 8192, 16 queries of one head of
+// 128: 14.8 us in 176 pieces against 17.8 in 512; 4 of 1024, 8 heads with 8 queries: 11.4 in 160, 12.9 in 256 of 5 units; 16 of 1024, 8 heads with 16
+// queries in 4 bits: 17.1 in 256, 18.6 in 512.
 BW_DEV Split split_of(const AttentionArgs& a, uint32_t units, uint32_t grid) {
-    const uint32_t total = units * (uint32_t)(a.kv_heads * a.q_groups), pieces = (total + a.min_units - 1) / (uint32_t)a.min_units;
+    const uint32_t total = units * (uint32_t)(a.kv_heads * a.q_groups), round = (uint32_t)(a.cus * kWaves);
+    const uint32_t size = (total + round - 1) / round * kWaves, pieces = total >= grid * kManyUnits ? grid : size ? (total + size - 1) / size : 0;
     Split s = {};
     s.pieces = pieces < grid ? pieces : grid;
     s.size = s.pieces ? total / s.pieces : 0;
