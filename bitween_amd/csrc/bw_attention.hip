@@ -82,16 +82,19 @@ int attention_check(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages
     return BW_OK;
 }
 
-// Workgroups, and whether every segment gets one of its own.
+// Workgroups, and whether every segment gets one of its own: nothing to cut, nothing to join.  With room for 512 tokens to a sequence always (128
+// sequences of 12 heads of 64: 15.3 us against 20.0), with room for 1024 where there are segments for half the CUs at least (64 sequences of up to
+// 1000, 8 heads of 128 in 4 bits: 16.6 against 22.4; 4 such sequences: 15.2 against 10.1), beyond never (32 of up to 2000 in 8 bits: 28.7 against 22.0).
 struct Plan { uint32_t grid; bool whole; };
-constexpr int kWholeTokens = 512;
+constexpr int kWholeTokens = 512, kWholeMany = 1024;
 Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
-    const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries);
+    const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries), tokens = max_pages * c->page_size;
+    const int cus = bw_device_cus();
     Plan p;
-    p.whole = max_pages * c->page_size <= kWholeTokens && segments < (int64_t)1 << 24;          // (2^32 threads of a launch)
+    p.whole = tokens <= (2 * segments >= cus ? kWholeMany : kWholeTokens) && segments < (int64_t)1 << 24;          // (2^32 threads of a launch)
     // (no more than there can be pieces: workgroups that find nothing cost their launch)
-    const int64_t resident = (int64_t)bw_device_cus() * resident_workgroups(c->dim);
-    const int64_t pieces = (segments * ((max_pages * c->page_size + kTile - 1) / kTile + kSegmentCost) + kWaves - 1) / kWaves;
+    const int64_t resident = (int64_t)cus * resident_workgroups(c->dim);
+    const int64_t pieces = (segments * ((tokens + kTile - 1) / kTile + kSegmentCost) + kWaves - 1) / kWaves;
     p.grid = (uint32_t)(p.whole ? segments : resident < pieces ? resident : pieces);
     return p;
 }

@@ -32,7 +32,9 @@
 #include "bw_cache.h"
 
 constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
-constexpr uint32_t kSegmentCost = 8;             // tiles
+// Tiles that beginning and joining a segment is worth: with 2 the pieces of many short segments are waited for (32 sequences of up to 1000 tokens, 8 heads of
+// 128 in 8 bits: 29.4 us; 5: 23.7; 8 and 12: 20.4), with 12 the long ones (64 of up to 8192 in 16 bits: 166.4 against 165.2 with 8 and 163.3 with 2).
+constexpr uint32_t kSegmentCost = 8;
 constexpr uint32_t kManyUnits = 16;              // see split_of
 constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
 
@@ -576,7 +578,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
         for (int c = 0; c < F::kGroups; c++) zeros[c] = f4{0.f, 0.f, 0.f, 0.f};
         auto step = [&](Tile<F>& tile, const uint32_t t) __attribute__((always_inline)) {
             // The second half of the workgroups shares its CUs with the first, whose waves, being older, go before: 17 against 21 us of a launch's 24.
-            // Going first every other tile evens it out (3 % of it).
+            // Going first every other tile evens it out (48 sequences of up to 8192 tokens, 8 heads of 128 in 8 bits: 46.2 against 47.4 us).
             __builtin_amdgcn_s_setprio(0);
             if (blockIdx.x >= gridDim.x / 2 && (t / kWaves & 1)) __builtin_amdgcn_s_setprio(1);
             const uint32_t next = t + kAhead * kWaves;

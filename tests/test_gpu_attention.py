@@ -51,6 +51,15 @@ def test_lengths(lengths, bits, group):
     b.check(b.attend())
 
 
+@pytest.mark.parametrize("room", [513, 1000, 1024, 1025])
+@pytest.mark.parametrize("bits,group,dtype", [(16, 0, torch.float16), (8, 128, torch.bfloat16), (4, 64, torch.float16)])
+def test_many_sequences_with_room_for_about_1024(room, bits, group, dtype):
+    b = Batch([room] + [(37 * i) % 1000 for i in range(35)], 8, 4, 128, 16, bits, group or 64, dtype, seed=room)
+    b.check(b.attend())
+    b = Batch([5, room, 0, 200], 8, 4, 128, 16, bits, group or 64, dtype, seed=room + 1)
+    b.check(b.attend())
+
+
 @pytest.mark.parametrize("bits,group,dtype", [(16, 0, torch.bfloat16), (4, 128, torch.float16), (8, 64, torch.float16)])
 def test_one_long_sequence(bits, group, dtype):
     b = Batch([100003], 32, 8, 128, 64, bits, group or 64, dtype, seed=1)
