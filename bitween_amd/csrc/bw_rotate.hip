@@ -250,27 +250,35 @@ __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
     }
 }
 
-// dw = the sum of its blocks' rows: one workgroup for 32 columns of a weight, 32 rows at a time, four of a thread under way
+// dw = the sum of its blocks' rows: one workgroup for 32 columns of a weight, 128 rows at a time, four of a thread under way (32 rows at a time: 4.9 us
+// for 819 and 205 rows).
 template <int DT>
-__global__ __launch_bounds__(256) void weight_grad_kernel(const float* partial, int dim, int q_blocks, int blocks, void* q_grad, void* k_grad, int f32) {
-    __shared__ f4 sums[32][8];
+__global__ __launch_bounds__(1024) void weight_grad_kernel(const float* partial, int dim, int q_blocks, int blocks, void* q_grad, void* k_grad, int f32) {
+    __shared__ f4 sums[128][8];
     const bool is_k = blockIdx.y == 1;
     void* out = is_k ? k_grad : q_grad;
     if (!out) return;
     const int to = is_k ? blocks : q_blocks, x = (int)threadIdx.x & 7, y = (int)threadIdx.x >> 3, d = (int)blockIdx.x * 32 + 4 * x;
     f4 s = {0.f, 0.f, 0.f, 0.f};
     if (d < dim)
-        for (int b = (is_k ? q_blocks : 0) + y; b < to; b += 128) {
+        for (int b = (is_k ? q_blocks : 0) + y; b < to; b += 512) {
             f4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = b + 32 * i < to ? *reinterpret_cast<const f4*>(partial + (int64_t)(b + 32 * i) * dim + d) : f4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4; i++) v[i] = b + 128 * i < to ? *reinterpret_cast<const f4*>(partial + (int64_t)(b + 128 * i) * dim + d) : f4{0.f, 0.f, 0.f, 0.f};
             s += (v[0] + v[1]) + (v[2] + v[3]);
         }
     sums[y][x] = s;
     __syncthreads();
+    if (y < 8) {
+#pragma unroll
+        for (int i = 1; i < 16; i++) s += sums[y + 8 * i][x];
+    }
+    __syncthreads();
+    if (y < 8) sums[y][x] = s;
+    __syncthreads();
     if (y || d >= dim) return;
 #pragma unroll
-    for (int i = 1; i < 32; i++) s += sums[i][x];
+    for (int i = 1; i < 8; i++) s += sums[i][x];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if (f32) ((float*)out)[d + j] = s[j];
@@ -382,9 +390,9 @@ extern "C" int bw_rotate_heads_grad(const bw_heads* h, int act_dtype, const void
     }
     if (sums) {                                               // (without tokens: zeros)
         if (act_dtype == BW_F16)
-            hipLaunchKernelGGL(weight_grad_kernel<BW_F16>, dim3((h->dim + 31) / 32, 2), dim3(256), 0, (hipStream_t)stream, a.partial, h->dim, a.q_blocks, blocks, q_weight_grad, k_weight_grad, a.weight_f32);
+            hipLaunchKernelGGL(weight_grad_kernel<BW_F16>, dim3((h->dim + 31) / 32, 2), dim3(1024), 0, (hipStream_t)stream, a.partial, h->dim, a.q_blocks, blocks, q_weight_grad, k_weight_grad, a.weight_f32);
         else
-            hipLaunchKernelGGL(weight_grad_kernel<BW_BF16>, dim3((h->dim + 31) / 32, 2), dim3(256), 0, (hipStream_t)stream, a.partial, h->dim, a.q_blocks, blocks, q_weight_grad, k_weight_grad, a.weight_f32);
+            hipLaunchKernelGGL(weight_grad_kernel<BW_BF16>, dim3((h->dim + 31) / 32, 2), dim3(1024), 0, (hipStream_t)stream, a.partial, h->dim, a.q_blocks, blocks, q_weight_grad, k_weight_grad, a.weight_f32);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;
