@@ -35,7 +35,7 @@ constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
 // Tiles that beginning and joining a segment is worth: with 2 the pieces of many short segments are waited for (32 sequences of up to 1000 tokens, 8 heads of
 // 128 in 8 bits: 29.4 us; 5: 23.7; 8 and 12: 20.4), with 12 the long ones (64 of up to 8192 in 16 bits: 166.4 against 165.2 with 8 and 163.3 with 2).
 constexpr uint32_t kSegmentCost = 8;
-constexpr uint32_t kManyUnits = 16;              // see split_of
+BW_DEV uint32_t many_units(int queries) { return queries > 8 ? 16 : 6; }          // see split_of
 constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
 
 // A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
@@ -75,13 +75,14 @@ struct Split {
         return unit < head ? unit / (size + 1) : longer + (unit - head) / size;
     }
 };
-// Less than kManyUnits for every workgroup that can be resident: one piece for a CU at most, of so many units that its waves have equally many.
-// Smaller ones cost more in parts to join, and a second piece on some of the CUs is waited for by all.  8 sequences of 8192, 16 queries of one head of
-// 128: 14.8 us in 176 pieces against 17.8 in 512; 4 of 1024, 8 heads with 8 queries: 11.4 in 160, 12.9 in 256 of 5 units; 16 of 1024, 8 heads with 16
-// queries in 4 bits: 17.1 in 256, 18.6 in 512.
+// Less than many_units for every workgroup that can be resident: one piece for a CU at most, of so many units that its waves have equally many.
+// Smaller ones cost more in parts to join, the more the queries of each, and a second piece on some of the CUs is waited for by all.  8 sequences of
+// 8192, 16 queries of one head of 128: 14.8 us in 176 pieces against 17.8 in 512; 4 of 1024, 8 heads with 8 queries: 11.4 in 160, 12.9 in 256 of 5 units;
+// 16 of 8192 with 16 queries of one head (8 units for each of 512): 19.5 in 212, 20.8 in 512.  4 sequences of 4096, 8 heads with 4 queries in 8 bits
+// (8.5 units): 17.7 in 242, 15.9 in 512; one of 2048, 32 heads in 8 bits (4.5 units): 13.8 in 192, 13.0 in 512, but 4 of 2000 with 16 queries 16.4 and 17.3.
 BW_DEV Split split_of(const AttentionArgs& a, uint32_t units, uint32_t grid) {
     const uint32_t total = units * (uint32_t)(a.kv_heads * a.q_groups), round = (uint32_t)(a.cus * kWaves);
-    const uint32_t size = (total + round - 1) / round * kWaves, pieces = total >= grid * kManyUnits ? grid : size ? (total + size - 1) / size : 0;
+    const uint32_t size = (total + round - 1) / round * kWaves, pieces = total >= grid * many_units(a.queries) ? grid : size ? (total + size - 1) / size : 0;
     Split s = {};
     s.pieces = pieces < grid ? pieces : grid;
     s.size = s.pieces ? total / s.pieces : 0;
