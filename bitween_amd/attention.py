@@ -32,7 +32,10 @@ def _whole(t, what, dtype):
     _tensor(t, what)
     if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
         raise TypeError(f"{what} must hold whole numbers, got {str(t.dtype)[6:]}")
-    return _hip._plain(t).to(dtype).contiguous()
+    t = _hip._plain(t)
+    if dtype is torch.int32 and t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        t = t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)       # what lies outside stays outside
+    return t.to(dtype).contiguous()
 
 
 def _one_gpu(what, *tensors):
@@ -169,8 +172,8 @@ def read_cache(slots, keys, values, key_meta=None, value_meta=None, bits=16, gro
     bfloat16; the cache's own type at 16 bits, float16 otherwise where none is given.  Codes come back as scale * (code - zero point),
     rounded once; a slot outside the cache gives zeros."""
     if dtype is None:
-        dtype = keys.dtype if bits == 16 else torch.float16
-    if dtype not in _HALF or (bits == 16 and dtype != keys.dtype):
+        dtype = getattr(keys, "dtype", None) if bits == 16 else torch.float16
+    if dtype not in _HALF or (bits == 16 and dtype != getattr(keys, "dtype", None)):
         raise TypeError(f"read_cache gives float16 or bfloat16 (a 16-bit cache its own type), not {dtype}")
     code = _hip._DTYPE_CODE[dtype]
     out = _native("cache_read")(slots, keys, values, key_meta, value_meta, bits, group_size, code)
@@ -197,7 +200,7 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
     rows nor the table's entries.  An infinity or a NaN among its cached values leaves nothing finite where it enters.  A length beyond the table is cut to it; a page number outside the cache is a page without tokens.  Lengths
     and table are read on the GPU when the kernel runs, so a captured call follows them.  No gradients."""
     if scale is None:
-        scale = q.shape[-1] ** -0.5
+        scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
     out = _native("cache_attention")(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale)
     if out is not None:
         return out

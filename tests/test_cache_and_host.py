@@ -208,3 +208,19 @@ def test_slots_of_positions_without_a_page_are_padding():
     assert c.slots(table, torch.tensor([31, 16, 5, 17, 31], dtype=torch.int32), torch.tensor([0, 1, 2, 2, 0])).tolist() == [15, -1, 21, 17, 15]
     with pytest.raises(ValueError):
         c.slots(table, torch.tensor([1]))
+
+
+def test_what_is_no_tensor_is_named():
+    t = torch.zeros(1)
+    with pytest.raises(TypeError):
+        bw.read_cache(t, None, None)
+    with pytest.raises(TypeError):
+        bw.read_cache(t, None, None, bits=8)
+    with pytest.raises(TypeError):
+        bw.cache_attention(None, t, t, None, None)
+    with pytest.raises(TypeError):
+        bw.cache_attention(t, t, t, None, None)
+    with pytest.raises(TypeError):
+        bw.write_cache(None, None, None, None, None)
+    with pytest.raises(TypeError):
+        bw.rotate_heads(None, None, None, None, None)

@@ -286,3 +286,25 @@ def test_a_padded_step_is_the_step_of_its_sequences(bits, group, dtype):
             assert a is None and b is None or torch.equal(a, b)
         positions += (positions >= 0).long()
         lengths += (lengths > 0).int()
+
+
+def test_wide_whole_numbers_outside_stay_outside():
+    """int64 tables and lengths: what does not fit 32 bits must not come back as a page or a length that does."""
+    b = Batch([64, 64, 5], 8, 2, 64, 16, 16, 64, torch.float16)
+    table, lengths = b.table.long(), b.lengths.long()
+    table[0, 2:] = 2 ** 32 + table[0, 2:]
+    table[1, :] -= 2 ** 33
+    lengths[1] += 2 ** 32
+    out = b.cache.attend(b.q, table, lengths)
+    b.check(out, lengths=[32, 0, 5])
+    full = b.cache.attend(b.q, b.table, torch.tensor([2 ** 32 + 1, 64, -2 ** 32 + 5], device="cuda"))
+    b.check(full, lengths=[64, 64, 0])
+
+
+@pytest.mark.parametrize("bits,group,pages", [(16, 0, 66000), (8, 64, 132000), (4, 128, 264000)])
+def test_pages_behind_four_gibibytes(bits, group, pages):
+    """8.6 GB of keys, so that every other page lies behind 32 bits of bytes (and behind 31 bits of values)."""
+    b = Batch([1000, 70, 0, 300], 8, 8, 128, 64, bits, group or 64, torch.float16, spare=pages)
+    page_bytes = b.cache.keys[0].nbytes
+    assert int(b.table[b.table < 2 ** 30].max()) * page_bytes > 2 ** 32
+    b.check(b.attend())
