@@ -51,7 +51,6 @@ struct AttentionArgs {
     uint16_t* out;
     Joint* joints;                               // what each workgroup leaves to join
     float* partial;                              // 2 slots for each workgroup: r [16], l [16], O [queries][dim]
-    int64_t page_bytes, meta_words;              // of one head in one page: row bytes * page_size; pairs
     uint32_t pages;
     int B, q_heads, kv_heads, share, queries, q_groups;   // queries: of a segment, at most 16; q_groups: segments of a key-value head
     int dim, row_bytes, page_shift, max_tokens, q_bf16, cus, whole;
