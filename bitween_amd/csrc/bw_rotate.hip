@@ -77,8 +77,16 @@ BW_DEV void chunks_of(const RotateArgs& a, int c, int& first, int& second, bool&
     second = turns ? first + a.half : first + CH;
 }
 
+// Over the 2^shift lanes of a head, each with the sum: neighbours, pairs, then mirrored halves of 8 and of 16, whose lanes hold the same by then.
+template <int CTRL> BW_DEV float from_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
 BW_DEV float head_sum(float v, int shift) {
-    for (int o = 1; o < 1 << shift; o <<= 1) v += __shfl_xor(v, o, 64);
+    if (shift > 0) v += from_lane<0xB1>(v);
+    if (shift > 1) v += from_lane<0x4E>(v);
+    if (shift > 2) v += from_lane<0x141>(v);
+    if (shift > 3) v += from_lane<0x140>(v);
+    if (shift > 4) v += __shfl_xor(v, 16, 64);
     return v;
 }
 
