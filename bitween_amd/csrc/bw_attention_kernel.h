@@ -15,6 +15,10 @@
 // The order of the head's values in an MFMA is free as long as K and Q agree, and that of the tokens as long as P and V agree, so nothing
 // crosses lanes: no LDS, no shuffles until the waves are joined.  r is only raised when a score passes it by 2^8 (one vote a tile).
 //
+// P enters as 16-bit numbers, each rounded to nearest, whose sum it is: three in bfloat16, which hold all of a float32 (two, cut to 16 bits, gave every
+// 170th result of the largest case another bfloat16 neighbour than the exact value's, where float32 weights give every 1500th; three cost 0 ... 2 %), two in
+// float16.
+//
 // Fewer than 16 queries leave columns of the MFMAs empty: the matrix cores have room (16 KB of a 16-bit tile take 32 MFMAs, some 500 cycles
 // of one SIMD, and about 8000 cycles of a SIMD's share of HBM).
 //
@@ -181,11 +185,8 @@ template <bool BF16> BW_DEV f4 mfma(u4 a, u4 b, f4 c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// Two float32 as 16-bit numbers, towards zero; split_pair leaves in x and y what is missing.
-template <bool BF16> BW_DEV uint32_t pair_of(float x, float y) {
-    if constexpr (BF16) return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
-    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
-}
+// Two float32 as 16-bit numbers, to nearest; split_pair leaves in x and y what is missing (exactly).
+template <bool BF16> BW_DEV uint32_t pair_of(float x, float y) { return narrow_pair<BF16 ? BW_BF16 : BW_F16>(x, y); }
 template <bool BF16> BW_DEV uint32_t split_pair(float& x, float& y) {
     const uint32_t p = pair_of<BF16>(x, y);
     if constexpr (BF16) {
@@ -735,19 +736,21 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
 #pragma unroll
                         for (int w = 0; w < F::kValueWords; w++) tile.value[e][w] = seen(e) ? tile.value[e][w] : 0u;
                 }
-                u4 hi, lo;
+                constexpr int kParts = F::kBf16 ? 3 : 2;
+                u4 part[kParts];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    hi[i] = split_pair<F::kBf16>(p[2 * i], p[2 * i + 1]);
-                    lo[i] = pair_of<F::kBf16>(p[2 * i], p[2 * i + 1]);
+#pragma unroll
+                    for (int n = 0; n < kParts - 1; n++) part[n][i] = split_pair<F::kBf16>(p[2 * i], p[2 * i + 1]);
+                    part[kParts - 1][i] = pair_of<F::kBf16>(p[2 * i], p[2 * i + 1]);
                 }
                 static_for<0, F::NV>([&](auto jc) {
                     constexpr int j = decltype(jc)::value;
                     u4 v;
 #pragma unroll
                     for (int i = 0; i < 4; i++) v[i] = token_pair<(j & 1) != 0>(tile.value[2 * i + 1][j / 2], tile.value[2 * i][j / 2]);
-                    acc[j] = mfma<F::kBf16>(v, hi, acc[j]);
-                    acc[j] = mfma<F::kBf16>(v, lo, acc[j]);
+#pragma unroll
+                    for (int n = 0; n < kParts; n++) acc[j] = mfma<F::kBf16>(v, part[n], acc[j]);
                 });
             }
             if (more) load_values(tile, g, next);
