@@ -13,11 +13,12 @@
 //   O^T[d][query] += V^T P^T         B = P^T as it lies there; A = V^T: a lane loads a piece of the rows of just those 8 tokens and pairs
 //                                    the tokens with byte permutes
 // The order of the head's values in an MFMA is free as long as K and Q agree, and that of the tokens as long as P and V agree, so nothing
-// crosses lanes: no LDS, no shuffles until the waves are joined.  r is only raised when a score passes it by 2^8 (one vote a tile).
+// crosses lanes: no LDS, no shuffles until the waves are joined.  r is only raised when a score passes it by some powers of two (one vote a tile).
 //
 // P enters as 16-bit numbers, each rounded to nearest, whose sum it is: three in bfloat16, which hold all of a float32 (two, cut to 16 bits, gave every
 // 170th result of the largest case another bfloat16 neighbour than the exact value's, where float32 weights give every 1500th; three cost 0 ... 2 %), two in
-// float16.
+// float16.  Its steps end at 2^-24, so r is kept where the largest P is 2^12 ... 2^15: a weight errs by 2^-22 of itself or 2^-37 of the largest.  (With
+// the largest at 1 ... 2^8, and cut instead of rounded, 8192 weights e^-14 of one more came out 0.9 % low.)
 //
 // Fewer than 16 queries leave columns of the MFMAs empty: the matrix cores have room (16 KB of a 16-bit tile take 32 MFMAs, some 500 cycles
 // of one SIMD, and about 8000 cycles of a SIMD's share of HBM).
@@ -29,9 +30,10 @@
 // Scales and zero points are applied in float32:
 //   K: S = s (Q . c - z sum Q) for each group
 //   V: O += (P s) c, and another MFMA whose rows are the zero points sums (P s) z, which is taken off at the end
-// so no value is rounded on its way in.  P s can be anything from 2^-24 to 2^16 times P: r then follows score + log2 of the token's scale
-// (a power of two 2^e), P is held relative to that and l adds P 2^-e.  P goes in as two 16-bit numbers whose sum it is (to 2^-16 and better):
-// one alone would err as much as the result's own rounding.
+// so no value is rounded on its way in.  What enters, P s, can be anything from 2^-24 to 2^16 times P, and a head's groups may be that far apart, so
+// every group has a power of two of its own for every query, its reach: P s times it is 2^12 ... 2^15 at its largest too, and the group's sums are
+// divided by it at the end.  P itself stays float32, and so do r and l.  (With one reference for all groups of a token a group 2^-10 of the largest
+// erred by 2^-10.  The reach costs 1 ... 3 % with heads of 128, 16 % with four groups of 64 to a head: one vote for each group.)
 #pragma once
 #include "bw_cache.h"
 
@@ -40,7 +42,11 @@ constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
 // 128 in 8 bits: 29.4 us; 5: 23.7; 8 and 12: 20.4), with 12 the long ones (64 of up to 8192 in 16 bits: 166.4 against 165.2 with 8 and 163.3 with 2).
 constexpr uint32_t kSegmentCost = 8;
 BW_DEV uint32_t many_units(int queries) { return queries > 8 ? 16 : 6; }          // see split_of
-constexpr float kSlack = 8.f;                    // scores may pass the reference by 2^8 before it is raised: P stays below 2^9 of float16's 2^16
+// Where weights lie in their 16-bit type: the largest at 2^kTop and more when its reference is set, below 2^kMost until the reference is raised.
+constexpr int kTop = 12, kMost = 15;
+// Over codes P itself stays float32 and may pass its reference by 2^8; a group's reach begins at 2^100.
+constexpr float kSlack = 8.f;
+constexpr int kFirstReach = 100;
 
 // A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
 struct Joint { uint32_t b, hq, parts, unused; };
@@ -572,11 +578,14 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
 
         // ---- tiles ----
         f4 acc[F::NV], zeros[F::kGroups];                         // zeros: sums of (P s) z, the same in every row
-        float r = -INFINITY, l = 0.f;
+        float r = -INFINITY, l = 0.f, reach[F::kGroups];
 #pragma unroll
         for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < F::kGroups; c++) zeros[c] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < F::kGroups; c++) {
+            zeros[c] = f4{0.f, 0.f, 0.f, 0.f};
+            reach[c] = __builtin_ldexpf(1.f, kFirstReach);
+        }
         auto step = [&](Tile<F>& tile, const uint32_t t) __attribute__((always_inline)) {
             // The second half of the workgroups shares its CUs with the first, whose waves, being older, go before: 17 against 21 us of a launch's 24.
             // Going first every other tile evens it out (48 sequences of up to 8192 tokens, 8 heads of 128 in 8 bits: 46.2 against 47.4 us).
@@ -646,43 +655,37 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                 tile.h = hn;
                 load_keys(tile, g, next);
             }
-            // reference: for codes the scores are raised by the exponent of the token's largest value scale
-            float unit[Z::kTokens], value_scale[F::kGroups][Z::kTokens];        // 2^-e; scales times that
             if constexpr (F::kCodes) {
-                static_for<0, Z::kTokens>([&](auto jc) {
-                    constexpr int j = decltype(jc)::value;
-                    float top = 0.f;
 #pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) {
-                        value_scale[c][j] = f16_bits(Z::template value_pair<j>(pairs[0][c], pairs[Z::kRegisters - 1][c]));
-                        top = c ? fmaxf(top, value_scale[c][j]) : value_scale[c][j];
-                    }
-                    const int ex = __builtin_amdgcn_frexp_expf(top);
-                    x[j] = __builtin_fmaf(x[j], score_scale, (float)ex);
-                    unit[j] = __builtin_ldexpf(1.f, -ex);
-#pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) value_scale[c][j] *= unit[j];
-                });
+                for (int j = 0; j < Z::kTokens; j++) x[j] *= score_scale;
             }
             if (!full) {
 #pragma unroll
                 for (int j = 0; j < Z::kTokens; j++) x[j] = own(j) ? x[j] : -INFINITY;
             }
+            auto over_lanes = [&](float top) {                   // of a query's column
+                top = Z::max(top);
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                return fmaxf(top, __shfl_xor(top, 32, 64));
+            };
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < Z::kTokens; j++) top = fmaxf(top, x[j]);
-            if (__builtin_amdgcn_ballot_w64(top > r + kSlack)) {
-                top = Z::max(top);
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), r);
-                const float keep = top == r ? 1.f : __builtin_amdgcn_exp2f(r - top);
-                r = top;
-                l *= keep;
+            const bool passed = __builtin_amdgcn_ballot_w64(top > r + (F::kCodes ? kSlack : kMost));
+            int up = 0;
+            if (passed) {
+                top = over_lanes(top);
+                if constexpr (F::kCodes) {                       // by whole powers of two, which round nothing
+                    const float raised = fmaxf(__builtin_ceilf(top), r);
+                    up = raised == r ? 0 : (int)fminf(raised - r, 300.f);
+                    r = raised;
+                    l = __builtin_ldexpf(l, -up);
+                } else {
+                    const float raised = fmaxf(top - kTop, r), keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
+                    r = raised;
+                    l *= keep;
 #pragma unroll
-                for (int j = 0; j < F::NV; j++) acc[j] *= keep;
-                if constexpr (F::kCodes) {
-#pragma unroll
-                    for (int c = 0; c < F::kGroups; c++) zeros[c] *= keep;
+                    for (int j = 0; j < F::NV; j++) acc[j] *= keep;
                 }
             }
             float p[Z::kTokens];
@@ -693,7 +696,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                 for (int j = 0; j < Z::kTokens; j++) p[j] = own(j) ? p[j] : 0.f;
             }
 #pragma unroll
-            for (int j = 0; j < Z::kTokens; j++) l = F::kCodes ? __builtin_fmaf(p[j], unit[j], l) : l + p[j];
+            for (int j = 0; j < Z::kTokens; j++) l += p[j];
             // weighted values
             if constexpr (F::kCodes) {
                 if constexpr (F::kMerge > 1) {
@@ -704,14 +707,31 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                 }
                 static_for<0, F::kGroups>([&](auto cc) {
                     constexpr int c = decltype(cc)::value;
-                    float pg[Z::kTokens];
+                    float ps[Z::kTokens], most = 0.f;             // P s, times the group's reach
+                    static_for<0, Z::kTokens>([&](auto jc) {
+                        constexpr int j = decltype(jc)::value;
+                        ps[j] = p[j] * f16_bits(Z::template value_pair<j>(pairs[0][c], pairs[Z::kRegisters - 1][c])) * reach[c];
+                        most = fmaxf(most, __builtin_fabsf(ps[j]));
+                    });
+                    if (passed || __builtin_amdgcn_ballot_w64(most > (float)(1 << kMost))) {
+                        most = over_lanes(most);
+                        // up with the reference, so that the group's weights stay where they are; down where they would pass 2^kMost
+                        const int was = __builtin_amdgcn_frexp_expf(reach[c]) - 1, high = most > 0.f ? __builtin_amdgcn_frexp_expf(most) - was : -1000;
+                        int now = min(was + up, kFirstReach);
+                        if (high + now > kMost) now = min(kTop + 1 - high, now);
+                        reach[c] = __builtin_ldexpf(1.f, now);
+#pragma unroll
+                        for (int j = 0; j < Z::kTokens; j++) ps[j] = __builtin_ldexpf(ps[j], now - was);
+                        const float by = __builtin_ldexpf(1.f, now - was - up);
+#pragma unroll
+                        for (int j = 0; j < F::kPerV; j++) acc[c * F::kPerV + j] *= by;
+                        zeros[c] *= by;
+                    }
                     uint32_t own_hi[Z::kTokens / 2], own_lo[Z::kTokens / 2];
 #pragma unroll
-                    for (int j = 0; j < Z::kTokens; j++) pg[j] = p[j] * value_scale[c][j];
-#pragma unroll
                     for (int i = 0; i < Z::kTokens / 2; i++) {
-                        own_hi[i] = split_pair<false>(pg[2 * i], pg[2 * i + 1]);
-                        own_lo[i] = pair_of<false>(pg[2 * i], pg[2 * i + 1]);
+                        own_hi[i] = split_pair<false>(ps[2 * i], ps[2 * i + 1]);
+                        own_lo[i] = pair_of<false>(ps[2 * i], ps[2 * i + 1]);
                     }
                     const u4 hi = Z::all(own_hi), lo = Z::all(own_lo);
                     const uint32_t pair = pairs[Z::kRegisters - 1][c], both = token_pair<true>((uint32_t)__builtin_amdgcn_mov_dpp((int)pair, 0xB1, 0xF, 0xF, true), pair);
@@ -802,7 +822,8 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         float o = acc[j][i];
-                        if constexpr (F::kCodes) o = __builtin_fmaf(o, (float)(1 << kUnit<F::kBits>), -zeros[j / F::kPerV][i]);
+                        if constexpr (F::kCodes)
+                            o = __builtin_ldexpf(__builtin_fmaf(o, (float)(1 << kUnit<F::kBits>), -zeros[j / F::kPerV][i]), 1 - __builtin_amdgcn_frexp_expf(reach[j / F::kPerV]));
                         outs[wave][m][F::v_at(4 * kg + i, j) - c * kChunk] = o * f;
                     }
             }

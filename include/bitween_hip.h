@@ -288,10 +288,12 @@ int bw_cache_read(const bw_cache* cache, int out_dtype, int64_t T, const int64_t
 
 /* Attention of one new token of each of B sequences over its cached tokens:
  *   out = sum_t softmax_t(scale q . k_t) v_t,  t < lengths[b],  token t in row t % page_size of page page_table[b][t / page_size]
- * Query head h reads key-value head h / (q_heads / kv_heads).  Codes enter with their exact values scale * (code - zero point), sums and
- * softmax are float32, out is rounded once.  A sequence without tokens (length 0 or less) gets zeros.  A length beyond
- * max_pages * page_size is taken as that; a page number outside the cache is a page without tokens.  Rows behind a sequence's last token
- * are not looked at, whatever they hold; an infinity or a NaN among the cached values leaves nothing finite where it enters.
+ * Query head h reads key-value head h / (q_heads / kv_heads).  Codes enter with their exact values scale * (code - zero point); scores, the
+ * softmax and all sums are float32.  Over a bfloat16 cache the weights meet the values as float32 too; otherwise they err by 2^-22 of themselves
+ * or, if more, 2^-37 of the largest (over codes: of the largest weight times scale of the same group).  out is rounded once.
+ * A sequence without tokens (length 0 or less) gets zeros.  A length beyond max_pages * page_size is taken as that; a page number outside
+ * the cache is a page without tokens.  Rows behind a sequence's last token are not looked at, whatever they hold; an infinity or a NaN among
+ * the cached values leaves nothing finite where it enters.
  *   q [B][q_heads][dim] act_dtype, strided as above; page_table int32, `table_row` elements from sequence to sequence; out contiguous
  * The cache is cut into equal pieces of work over all sequences; the parts of a sequence that lie in several of them are joined by a second
  * kernel in a fixed order, through a workspace of bw_cache_attention_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed). */
