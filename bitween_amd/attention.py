@@ -197,8 +197,10 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
     h // (q_heads // kv_heads).  scale: 1 / sqrt(dim) where none is given.  q has the type of a 16-bit cache, float16 or bfloat16 over codes.
 
     A sequence of length 0 (an idle row of a padded batch) gives zeros.  What lies behind a sequence's last token is not looked at - neither the
-    rows nor the table's entries.  An infinity or a NaN among its cached values leaves nothing finite where it enters.  A length beyond the table is cut to it; a page number outside the cache is a page without tokens.  Lengths
-    and table are read on the GPU when the kernel runs, so a captured call follows them.  No gradients."""
+    rows nor the table's entries.  A score of minus infinity (an infinity among the keys) has weight 0, and a sequence without any other score gives NaN, as
+    one of plus infinity or NaN does; an infinity or a NaN among the values leaves nothing finite in its channel, whatever its weight.  A length beyond
+    the table is cut to it; a page number outside the cache is a page without tokens.  Lengths and table are read on the GPU when the kernel runs, so a
+    captured call follows them.  No gradients."""
     if scale is None:
         scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
     out = _native("cache_attention")(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale)

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(32 * ROWS) void attention_join_kernel(AttentionArgs
         sum += f * sums[i][x];
         o += f * outs[i][x];
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = top == -INFINITY ? 0.f : 1.f / sum;           // no tokens: 0; none with a finite score: 0 / 0
     store_out(a, (int64_t)b * a.q_heads + head * a.share + first_query + query, e - query * a.dim, o * inv);
 }
 

@@ -47,6 +47,9 @@ constexpr int kTop = 12, kMost = 15;
 // Over codes P itself stays float32 and may pass its reference by 2^8; a group's reach begins at 2^100.
 constexpr float kSlack = 8.f;
 constexpr int kFirstReach = 100;
+// The reference before any finite score: a score of minus infinity lies as far below it as below any other, and weighs 0.  A wave that has met no token
+// hands on minus infinity instead.
+constexpr float kLowest = -3.4028235e38f;
 
 // A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
 struct Joint { uint32_t b, hq, parts, unused; };
@@ -578,7 +581,8 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
 
         // ---- tiles ----
         f4 acc[F::NV], zeros[F::kGroups];                         // zeros: sums of (P s) z, the same in every row
-        float r = -INFINITY, l = 0.f, reach[F::kGroups];
+        float r = kLowest, l = 0.f, reach[F::kGroups];
+        bool any = false;                                         // a token that counts, for any lane
 #pragma unroll
         for (int j = 0; j < F::NV; j++) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -598,6 +602,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             // Tokens that do not count: behind the end, or on a page outside the cache.
             const bool full = (int)t * kTile + kTile <= n && tile.h.page[0] < a.pages && tile.h.page[1] < a.pages;
             const Halves h = tile.h;
+            any |= h.page[0] < a.pages || h.page[1] < a.pages;
             auto counts = [&](int half, int i) { return (int)t * kTile + 16 * half + 4 * kg + i < n && h.page[half] < a.pages; };
             auto seen = [&](int e) { return counts(e >> 2, e & 3); };               // of the lane's 8 tokens
             auto own = [&](int j) { const int e = fold.token(j); return e & 4 ? counts(1, e & 3) : counts(0, e & 3); };
@@ -690,11 +695,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             }
             float p[Z::kTokens];
 #pragma unroll
-            for (int j = 0; j < Z::kTokens; j++) p[j] = __builtin_amdgcn_exp2f(x[j] - r);
-            if (!full) {
-#pragma unroll
-                for (int j = 0; j < Z::kTokens; j++) p[j] = own(j) ? p[j] : 0.f;
-            }
+            for (int j = 0; j < Z::kTokens; j++) p[j] = __builtin_amdgcn_exp2f(x[j] - r);       // (r is never minus infinity: 0 where x is)
 #pragma unroll
             for (int j = 0; j < Z::kTokens; j++) l += p[j];
             // weighted values
@@ -783,6 +784,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
         if (more_segments) begin(after);
 
         // ---- the four waves of the workgroup joined ----
+        if (!any) r = -INFINITY;
         l = Z::sum(l);
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
@@ -836,7 +838,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                 for (int w = 1; w < kWaves; w++) o += *reinterpret_cast<const f4*>(&outs[w][query][d]);
                 if (complete) {
                     float top;
-                    const float sum = joined(query, top), inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const float sum = joined(query, top), inv = top == -INFINITY ? 0.f : 1.f / sum;
                     store_out(a, (int64_t)g.b * a.q_heads + g.q_head + query, c * kChunk + d, o * inv);
                 } else {
                     *reinterpret_cast<f4*>(slot + 2 * kQueries + query * a.dim + c * kChunk + d) = o;

@@ -292,8 +292,9 @@ int bw_cache_read(const bw_cache* cache, int out_dtype, int64_t T, const int64_t
  * softmax and all sums are float32.  Over a bfloat16 cache the weights meet the values as float32 too; otherwise they err by 2^-22 of themselves
  * or, if more, 2^-37 of the largest (over codes: of the largest weight times scale of the same group).  out is rounded once.
  * A sequence without tokens (length 0 or less) gets zeros.  A length beyond max_pages * page_size is taken as that; a page number outside
- * the cache is a page without tokens.  Rows behind a sequence's last token are not looked at, whatever they hold; an infinity or a NaN among
- * the cached values leaves nothing finite where it enters.
+ * the cache is a page without tokens.  Rows behind a sequence's last token are not looked at, whatever they hold.  A score of minus infinity
+ * has weight 0; a sequence without any other score gives NaN, as one of plus infinity or NaN does; an infinity or a NaN among the cached
+ * values leaves nothing finite in its channel, whatever its weight.
  *   q [B][q_heads][dim] act_dtype, strided as above; page_table int32, `table_row` elements from sequence to sequence; out contiguous
  * The cache is cut into equal pieces of work over all sequences; the parts of a sequence that lie in several of them are joined by a second
  * kernel in a fixed order, through a workspace of bw_cache_attention_workspace_bytes(...) bytes (16-byte aligned; 0 = none needed). */
