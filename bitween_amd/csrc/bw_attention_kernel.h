@@ -42,8 +42,10 @@ constexpr int kTile = 32, kTileShift = 5, kWaves = 4, kQueries = 16;
 // 128 in 8 bits: 29.4 us; 5: 23.7; 8 and 12: 20.4), with 12 the long ones (64 of up to 8192 in 16 bits: 166.4 against 165.2 with 8 and 163.3 with 2).
 constexpr uint32_t kSegmentCost = 8;
 BW_DEV uint32_t many_units(int queries) { return queries > 8 ? 16 : 6; }          // see split_of
-// Where weights lie in their 16-bit type: the largest at 2^kTop and more when its reference is set, below 2^kMost until the reference is raised.
-constexpr int kTop = 12, kMost = 15;
+// Where weights lie in their 16-bit type: the largest at 2^kTop and more when its reference is set, up to 2^kMost until the reference is raised.  In
+// bfloat16, whose steps have no end but whose values reach 2^128, never above 1: the products are no larger than the values.
+template <bool BF16> constexpr int kTop = BF16 ? -8 : 12;
+template <bool BF16> constexpr int kMost = BF16 ? 0 : 15;
 // Over codes P itself stays float32 and may pass its reference by 2^8; a group's reach begins at 2^100.
 constexpr float kSlack = 8.f;
 constexpr int kFirstReach = 100;
@@ -676,7 +678,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < Z::kTokens; j++) top = fmaxf(top, x[j]);
-            const bool passed = __builtin_amdgcn_ballot_w64(top > r + (F::kCodes ? kSlack : kMost));
+            const bool passed = __builtin_amdgcn_ballot_w64(top > r + (F::kCodes ? kSlack : kMost<F::kBf16>));
             int up = 0;
             if (passed) {
                 top = over_lanes(top);
@@ -686,7 +688,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                     r = raised;
                     l = __builtin_ldexpf(l, -up);
                 } else {
-                    const float raised = fmaxf(top - kTop, r), keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
+                    const float raised = fmaxf(top - kTop<F::kBf16>, r), keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
                     r = raised;
                     l *= keep;
 #pragma unroll
@@ -714,12 +716,12 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                         ps[j] = p[j] * f16_bits(Z::template value_pair<j>(pairs[0][c], pairs[Z::kRegisters - 1][c])) * reach[c];
                         most = fmaxf(most, __builtin_fabsf(ps[j]));
                     });
-                    if (passed || __builtin_amdgcn_ballot_w64(most > (float)(1 << kMost))) {
+                    if (passed || __builtin_amdgcn_ballot_w64(most > (float)(1 << kMost<false>))) {
                         most = over_lanes(most);
                         // up with the reference, so that the group's weights stay where they are; down where they would pass 2^kMost
                         const int was = __builtin_amdgcn_frexp_expf(reach[c]) - 1, high = most > 0.f ? __builtin_amdgcn_frexp_expf(most) - was : -1000;
                         int now = min(was + up, kFirstReach);
-                        if (high + now > kMost) now = min(kTop + 1 - high, now);
+                        if (high + now > kMost<false>) now = min(kTop<false> + 1 - high, now);
                         reach[c] = __builtin_ldexpf(1.f, now);
 #pragma unroll
                         for (int j = 0; j < Z::kTokens; j++) ps[j] = __builtin_ldexpf(ps[j], now - was);

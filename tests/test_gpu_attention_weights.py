@@ -161,3 +161,28 @@ def test_values_that_cancel(dtype):
         bound = half_step(dtype) * want.abs() + (16 + n) * 2.0 ** -24 + 2.0 ** -25
         worst = max(worst, ((out[s].double() - want).abs() / bound).max().item())
     assert worst <= 1, f"{worst:.3f} times the bound"
+
+
+@pytest.mark.parametrize("tokens", [2, 40, 700])
+@pytest.mark.parametrize("gap", [20.0, 24.0, 27.0, 30.0, 40.0])
+def test_values_at_the_upper_end_of_bfloat16(gap, tokens):
+    """Values up to 2^127 under one weight near 1 among small ones: finite, as products of float32 weights are.  The token far above is the last, so that
+    its score is met after the others' (2^(gap / ln 2) lower)."""
+    b = Batch([tokens, tokens], 8, 2, 128, 32, 16, 64, torch.bfloat16, seed=int(gap), spread=0.02)
+    b.q = b.q[:, ::4].repeat_interleave(4, 1)
+    for s in range(2):
+        q = b.q[s, ::4].float()
+        for step in range(5):                                    # several raised scores, a fifth of the gap apart
+            at = (s + 1) * tokens - 1 - 16 * step
+            if at >= s * tokens:
+                b.k[at] = (q * ((gap - step * gap / 5) * 128 ** 0.5 / q.pow(2).sum(-1, keepdim=True))).bfloat16()
+    b.v = (b.v.float().clamp(-1.9, 1.9) * 2.0 ** 127).bfloat16()
+    _filled(b)
+    out = b.attend().double()
+    for s in range(2):
+        k, v = (x[s * tokens:(s + 1) * tokens].double().transpose(0, 1) for x in (b.k, b.v))
+        w = torch.softmax(torch.matmul(b.q[s].double().view(2, 4, 128), k.transpose(1, 2).contiguous()) * 128 ** -0.5, -1)
+        want = torch.matmul(w, v.contiguous()).reshape(8, 128)
+        # scores in float32: 2 (dim + 16) 2^-24 of at most gap + 1, of values below 2^128
+        assert torch.isfinite(out[s]).all()
+        assert bool(((out[s] - want).abs() <= half_step(torch.bfloat16) * want.abs() + 2 * 144 * 2.0 ** -24 * (gap + 1) * 2.0 ** 128).all())
