@@ -10,6 +10,7 @@ weights); they run on torch's current stream, allocate their outputs and workspa
 graphs.  There is no CPU path: CPU tensors raise.  The reference has no counterpart; its models bring these as eager torch operations.
 """
 import torch
+from torch.autograd import forward_ad
 
 from .kernels import hip_loader as _hip
 
@@ -45,6 +46,12 @@ def _one_gpu(what, *tensors):
     devices = {t.device for t in tensors if t is not None}
     if len(devices) > 1:
         raise ValueError(f"{what}: tensors on {', '.join(sorted(map(str, devices)))}; one GPU is wanted")
+
+
+def _no_tangent(what, *tensors):
+    """Forward-mode derivatives are refused, with and without grad mode: a result without its tangent would be wrong without a word."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _hip.BitweenHipError(f"{what} has no forward-mode derivative")
 
 
 def _no_grad(what, *tensors):
@@ -117,6 +124,7 @@ def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
         raise ValueError("cos and sin must both be [table rows, rotary / 2]")
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise NotImplementedError("rotate_heads has no gradient of cos and sin")
+    _no_tangent(what, cos, sin)
     for t, name in ((q, "q"), (k, "k")):
         if t.dim() != positions.dim() + 2 or t.shape[:-2] != positions.shape or 0 in t.shape[-2:]:
             raise ValueError(f"{name} must be [..., heads, dim] with the leading dimensions of positions {list(positions.shape)}, got {list(t.shape)}")
@@ -160,6 +168,7 @@ def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=
         raise ValueError("slots must be [tokens], one for every row of k and v")
     _one_gpu(what, keys, k, v, slots)
     _no_grad(what, k, v, keys, values)
+    _no_tangent(what, k, v, keys, values, key_meta, value_meta)
     for a, b in ((keys, values), (key_meta, value_meta)):
         if a is not None and a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes:
             raise ValueError(f"{what}: keys and values of a cache that is written must not share memory")
@@ -184,6 +193,7 @@ def read_cache(slots, keys, values, key_meta=None, value_meta=None, bits=16, gro
     if slots.dim() != 1:
         raise ValueError("slots must be [tokens]")
     _one_gpu("read_cache", keys, slots)
+    _no_tangent("read_cache", keys, values, key_meta, value_meta)
     return _taken("read_cache", _native("cache_read")(_whole(slots, "slots", torch.int64), *_cache_args(keys, values, key_meta, value_meta, bits, group_size), code))
 
 
@@ -217,6 +227,7 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
         raise ValueError(f"page_table must be [{q.shape[0]}, pages] and lengths [{q.shape[0]}]")
     _one_gpu(what, keys, q, page_table, lengths)
     _no_grad(what, q)
+    _no_tangent(what, q, keys, values, key_meta, value_meta)
     return _taken(what, _native("cache_attention")(_hip._plain(q), _whole(page_table, "page_table", torch.int32), _whole(lengths, "lengths", torch.int32),
                                                    *_cache_args(keys, values, key_meta, value_meta, bits, group_size), float(scale)))
 

@@ -516,6 +516,11 @@ struct Rows {
     }
 };
 
+// Forward-mode derivatives are refused, with and without grad mode: a result without its tangent would be wrong without a word.
+void check_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 inline bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 inline bool on_gpu(const Tensor& t, const Tensor& like) { return t.is_cuda() && t.has_storage() && t.device() == like.device(); }
 
@@ -638,12 +643,9 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const Tensor qw = args[5] == Py_None ? Tensor() : unpack(args[5]), kw = args[6] == Py_None ? Tensor() : unpack(args[6]);
         Rotation r;
         if (!rotation_of(q, k, cos, sin, positions, qw, kw, eps, r)) return none();
+        check_tangents("rotate_heads", {&q, &k, &qw, &kw, &cos, &sin});
         bool recorded = false;
-        for (const Tensor* t : {&q, &k, &qw, &kw}) {
-            if (!t->defined()) continue;
-            recorded |= t->requires_grad();
-            TORCH_CHECK(!t->_fw_grad(0).defined(), "rotate_heads has no forward-mode derivative");
-        }
+        for (const Tensor* t : {&q, &k, &qw, &kw}) recorded |= t->defined() && t->requires_grad();
         recorded &= c10::GradMode::is_enabled();
         if (c10::GradMode::is_enabled()) {
             if (cos.requires_grad() || sin.requires_grad()) return none();
@@ -746,6 +748,7 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                 t->size(2) != h.c.dim || wants_grad(*t))
                 return none();
         if (k.scalar_type() != v.scalar_type() || (h.c.bits == 16 && k.scalar_type() != h.keys.scalar_type())) return none();
+        check_tangents("write_cache", {&k, &v, &h.keys, &h.values, &h.key_meta, &h.value_meta});
         if (wants_grad(h.keys) || wants_grad(h.values) || overlap(h.keys, h.values) || (h.key_meta.defined() && overlap(h.key_meta, h.value_meta))) return none();
         int status = 0;
         {
@@ -780,6 +783,7 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const int code = (int)PyLong_AsLong(args[7]);
         if (PyErr_Occurred()) return nullptr;
         if ((code != BW_F16 && code != BW_BF16) || (h.c.bits == 16 && code != h.c.dtype)) return none();
+        check_tangents("read_cache", {&h.keys, &h.values, &h.key_meta, &h.value_meta});
         Tensor k, v;
         int status = 0;
         {
@@ -822,6 +826,7 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch || table.size(1) < 1 || (table.size(1) > 1 && table.stride(1) != 1) ||
             lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != batch || !lengths.is_contiguous())
             return none();
+        check_tangents("cache_attention", {&q, &h.keys, &h.values, &h.key_meta, &h.value_meta});
         Tensor out;
         int status = 0;
         {
