@@ -55,7 +55,7 @@ def _no_tangent(what, *tensors):
 
 
 def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise _hip.BitweenHipError(f"{what} has no gradient: call it under torch.no_grad(), or on detached tensors")
 
 
@@ -167,7 +167,7 @@ def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=
     if slots.dim() != 1 or not len(slots) == len(k) == len(v):
         raise ValueError("slots must be [tokens], one for every row of k and v")
     _one_gpu(what, keys, k, v, slots)
-    _no_grad(what, k, v, keys, values)
+    _no_grad(what, k, v, keys, values, key_meta, value_meta)
     _no_tangent(what, k, v, keys, values, key_meta, value_meta)
     for a, b in ((keys, values), (key_meta, value_meta)):
         if a is not None and a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes:
@@ -193,6 +193,7 @@ def read_cache(slots, keys, values, key_meta=None, value_meta=None, bits=16, gro
     if slots.dim() != 1:
         raise ValueError("slots must be [tokens]")
     _one_gpu("read_cache", keys, slots)
+    _no_grad("read_cache", keys, values, key_meta, value_meta)
     _no_tangent("read_cache", keys, values, key_meta, value_meta)
     return _taken("read_cache", _native("cache_read")(_whole(slots, "slots", torch.int64), *_cache_args(keys, values, key_meta, value_meta, bits, group_size), code))
 
@@ -226,7 +227,7 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
     if page_table.dim() != 2 or page_table.shape[0] != q.shape[0] or page_table.shape[1] < 1 or lengths.shape != q.shape[:1]:
         raise ValueError(f"page_table must be [{q.shape[0]}, pages] and lengths [{q.shape[0]}]")
     _one_gpu(what, keys, q, page_table, lengths)
-    _no_grad(what, q)
+    _no_grad(what, q, keys, values, key_meta, value_meta)
     _no_tangent(what, q, keys, values, key_meta, value_meta)
     return _taken(what, _native("cache_attention")(_hip._plain(q), _whole(page_table, "page_table", torch.int32), _whole(lengths, "lengths", torch.int32),
                                                    *_cache_args(keys, values, key_meta, value_meta, bits, group_size), float(scale)))

@@ -732,6 +732,12 @@ inline bool overlap(const Tensor& a, const Tensor& b) {
 }
 
 inline bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// A cache that asks for gradients, which neither its reader nor its writer gives (the Python functions refuse it).
+inline bool wants_grad(const Cache& h) {
+    for (const Tensor* t : {&h.keys, &h.values, &h.key_meta, &h.value_meta})
+        if (t->defined() && wants_grad(*t)) return true;
+    return false;
+}
 
 // cache_write(k, v, slots, keys, values, key_meta, value_meta, bits, group_size) -> True or None
 PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -749,7 +755,7 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                 return none();
         if (k.scalar_type() != v.scalar_type() || (h.c.bits == 16 && k.scalar_type() != h.keys.scalar_type())) return none();
         check_tangents("write_cache", {&k, &v, &h.keys, &h.values, &h.key_meta, &h.value_meta});
-        if (wants_grad(h.keys) || wants_grad(h.values) || overlap(h.keys, h.values) || (h.key_meta.defined() && overlap(h.key_meta, h.value_meta))) return none();
+        if (wants_grad(h) || overlap(h.keys, h.values) || (h.key_meta.defined() && overlap(h.key_meta, h.value_meta))) return none();
         int status = 0;
         {
             Unlocked unlocked;
@@ -782,7 +788,7 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         }
         const int code = (int)PyLong_AsLong(args[7]);
         if (PyErr_Occurred()) return nullptr;
-        if ((code != BW_F16 && code != BW_BF16) || (h.c.bits == 16 && code != h.c.dtype)) return none();
+        if ((code != BW_F16 && code != BW_BF16) || (h.c.bits == 16 && code != h.c.dtype) || wants_grad(h)) return none();
         check_tangents("read_cache", {&h.keys, &h.values, &h.key_meta, &h.value_meta});
         Tensor k, v;
         int status = 0;
@@ -820,7 +826,7 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         for (const Tensor* t : {&q, &table, &lengths})
             if (!on_gpu(*t, h.keys)) return none();
         if (!half_type(q.scalar_type()) || (h.c.bits == 16 && q.scalar_type() != h.keys.scalar_type()) || q.dim() != 3 || q.size(2) != h.c.dim ||
-            q.size(1) < 1 || q.size(1) > 65535 || q.size(1) % h.c.kv_heads || wants_grad(q))
+            q.size(1) < 1 || q.size(1) > 65535 || q.size(1) % h.c.kv_heads || wants_grad(q) || wants_grad(h))
             return none();
         const int64_t batch = q.size(0);
         if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch || table.size(1) < 1 || (table.size(1) > 1 && table.stride(1) != 1) ||

@@ -4,6 +4,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import bitween_amd as bw
+from bitween_amd.kernels.hip_loader import BitweenHipError
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,23 @@ def test_forward_mode_of_the_rotation_s_tables_is_refused(converted):
             for context in (torch.enable_grad(), torch.no_grad()):
                 with context, pytest.raises(RuntimeError, match="no forward-mode derivative"):
                     bw.rotate_heads(q, q, *tables, positions)
+
+
+@pytest.mark.parametrize("name", ["write", "read", "attend"])
+@pytest.mark.parametrize("converted", [False, True])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_tensors_that_ask_for_gradients_are_refused(bits, converted, name):
+    """Queries, new rows, 16-bit keys and values, scales: with grad mode a call that would leave their gradients out raises, without it the call is made."""
+    types = (torch.int32, torch.int64) if converted else (torch.int64, torch.int32)
+    inputs, call = _calls(bits, *types)[name]
+    want = call(inputs)
+    for i, t in enumerate(inputs):
+        if not t.is_floating_point():
+            continue
+        asking = [x.detach().requires_grad_(True) if j == i else x for j, x in enumerate(inputs)]
+        with pytest.raises(BitweenHipError, match="no gradient"):
+            call(asking)
+        with torch.no_grad():
+            got = call(asking)
+        for a, b in zip(*((x if isinstance(x, tuple) else (x,)) for x in (got, want))):
+            assert a is None and b is None or torch.equal(a, b)
