@@ -360,7 +360,7 @@ extern "C" int bw_rotate_heads(const bw_heads* h, int act_dtype, const void* q, 
 }
 
 extern "C" size_t bw_rotate_heads_grad_workspace_bytes(const bw_heads* h) {
-    if (!h || heads_check(h, h->weight_dtype == BW_BF16 ? BW_BF16 : BW_F16) == BW_EINVAL || (!h->q_weight && !h->k_weight)) return 0;
+    if (heads_check(h, h && h->weight_dtype == BW_BF16 ? BW_BF16 : BW_F16) != BW_OK || (!h->q_weight && !h->k_weight)) return 0;
     return (size_t)(grad_blocks(h, h->q_heads) + grad_blocks(h, h->k_heads)) * h->dim * sizeof(float);
 }
 
