@@ -77,7 +77,7 @@ __global__ __launch_bounds__(32 * ROWS) void attention_join_kernel(AttentionArgs
 int attention_check(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
     if (int st = bw_cache_check(c)) return st;
     if (B < 0 || q_heads < 1 || q_heads % c->kv_heads || max_pages < 1) return BW_EINVAL;
-    if (B > 1 << 20 || q_heads > 65535 || max_pages * c->page_size >= (int64_t)1 << 25) return BW_EUNSUPPORTED;
+    if (B > 1 << 20 || q_heads > 65535 || max_pages >= ((int64_t)1 << 25) / c->page_size) return BW_EUNSUPPORTED;
     if (B * ((max_pages * c->page_size + kTile - 1) / kTile + kSegmentCost) >= ((int64_t)1 << 31) / q_heads || B * q_heads >= (int64_t)1 << 29) return BW_EUNSUPPORTED;
     return BW_OK;
 }

@@ -14,7 +14,7 @@ static inline int bw_cache_check(const bw_cache* c) {
         if (!bw_aligned(c->key_meta, 16) || !bw_aligned(c->value_meta, 16)) return BW_EALIGN;
     }
     if (c->dim % 8 || c->dim > 256 || c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return BW_EUNSUPPORTED;
-    if (c->pages >= (int64_t)1 << 31 || c->kv_heads > 65535) return BW_EUNSUPPORTED;
+    if (c->pages >= (int64_t)1 << 31 || c->kv_heads > 65535 || c->pages * c->page_size * c->kv_heads >= (int64_t)1 << 53) return BW_EUNSUPPORTED;
     if (!bw_aligned(c->keys, 16) || !bw_aligned(c->values, 16)) return BW_EALIGN;
     return BW_OK;
 }

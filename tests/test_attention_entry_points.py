@@ -24,3 +24,26 @@ def test_no_workspace_for_a_gradient_that_is_refused(fields):
 def test_a_workspace_for_a_gradient_that_is_taken(fields):
     h = _heads(**fields)
     assert hip_loader.load().bw_rotate_heads_grad_workspace_bytes(h) >= 2 * h.dim * 4          # a row of each kind at least
+
+
+def _cache(**other):
+    fields = dict(keys=P, values=P, key_meta=P, value_meta=P, pages=4, kv_heads=2, page_size=16, dim=64, bits=8, group=32, dtype=0)
+    return hip_loader.Cache(**{**fields, **other})
+
+
+@pytest.mark.parametrize("page_size", [16, 1024])
+@pytest.mark.parametrize("power", [53, 54, 55, 58, 59, 60, 61, 62])
+def test_tables_whose_tokens_pass_64_bits_are_refused(power, page_size):
+    """2^54 pages of 1024 tokens are 2^64: a table without room, if the product wraps."""
+    lib, c = hip_loader.load(), _cache(page_size=page_size)
+    for extra in (0, 1):
+        assert lib.bw_cache_attention(c, 0, P, 1, 2, 128, 64, P, (1 << power) + extra, 4, P, 1.0, P, P, 1 << 30, None) == EUNSUPPORTED
+        assert lib.bw_cache_attention_workspace_bytes(c, 1, 2, (1 << power) + extra) == 0
+
+
+def test_caches_whose_values_pass_63_bits_are_refused():
+    """(2^31 - 1) pages of 1024 rows, 65535 heads of 256 values: two such tensors share memory wherever they lie, if their size wraps to nothing they do not."""
+    lib, c = hip_loader.load(), _cache(pages=(1 << 31) - 1, page_size=1024, kv_heads=65535, dim=256, values=2 * P, value_meta=3 * P)
+    assert lib.bw_cache_write(c, 0, 1, P, 16776960, 256, P, 16776960, 256, P, None) == EUNSUPPORTED
+    assert lib.bw_cache_read(c, 0, 1, P, P, P, None) == EUNSUPPORTED
+    assert lib.bw_cache_attention_workspace_bytes(c, 1, 65535, 4) == 0
