@@ -291,6 +291,8 @@ class PagedCache:
             pages = page_table
         else:
             pages = page_table[sequences]
+        if pages.shape[1] == 0:                                  # (nothing that could be looked up)
+            return torch.full_like(positions, -1, dtype=torch.int64)
         column = positions // size
         kept = (column >= 0) & (column < pages.shape[1])
         page = pages.gather(1, column.clamp(0, pages.shape[1] - 1).long()[:, None])[:, 0].long()
