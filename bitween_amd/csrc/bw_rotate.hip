@@ -307,7 +307,7 @@ int heads_check(const bw_heads* h, int act_dtype) {
     if (h->dim % 8 || h->rotary % 8 || h->dim > kMaxDim) return BW_EUNSUPPORTED;
     if (h->q_heads > 65535 || h->k_heads > 65535 || h->tokens >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
     const int64_t items = h->tokens * ((int64_t)h->q_heads + h->k_heads);
-    if (items >= (int64_t)1 << 31 || items << bw_log2(h->dim / (2 * chunk_of(h))) >= (int64_t)1 << 32) return BW_EUNSUPPORTED;   // threads of a launch
+    if (items >= (int64_t)1 << 31 || items * h->dim >= (int64_t)1 << 36) return BW_EUNSUPPORTED;
     if (!bw_aligned(h->cos, 16) || !bw_aligned(h->sin, 16) || !bw_aligned(h->positions, 8) || !bw_aligned(h->q_weight, 16) || !bw_aligned(h->k_weight, 16))
         return BW_EALIGN;
     return BW_OK;
@@ -350,13 +350,21 @@ extern "C" int bw_rotate_heads(const bw_heads* h, int act_dtype, const void* q, 
     a.q = (const uint16_t*)q; a.k = (const uint16_t*)k;
     a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head;
     a.q_out = (uint16_t*)q_out; a.k_out = (uint16_t*)k_out;
-    const int64_t items = h->tokens * (h->q_heads + h->k_heads), per_block = 256 >> a.lane_shift;
-    const dim3 grid((unsigned)((items + per_block - 1) / per_block)), block(256);
+    // In several launches where a head's lanes, filled up to a power of two, would pass the 2^32 threads of one.
+    const int64_t heads = h->q_heads + h->k_heads, per_block = 256 >> a.lane_shift, most = (((int64_t)1 << 32) - 256) / (heads << a.lane_shift);
+    for (int64_t at = 0; at < h->tokens; at += most) {
+        a.T = (int)(h->tokens - at < most ? h->tokens - at : most);
+        const dim3 grid((unsigned)((a.T * heads + per_block - 1) / per_block)), block(256);
 #define BW_ROTATE(DT, CH) \
     if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_kernel<DT, CH>), grid, block, 0, (hipStream_t)stream, a);
-    BW_ROTATE(BW_F16, 8) BW_ROTATE(BW_F16, 4) BW_ROTATE(BW_BF16, 8) BW_ROTATE(BW_BF16, 4)
+        BW_ROTATE(BW_F16, 8) BW_ROTATE(BW_F16, 4) BW_ROTATE(BW_BF16, 8) BW_ROTATE(BW_BF16, 4)
 #undef BW_ROTATE
-    return hipGetLastError() == hipSuccess ? BW_OK : BW_ELAUNCH;
+        if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
+        a.positions += a.T;
+        a.q += a.T * q_row; a.k += a.T * k_row;
+        a.q_out += (int64_t)a.T * h->q_heads * h->dim; a.k_out += (int64_t)a.T * h->k_heads * h->dim;
+    }
+    return BW_OK;
 }
 
 extern "C" size_t bw_rotate_heads_grad_workspace_bytes(const bw_heads* h) {

@@ -47,3 +47,18 @@ def test_caches_whose_values_pass_63_bits_are_refused():
     assert lib.bw_cache_write(c, 0, 1, P, 16776960, 256, P, 16776960, 256, P, None) == EUNSUPPORTED
     assert lib.bw_cache_read(c, 0, 1, P, P, P, None) == EUNSUPPORTED
     assert lib.bw_cache_attention_workspace_bytes(c, 1, 65535, 4) == 0
+
+
+@pytest.mark.parametrize("dim,rotary", [(80, 40), (40, 40), (136, 136), (24, 8), (64, 64), (256, 256)])
+def test_rotations_are_refused_from_2_31_heads_and_2_36_values_on(dim, rotary):
+    """Whatever lanes a head has: the limits that the header states, for the forward and its gradient (refused here by their pointers' alignment instead)."""
+    lib = hip_loader.load()
+    tokens = min((1 << 31) - 1, ((1 << 36) - 1) // dim) // 3     # of 3 heads
+
+    def status(tokens):
+        h = _heads(tokens=tokens, dim=dim, rotary=rotary, cos=P + 4)
+        return lib.bw_rotate_heads(h, 0, P, 3 * dim, dim, P, 3 * dim, dim, P, P, None), lib.bw_rotate_heads_grad(
+            h, 0, P, 3 * dim, dim, P, 3 * dim, dim, P, 3 * dim, dim, None, 0, 0, P, P, None, None, None, 0, None)
+
+    assert status(tokens) == (EALIGN, EALIGN)
+    assert status(tokens + 1) == (EUNSUPPORTED, EUNSUPPORTED)
