@@ -136,8 +136,8 @@ def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
         _tensor(w, "q_weight / k_weight", q.dtype, torch.float32)
         if w.shape != (dim,) or w.dtype != weights[0].dtype:
             raise ValueError(f"q_weight and k_weight must be [{dim}] of one type")
-    plain = [None if t is None else t.as_subclass(torch.Tensor) for t in (q, k, q_weight, k_weight)]
-    plain[2:] = [None if w is None else w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format) for w in plain[2:]]
+    # (a leaf goes on as it is: what a capture asks of its gradient's accumulation is asked of the leaf itself)
+    plain = [t if t is None or type(t) in (torch.Tensor, torch.nn.Parameter) else t.as_subclass(torch.Tensor) for t in (q, k, q_weight, k_weight)]
     tables = [t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (_hip._plain(t).float() for t in (cos, sin))]
     return _taken(what, _native("rotate_heads")(plain[0], plain[1], *tables, _whole(positions, "positions", torch.int64), plain[2], plain[3], float(eps)))
 

@@ -532,6 +532,7 @@ bool heads_of(const Tensor& t, at::IntArrayRef lead) {
 struct Rotation {
     bw_heads heads;
     int act;
+    Tensor weights[2];                                          // the queries' and the keys', as the kernels read them
 };
 
 bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions, const Tensor& qw, const Tensor& kw,
@@ -548,15 +549,23 @@ bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tens
     at::ScalarType wt = q.scalar_type();
     for (const Tensor* t : {&qw, &kw})
         if (t->defined()) {
-            if (!on_gpu(*t, q) || t->dim() != 1 || t->size(0) != dim || !t->is_contiguous() || !aligned16(t->const_data_ptr())) return false;
+            if (!on_gpu(*t, q) || t->dim() != 1 || t->size(0) != dim) return false;
             wt = t->scalar_type();
         }
     if (wt != q.scalar_type() && wt != at::kFloat) return false;
     if (qw.defined() && kw.defined() && qw.scalar_type() != kw.scalar_type()) return false;
+    r.weights[0] = qw;
+    r.weights[1] = kw;
+    for (Tensor& w : r.weights)
+        if (w.defined() && (!w.is_contiguous() || !aligned16(w.const_data_ptr()))) {
+            c10::AutoGradMode off(false);
+            OnDevice on(q.device());
+            w = w.clone(at::MemoryFormat::Contiguous);
+        }
     r.act = dtype_code(q.scalar_type());
     r.heads = {positions.numel(), (int)q.size(-2), (int)k.size(-2), (int)dim, (int)(2 * cos.size(1)), (const float*)cos.const_data_ptr(),
-               (const float*)sin.const_data_ptr(), cos.size(0), (const int64_t*)positions.const_data_ptr(), qw.defined() ? qw.const_data_ptr() : nullptr,
-               kw.defined() ? kw.const_data_ptr() : nullptr, dtype_code(wt), (float)eps};
+               (const float*)sin.const_data_ptr(), cos.size(0), (const int64_t*)positions.const_data_ptr(), qw.defined() ? r.weights[0].const_data_ptr() : nullptr,
+               kw.defined() ? r.weights[1].const_data_ptr() : nullptr, dtype_code(wt), (float)eps};
     return true;
 }
 
