@@ -12,16 +12,17 @@
 //   P^T = exp2(S^T c - r)            a lane holds query lane % 16, tokens 4 (lane / 16) + i of each half of the tile
 //   O^T[d][query] += V^T P^T         B = P^T as it lies there; A = V^T: a lane loads a piece of the rows of just those 8 tokens and pairs
 //                                    the tokens with byte permutes
-// The order of the head's values in an MFMA is free as long as K and Q agree, and that of the tokens as long as P and V agree, so nothing
-// crosses lanes: no LDS, no shuffles until the waves are joined.  r is only raised when a score passes it by some powers of two (one vote a tile).
+// The order of the head's values in an MFMA is free as long as K and Q agree, and that of the tokens as long as P and V agree, so between the two
+// products nothing crosses lanes, and there is no LDS before the waves are joined.  r is only raised when a score passes it by some powers of two (one vote
+// a tile, shuffles where it is raised).  Over codes pairs, weights and narrow pieces of V go from lane to lane in registers (DPP), see Fold and Exchange.
 //
 // P enters as 16-bit numbers, each rounded to nearest, whose sum it is: three in bfloat16, which hold all of a float32 (two, cut to 16 bits, gave every
 // 170th result of the largest case another bfloat16 neighbour than the exact value's, where float32 weights give every 1500th; three cost 0 ... 2 %), two in
 // float16.  Its steps end at 2^-24, so r is kept where the largest P is 2^12 ... 2^15: a weight errs by 2^-22 of itself or 2^-37 of the largest.  (With
 // the largest at 1 ... 2^8, and cut instead of rounded, 8192 weights e^-14 of one more came out 0.9 % low.)
 //
-// Fewer than 16 queries leave columns of the MFMAs empty: the matrix cores have room (16 KB of a 16-bit tile take 32 MFMAs, some 500 cycles
-// of one SIMD, and about 8000 cycles of a SIMD's share of HBM).
+// Fewer than 16 queries leave columns of the MFMAs empty: the matrix cores have room (16 KB of a 16-bit tile take 24 MFMAs in float16, 32 in
+// bfloat16, 400 and 500 cycles of one SIMD, and about 6000 cycles of a SIMD's share of HBM).
 //
 // Codes enter the MFMAs as they are: a whole number in the low bits of a 16-bit float is that number times 2^-24, a subnormal, which the matrix cores
 // take, so that unpacking is a byte permute or a shift and an AND for two codes.  They line products up as if a subnormal were 2^-14 and cut them
@@ -54,7 +55,7 @@ constexpr int kFirstReach = 100;
 constexpr float kLowest = -3.4028235e38f;
 
 // A segment that begins in a workgroup's piece (in its second slot) and goes on in the first slots of the next parts - 1 pieces; parts 0: none.
-struct Joint { uint32_t b, hq, parts, unused; };
+struct alignas(16) Joint { uint32_t b, hq, parts; };          // (what lies behind them in the workspace begins at 16 bytes)
 
 struct AttentionArgs {
     const uint16_t* q;
@@ -254,8 +255,8 @@ template <int N> BW_DEV uint32_t lane_after(uint32_t v) { return (uint32_t)__bui
 
 // Groups whose part for a lane is 1 or 2 bytes of a row of V: instead of that from each, lane m loads word m / MERGE of group m % MERGE, and the MERGE lanes of
 // one word index exchange their bytes or halves, so that each has its part of every group in one register.
-// 4 bits in groups of 32, 8 heads of 128: 104 against 118 us with 4 queries each (64 sequences of up to 8192 tokens), 67 against 80 with 16 (32 sequences);
-// 8 bits 125 against 122 and 84 against 89.
+// Groups of 32, 8 heads of 128: 102 against 169 us with 4 queries each (64 sequences of up to 8192 tokens), 68 against 98 with 16 (32 sequences);
+// 8 bits 127 against 175 and 91 against 111.
 template <int MERGE> struct Exchange {
     uint32_t pairs, quads;                       // byte selectors
     BW_DEV explicit Exchange(int m) : pairs(m & 1 ? 0x03070105u : 0x06020400u), quads(m & (MERGE / 2) ? 0x03020706u : 0x05040100u) {}
@@ -268,8 +269,8 @@ template <int MERGE> struct Exchange {
 // Few queries leave columns of the MFMAs empty, and with them most of what a lane does between the two products: over codes that is more than the
 // unpacking.  With 8 or fewer queries (FOLD 2) or 4 (FOLD 4) they are there 2 or 4 times, and the lanes of each copy ("part" m / (16 / FOLD)) take only
 // their share of the tile's tokens, kTokens = 8 / FOLD instead of 8 each; the weights go back to the first copy's lanes for the second product.
-// 64 sequences of up to 8192 tokens, 8 heads of 128, groups of 32, 4 queries: 119 against 144 us in 4 bits, 125 against 187 us in 8 (fewer registers go
-// to memory, too); groups of 128: 75.5 against 78 and 96 against 98 us.
+// 64 sequences of up to 8192 tokens, 8 heads of 128, groups of 32, 4 queries: 102 against 113 us in 4 bits, 127 against 152 us in 8 (fewer registers go
+// to memory, too); groups of 128: no difference; one sequence of 65537: 27.0 against 28.2.
 //   token j of part p is token 4 h + i of the lane's 8: FOLD 1: j;  2: h = p, i = j;  4: h = p / 2, i = 2 (p % 2) + j
 //   a group's pairs, one load for all: FOLD 1: lanes 0 ... 7 the keys' 8 tokens, 8 ... 15 the values';  2: lanes 4 c + i of part p the keys' and, in a
 //   second register, the values' token j = i;  4: lanes 0, 1 of the four of part p the keys' tokens, 2, 3 the values'
@@ -344,8 +345,8 @@ template <class F> constexpr bool kPast = F::kDim > 64;
 // Three for heads of 128 leave too few for groups of 32 (175 against 118 us in 4 bits) and won 4 % over groups of 128, nothing in 8 bits.
 constexpr int resident_workgroups(int dim) { return dim > 128 ? 1 : dim > 64 ? 2 : 3; }
 
-// Tiles that a wave has asked for.  Two where the registers hold them: 70 us against 74.5 at 64 sequences of up to 8192 tokens, 8 heads of 128, 4 bits in
-// groups of 128, 100 against 104 in groups of 32; with more of them in registers (8 or more queries) 67 us became 74, and 8 and 16 bits, whose
+// Tiles that a wave has asked for.  Two where the registers hold them: 74.3 us against 75.6 at 64 sequences of up to 8192 tokens, 8 heads of 128, 4 bits in
+// groups of 128, 102 against 104 in groups of 32; with more of them in registers (8 or more queries) 67 us became 74, and 8 and 16 bits, whose
 // tiles are larger, gain nothing or lose.
 template <class F, int FOLD> constexpr int tiles_ahead = F::kBits == 4 && F::kDim <= 128 && (F::kGroups <= 2 || FOLD == 4) ? 2 : 1;
 
@@ -800,7 +801,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
         const bool complete = g.from == 0 && to == g.tiles;
         float* slot = complete ? nullptr : a.partial + (int64_t)(2 * blockIdx.x + (g.from == 0)) * (2 * kQueries + a.queries * a.dim);
         if (!complete && g.from == 0 && threadIdx.x == 0)         // (the segment ends tiles - to units behind this piece)
-            a.joints[blockIdx.x] = Joint{g.b, g.hq, min(s.piece_of(position + g.units + g.tiles - to - 1), s.pieces - 1) - blockIdx.x + 1, 0};
+            a.joints[blockIdx.x] = Joint{g.b, g.hq, min(s.piece_of(position + g.units + g.tiles - to - 1), s.pieces - 1) - blockIdx.x + 1};
         auto joined = [&](int query, float& top) {                // sum of the waves' l, relative to the largest r
             top = fmaxf(fmaxf(stats[0][0][query], stats[1][0][query]), fmaxf(stats[2][0][query], stats[3][0][query]));
             float sum = 0.f;
