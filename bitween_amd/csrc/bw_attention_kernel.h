@@ -680,16 +680,19 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
 #pragma unroll
             for (int j = 1; j < Z::kTokens; j++) top = fmaxf(top, x[j]);
             const bool passed = __builtin_amdgcn_ballot_w64(top > r + (F::kCodes ? kSlack : kMost<F::kBf16>));
+            float keep = 1.f;
             int up = 0;
             if (passed) {
                 top = over_lanes(top);
-                if constexpr (F::kCodes) {                       // by whole powers of two, which round nothing
-                    const float raised = fmaxf(__builtin_ceilf(top), r);
-                    up = raised == r ? 0 : (int)fminf(raised - r, 300.f);
+                if constexpr (F::kCodes) {                       // by 2^up / keep, 2^up of it with the groups' reach
+                    const float raised = fmaxf(top, r), by = raised == r ? 0.f : fminf(raised - r, 300.f);
+                    up = (int)by;
+                    keep = __builtin_amdgcn_exp2f((float)up - by);
                     r = raised;
-                    l = __builtin_ldexpf(l, -up);
+                    l = __builtin_ldexpf(l * keep, -up);
                 } else {
-                    const float raised = fmaxf(top - kTop<F::kBf16>, r), keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
+                    const float raised = fmaxf(top - kTop<F::kBf16>, r);
+                    keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
                     r = raised;
                     l *= keep;
 #pragma unroll
@@ -726,7 +729,7 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                         reach[c] = __builtin_ldexpf(1.f, now);
 #pragma unroll
                         for (int j = 0; j < Z::kTokens; j++) ps[j] = __builtin_ldexpf(ps[j], now - was);
-                        const float by = __builtin_ldexpf(1.f, now - was - up);
+                        const float by = __builtin_ldexpf(keep, now - was - up);
 #pragma unroll
                         for (int j = 0; j < F::kPerV; j++) acc[c * F::kPerV + j] *= by;
                         zeros[c] *= by;

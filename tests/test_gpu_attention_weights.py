@@ -186,3 +186,26 @@ def test_values_at_the_upper_end_of_bfloat16(gap, tokens):
         # scores in float32: 2 (dim + 16) 2^-24 of at most gap + 1, of values below 2^128
         assert torch.isfinite(out[s]).all()
         assert bool(((out[s] - want).abs() <= half_step(torch.bfloat16) * want.abs() + 2 * 144 * 2.0 ** -24 * (gap + 1) * 2.0 ** 128).all())
+
+
+@pytest.mark.parametrize("bits,group,dtype", FORMATS)
+@pytest.mark.parametrize("heads", [2, 12, 32])
+def test_one_token_gives_its_values(heads, bits, group, dtype):
+    """A weight of 1 is exact: a sequence of one token gives what the cache holds, rounded once, whatever its score."""
+    b = Batch([1] * 70, heads, 2, 128, 16, bits, group or 64, dtype, seed=heads, spread=3.0)
+    c = b.cache
+    want = rows(c.values, c.value_meta, torch.cat(b.slots), bits, b.group).to(dtype).repeat_interleave(heads // 2, 1)
+    assert torch.equal(b.attend(), want)
+
+
+@pytest.mark.parametrize("bits,group,dtype", FORMATS)
+def test_one_token_above_all_gives_its_values(bits, group, dtype):
+    """So does the only token with a weight, wherever it lies: the others' scores are 2000 lower."""
+    for at in (0, 33, 299):
+        b = Batch([300, 700], 4, 2, 128, 16, bits, group or 64, dtype, seed=at)
+        b.q.fill_(1.0)
+        b.k[:300].fill_(-177.0)
+        b.k[at].fill_(1.0)
+        _filled(b)
+        want = rows(b.cache.values, b.cache.value_meta, b.slots[0][at:at + 1], bits, b.group).to(dtype).repeat_interleave(2, 1)
+        assert torch.equal(b.attend()[0], want[0])
