@@ -680,19 +680,16 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
 #pragma unroll
             for (int j = 1; j < Z::kTokens; j++) top = fmaxf(top, x[j]);
             const bool passed = __builtin_amdgcn_ballot_w64(top > r + (F::kCodes ? kSlack : kMost<F::kBf16>));
-            float keep = 1.f;
-            int up = 0;
+            float raise = 0.f;                                    // of r, over codes
             if (passed) {
                 top = over_lanes(top);
-                if constexpr (F::kCodes) {                       // by 2^up / keep, 2^up of it with the groups' reach
-                    const float raised = fmaxf(top, r), by = raised == r ? 0.f : fminf(raised - r, 300.f);
-                    up = (int)by;
-                    keep = __builtin_amdgcn_exp2f((float)up - by);
+                if constexpr (F::kCodes) {
+                    const float raised = fmaxf(top, r);
+                    raise = raised == r ? 0.f : fminf(raised - r, 300.f);
                     r = raised;
-                    l = __builtin_ldexpf(l * keep, -up);
+                    l *= __builtin_amdgcn_exp2f(-raise);
                 } else {
-                    const float raised = fmaxf(top - kTop<F::kBf16>, r);
-                    keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
+                    const float raised = fmaxf(top - kTop<F::kBf16>, r), keep = raised == r ? 1.f : __builtin_amdgcn_exp2f(r - raised);
                     r = raised;
                     l *= keep;
 #pragma unroll
@@ -722,14 +719,16 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                     });
                     if (passed || __builtin_amdgcn_ballot_w64(most > (float)(1 << kMost<false>))) {
                         most = over_lanes(most);
-                        // up with the reference, so that the group's weights stay where they are; down where they would pass 2^kMost
+                        // up with the reference (by whole powers of two; the rest goes into the sums), so that the group's weights stay where they
+                        // are; down where they would pass 2^kMost
+                        const int up = (int)raise;
                         const int was = __builtin_amdgcn_frexp_expf(reach[c]) - 1, high = most > 0.f ? __builtin_amdgcn_frexp_expf(most) - was : -1000;
                         int now = min(was + up, kFirstReach);
                         if (high + now > kMost<false>) now = min(kTop<false> + 1 - high, now);
                         reach[c] = __builtin_ldexpf(1.f, now);
 #pragma unroll
                         for (int j = 0; j < Z::kTokens; j++) ps[j] = __builtin_ldexpf(ps[j], now - was);
-                        const float by = __builtin_ldexpf(keep, now - was - up);
+                        const float by = __builtin_ldexpf(__builtin_amdgcn_exp2f((float)up - raise), now - was - up);
 #pragma unroll
                         for (int j = 0; j < F::kPerV; j++) acc[c * F::kPerV + j] *= by;
                         zeros[c] *= by;
