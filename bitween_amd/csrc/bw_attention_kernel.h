@@ -34,7 +34,8 @@
 // so no value is rounded on its way in.  What enters, P s, can be anything from 2^-24 to 2^16 times P, and a head's groups may be that far apart, so
 // every group has a power of two of its own for every query, its reach: P s times it is 2^12 ... 2^15 at its largest too, and the group's sums are
 // divided by it at the end.  P itself stays float32, and so do r and l.  (With one reference for all groups of a token a group 2^-10 of the largest
-// erred by 2^-10.  The reach costs 1 ... 3 % with heads of 128, 16 % with four groups of 64 to a head: one vote for each group.)
+// erred by 2^-10.  The reach and its vote for each group cost 1 ... 4 % with heads of 128, 9 % with 16 queries over groups of 32 in 8 bits, 18 % with four groups
+// of 64 to a head.)
 #pragma once
 #include "bw_cache.h"
 
@@ -337,7 +338,7 @@ template <int WORDS, bool NT = false> BW_DEV void load_words(const uint8_t* p, u
 }
 
 // Values are read past the caches, which leaves those to the keys, whose cache lines are taken by more than one load: 165 against 182 us at 64 sequences
-// of 2048 ... 8192 16-bit tokens (8 heads of 128), 96 against 106 us in 8 bits, the keys too no further use.  Not with 64 values to a head, whose loads
+// of up to 8192 16-bit tokens (8 heads of 128), 96 against 106 us in 8 bits, the keys too no further use.  Not with 64 values to a head, whose loads
 // of values share lines as well: 15.2 against 16.1 us at 128 sequences of 512.
 template <class F> constexpr bool kPast = F::kDim > 64;
 

@@ -290,7 +290,9 @@ int bw_cache_read(const bw_cache* cache, int out_dtype, int64_t T, const int64_t
  *   out = sum_t softmax_t(scale q . k_t) v_t,  t < lengths[b],  token t in row t % page_size of page page_table[b][t / page_size]
  * Query head h reads key-value head h / (q_heads / kv_heads).  Codes enter with their exact values scale * (code - zero point); scores, the
  * softmax and all sums are float32.  Over a bfloat16 cache the weights meet the values as float32 too; otherwise they err by 2^-22 of themselves
- * or, if more, 2^-37 of the largest (over codes: of the largest weight times scale of the same group).  out is rounded once.
+ * or, if more, 2^-37 of the largest (over codes: of the largest weight times scale of the same group).  Over codes a weight multiplies code and
+ * zero point apart, and sums of 32 products are cut 2^-16 (8 bits) or 2^-20 (4 bits) of a code's unit below the largest: at most 2^-18.9 of
+ * a group's range.  out is rounded once.
  * A sequence without tokens (length 0 or less) gets zeros.  A length beyond max_pages * page_size is taken as that; a page number outside
  * the cache is a page without tokens.  Rows behind a sequence's last token are not looked at, whatever they hold.  A score of minus infinity
  * has weight 0; a sequence without any other score gives NaN, as one of plus infinity or NaN does; an infinity or a NaN among the cached
