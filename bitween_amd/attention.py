@@ -7,7 +7,8 @@ key-value cache that may hold 8- or 4-bit codes, and the attention of one new to
 
 Each is one HIP kernel of libbitween_hip.so (the attention is joined by a second one where a sequence is cut, and so are the gradients of norm
 weights); they run on torch's current stream, allocate their outputs and workspaces from its allocator, and can be captured in HIP
-graphs.  There is no CPU path: CPU tensors raise.  The reference has no counterpart; its models bring these as eager torch operations.
+graphs.  Cache and attention have no derivatives: under grad mode a tensor that asks for gradients raises, a forward-mode tangent always (for the
+rotation too).  There is no CPU path: CPU tensors raise.  The reference has no counterpart; its models bring these as eager torch operations.
 """
 import torch
 from torch.autograd import forward_ad

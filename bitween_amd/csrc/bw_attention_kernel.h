@@ -720,9 +720,9 @@ __global__ __launch_bounds__(256, resident_workgroups(F::kDim)) void attention_k
                     });
                     if (passed || __builtin_amdgcn_ballot_w64(most > (float)(1 << kMost<false>))) {
                         most = over_lanes(most);
-                        // up with the reference (by whole powers of two; the rest goes into the sums), so that the group's weights stay where they
-                        // are; down where they would pass 2^kMost
-                        const int up = (int)raise;
+                        // up with the reference (by whole powers of two; what they are more goes into the sums), so that the group's weights do not
+                        // sink; down where they would pass 2^kMost
+                        const int up = (int)__builtin_ceilf(raise);
                         const int was = __builtin_amdgcn_frexp_expf(reach[c]) - 1, high = most > 0.f ? __builtin_amdgcn_frexp_expf(most) - was : -1000;
                         int now = min(was + up, kFirstReach);
                         if (high + now > kMost<false>) now = min(kTop<false> + 1 - high, now);
