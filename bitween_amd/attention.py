@@ -234,6 +234,62 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
                                                    *_cache_args(keys, values, key_meta, value_meta, bits, group_size), float(scale)))
 
 
+def _window(what, window, sinks):
+    """window (0: all tokens) and sinks as whole numbers."""
+    for n, name, least in ((window, "window", 1), (sinks, "sinks", 0)):
+        if n is None and name == "window":
+            continue
+        if not isinstance(n, int) or isinstance(n, bool):
+            raise TypeError(f"{what}: {name} must be a whole number, got {type(n).__name__}")
+        if n < least:
+            raise ValueError(f"{what}: {name} must be at least {least}, got {n}")
+    return min(window or 0, 2 ** 62), min(sinks, 2 ** 62)
+
+
+def prompt_attention(q, k, v, q_starts=None, k_starts=None, window=None, sinks=0, scale=None):
+    """Causal attention of many tokens of each sequence: a prompt's, a part of a long one's, training sequences'.
+
+        out = sum_t softmax_t(scale q . k_t) v_t   over the tokens t up to q's own: the last `window` of them (all where none is given) and the first `sinks`
+
+    q [batch, tokens, q_heads, dim], k and v [batch, all tokens, kv_heads, dim], or without the batch dimension for one sequence; or, with starts, the tokens of several
+    sequences one behind the other: q [tokens, q_heads, dim], sequence s from q_starts[s] to q_starts[s + 1] - 1 (int32 [sequences + 1]), and k and v likewise by k_starts (by
+    q_starts where none are given).  The tokens of q are the last ones of their sequence: with more keys than queries the first keys are those of a prompt's earlier
+    parts (as read_cache returns them).  kv_heads divides q_heads; query head h reads head h // (q_heads // kv_heads).  scale: 1 / sqrt(dim) where none is given.
+
+    Gradients of q, k and v; no second derivatives.  float16 or bfloat16; scores, softmax and sums are float32, a weight is rounded once to the type.  A token with nothing
+    to see (more queries than keys) gives zeros, and so do rows of q that belong to no sequence; other rows of k and v are not looked at.  Infinities and NaN
+    of one token touch what sees it, nothing else.  Starts are read on the GPU, so a captured call follows them; they must not decrease.  dim is a multiple
+    of 8 up to 256.  Leading dimensions that are not one stride are copied first."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
+    what = "prompt_attention"
+    width, first = _window(what, window, sinks)
+    if k_starts is None:
+        k_starts = q_starts
+    out = _native(what)(q, k, v, q_starts, k_starts, width, first, scale)
+    if out is not None:
+        return out
+    _tensor(q, "q", *_HALF)
+    _tensor(k, "k", q.dtype)
+    _tensor(v, "v", q.dtype)
+    if q.dim() not in ((3,) if q_starts is not None or k_starts is not None else (3, 4)) or 0 in q.shape[-2:]:
+        raise ValueError(f"q must be [batch, tokens, heads, dim], or [tokens, heads, dim] of one sequence or with starts, got {list(q.shape)}")
+    if k.dim() != q.dim() or k.shape != v.shape or k.shape[-1] != q.shape[-1] or k.shape[-2] < 1 or q.shape[-2] % k.shape[-2] or k.shape[:-3] != q.shape[:-3]:
+        raise ValueError(f"k and v must both be [..., tokens, a divisor of {q.shape[-2]} heads, {q.shape[-1]}] with q's batch, got {list(k.shape)} and {list(v.shape)}")
+    starts = [q_starts, k_starts]
+    if (q_starts is None) != (k_starts is None):
+        raise ValueError("k_starts without q_starts")
+    _one_gpu(what, q, k, v, *starts)
+    if q_starts is not None:
+        for t, name in zip(starts, ("q_starts", "k_starts")):
+            _tensor(t, name)
+            if t.dim() != 1 or len(t) < 2 or len(t) != len(q_starts):
+                raise ValueError("q_starts and k_starts must both be [sequences + 1], at least one sequence")
+        starts = [_whole(t, "q_starts / k_starts", torch.int32) for t in starts]
+    plain = [t if type(t) in (torch.Tensor, torch.nn.Parameter) else t.as_subclass(torch.Tensor) for t in (q, k, v)]
+    return _taken(what, _native(what)(*plain, *starts, width, first, float(scale)))
+
+
 class PagedCache:
     """The tensors of one layer's paged key-value cache and the calls on them.
 

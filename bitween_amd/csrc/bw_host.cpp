@@ -46,6 +46,10 @@ struct Library {
     decltype(&bw_cache_read) cache_read = nullptr;
     decltype(&bw_cache_attention) attention = nullptr;
     decltype(&bw_cache_attention_workspace_bytes) attention_ws_bytes = nullptr;
+    decltype(&bw_prompt_attention) prompt = nullptr;
+    decltype(&bw_prompt_attention_workspace_bytes) prompt_ws_bytes = nullptr;
+    decltype(&bw_prompt_attention_grad) prompt_grad = nullptr;
+    decltype(&bw_prompt_attention_grad_workspace_bytes) prompt_grad_ws_bytes = nullptr;
 } lib;
 
 PyObject* g_check = nullptr;          // Python: check(status, entry point's name) raises for a status other than 0
@@ -569,6 +573,16 @@ bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tens
     return true;
 }
 
+// Under create_graph: gradients that have no derivative of their own.
+void no_second_derivative(const char* what, torch::autograd::variable_list& grads) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (auto& v : grads)
+        if (v.defined()) {
+            auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", 1);
+            v = error->apply({v.detach().requires_grad_(true)})[0];
+        }
+}
+
 struct RotateHeadsBackward : public torch::autograd::Node {
     enum { Q, K, QW, KW, COS, SIN, POSITIONS };
     torch::autograd::SavedVariable saved[7];
@@ -613,20 +627,14 @@ struct RotateHeadsBackward : public torch::autograd::Node {
         }
         for (int i : {0, 1})
             if (!task_should_compute_output(i)) out[i] = Tensor();
-        if (c10::GradMode::is_enabled()) {                      // create_graph: these gradients have no derivative of their own
-            for (auto& v : out)
-                if (v.defined()) {
-                    auto error = std::make_shared<torch::autograd::DelayedError>("rotate_heads has no second derivative", 1);
-                    v = error->apply({v.detach().requires_grad_(true)})[0];
-                }
-        }
+        no_second_derivative("rotate_heads", out);
         return out;
     }
 };
 
 // Autograd runs a leaf's accumulation on the stream where its node was made.  A node that an eager graph keeps alive on another stream would
 // be waited for inside the capture, which a capture cannot do: refused here, while nothing is recorded yet.
-void check_capture(std::initializer_list<const Tensor*> inputs, at::DeviceIndex index) {
+void check_capture(const char* what, std::initializer_list<const Tensor*> inputs, at::DeviceIndex index) {
     const auto stream = c10::hip::getCurrentHIPStream(index);
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
@@ -635,7 +643,7 @@ void check_capture(std::initializer_list<const Tensor*> inputs, at::DeviceIndex 
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!node) continue;
         const auto on = node->stream();
-        TORCH_CHECK(!on || *on == stream.unwrap(), "rotate_heads: a graph recorded on another stream still holds the gradient accumulation of an input of this "
+        TORCH_CHECK(!on || *on == stream.unwrap(), what, ": a graph recorded on another stream still holds the gradient accumulation of an input of this "
                     "captured call; drop that graph (its outputs) before the capture");
     }
 }
@@ -659,7 +667,7 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if (c10::GradMode::is_enabled()) {
             if (cos.requires_grad() || sin.requires_grad()) return none();
         }
-        if (recorded) check_capture({&q, &k, &qw, &kw}, q.device().index());
+        if (recorded) check_capture("rotate_heads", {&q, &k, &qw, &kw}, q.device().index());
         Tensor q_out, k_out;
         int status = 0;
         {
@@ -864,6 +872,137 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     });
 }
 
+// ---- attention of prompts ----
+
+// What a call of prompt_attention is given: q, k, v [tokens, heads, dim] of sequences that begin at q_starts and k_starts, or [batch, tokens, heads, dim] (one
+// sequence without the first dimension) without them.
+bool prompt_of(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_starts, const Tensor& k_starts, int64_t window, int64_t sinks, double scale, bw_prompt& p) {
+    if (!lib.prompt || !q.is_cuda() || !q.has_storage() || !half_type(q.scalar_type()) || (q.dim() != 3 && q.dim() != 4)) return false;
+    for (const Tensor* t : {&k, &v})
+        if (!on_gpu(*t, q) || t->scalar_type() != q.scalar_type() || t->dim() != q.dim() || t->size(-1) != q.size(-1)) return false;
+    const int64_t heads = q.size(-2), kv = k.size(-2), dim = q.size(-1);
+    if (!v.sizes().equals(k.sizes()) || dim < 1 || dim > 65535 || kv < 1 || heads < 1 || heads > 65535 || heads % kv) return false;
+    int64_t sequences = 1;
+    if (q_starts.defined() != k_starts.defined()) return false;
+    if (q_starts.defined()) {
+        if (q.dim() != 3) return false;
+        for (const Tensor* t : {&q_starts, &k_starts})
+            if (!on_gpu(*t, q) || t->scalar_type() != at::kInt || t->dim() != 1 || !t->is_contiguous() || t->size(0) < 2 || t->size(0) >= (int64_t)1 << 31) return false;
+        if (q_starts.size(0) != k_starts.size(0)) return false;
+        sequences = q_starts.size(0) - 1;
+    } else if (q.dim() == 4) {
+        if (q.size(0) != k.size(0) || q.size(0) >= (int64_t)1 << 31) return false;
+        sequences = std::max<int64_t>(q.size(0), 1);
+    }
+    if (window < 0 || sinks < 0) return false;
+    const bool dense = q.dim() == 4;
+    p = {dense ? q.size(0) * q.size(1) : q.size(0), dense ? k.size(0) * k.size(1) : k.size(0), q_starts.defined() ? (const int32_t*)q_starts.const_data_ptr() : nullptr,
+         k_starts.defined() ? (const int32_t*)k_starts.const_data_ptr() : nullptr, (int)sequences, (int)heads, (int)kv, (int)dim, window, sinks, (float)scale};
+    return true;
+}
+
+// Rows whose distances are those that the kernels take: a copy otherwise.
+Rows prompt_rows(const Tensor& t, int64_t tokens, int64_t heads_together) {
+    Rows r(t, tokens);
+    if (r.row >= 1 << 24 || (heads_together - 1) * r.head + 65 * r.row >= (int64_t)1 << 31 || r.head >= (int64_t)1 << 30) {
+        r.held = r.held.clone(at::MemoryFormat::Contiguous);
+        r.data = r.held.const_data_ptr();
+        r.row = tokens <= 1 ? 0 : r.held.stride(0);
+        r.head = r.held.size(1) <= 1 ? 0 : r.held.stride(1);
+    }
+    return r;
+}
+
+struct PromptAttentionBackward : public torch::autograd::Node {
+    enum { Q, K, V, Q_STARTS, K_STARTS, LSE, OUT };
+    torch::autograd::SavedVariable saved[7];
+    int64_t window = 0, sinks = 0;
+    double scale = 0;
+    std::string name() const override { return "PromptAttentionBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (auto& v : saved) v.reset_data();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list out(3);
+        if (!grads[0].defined()) return out;
+        Tensor t[7];
+        for (int i = 0; i < 7; i++) t[i] = i == OUT ? saved[i].unpack(shared_from_this()) : saved[i].unpack();
+        const Tensor& g = grads[0];
+        OnDevice on(g.device());
+        {
+            c10::AutoGradMode off(false);
+            bw_prompt p;
+            TORCH_CHECK(prompt_of(t[Q], t[K], t[V], t[Q_STARTS], t[K_STARTS], window, sinks, scale, p) && g.sizes().equals(t[Q].sizes()) && g.scalar_type() == t[Q].scalar_type(),
+                        "bw_prompt_attention_grad: the gradient or what the forward saved has changed");
+            const int64_t share = p.q_heads / p.kv_heads;
+            const Rows rg = prompt_rows(g, p.q_tokens, share), rq = prompt_rows(t[Q], p.q_tokens, share), rk = prompt_rows(t[K], p.k_tokens, 1), rv = prompt_rows(t[V], p.k_tokens, 1);
+            for (int i : {0, 1, 2})
+                if (task_should_compute_output(i)) out[i] = empty(t[i].sizes(), t[i].scalar_type(), g.device());
+            const size_t bytes = lib.prompt_grad_ws_bytes(&p);
+            Tensor ws;
+            if (bytes) ws = empty({(int64_t)bytes}, at::kByte, g.device());
+            auto to = [&](int i) { return out[i].defined() ? out[i].mutable_data_ptr() : nullptr; };
+            const int st = lib.prompt_grad(&p, dtype_code(g.scalar_type()), rg.data, rg.row, rg.head, rq.data, rq.row, rq.head, rk.data, rk.row, rk.head, rv.data, rv.row, rv.head,
+                                           t[OUT].const_data_ptr(), (const float*)t[LSE].const_data_ptr(), to(0), to(1), to(2), bytes ? ws.mutable_data_ptr() : nullptr, bytes,
+                                           stream_of(g.device().index()));
+            TORCH_CHECK(st == BW_OK, "bw_prompt_attention_grad failed (status ", st, ")");
+        }
+        no_second_derivative("prompt_attention", out);
+        return out;
+    }
+};
+
+// prompt_attention(q, k, v, q_starts or None, k_starts or None, window (0: none), sinks, scale) -> out or None
+PyObject* py_prompt_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 8) return none();
+        for (int i = 0; i < 5; i++)
+            if (!plain(args[i]) && !(i >= 3 && args[i] == Py_None)) return none();
+        if (!PyLong_Check(args[5]) || !PyLong_Check(args[6])) return none();
+        const int64_t window = PyLong_AsLongLong(args[5]), sinks = PyLong_AsLongLong(args[6]);
+        const double scale = PyFloat_AsDouble(args[7]);
+        if (PyErr_Occurred()) return nullptr;
+        const Tensor q = unpack(args[0]), k = unpack(args[1]), v = unpack(args[2]);
+        const Tensor q_starts = args[3] == Py_None ? Tensor() : unpack(args[3]), k_starts = args[4] == Py_None ? Tensor() : unpack(args[4]);
+        bw_prompt p;
+        if (!prompt_of(q, k, v, q_starts, k_starts, window, sinks, scale, p)) return none();
+        check_tangents("prompt_attention", {&q, &k, &v});
+        const bool recorded = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+        if (recorded) check_capture("prompt_attention", {&q, &k, &v}, q.device().index());
+        Tensor out, lse;
+        int status = 0;
+        {
+            Unlocked unlocked;
+            c10::AutoGradMode off(false);
+            OnDevice on(q.device());
+            out = empty(q.sizes(), q.scalar_type(), q.device());
+            if (recorded) lse = empty({p.q_tokens * p.q_heads}, at::kFloat, q.device());
+            const int64_t share = p.q_heads / p.kv_heads;
+            const Rows rq = prompt_rows(q, p.q_tokens, share), rk = prompt_rows(k, p.k_tokens, 1), rv = prompt_rows(v, p.k_tokens, 1);
+            const size_t bytes = lib.prompt_ws_bytes(&p);
+            Tensor ws;
+            if (bytes) ws = empty({(int64_t)bytes}, at::kByte, q.device());
+            status = lib.prompt(&p, dtype_code(q.scalar_type()), rq.data, rq.row, rq.head, rk.data, rk.row, rk.head, rv.data, rv.row, rv.head, out.mutable_data_ptr(),
+                                recorded ? (float*)lse.mutable_data_ptr() : nullptr, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(q.device().index()));
+        }
+        if (status) return checked({}, status, "bw_prompt_attention");
+        if (recorded) {
+            std::shared_ptr<PromptAttentionBackward> node(new PromptAttentionBackward(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
+            const Tensor* keep[6] = {&q, &k, &v, &q_starts, &k_starts, &lse};
+            for (int i = 0; i < 6; i++) node->saved[i] = torch::autograd::SavedVariable(*keep[i], false);
+            node->window = window;
+            node->sinks = sinks;
+            node->scale = scale;
+            torch::autograd::set_history(out, node);
+            node->saved[PromptAttentionBackward::OUT] = torch::autograd::SavedVariable(out, true);
+        }
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 // bind({entry point name: address}, check, dict with the fused gradient's row limits): once, after the kernel library is loaded
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject *table, *check, *limits;
@@ -892,8 +1031,12 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(l.cache_read, "bw_cache_read");
     get(l.attention, "bw_cache_attention");
     get(l.attention_ws_bytes, "bw_cache_attention_workspace_bytes");
+    get(l.prompt, "bw_prompt_attention");
+    get(l.prompt_ws_bytes, "bw_prompt_attention_workspace_bytes");
+    get(l.prompt_grad, "bw_prompt_attention_grad");
+    get(l.prompt_grad_ws_bytes, "bw_prompt_attention_grad_workspace_bytes");
     if (PyErr_Occurred()) return nullptr;
-    if (!ok) l.rotate = nullptr, l.attention = nullptr;
+    if (!ok) l.rotate = nullptr, l.attention = nullptr, l.prompt = nullptr;
     if (!linears) {
         PyErr_SetString(PyExc_RuntimeError, "bind: an entry point is missing");
         return nullptr;
@@ -917,6 +1060,7 @@ PyMethodDef methods[] = {
     {"cache_write", (PyCFunction)(void*)py_cache_write, METH_FASTCALL, nullptr},
     {"cache_read", (PyCFunction)(void*)py_cache_read, METH_FASTCALL, nullptr},
     {"cache_attention", (PyCFunction)(void*)py_cache_attention, METH_FASTCALL, nullptr},
+    {"prompt_attention", (PyCFunction)(void*)py_prompt_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_bw_host", "Native host path of bitween_amd", -1, methods};

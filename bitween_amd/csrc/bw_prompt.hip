@@ -1,0 +1,248 @@
+// Causal attention of many tokens of each sequence (prompts, training), with a window and sinks, and its gradients: the C entry points, and the joins of what was
+// cut into parts.  The kernels are in bw_prompt_kernel.h and bw_prompt_grad_kernel.h, instantiated by bw_prompt_*.hip for each type.
+#include "bw_prompt_grad.h"
+
+#include <utility>
+
+namespace {
+
+// out = the parts of a row put together; a row's part: reference, sum, two unused, sums of the values [dim].  A thread has 4 values of a row.
+template <int DT>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, int threads, uint32_t rows) {
+    const uint32_t i = blockIdx.x * (256 / threads) + threadIdx.x / threads;
+    const int d = (int)(threadIdx.x % threads) * 4;
+    if (threadIdx.x / threads >= 256 / threads || i >= rows) return;
+    const int64_t pitch = a.dim + 4;
+    const float* part = a.partial + (int64_t)i * a.splits * pitch;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; s++) top = fmaxf(top, part[s * pitch]);
+    float sum = 0.f;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; s++) {
+        const float r = part[s * pitch];
+        if (r == -INFINITY) continue;                              // no key of this part is seen
+        const float f = __builtin_amdgcn_exp2f(r - top);
+        sum += f * part[s * pitch + 1];
+        o += f * *reinterpret_cast<const f4*>(part + s * pitch + 4 + d);
+    }
+    const bool empty = top == -INFINITY;
+    o *= empty ? 0.f : 1.f / sum;
+    uint32_t rest;
+    const uint32_t token_head = i / (uint32_t)a.share, j = i - token_head * a.share, head = token_head / (uint32_t)a.q_tokens;
+    rest = token_head - head * a.q_tokens;
+    store4<DT>(a.out + ((int64_t)rest * a.q_heads + head * a.share + j) * a.dim + d, o[0], o[1], o[2], o[3]);
+    if (a.lse && d == 0) a.lse[i] = empty ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+int prompt_check(const bw_prompt* p, int act_dtype) {
+    if (!p || p->q_tokens < 0 || p->k_tokens < 0 || p->sequences < 1 || p->q_heads < 1 || p->kv_heads < 1 || p->q_heads % p->kv_heads || p->dim < 1 || p->window < 0 ||
+        p->sinks < 0)
+        return BW_EINVAL;
+    if (!p->q_starts != !p->k_starts) return BW_EINVAL;
+    if (!p->q_starts && (p->q_tokens % p->sequences || p->k_tokens % p->sequences)) return BW_EINVAL;
+    if (act_dtype != BW_F16 && act_dtype != BW_BF16) return BW_EUNSUPPORTED;
+    if (p->dim % 8 || p->dim > 256 || p->q_heads > 65535 || p->sequences > 1 << 20) return BW_EUNSUPPORTED;
+    if (p->q_tokens >= (int64_t)1 << 31 || p->k_tokens >= (int64_t)1 << 31 || p->q_tokens + p->k_tokens >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    if (p->q_tokens * p->q_heads >= (int64_t)1 << 31 || (p->k_tokens + p->q_tokens) * p->kv_heads >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    if (!bw_aligned(p->q_starts, 4) || !bw_aligned(p->k_starts, 4)) return BW_EALIGN;
+    return BW_OK;
+}
+
+// Workgroups of `tile` rows (or keys) each: of a sequence, or slots for all of them.
+int64_t tiles_of(const bw_prompt* p, int64_t tokens, int share, int tile) {
+    return p->q_starts ? tokens * share / tile + p->sequences + 2 : (tokens / p->sequences * share + tile - 1) / tile;
+}
+
+PromptArgs args_of(const bw_prompt* p) {
+    PromptArgs a = {};
+    a.q_starts = p->q_starts; a.k_starts = p->k_starts;
+    a.q_tokens = (int)p->q_tokens; a.k_tokens = (int)p->k_tokens;
+    a.sequences = p->sequences;
+    a.seq_q = (int)(p->q_tokens / p->sequences); a.seq_k = (int)(p->k_tokens / p->sequences);
+    a.q_heads = p->q_heads; a.kv_heads = p->kv_heads; a.share = p->q_heads / p->kv_heads;
+    a.dim = p->dim;
+    // (a window of all tokens hides none)
+    a.window = (int)(p->window && p->window < p->k_tokens ? p->window : p->k_tokens > 0 ? p->k_tokens : 1);
+    a.sinks = (int)(p->sinks < p->k_tokens ? p->sinks : p->k_tokens);
+    a.combos = (uint32_t)(p->kv_heads * (int64_t)(p->q_starts ? 1 : p->sequences));
+    a.by_share = FastDiv((uint32_t)a.share);
+    a.by_combos = FastDiv(a.combos);
+    a.by_heads = FastDiv((uint32_t)p->kv_heads);
+    a.flip = p->scale < 0.f ? 0x80008000u : 0u;
+    // (scale 0: all scores that are numbers weigh the same, and hidden ones, minus infinity, stay hidden)
+    const float scale = __builtin_fabsf(p->scale) * 1.44269504088896340736f;
+    a.scale = scale < 1e-38f ? 1e-38f : scale;
+    return a;
+}
+
+int key_tile(int dim) { return dim > 128 ? 32 : 64; }
+
+// Parts that the keys of a tile of rows are cut into: where there are fewer tiles of rows than workgroups that the chip holds.
+constexpr int kPartTiles = 4;
+int splits_of(const bw_prompt* p) {
+    const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), resident = bw_device_cus() * (p->dim > 128 ? 1 : 2);
+    const int64_t blocks = p->kv_heads * (p->q_starts ? (p->q_tokens * share + kRows - 1) / kRows : p->sequences * tiles_of(p, p->q_tokens, share, kRows));
+    int64_t keys = p->k_tokens / (p->q_starts ? 1 : p->sequences);
+    const int64_t reach = p->window ? p->window + p->sinks + kRows / share + 2 : keys;
+    if (reach < keys) keys = reach;
+    const int64_t most = (keys + tile - 1) / tile / kPartTiles, want = blocks > 0 ? resident / blocks : 1;
+    const int64_t splits = want < most ? want : most;
+    return (int)(splits < 1 ? 1 : splits < 64 ? splits : 64);
+}
+
+// Gradients of keys and values from their parts: a thread has 4 values.
+template <int DT>
+__global__ __launch_bounds__(256) void prompt_grad_join_kernel(const float* parts, int splits, int64_t all, int dim, uint16_t* k_grad, uint16_t* v_grad) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;                 // of [keys][2][dim]
+    if (at >= all) return;
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; s++) x += *reinterpret_cast<const f4*>(parts + s * all + at);
+    const int64_t pair = at / dim;
+    uint16_t* out = pair & 1 ? v_grad : k_grad;
+    if (out) store4<DT>(out + (pair >> 1) * dim + (at - pair * dim), x[0], x[1], x[2], x[3]);
+}
+
+// How the gradients' work is cut, and where their workspace has what.
+constexpr int kGradKeys = 32 * kPromptWaves;
+struct GradPlan {
+    int splits, far, sinks;
+    size_t delta, parts, sink_parts;             // bytes
+};
+GradPlan grad_plan(const bw_prompt* p) {
+    const PromptArgs a = args_of(p);
+    const int64_t resident = bw_device_cus() * (p->dim > 128 ? 1 : 2), seq_q = p->q_tokens / (p->q_starts ? 1 : p->sequences);
+    const int64_t blocks = p->kv_heads * (p->q_starts ? (p->k_tokens + kGradKeys - 1) / kGradKeys : p->sequences * tiles_of(p, p->k_tokens, 1, kGradKeys));
+    const bool window = a.window < p->k_tokens;
+    // tiles of rows that a tile of keys meets, and all that there are
+    const int tile = key_tile(p->dim);
+    const int64_t all = (seq_q * a.share + tile - 1) / tile, near_ = window ? ((int64_t)(a.window + kGradKeys) * a.share + tile - 1) / tile : all;
+    GradPlan g = {};
+    const int64_t most = (near_ < all ? near_ : all) / kPartTiles, want = blocks > 0 ? (resident + blocks - 1) / blocks : 1, splits = want < most ? want : most;
+    g.splits = (int)(splits < 1 ? 1 : splits < 16 ? splits : 16);
+    if (window && a.sinks > 0 && p->q_tokens > 0) {
+        g.sinks = a.sinks;
+        const size_t one = (size_t)p->sequences * p->kv_heads * g.sinks * 2 * p->dim * sizeof(float);
+        int64_t far = (all + near_ - 1) / near_;
+        while (far > 1 && one * far > (size_t)256 << 20) far /= 2;
+        g.far = (int)(far < 64 ? far : 64);
+        g.sink_parts = one * g.far;
+    }
+    g.delta = ((size_t)(p->q_tokens * p->q_heads) + 3) / 4 * 16;
+    if (g.splits > 1) g.parts = (size_t)g.splits * p->k_tokens * p->kv_heads * 2 * p->dim * sizeof(float);
+    return g;
+}
+
+}  // namespace
+
+extern "C" size_t bw_prompt_attention_workspace_bytes(const bw_prompt* p) {
+    if (prompt_check(p, BW_F16) != BW_OK || p->q_tokens == 0) return 0;
+    const int splits = splits_of(p);
+    return splits > 1 ? (size_t)(p->q_tokens * p->q_heads) * splits * (p->dim + 4) * sizeof(float) : 0;
+}
+
+extern "C" int bw_prompt_attention(const bw_prompt* p, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                                   const void* v, int64_t v_row, int64_t v_head, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int st = prompt_check(p, act_dtype)) return st;
+    if (p->q_tokens == 0) return BW_OK;
+    if (!q || !out || (p->k_tokens > 0 && (!k || !v))) return BW_EINVAL;
+    if (!bw_aligned(q, 16) || !bw_aligned(k, 16) || !bw_aligned(v, 16) || !bw_aligned(out, 16) || !bw_aligned(lse, 4) || (q_row | q_head | k_row | k_head | v_row | v_head) % 8)
+        return BW_EALIGN;
+    // (a row's place in its tile of 64 is 32 bits of bytes)
+    if (k_row < 0 || v_row < 0 || k_row >= 1 << 24 || v_row >= 1 << 24) return BW_EUNSUPPORTED;
+    PromptArgs a = args_of(p);
+    a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+    a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+    a.out = (uint16_t*)out;
+    a.lse = lse;
+    a.splits = splits_of(p);
+    const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos * a.splits;
+    if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
+    a.tiles = (uint32_t)tiles;
+    const size_t bytes = bw_prompt_attention_workspace_bytes(p);
+    if (bytes) {
+        if (!workspace || workspace_bytes < bytes) return BW_EWORKSPACE;
+        if (!bw_aligned(workspace, 16)) return BW_EALIGN;
+        a.partial = (float*)workspace;
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    if (int failed = act_dtype == BW_F16 ? bw_launch_prompt_f16(a, (uint32_t)grid, st) : bw_launch_prompt_bf16(a, (uint32_t)grid, st)) return failed;
+    if (a.splits > 1) {
+        const int threads = p->dim / 4;
+        const uint32_t rows = (uint32_t)(p->q_tokens * p->q_heads), per = 256 / threads;
+        if (act_dtype == BW_F16) hipLaunchKernelGGL(prompt_join_kernel<BW_F16>, dim3((rows + per - 1) / per), dim3(256), 0, st, a, threads, rows);
+        else hipLaunchKernelGGL(prompt_join_kernel<BW_BF16>, dim3((rows + per - 1) / per), dim3(256), 0, st, a, threads, rows);
+        if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
+    }
+    return BW_OK;
+}
+
+extern "C" size_t bw_prompt_attention_grad_workspace_bytes(const bw_prompt* p) {
+    if (prompt_check(p, BW_F16) != BW_OK) return 0;
+    const GradPlan plan = grad_plan(p);
+    return plan.delta + plan.parts + plan.sink_parts;
+}
+
+extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const void* grad, int64_t grad_row, int64_t grad_head, const void* q, int64_t q_row,
+                                        int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* out,
+                                        const float* lse, void* q_grad, void* k_grad, void* v_grad, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int st = prompt_check(p, act_dtype)) return st;
+    if (p->q_tokens > 0 && (!grad || !q || !out || !lse)) return BW_EINVAL;
+    if (p->k_tokens > 0 && (!k || !v)) return BW_EINVAL;
+    if (!bw_aligned(grad, 16) || !bw_aligned(q, 16) || !bw_aligned(k, 16) || !bw_aligned(v, 16) || !bw_aligned(out, 16) || !bw_aligned(lse, 4) || !bw_aligned(q_grad, 16) ||
+        !bw_aligned(k_grad, 16) || !bw_aligned(v_grad, 16) || (grad_row | grad_head | q_row | q_head | k_row | k_head | v_row | v_head) % 8)
+        return BW_EALIGN;
+    const int64_t share = p->q_heads / p->kv_heads;
+    for (int64_t row : {k_row, v_row, q_row, grad_row})
+        if (row < 0 || row >= 1 << 24) return BW_EUNSUPPORTED;
+    // (a row's place in a tile of rows of a key head's query heads is 32 bits of bytes)
+    for (auto [row, head] : {std::pair<int64_t, int64_t>{q_row, q_head}, {grad_row, grad_head}})
+        if (head < 0 || head >= (int64_t)1 << 30 || (share - 1) * head + 65 * row >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    const GradPlan plan = grad_plan(p);
+    const size_t bytes = plan.delta + plan.parts + plan.sink_parts;
+    if (bytes) {
+        if (!workspace || workspace_bytes < bytes) return BW_EWORKSPACE;
+        if (!bw_aligned(workspace, 16)) return BW_EALIGN;
+    }
+    PromptGradArgs g = {};
+    g.p = args_of(p);
+    PromptArgs& a = g.p;
+    a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+    a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+    a.lse = const_cast<float*>(lse);
+    g.grad = (const uint16_t*)grad; g.grad_row = grad_row; g.grad_head = grad_head;
+    g.result = (const uint16_t*)out;
+    g.q_grad = (uint16_t*)q_grad; g.k_grad = (uint16_t*)k_grad; g.v_grad = (uint16_t*)v_grad;
+    g.delta = (float*)workspace;
+    g.parts = (float*)((char*)workspace + plan.delta);
+    g.sink_parts = (float*)((char*)workspace + plan.delta + plan.parts);
+    g.far = plan.far;
+    g.plain_scale = p->scale;
+    PromptGrids grids = {};
+    const bool keys = (k_grad || v_grad) && p->k_tokens > 0;
+    if (p->q_tokens > 0) {
+        const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos;
+        if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
+        grids.rows = (uint32_t)grid;
+        grids.row_tiles = (uint32_t)tiles;
+    }
+    if (keys) {
+        const int64_t tiles = tiles_of(p, p->k_tokens, 1, kGradKeys), grid = tiles * a.combos * plan.splits;
+        const int64_t far_combos = (int64_t)p->sequences * p->kv_heads, far = plan.far ? far_combos * plan.far * ((plan.sinks + kGradKeys - 1) / kGradKeys) : 0;
+        if (grid >= (int64_t)1 << 24 || far >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
+        grids.keys = (uint32_t)grid;
+        grids.key_tiles = (uint32_t)tiles;
+        grids.key_splits = (uint32_t)plan.splits;
+        grids.far = (uint32_t)far;
+        grids.far_combos = (uint32_t)far_combos;
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    if (int failed = act_dtype == BW_F16 ? bw_launch_prompt_grad_f16(g, grids, st) : bw_launch_prompt_grad_bf16(g, grids, st)) return failed;
+    if (keys && plan.splits > 1) {
+        const int64_t all = p->k_tokens * p->kv_heads * 2 * p->dim;
+        const dim3 grid((unsigned)((all / 4 + 255) / 256));
+        if (act_dtype == BW_F16) hipLaunchKernelGGL(prompt_grad_join_kernel<BW_F16>, grid, dim3(256), 0, st, g.parts, plan.splits, all, p->dim, g.k_grad, g.v_grad);
+        else hipLaunchKernelGGL(prompt_grad_join_kernel<BW_BF16>, grid, dim3(256), 0, st, g.parts, plan.splits, all, p->dim, g.k_grad, g.v_grad);
+        if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
+    }
+    return BW_OK;
+}

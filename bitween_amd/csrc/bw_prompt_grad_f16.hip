@@ -1,0 +1,6 @@
+// Gradients of the attention of prompts in float16.
+#include "bw_prompt_grad.h"
+
+int bw_launch_prompt_grad_f16(const PromptGradArgs& g, const PromptGrids& grids, hipStream_t stream) {
+    return with_head<BW_F16>(g.p.dim, [&](auto head) { return launch_prompt_grad<decltype(head)>(g, grids, stream); });
+}

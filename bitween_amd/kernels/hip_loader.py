@@ -24,7 +24,8 @@ _DTYPE_CODE = {torch.float16: BW_F16, torch.bfloat16: BW_BF16, torch.float32: BW
 ABI_VERSION = 10           # what bw_abi_version() of a matching library returns
 ENTRY_POINTS = ("bw_abi_version", "bw_strerror", "bw_quantize_pack", "bw_quantize_pack_add", "bw_dequantize", "bw_qgemv", "bw_qgemm",
                 "bw_qgemm_ws", "bw_qgemm_static", "bw_qgemm_workspace_bytes", "bw_qgemm_tile_rows", "bw_qgemm_tile_cols", "bw_qlinear", "bw_qlinear_ws", "bw_qlinear_workspace_bytes", "bw_qdgrad", "bw_qdgrad_workspace_bytes", "bw_qdgrad_tile_rows", "bw_qdgrad_rows_slices", "bw_cast_bf16_f16", "bw_qlinear_decode_rows", "bw_qgemv_last_kernel",
-                "bw_rotate_heads", "bw_rotate_heads_grad", "bw_rotate_heads_grad_workspace_bytes", "bw_cache_write", "bw_cache_read", "bw_cache_attention", "bw_cache_attention_workspace_bytes")
+                "bw_rotate_heads", "bw_rotate_heads_grad", "bw_rotate_heads_grad_workspace_bytes", "bw_cache_write", "bw_cache_read", "bw_cache_attention", "bw_cache_attention_workspace_bytes",
+                "bw_prompt_attention", "bw_prompt_attention_workspace_bytes", "bw_prompt_attention_grad", "bw_prompt_attention_grad_workspace_bytes")
 
 
 class BitweenHipError(RuntimeError):
@@ -43,6 +44,13 @@ class Cache(ctypes.Structure):
     _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("key_meta", ctypes.c_void_p), ("value_meta", ctypes.c_void_p),
                 ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int), ("page_size", ctypes.c_int), ("dim", ctypes.c_int), ("bits", ctypes.c_int),
                 ("group", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class Prompt(ctypes.Structure):
+    """bw_prompt"""
+    _fields_ = [("q_tokens", ctypes.c_int64), ("k_tokens", ctypes.c_int64), ("q_starts", ctypes.c_void_p), ("k_starts", ctypes.c_void_p),
+                ("sequences", ctypes.c_int), ("q_heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dim", ctypes.c_int), ("window", ctypes.c_int64),
+                ("sinks", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
 def library_path():
@@ -108,9 +116,13 @@ def load():
     lib.bw_cache_read.argtypes = [cache, i32, i64, vp, vp, vp, vp]
     lib.bw_cache_attention.argtypes = [cache, i32, vp, i64, i32, i64, i64, vp, i64, i64, vp, ctypes.c_float, vp, vp, size, vp]
     lib.bw_cache_attention_workspace_bytes.argtypes = [cache, i64, i32, i64]
-    for name in ("bw_rotate_heads_grad_workspace_bytes", "bw_cache_attention_workspace_bytes"):
+    prompt = ctypes.POINTER(Prompt)
+    lib.bw_prompt_attention.argtypes = [prompt, i32] + [vp, i64, i64] * 3 + [vp, vp, vp, size, vp]
+    lib.bw_prompt_attention_grad.argtypes = [prompt, i32] + [vp, i64, i64] * 4 + [vp] * 6 + [size, vp]
+    lib.bw_prompt_attention_workspace_bytes.argtypes = lib.bw_prompt_attention_grad_workspace_bytes.argtypes = [prompt]
+    for name in ("bw_rotate_heads_grad_workspace_bytes", "bw_cache_attention_workspace_bytes", "bw_prompt_attention_workspace_bytes", "bw_prompt_attention_grad_workspace_bytes"):
         getattr(lib, name).restype = size
-    for name in ("bw_rotate_heads", "bw_rotate_heads_grad", "bw_cache_write", "bw_cache_read", "bw_cache_attention"):
+    for name in ("bw_rotate_heads", "bw_rotate_heads_grad", "bw_cache_write", "bw_cache_read", "bw_cache_attention", "bw_prompt_attention", "bw_prompt_attention_grad"):
         getattr(lib, name).restype = i32
     for name in ("bw_quantize_pack", "bw_quantize_pack_add", "bw_dequantize", "bw_qgemv", "bw_qgemm", "bw_qgemm_ws", "bw_qgemm_static", "bw_qlinear"):
         getattr(lib, name).restype = i32

@@ -306,6 +306,49 @@ int bw_cache_attention(const bw_cache* cache, int act_dtype, const void* q, int6
                        const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, void* out,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Attention of many tokens of each sequence: prompts, training ----
+ *   out = sum_t softmax_t(scale q . k_t) v_t   over the tokens t that a new token sees: those up to its own, of them the last `window` and the first
+ *   `sinks` (window 0: all)
+ * The new tokens of a sequence are its last ones: the i-th of n new tokens among m has position m - n + i.  One without a token to see (m < n) gets zeros.
+ * Query head h reads key-value head h / (q_heads / kv_heads).
+ *   q, k, v   act_dtype (BW_F16 | BW_BF16): rows of tokens, `*_row` elements apart, a head `*_head` apart, a head's values adjacent; out [q_tokens][q_heads][dim]
+ *   q_starts, k_starts   int32 [sequences + 1], read on the GPU: sequence s has the new tokens q_starts[s] ... q_starts[s + 1] - 1 and the tokens k_starts[s] ...
+ *             k_starts[s + 1] - 1 of k and v.  Both NULL: q_tokens / sequences and k_tokens / sequences tokens each.  Rows of q that belong to no sequence get
+ *             zeros, rows of k and v that belong to none are not looked at.  A number outside the tensor is taken as its end; numbers that decrease leave
+ *             undefined results (and nothing outside the tensors is touched).
+ * Scores, the softmax and all sums are float32; a weight meets its value rounded once to act_dtype (in float16 scaled so that the largest of a row is near its upper end).
+ * A score of minus infinity has weight 0, and a row without any other score gives NaN, as one of plus infinity or NaN does; an infinity or a NaN among the values leaves
+ * nothing finite in its channel of the rows that see it, whatever its weight, and touches no others.
+ * dim a multiple of 8 up to 256, pointers, rows and heads aligned to 16 bytes, rows of k and v 0 ... 2^24 - 1 elements apart; fewer than 2^31 tokens and heads of tokens.
+ *   lse   float32 [q_tokens * q_heads] or NULL: what the gradients need of the forward
+ * Where there are few rows their keys are cut into parts, joined in a fixed order through a workspace of bw_prompt_attention_workspace_bytes(...) bytes (16-byte aligned; 0 =
+ * none needed). */
+typedef struct bw_prompt {
+    int64_t q_tokens, k_tokens;
+    const int32_t *q_starts, *k_starts;
+    int sequences, q_heads, kv_heads, dim;
+    int64_t window, sinks;
+    float scale;
+} bw_prompt;
+
+size_t bw_prompt_attention_workspace_bytes(const bw_prompt* prompt);
+
+int bw_prompt_attention(const bw_prompt* prompt, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                        const void* v, int64_t v_row, int64_t v_head, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients: q_grad [q_tokens][q_heads][dim], k_grad and v_grad [k_tokens][kv_heads][dim], each of which may be NULL, from grad, the gradient of out (strided like q).
+ * q, k, v, out and lse as the forward had and left them.  With P the weights: dV = P^T grad, dS = P (grad V^T - rowsum(grad out)), dQ = scale dS K, dK = scale dS^T Q; all sums
+ * float32, each in one order (the same inputs give the same bits); P and dS enter their second products rounded once to act_dtype (in float16 as a power of two times that of
+ * their row or key, so that small gradients keep their bits).  Rows of k and v that belong to no sequence get zeros; what an infinity or a NaN of one token touches is what
+ * sees it, or what it sees.
+ * Beside the forward's: rows of q and grad 0 ... 2^24 - 1 elements apart, a key head's query heads and 65 rows within 2^31 elements; a workspace of
+ * bw_prompt_attention_grad_workspace_bytes(...) bytes (16-byte aligned). */
+size_t bw_prompt_attention_grad_workspace_bytes(const bw_prompt* prompt);
+
+int bw_prompt_attention_grad(const bw_prompt* prompt, int act_dtype, const void* grad, int64_t grad_row, int64_t grad_head, const void* q, int64_t q_row, int64_t q_head,
+                             const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* out, const float* lse,
+                             void* q_grad, void* k_grad, void* v_grad, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
