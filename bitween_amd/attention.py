@@ -10,6 +10,8 @@ weights); they run on torch's current stream, allocate their outputs and workspa
 graphs.  Cache and attention have no derivatives: under grad mode a tensor that asks for gradients raises, a forward-mode tangent always (for the
 rotation too).  There is no CPU path: CPU tensors raise.  The reference has no counterpart; its models bring these as eager torch operations.
 """
+import operator
+
 import torch
 from torch.autograd import forward_ad
 
@@ -100,7 +102,26 @@ def _taken(what, out):
     return out
 
 
-def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e-6):
+def _axes(what, sections, interleaved, half):
+    """sections as a tuple of whole numbers that take all of a head's `half` pairs, or None."""
+    if not isinstance(interleaved, bool):
+        raise TypeError(f"{what}: interleaved must be True or False, got {type(interleaved).__name__}")
+    if sections is None:
+        if interleaved:
+            raise ValueError(f"{what}: interleaved without sections")
+        return None
+    try:
+        counts = tuple(operator.index(n) for n in sections)
+    except TypeError:
+        raise TypeError(f"{what}: sections must be whole numbers, got {sections!r}") from None
+    if not 1 <= len(counts) <= 4 or min(counts) < 0 or sum(counts) != half:
+        raise ValueError(f"{what}: sections must be one to four numbers of pairs, {half} in all, got {sections!r}")
+    if interleaved and any(n and (n - 1) * len(counts) + i >= half for i, n in enumerate(counts) if i):
+        raise ValueError(f"{what}: interleaved sections {counts} do not find their pairs among {half}")
+    return counts
+
+
+def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e-6, sections=None, interleaved=False):
     """Queries [..., q_heads, dim] and keys [..., k_heads, dim] turned by the angle of their token's position, as two new tensors:
 
         y = x * rsqrt(mean(x^2) + eps) * weight             (y = x without a weight)
@@ -111,10 +132,14 @@ def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     each may be None.  float16 or bfloat16; float32 arithmetic, one rounding.  Gradients of q, k and the weights (sums in a fixed order);
     none of cos and sin, and no second derivatives.  dim and 2 h are multiples of 8, dim up to 256.
     Leading dimensions that are not one stride (a transposed [batch, heads, tokens, dim]) are copied first."""
-    out = _native("rotate_heads")(q, k, cos, sin, positions, q_weight, k_weight, eps)
+    out = _native("rotate_heads")(q, k, cos, sin, positions, q_weight, k_weight, eps, sections, interleaved)
     if out is not None:
         return out
-    what = "rotate_heads"
+    return _taken("rotate_heads", _native("rotate_heads")(*_rotation("rotate_heads", q, k, cos, sin, positions, q_weight, k_weight, eps, sections, interleaved)))
+
+
+def _rotation(what, q, k, cos, sin, positions, q_weight, k_weight, eps, sections, interleaved):
+    """The arguments of a rotation, checked and as the kernels read them."""
     _tensor(q, "q", *_HALF)
     _tensor(k, "k", q.dtype)
     _tensor(cos, "cos", torch.float32, torch.float16, torch.bfloat16)
@@ -124,11 +149,15 @@ def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     if cos.dim() != 2 or cos.shape != sin.shape or 0 in cos.shape:
         raise ValueError("cos and sin must both be [table rows, rotary / 2]")
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
-        raise NotImplementedError("rotate_heads has no gradient of cos and sin")
+        raise NotImplementedError(f"{what} has no gradient of cos and sin")
     _no_tangent(what, cos, sin)
+    axes = _axes(what, sections, interleaved, cos.shape[1])
+    if axes and (positions.dim() < 1 or len(positions) != len(axes)):
+        raise ValueError(f"positions must be [{len(axes)}, ...], a row for each of the sections, got {list(positions.shape)}")
+    lead = positions.shape[1:] if axes else positions.shape
     for t, name in ((q, "q"), (k, "k")):
-        if t.dim() != positions.dim() + 2 or t.shape[:-2] != positions.shape or 0 in t.shape[-2:]:
-            raise ValueError(f"{name} must be [..., heads, dim] with the leading dimensions of positions {list(positions.shape)}, got {list(t.shape)}")
+        if t.dim() != len(lead) + 2 or t.shape[:-2] != lead or 0 in t.shape[-2:]:
+            raise ValueError(f"{name} must be [..., heads, dim] with the leading dimensions of positions {list(lead)}, got {list(t.shape)}")
     dim = q.shape[-1]
     if k.shape[-1] != dim or 2 * cos.shape[1] > dim:
         raise ValueError(f"q and k must have one head dimension, at least twice the {cos.shape[1]} columns of cos")
@@ -140,7 +169,7 @@ def rotate_heads(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     # (a leaf goes on as it is: what a capture asks of its gradient's accumulation is asked of the leaf itself)
     plain = [t if t is None or type(t) in (torch.Tensor, torch.nn.Parameter) else t.as_subclass(torch.Tensor) for t in (q, k, q_weight, k_weight)]
     tables = [t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (_hip._plain(t).float() for t in (cos, sin))]
-    return _taken(what, _native("rotate_heads")(plain[0], plain[1], *tables, _whole(positions, "positions", torch.int64), plain[2], plain[3], float(eps)))
+    return plain[0], plain[1], *tables, _whole(positions, "positions", torch.int64), plain[2], plain[3], float(eps), axes, interleaved
 
 
 def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=16, group_size=64):
@@ -158,6 +187,13 @@ def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=
     if _native("cache_write")(k, v, slots, keys, values, key_meta, value_meta, bits, group_size):
         return
     what = "write_cache"
+    _checked_written(what, k, v, slots, keys, values, key_meta, value_meta, bits, group_size)
+    _taken(what, _native("cache_write")(_hip._plain(k), _hip._plain(v), _whole(slots, "slots", torch.int64),
+                                        *_cache_args(keys, values, key_meta, value_meta, bits, group_size)))
+
+
+def _checked_written(what, k, v, slots, keys, values, key_meta, value_meta, bits, group_size):
+    """Keys and values that fit their slots and the cache that they are written into."""
     dim = _checked_cache(what, keys, values, key_meta, value_meta, bits, group_size)
     for t, name in ((k, "k"), (v, "v")):
         _tensor(t, name, *((keys.dtype,) if bits == 16 else _HALF))
@@ -173,8 +209,31 @@ def write_cache(k, v, slots, keys, values, key_meta=None, value_meta=None, bits=
     for a, b in ((keys, values), (key_meta, value_meta)):
         if a is not None and a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes:
             raise ValueError(f"{what}: keys and values of a cache that is written must not share memory")
-    _taken(what, _native("cache_write")(_hip._plain(k), _hip._plain(v), _whole(slots, "slots", torch.int64),
-                                        *_cache_args(keys, values, key_meta, value_meta, bits, group_size)))
+
+
+def append_cache(q, k, v, cos, sin, positions, slots, keys, values, key_meta=None, value_meta=None, bits=16, group_size=64, q_weight=None, k_weight=None, eps=1e-6, sections=None,
+                 interleaved=False):
+    """rotate_heads and write_cache in one kernel: queries [tokens, q_heads, dim] and keys [tokens, kv_heads, dim] turned by their token's position, the keys and the values
+    [tokens, kv_heads, dim] written into the rows `slots` of the cache.  Returns the rotated queries.
+
+    Arguments as those two take them (positions [tokens], or [axes, tokens] with sections).  A norm's 1 / sqrt(mean(x^2) + eps) is formed in float64 and
+    rounded once; a key is rounded to its type before it is quantised: without norms, queries and cache are the bits that the two calls leave.  A token whose position
+    lies outside the table gets zeros as queries and is left out of the cache.  No gradients."""
+    out = _native("cache_append")(q, k, v, cos, sin, positions, slots, keys, values, key_meta, value_meta, bits, group_size, q_weight, k_weight, eps, sections, interleaved)
+    if out is not None:
+        return out
+    what = "append_cache"
+    _checked_written(what, k, v, slots, keys, values, key_meta, value_meta, bits, group_size)
+    _tensor(q, "q", k.dtype)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [tokens, heads, dim], got {list(q.shape)}")
+    q, k, cos, sin, positions, q_weight, k_weight, eps, sections, interleaved = _rotation(what, q, k, cos, sin, positions, q_weight, k_weight, eps, sections, interleaved)
+    _one_gpu(what, keys, q)
+    _no_grad(what, q, cos, sin, q_weight, k_weight)
+    _no_tangent(what, q, q_weight, k_weight)
+    return _taken(what, _native("cache_append")(*map(_hip._plain, (q, k, v, cos, sin)), positions, _whole(slots, "slots", torch.int64),
+                                                *_cache_args(keys, values, key_meta, value_meta, bits, group_size),
+                                                *(None if w is None else _hip._plain(w) for w in (q_weight, k_weight)), eps, sections, interleaved))
 
 
 def read_cache(slots, keys, values, key_meta=None, value_meta=None, bits=16, group_size=64, dtype=None):
@@ -329,6 +388,11 @@ class PagedCache:
     def write(self, k, v, slots):
         """write_cache into this cache."""
         write_cache(k, v, slots, self.keys, self.values, self.key_meta, self.value_meta, self.bits, self.group_size)
+
+    def append(self, q, k, v, cos, sin, positions, slots, q_weight=None, k_weight=None, eps=1e-6, sections=None, interleaved=False):
+        """append_cache into this cache; the rotated queries."""
+        return append_cache(q, k, v, cos, sin, positions, slots, self.keys, self.values, self.key_meta, self.value_meta, self.bits, self.group_size, q_weight, k_weight, eps,
+                            sections, interleaved)
 
     def read(self, slots):
         """read_cache of this cache, in its dtype."""

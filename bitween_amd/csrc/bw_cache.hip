@@ -4,15 +4,7 @@
 // cross-lane moves (their number divides 64 and every row starts at a multiple of it, so a group never leaves its wave), and the first of
 // them stores the group's pair.
 //
-// The code of x is rint(x / s) of the exact quotient: with r = 1 / s to within a unit of its last place, t = x r and one step t + (x - t s) r the
-// result is the correctly rounded quotient wherever rint could tell a difference - x has at most 11 significant bits and s 11, so a
-// quotient up to 256 that is not exactly half way between two whole numbers lies at least 2^-13 from half way, and one that is half way has at
-// most 10 bits, which the step returns exactly (the residual is exact in the fused operation).  The range over 15 or 255 is that step too, with the
-// correctly rounded reciprocal: the correctly rounded quotient (checked over a whole binade and samples of all others).
-//
-// Extrema of 16-bit floats are whole-number maxima of their bits: a positive value's bits grow with it, a negative one's are negative, so
-// max(0, bits) over a group is its largest value (or 0), max(0, bits ^ sign) its most negative one, and an infinity or a NaN shows as bits from the
-// infinity's on.  Both fit one register on the way over the lanes.
+// How a group's scale and codes are found is in bw_cache.h.
 //
 // Both kernels are one pass over memory: what bounds them is HBM beyond a few hundred tokens and the launch below.  32768 tokens of 8 heads of 128
 // at 8 bits (203 MB each way): 38 us to write, 36 us to read back, 5.3 and 5.6 TB/s; a copy reaches 5.2.
@@ -55,9 +47,6 @@ BW_DEV Unit unit_of(const CacheArgs& a, uint32_t i) {
     return u;
 }
 
-// Larger of the two 16-bit whole numbers of each half.
-typedef short s2 __attribute__((ext_vector_type(2)));
-BW_DEV uint32_t max16(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s2, a), __builtin_bit_cast(s2, b))); }
 template <int CTRL> BW_DEV uint32_t max16_over(uint32_t v) { return max16(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false)); }
 
 // Workgroups go to the eight dies in turn: here each die gets kRun neighbouring ones of every 8 kRun, so that the pairs of neighbouring tokens,
@@ -92,55 +81,24 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheArgs a) {
     if constexpr (BITS == 16) {
         if (kept) *reinterpret_cast<u4*>(out + (row_index(a, slot, u.head) * a.dim + u.chunk * 8) * 2) = u4{w[0], w[1], w[2], w[3]};
     } else {
-        constexpr float top = (float)((1 << BITS) - 1), inv_top = 1.f / top;
-        uint32_t hi = 0, lo = 0;
-#pragma unroll
-        for (int j = 0; j < V / 2; j++) {
-            hi = max16(hi, w[j]);
-            lo = max16(lo, w[j] ^ 0x80008000u);
-        }
-        // low half: the largest value, high half: the size of the most negative one
-        uint32_t both = max16(__builtin_amdgcn_perm(lo, hi, 0x05040100u), __builtin_amdgcn_perm(lo, hi, 0x07060302u));
+        uint32_t both = extrema_of<V / 2>(w);
         both = max16_over<0xB1>(both);                          // quad_perm: the neighbour
         if (a.group_shift > 1) both = max16_over<0x4E>(both);   // ... and the other two of four
         if (a.group_shift > 2) both = max16_over<0x141>(both);  // row_half_mirror: the other four of eight
-        constexpr uint32_t inf = DT == BW_F16 ? 0x7C00u : 0x7F80u;
-        const bool bad = (both & 0xFFFFu) >= inf || (both >> 16) >= inf;
-        const float largest = widen16<DT>((uint16_t)both), smallest = -widen16<DT>((uint16_t)(both >> 16));
-        // the scale rounds up, so that no code has to be clipped for its rounding; never 0
-        const float range = largest - smallest, t0 = range * inv_top;
-        const float step = fminf(__builtin_fmaf(__builtin_fmaf(-t0, top, range), inv_top, t0), 65504.f);
-        uint32_t sb = __builtin_bit_cast(uint16_t, (_Float16)step);
-        sb += f16_bits(sb) < step ? 1 : 0;
-        sb = sb ? sb : 1;
-        const float s = f16_bits(sb), r = __builtin_amdgcn_rcpf(s);
-        // 1.5 2^23 added: the nearest whole number (ties to even) in the low bits, and whole numbers may be added to it
-        constexpr float kWhole = 12582912.f;
-        auto whole = [&](float v) {
-            const float t = v * r;
-            return __builtin_fmaf(__builtin_fmaf(-t, s, v), r, t) + kWhole;
-        };
-        const float z = fminf(whole(-smallest) - kWhole, top);
+        const GroupCoder<DT, BITS> group(both);
         uint32_t q[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const float x = whole(widen16<DT>((uint16_t)(w[j / 2] >> (16 * (j & 1))))) + z;
-            q[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_fmed3f(x, kWhole, kWhole + top));   // (a group with a NaN is marked by its scale)
-        }
+        for (int j = 0; j < V; j++) q[j] = group.code(widen16<DT>((uint16_t)(w[j / 2] >> (16 * (j & 1)))));
         if (kept) {
-            auto bytes = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
-                return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0C0C0400u), __builtin_amdgcn_perm(b1, b0, 0x0C0C0400u), 0x05040100u);
-            };
             uint8_t* dst = out + row_index(a, slot, u.head) * (a.dim * BITS / 8) + u.chunk * (V * BITS / 8);
             if constexpr (BITS == 8) {
-                *reinterpret_cast<u4*>(dst) = u4{bytes(q[0], q[1], q[2], q[3]), bytes(q[4], q[5], q[6], q[7]), bytes(q[8], q[9], q[10], q[11]), bytes(q[12], q[13], q[14], q[15])};
+                *reinterpret_cast<u4*>(dst) = u4{bytes_of(q[0], q[1], q[2], q[3]), bytes_of(q[4], q[5], q[6], q[7]), bytes_of(q[8], q[9], q[10], q[11]), bytes_of(q[12], q[13], q[14], q[15])};
             } else {
-                *reinterpret_cast<u2*>(dst) = u2{bytes(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4),
-                                                 bytes(q[8] | q[9] << 4, q[10] | q[11] << 4, q[12] | q[13] << 4, q[14] | q[15] << 4)};
+                *reinterpret_cast<u2*>(dst) = u2{bytes_of(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4),
+                                                 bytes_of(q[8] | q[9] << 4, q[10] | q[11] << 4, q[12] | q[13] << 4, q[14] | q[15] << 4)};
             }
             if ((u.chunk & ((1 << a.group_shift) - 1)) == 0)
-                (u.value ? a.value_meta : a.key_meta)[pair_index(a, slot, u.head, u.chunk >> a.group_shift)] =
-                    (bad ? 0x7E00u : sb) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)z) << 16;
+                (u.value ? a.value_meta : a.key_meta)[pair_index(a, slot, u.head, u.chunk >> a.group_shift)] = group.pair;
         }
     }
 }
@@ -203,12 +161,6 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheArgs a) {
         if constexpr (UN > 1) __builtin_nontemporal_store(w[n], reinterpret_cast<u4*>(out));
         else *reinterpret_cast<u4*>(out) = w[n];
     }
-}
-
-// Two pieces of memory of `bytes` that share some.
-bool overlap(const void* a, const void* b, int64_t bytes) {
-    const int64_t apart = (int64_t)((const char*)a - (const char*)b);
-    return apart < bytes && apart > -bytes;
 }
 
 CacheArgs args_of(const bw_cache* c, int values) {
@@ -277,7 +229,7 @@ extern "C" int bw_cache_write(const bw_cache* c, int act_dtype, int64_t T, const
     if (T == 0) return BW_OK;
     if (!bw_aligned(k, 16) || !bw_aligned(v, 16) || !bw_aligned(slots, 8) || (k_row | k_head | v_row | v_head) % 8) return BW_EALIGN;
     const int64_t values = c->pages * c->page_size * c->kv_heads * c->dim;
-    if (overlap(c->keys, c->values, values / 8 * c->bits) || (c->bits != 16 && overlap(c->key_meta, c->value_meta, values / c->group * 4))) return BW_EINVAL;
+    if (bw_overlap(c->keys, c->values, values / 8 * c->bits) || (c->bits != 16 && bw_overlap(c->key_meta, c->value_meta, values / c->group * 4))) return BW_EINVAL;
     CacheArgs a = args_of(c, c->bits == 16 ? kWriteValues<16> : kWriteValues<8>);
     a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
     a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;

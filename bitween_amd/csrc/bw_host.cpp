@@ -42,6 +42,9 @@ struct Library {
     decltype(&bw_rotate_heads) rotate = nullptr;
     decltype(&bw_rotate_heads_grad) rotate_grad = nullptr;
     decltype(&bw_rotate_heads_grad_workspace_bytes) rotate_grad_ws_bytes = nullptr;
+    decltype(&bw_rotate_axes) rotate_axes = nullptr;
+    decltype(&bw_rotate_axes_grad) rotate_axes_grad = nullptr;
+    decltype(&bw_cache_append) append = nullptr;
     decltype(&bw_cache_write) cache_write = nullptr;
     decltype(&bw_cache_read) cache_read = nullptr;
     decltype(&bw_cache_attention) attention = nullptr;
@@ -539,12 +542,31 @@ struct Rotation {
     Tensor weights[2];                                          // the queries' and the keys', as the kernels read them
 };
 
+// sections (None or a tuple of up to four numbers) and interleaved; count 0: one position for each token.
+bool axes_of(PyObject* sections, PyObject* interleaved, bw_axes& axes) {
+    axes = {};
+    if (sections == Py_None) return interleaved == Py_False;
+    if (!PyTuple_Check(sections) || PyTuple_GET_SIZE(sections) < 1 || PyTuple_GET_SIZE(sections) > 4 || !PyBool_Check(interleaved)) return false;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sections); i++) {
+        PyObject* n = PyTuple_GET_ITEM(sections, i);
+        if (!PyLong_CheckExact(n)) return false;
+        const long v = PyLong_AsLong(n);
+        if (PyErr_Occurred() || v < 0 || v > 65535) return false;
+        axes.sections[i] = (int)v;
+    }
+    axes.count = (int)PyTuple_GET_SIZE(sections);
+    axes.interleaved = interleaved == Py_True;
+    return true;
+}
+
 bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions, const Tensor& qw, const Tensor& kw,
-                 double eps, Rotation& r) {
+                 double eps, const bw_axes& axes, Rotation& r) {
     if (!lib.rotate || !q.is_cuda() || !q.has_storage() || !half_type(q.scalar_type()) || k.scalar_type() != q.scalar_type()) return false;
     for (const Tensor* t : {&k, &cos, &sin, &positions})
         if (!on_gpu(*t, q)) return false;
-    if (positions.scalar_type() != at::kLong || !positions.is_contiguous() || !heads_of(q, positions.sizes()) || !heads_of(k, positions.sizes())) return false;
+    if (positions.scalar_type() != at::kLong || !positions.is_contiguous() || (axes.count && (positions.dim() < 1 || positions.size(0) != axes.count))) return false;
+    const at::IntArrayRef lead = axes.count ? positions.sizes().slice(1) : positions.sizes();
+    if (!heads_of(q, lead) || !heads_of(k, lead)) return false;
     const int64_t dim = q.size(-1);
     if (k.size(-1) != dim || q.size(-2) > 65535 || k.size(-2) > 65535 || dim > 65535) return false;
     for (const Tensor* t : {&cos, &sin})
@@ -567,7 +589,15 @@ bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tens
             w = w.clone(at::MemoryFormat::Contiguous);
         }
     r.act = dtype_code(q.scalar_type());
-    r.heads = {positions.numel(), (int)q.size(-2), (int)k.size(-2), (int)dim, (int)(2 * cos.size(1)), (const float*)cos.const_data_ptr(),
+    if (axes.count) {
+        int64_t pairs = 0;
+        for (int i = 0; i < axes.count; i++) {
+            pairs += axes.sections[i];
+            if (axes.interleaved && i && axes.sections[i] && (axes.sections[i] - 1) * (int64_t)axes.count + i >= cos.size(1)) return false;
+        }
+        if (pairs != cos.size(1)) return false;
+    }
+    r.heads = {positions.numel() / std::max(axes.count, 1), (int)q.size(-2), (int)k.size(-2), (int)dim, (int)(2 * cos.size(1)), (const float*)cos.const_data_ptr(),
                (const float*)sin.const_data_ptr(), cos.size(0), (const int64_t*)positions.const_data_ptr(), qw.defined() ? r.weights[0].const_data_ptr() : nullptr,
                kw.defined() ? r.weights[1].const_data_ptr() : nullptr, dtype_code(wt), (float)eps};
     return true;
@@ -589,6 +619,7 @@ struct RotateHeadsBackward : public torch::autograd::Node {
     c10::SmallVector<int64_t, 5> q_sizes, k_sizes;
     at::ScalarType type = at::kHalf;
     double eps = 0;
+    bw_axes axes = {};
     std::string name() const override { return "RotateHeadsBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -605,7 +636,7 @@ struct RotateHeadsBackward : public torch::autograd::Node {
         {
             c10::AutoGradMode off(false);
             Rotation r;
-            TORCH_CHECK(rotation_of(gq, gk, t[COS], t[SIN], t[POSITIONS], t[QW], t[KW], eps, r), "bw_rotate_heads_grad: the gradients or what the forward saved have changed");
+            TORCH_CHECK(rotation_of(gq, gk, t[COS], t[SIN], t[POSITIONS], t[QW], t[KW], eps, axes, r), "bw_rotate_heads_grad: the gradients or what the forward saved have changed");
             const int64_t tokens = r.heads.tokens;
             const Rows rgq(gq, tokens), rgk(gk, tokens);
             Rows rq, rk;
@@ -619,10 +650,12 @@ struct RotateHeadsBackward : public torch::autograd::Node {
             size_t bytes = 0;
             if (out[2].defined() || out[3].defined()) bytes = lib.rotate_grad_ws_bytes(&r.heads);
             if (bytes) ws = empty({(int64_t)bytes}, at::kByte, gq.device());
-            const int st = lib.rotate_grad(&r.heads, r.act, rgq.data, rgq.row, rgq.head, rgk.data, rgk.row, rgk.head, rq.data, rq.row, rq.head, rk.data, rk.row,
-                                           rk.head, out[0].mutable_data_ptr(), out[1].mutable_data_ptr(), out[2].defined() ? out[2].mutable_data_ptr() : nullptr,
-                                           out[3].defined() ? out[3].mutable_data_ptr() : nullptr, bytes ? ws.mutable_data_ptr() : nullptr, bytes,
-                                           stream_of(gq.device().index()));
+            auto grad = [&](auto entry, auto... axes) {
+                return entry(&r.heads, axes..., r.act, rgq.data, rgq.row, rgq.head, rgk.data, rgk.row, rgk.head, rq.data, rq.row, rq.head, rk.data, rk.row, rk.head,
+                             out[0].mutable_data_ptr(), out[1].mutable_data_ptr(), out[2].defined() ? out[2].mutable_data_ptr() : nullptr,
+                             out[3].defined() ? out[3].mutable_data_ptr() : nullptr, bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(gq.device().index()));
+            };
+            const int st = axes.count ? grad(lib.rotate_axes_grad, (const bw_axes*)&axes) : grad(lib.rotate_grad);
             TORCH_CHECK(st == BW_OK, "bw_rotate_heads_grad failed (status ", st, ")");
         }
         for (int i : {0, 1})
@@ -648,10 +681,10 @@ void check_capture(const char* what, std::initializer_list<const Tensor*> inputs
     }
 }
 
-// rotate_heads(q, k, cos, sin, positions, q_weight or None, k_weight or None, eps) -> (q, k) or None
+// rotate_heads(q, k, cos, sin, positions, q_weight or None, k_weight or None, eps[, sections or None, interleaved]) -> (q, k) or None
 PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return guarded([&]() -> PyObject* {
-        if (nargs != 8) return none();
+        if (nargs != 8 && nargs != 10) return none();
         for (int i = 0; i < 7; i++)
             if (!plain(args[i]) && !(i >= 5 && args[i] == Py_None)) return none();
         const double eps = PyFloat_AsDouble(args[7]);
@@ -659,7 +692,11 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const Tensor q = unpack(args[0]), k = unpack(args[1]), cos = unpack(args[2]), sin = unpack(args[3]), positions = unpack(args[4]);
         const Tensor qw = args[5] == Py_None ? Tensor() : unpack(args[5]), kw = args[6] == Py_None ? Tensor() : unpack(args[6]);
         Rotation r;
-        if (!rotation_of(q, k, cos, sin, positions, qw, kw, eps, r)) return none();
+        bw_axes axes = {};
+        if ((nargs == 10 && !axes_of(args[8], args[9], axes)) || !rotation_of(q, k, cos, sin, positions, qw, kw, eps, axes, r)) {
+            if (PyErr_Occurred()) return nullptr;
+            return none();
+        }
         check_tangents("rotate_heads", {&q, &k, &qw, &kw, &cos, &sin});
         bool recorded = false;
         for (const Tensor* t : {&q, &k, &qw, &kw}) recorded |= t->defined() && t->requires_grad();
@@ -678,8 +715,11 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             k_out = empty(k.sizes(), q.scalar_type(), q.device());
             if (r.heads.tokens > 0) {
                 const Rows rq(q, r.heads.tokens), rk(k, r.heads.tokens);
-                status = lib.rotate(&r.heads, r.act, rq.data, rq.row, rq.head, rk.data, rk.row, rk.head, q_out.mutable_data_ptr(), k_out.mutable_data_ptr(),
-                                    stream_of(q.device().index()));
+                auto rotate = [&](auto entry, auto... axes) {
+                    return entry(&r.heads, axes..., r.act, rq.data, rq.row, rq.head, rk.data, rk.row, rk.head, q_out.mutable_data_ptr(), k_out.mutable_data_ptr(),
+                                 stream_of(q.device().index()));
+                };
+                status = axes.count ? rotate(lib.rotate_axes, (const bw_axes*)&axes) : rotate(lib.rotate);
             }
         }
         if (status) return checked({}, status, "bw_rotate_heads");
@@ -692,6 +732,7 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             node->k_sizes = k.sizes();
             node->type = q.scalar_type();
             node->eps = eps;
+            node->axes = axes;
             torch::autograd::set_history(torch::autograd::variable_list{q_out, k_out}, node);
         }
         PyObject* p = PyTuple_New(2);
@@ -791,6 +832,55 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         }
         if (status) return checked({}, status, "bw_cache_write");
         Py_RETURN_TRUE;
+    });
+}
+
+// cache_append(q, k, v, cos, sin, positions, slots, keys, values, key_meta, value_meta, bits, group_size, q_weight or None, k_weight or None, eps, sections or None, interleaved)
+// -> q or None
+PyObject* py_cache_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 18) return none();
+        for (int i : {0, 1, 2, 3, 4, 5, 13, 14})
+            if (!plain(args[i]) && !(i >= 13 && args[i] == Py_None)) return none();
+        Cache h;
+        Tensor slots;
+        bw_axes axes;
+        const double eps = PyFloat_AsDouble(args[15]);
+        if (PyErr_Occurred()) return nullptr;
+        if (!lib.append || !cache_of(args + 7, h) || !slots_of(args[6], h.keys, slots) || !axes_of(args[16], args[17], axes)) {
+            if (PyErr_Occurred()) return nullptr;
+            return none();
+        }
+        const Tensor q = unpack(args[0]), k = unpack(args[1]), v = unpack(args[2]), cos = unpack(args[3]), sin = unpack(args[4]), positions = unpack(args[5]);
+        const Tensor qw = args[13] == Py_None ? Tensor() : unpack(args[13]), kw = args[14] == Py_None ? Tensor() : unpack(args[14]);
+        Rotation r;
+        if (q.dim() != 3 || !on_gpu(q, h.keys) || !rotation_of(q, k, cos, sin, positions, qw, kw, eps, axes, r)) return none();
+        if (!on_gpu(v, h.keys) || v.scalar_type() != k.scalar_type() || !v.sizes().equals(k.sizes()) || k.size(0) != slots.size(0) || k.size(1) != h.c.kv_heads || k.size(2) != h.c.dim ||
+            (h.c.bits == 16 && k.scalar_type() != h.keys.scalar_type()))
+            return none();
+        for (const Tensor* t : {&q, &k, &v, &cos, &sin, &qw, &kw})
+            if (t->defined() && wants_grad(*t)) return none();
+        check_tangents("append_cache", {&q, &k, &v, &cos, &sin, &qw, &kw, &h.keys, &h.values, &h.key_meta, &h.value_meta});
+        if (wants_grad(h) || overlap(h.keys, h.values) || (h.key_meta.defined() && overlap(h.key_meta, h.value_meta))) return none();
+        Tensor q_out;
+        int status = 0;
+        {
+            Unlocked unlocked;
+            c10::AutoGradMode off(false);
+            for (const Tensor* t : {&h.keys, &h.values, &h.key_meta, &h.value_meta})       // written in place: what autograd saved of them is stale
+                if (t->defined()) torch::autograd::impl::bump_version(*t);
+            const int64_t tokens = slots.size(0);
+            OnDevice on(q.device());
+            q_out = empty(q.sizes(), q.scalar_type(), q.device());
+            if (tokens > 0) {
+                // (rows of this very cache: they may be written before they are read)
+                auto own = [&](const Tensor& t) { return t.is_alias_of(h.keys) || t.is_alias_of(h.values) ? t.clone() : t; };
+                const Rows rq(own(q), tokens), rk(own(k), tokens), rv(own(v), tokens);
+                status = lib.append(&h.c, &r.heads, axes.count ? &axes : nullptr, r.act, rq.data, rq.row, rq.head, rk.data, rk.row, rk.head, rv.data, rv.row, rv.head,
+                                    (const int64_t*)slots.const_data_ptr(), q_out.mutable_data_ptr(), stream_of(q.device().index()));
+            }
+        }
+        return checked(std::move(q_out), status, "bw_cache_append");
     });
 }
 
@@ -1027,6 +1117,9 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(l.rotate, "bw_rotate_heads");
     get(l.rotate_grad, "bw_rotate_heads_grad");
     get(l.rotate_grad_ws_bytes, "bw_rotate_heads_grad_workspace_bytes");
+    get(l.rotate_axes, "bw_rotate_axes");
+    get(l.rotate_axes_grad, "bw_rotate_axes_grad");
+    get(l.append, "bw_cache_append");
     get(l.cache_write, "bw_cache_write");
     get(l.cache_read, "bw_cache_read");
     get(l.attention, "bw_cache_attention");
@@ -1057,6 +1150,7 @@ PyMethodDef methods[] = {
     {"quantize", (PyCFunction)(void*)py_quantize, METH_FASTCALL, nullptr},
     {"dequantize", (PyCFunction)(void*)py_dequantize, METH_FASTCALL, nullptr},
     {"rotate_heads", (PyCFunction)(void*)py_rotate_heads, METH_FASTCALL, nullptr},
+    {"cache_append", (PyCFunction)(void*)py_cache_append, METH_FASTCALL, nullptr},
     {"cache_write", (PyCFunction)(void*)py_cache_write, METH_FASTCALL, nullptr},
     {"cache_read", (PyCFunction)(void*)py_cache_read, METH_FASTCALL, nullptr},
     {"cache_attention", (PyCFunction)(void*)py_cache_attention, METH_FASTCALL, nullptr},

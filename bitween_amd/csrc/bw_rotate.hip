@@ -1,8 +1,6 @@
 // Rotation of queries and keys by the angle of their token's position, with the norm of each head in the same pass, and its gradients.
 //
-// A thread owns CH values of a head and the CH values half a rotation further on, the pairs that turn together (behind the rotated part:
-// twice CH neighbours), so that a pair never leaves its thread.  2^lane_shift neighbouring threads hold a head (as many as it needs, filled up
-// to a power of two), and the sums that the norm needs go over them with cross-lane shuffles.
+// Which values a thread has, and its angles, are in bw_rotate.h.
 //
 // Gradients, with n = x r, r = rsqrt(mean(x^2) + eps) and g' the incoming gradient turned back:
 //   dx = r (g' w - n mean(g' w n)),  dw = sum over tokens and heads of g' n
@@ -12,103 +10,11 @@
 // One pass over memory, a dozen float32 operations a value: launch-bound up to a few hundred tokens (one token 2.3 us as a graph), HBM and, as every head
 // loads its token's cosines and sines, the L2 beyond: 2048 tokens of 32 and 8 heads of 128 in bfloat16 with both norms take 11 us (42 MB, 3.8 TB/s),
 // their gradients 17 (63 MB) and 4 for the sum; torch copies 21 MB in 7 us.
-#include "bw_cache.h"
+#include "bw_rotate.h"
 
 namespace {
 
-constexpr int kMaxDim = 256;
-
-struct RotateArgs {
-    const uint16_t *q, *k, *gq, *gk;
-    int64_t q_row, q_head, k_row, k_head, gq_row, gq_head, gk_row, gk_head;
-    uint16_t *q_out, *k_out;                     // rotated heads, or the gradients of the inputs
-    const float *cos, *sin;
-    const int64_t* positions;
-    const void *q_weight, *k_weight;
-    float* partial;                              // [blocks][dim]: sums of dw, the queries' blocks first
-    int64_t table_rows;
-    int T, q_heads, k_heads, dim, half, lanes, lane_shift, weight_f32;
-    int q_blocks;                                // gradient: blocks that serve the queries
-    float eps;
-};
-
-// CH 16-bit values as they come from memory, and as float32.
-template <int CH> using Raw = std::conditional_t<CH == 8, u4, u2>;
-template <int CH> BW_DEV Raw<CH> load_raw(const uint16_t* p) { return *reinterpret_cast<const Raw<CH>*>(p); }
-template <int DT, int CH> BW_DEV void widen_raw(const Raw<CH>& w, float* x) {
-#pragma unroll
-    for (int j = 0; j < CH; j++) x[j] = widen16<DT>((uint16_t)(w[j / 2] >> (16 * (j & 1))));
-}
-
-template <int DT, int CH>
-BW_DEV void store_chunk(uint16_t* p, const float* x) {
-    uint32_t w[CH / 2];
-#pragma unroll
-    for (int j = 0; j < CH / 2; j++) w[j] = narrow_pair<DT>(x[2 * j], x[2 * j + 1]);
-    if constexpr (CH == 8) *reinterpret_cast<u4*>(p) = u4{w[0], w[1], w[2], w[3]};
-    else *reinterpret_cast<u2*>(p) = u2{w[0], w[1]};
-}
-
-template <int DT, int CH>
-BW_DEV void load_weight(const void* w, int f32, int at, float* x) {
-    if (f32) {
-#pragma unroll
-        for (int j = 0; j < CH; j++) x[j] = ((const float*)w)[at + j];
-    } else {
-        widen_raw<DT, CH>(load_raw<CH>((const uint16_t*)w + at), x);
-    }
-}
-
-template <int CH>
-BW_DEV void load_floats(const float* p, float* x) {
-#pragma unroll
-    for (int j = 0; j < CH / 4; j++) {
-        const f4 v = *reinterpret_cast<const f4*>(p + 4 * j);
-        x[4 * j] = v[0]; x[4 * j + 1] = v[1]; x[4 * j + 2] = v[2]; x[4 * j + 3] = v[3];
-    }
-}
-
-// The two chunks of lane c of a head, and whether they turn.
-template <int CH>
-BW_DEV void chunks_of(const RotateArgs& a, int c, int& first, int& second, bool& turns) {
-    const int pairs = a.half / CH;
-    turns = c < pairs;
-    first = turns ? c * CH : 2 * a.half + 2 * (c - pairs) * CH;
-    second = turns ? first + a.half : first + CH;
-}
-
-// Over the 2^shift lanes of a head, each with the sum: neighbours, pairs, then mirrored halves of 8 and of 16, whose lanes hold the same by then.
-template <int CTRL> BW_DEV float from_lane(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-}
-BW_DEV float head_sum(float v, int shift) {
-    if (shift > 0) v += from_lane<0xB1>(v);
-    if (shift > 1) v += from_lane<0x4E>(v);
-    if (shift > 2) v += from_lane<0x141>(v);
-    if (shift > 3) v += from_lane<0x140>(v);
-    if (shift > 4) v += __shfl_xor(v, 16, 64);
-    return v;
-}
-
-// cos and sin of a thread's pairs.
-template <int CH> struct Angle {
-    float c[CH], s[CH];
-    BW_DEV void load(const RotateArgs& a, int64_t pos, int first) {
-        load_floats<CH>(a.cos + pos * a.half + first, c);
-        load_floats<CH>(a.sin + pos * a.half + first, s);
-    }
-    // SIGN 1: turned by the angle, -1: turned back
-    template <int SIGN> BW_DEV void turn(float* x, float* y) const {
-#pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const float u = x[j], v = y[j];
-            x[j] = u * c[j] - SIGN * v * s[j];
-            y[j] = v * c[j] + SIGN * u * s[j];
-        }
-    }
-};
-
-template <int DT, int CH>
+template <int DT, int CH, bool AXES>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     const uint32_t heads = (uint32_t)(a.q_heads + a.k_heads), item = (blockIdx.x * 256 + threadIdx.x) >> a.lane_shift;
     const int lane = (int)threadIdx.x & ((1 << a.lane_shift) - 1);
@@ -122,11 +28,11 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     bool turns;
     chunks_of<CH>(a, live ? lane : 0, first, second, turns);
     const uint16_t* src = is_k ? a.k + token * a.k_row + head * a.k_head : a.q + token * a.q_row + head * a.q_head;
-    const int64_t pos = a.positions[token];
+    const Position<AXES> pos(a, token);
     float x[CH], y[CH];
     widen_raw<DT, CH>(load_raw<CH>(src + first), x);
     widen_raw<DT, CH>(load_raw<CH>(src + second), y);
-    const bool kept = pos >= 0 && pos < a.table_rows;
+    const bool kept = pos.kept;
     Angle<CH> angle;
     if (kept && turns) angle.load(a, pos, first);
     if (a.q_weight || a.k_weight) {
@@ -161,7 +67,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
 }
 
 // One block serves the queries' heads or the keys', 256 >> lane_shift at a time.
-template <int DT, int CH>
+template <int DT, int CH, bool AXES>
 __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
     __shared__ float sums[256 * 2 * CH];
     const bool is_k = (int)blockIdx.x >= a.q_blocks;
@@ -188,8 +94,8 @@ __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
         const bool live = item < items && lane < a.lanes;
         const uint32_t it = live ? item : 0;
         const int token = (int)(it / heads), head = (int)(it - (uint32_t)token * heads);
-        const int64_t pos = a.positions[token];
-        const bool kept = pos >= 0 && pos < a.table_rows;
+        const Position<AXES> pos(a, token);
+        const bool kept = pos.kept;
         const uint16_t* g = gs + token * g_row + head * g_head;
         const uint16_t* in = xs + token * x_row + head * x_head;
         const Raw<CH> g1 = load_raw<CH>(g + first), g2 = load_raw<CH>(g + second);
@@ -296,40 +202,6 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* partial,
     }
 }
 
-// Values of a chunk: 8, where whole 16-byte chunks fill the rotated halves and what lies behind them.
-int chunk_of(const bw_heads* h) { return h->dim % 16 == 0 && h->rotary % 16 == 0 ? 8 : 4; }
-
-int heads_check(const bw_heads* h, int act_dtype) {
-    if (!h || h->tokens < 0 || h->q_heads < 1 || h->k_heads < 1 || h->dim < 1 || h->rotary < 1 || h->rotary > h->dim || h->table_rows < 1) return BW_EINVAL;
-    if (h->tokens > 0 && (!h->cos || !h->sin || !h->positions)) return BW_EINVAL;
-    if (act_dtype != BW_F16 && act_dtype != BW_BF16) return BW_EUNSUPPORTED;
-    if ((h->q_weight || h->k_weight) && h->weight_dtype != act_dtype && h->weight_dtype != BW_F32) return BW_EUNSUPPORTED;
-    if (h->dim % 8 || h->rotary % 8 || h->dim > kMaxDim) return BW_EUNSUPPORTED;
-    if (h->q_heads > 65535 || h->k_heads > 65535 || h->tokens >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
-    const int64_t items = h->tokens * ((int64_t)h->q_heads + h->k_heads);
-    if (items >= (int64_t)1 << 31 || items * h->dim >= (int64_t)1 << 36) return BW_EUNSUPPORTED;
-    if (!bw_aligned(h->cos, 16) || !bw_aligned(h->sin, 16) || !bw_aligned(h->positions, 8) || !bw_aligned(h->q_weight, 16) || !bw_aligned(h->k_weight, 16))
-        return BW_EALIGN;
-    return BW_OK;
-}
-
-RotateArgs args_of(const bw_heads* h) {
-    RotateArgs a = {};
-    a.cos = h->cos; a.sin = h->sin;
-    a.positions = h->positions;
-    a.q_weight = h->q_weight; a.k_weight = h->k_weight;
-    a.weight_f32 = h->weight_dtype == BW_F32;
-    a.table_rows = h->table_rows;
-    a.T = (int)h->tokens;
-    a.q_heads = h->q_heads; a.k_heads = h->k_heads;
-    a.dim = h->dim;
-    a.half = h->rotary / 2;
-    a.lanes = h->dim / (2 * chunk_of(h));
-    a.lane_shift = bw_log2(a.lanes);
-    a.eps = h->eps;
-    return a;
-}
-
 // Blocks of the gradient kernel for the queries or the keys: enough to fill the chip together, 1024 in proportion to their heads, so that the
 // sums over them stay short (2048 tokens of 32 and 8 heads of 128, forward and backward: 30.2 us; with 768 30.5, 1536 31.9, 2048 33.1).
 int grad_blocks(const bw_heads* h, int heads) {
@@ -338,15 +210,13 @@ int grad_blocks(const bw_heads* h, int heads) {
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
-}  // namespace
-
-extern "C" int bw_rotate_heads(const bw_heads* h, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
-                               int64_t k_head, void* q_out, void* k_out, void* stream) {
+int rotate(const bw_heads* h, const bw_axes* x, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, void* q_out,
+           void* k_out, void* stream) {
     if (int st = heads_check(h, act_dtype)) return st;
     if (h->tokens == 0) return BW_OK;
     if (!q || !k || !q_out || !k_out) return BW_EINVAL;
     if (!bw_aligned(q, 16) || !bw_aligned(k, 16) || !bw_aligned(q_out, 16) || !bw_aligned(k_out, 16) || (q_row | q_head | k_row | k_head) % 8) return BW_EALIGN;
-    RotateArgs a = args_of(h);
+    RotateArgs a = rotate_args(h, x);
     a.q = (const uint16_t*)q; a.k = (const uint16_t*)k;
     a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head;
     a.q_out = (uint16_t*)q_out; a.k_out = (uint16_t*)k_out;
@@ -356,7 +226,8 @@ extern "C" int bw_rotate_heads(const bw_heads* h, int act_dtype, const void* q, 
         a.T = (int)(h->tokens - at < most ? h->tokens - at : most);
         const dim3 grid((unsigned)((a.T * heads + per_block - 1) / per_block)), block(256);
 #define BW_ROTATE(DT, CH) \
-    if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_kernel<DT, CH>), grid, block, 0, (hipStream_t)stream, a);
+    if (act_dtype == DT && chunk_of(h) == CH && x) hipLaunchKernelGGL((rotate_kernel<DT, CH, true>), grid, block, 0, (hipStream_t)stream, a); \
+    else if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_kernel<DT, CH, false>), grid, block, 0, (hipStream_t)stream, a);
         BW_ROTATE(BW_F16, 8) BW_ROTATE(BW_F16, 4) BW_ROTATE(BW_BF16, 8) BW_ROTATE(BW_BF16, 4)
 #undef BW_ROTATE
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
@@ -367,15 +238,14 @@ extern "C" int bw_rotate_heads(const bw_heads* h, int act_dtype, const void* q, 
     return BW_OK;
 }
 
-extern "C" size_t bw_rotate_heads_grad_workspace_bytes(const bw_heads* h) {
+size_t grad_workspace(const bw_heads* h) {
     if (heads_check(h, h && h->weight_dtype == BW_BF16 ? BW_BF16 : BW_F16) != BW_OK || (!h->q_weight && !h->k_weight)) return 0;
     return (size_t)(grad_blocks(h, h->q_heads) + grad_blocks(h, h->k_heads)) * h->dim * sizeof(float);
 }
 
-extern "C" int bw_rotate_heads_grad(const bw_heads* h, int act_dtype, const void* gq, int64_t gq_row, int64_t gq_head, const void* gk, int64_t gk_row,
-                                    int64_t gk_head, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
-                                    void* q_grad, void* k_grad, void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
-                                    void* stream) {
+int rotate_grad(const bw_heads* h, const bw_axes* x, int act_dtype, const void* gq, int64_t gq_row, int64_t gq_head, const void* gk, int64_t gk_row, int64_t gk_head,
+                const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, void* q_grad, void* k_grad, void* q_weight_grad,
+                void* k_weight_grad, void* workspace, size_t workspace_bytes, void* stream) {
     if (int st = heads_check(h, act_dtype)) return st;
     if ((q_weight_grad && !h->q_weight) || (k_weight_grad && !h->k_weight)) return BW_EINVAL;
     if (h->tokens > 0) {
@@ -385,7 +255,7 @@ extern "C" int bw_rotate_heads_grad(const bw_heads* h, int act_dtype, const void
             return BW_EALIGN;
         if ((h->q_weight && (q_row | q_head) % 8) || (h->k_weight && (k_row | k_head) % 8)) return BW_EALIGN;
     }
-    RotateArgs a = args_of(h);
+    RotateArgs a = rotate_args(h, x);
     a.gq = (const uint16_t*)gq; a.gk = (const uint16_t*)gk;
     a.gq_row = gq_row; a.gq_head = gq_head; a.gk_row = gk_row; a.gk_head = gk_head;
     a.q = (const uint16_t*)q; a.k = (const uint16_t*)k;
@@ -395,13 +265,14 @@ extern "C" int bw_rotate_heads_grad(const bw_heads* h, int act_dtype, const void
     const int blocks = h->tokens ? a.q_blocks + grad_blocks(h, h->k_heads) : 0;
     const bool sums = q_weight_grad || k_weight_grad;
     if (sums && blocks) {
-        if (!workspace || workspace_bytes < bw_rotate_heads_grad_workspace_bytes(h)) return BW_EWORKSPACE;
+        if (!workspace || workspace_bytes < grad_workspace(h)) return BW_EWORKSPACE;
         if (!bw_aligned(workspace, 16)) return BW_EALIGN;
         a.partial = (float*)workspace;
     }
     if (blocks) {
 #define BW_ROTATE(DT, CH) \
-    if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_grad_kernel<DT, CH>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+    if (act_dtype == DT && chunk_of(h) == CH && x) hipLaunchKernelGGL((rotate_grad_kernel<DT, CH, true>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a); \
+    else if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_grad_kernel<DT, CH, false>), dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
         BW_ROTATE(BW_F16, 8) BW_ROTATE(BW_F16, 4) BW_ROTATE(BW_BF16, 8) BW_ROTATE(BW_BF16, 4)
 #undef BW_ROTATE
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
@@ -414,4 +285,35 @@ extern "C" int bw_rotate_heads_grad(const bw_heads* h, int act_dtype, const void
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;
+}
+
+}  // namespace
+
+extern "C" int bw_rotate_heads(const bw_heads* h, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                               int64_t k_head, void* q_out, void* k_out, void* stream) {
+    return rotate(h, nullptr, act_dtype, q, q_row, q_head, k, k_row, k_head, q_out, k_out, stream);
+}
+
+extern "C" int bw_rotate_axes(const bw_heads* h, const bw_axes* axes, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                              int64_t k_head, void* q_out, void* k_out, void* stream) {
+    if (int st = axes_check(axes, h ? h->rotary : 0)) return st;
+    return rotate(h, axes, act_dtype, q, q_row, q_head, k, k_row, k_head, q_out, k_out, stream);
+}
+
+extern "C" size_t bw_rotate_heads_grad_workspace_bytes(const bw_heads* h) { return grad_workspace(h); }
+
+extern "C" int bw_rotate_heads_grad(const bw_heads* h, int act_dtype, const void* gq, int64_t gq_row, int64_t gq_head, const void* gk, int64_t gk_row,
+                                    int64_t gk_head, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                                    void* q_grad, void* k_grad, void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+    return rotate_grad(h, nullptr, act_dtype, gq, gq_row, gq_head, gk, gk_row, gk_head, q, q_row, q_head, k, k_row, k_head, q_grad, k_grad, q_weight_grad, k_weight_grad,
+                       workspace, workspace_bytes, stream);
+}
+
+extern "C" int bw_rotate_axes_grad(const bw_heads* h, const bw_axes* axes, int act_dtype, const void* gq, int64_t gq_row, int64_t gq_head, const void* gk, int64_t gk_row,
+                                   int64_t gk_head, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, void* q_grad, void* k_grad,
+                                   void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int st = axes_check(axes, h ? h->rotary : 0)) return st;
+    return rotate_grad(h, axes, act_dtype, gq, gq_row, gq_head, gk, gk_row, gk_head, q, q_row, q_head, k, k_row, k_head, q_grad, k_grad, q_weight_grad, k_weight_grad,
+                       workspace, workspace_bytes, stream);
 }

@@ -258,6 +258,20 @@ int bw_rotate_heads_grad(const bw_heads* heads, int act_dtype, const void* gq, i
                          void* q_grad, void* k_grad, void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* Both with positions of several axes (time, height, width; up to 4): heads->positions is [count][tokens], and pair (i, i + h) of every head turns by the position on its own axis,
+ * c = cos[p_axis][i].  sections[a] pairs belong to axis a, h in all: the first ones to axis 0 and so on, or (interleaved) pair i to axis i % count as long as i < count *
+ * sections[i % count], and to axis 0 otherwise.  A token with a position outside the table on any axis is padding.  The workspace is that of bw_rotate_heads_grad. */
+typedef struct bw_axes {
+    int count, sections[4], interleaved;
+} bw_axes;
+
+int bw_rotate_axes(const bw_heads* heads, const bw_axes* axes, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                   int64_t k_head, void* q_out, void* k_out, void* stream);
+
+int bw_rotate_axes_grad(const bw_heads* heads, const bw_axes* axes, int act_dtype, const void* gq, int64_t gq_row, int64_t gq_head, const void* gk, int64_t gk_row,
+                        int64_t gk_head, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, void* q_grad, void* k_grad,
+                        void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes, void* stream);
+
 /* A paged key-value cache: `pages` pages of page_size token rows for each of kv_heads heads.
  *   bits 16   keys, values [pages][kv_heads][page_size][dim] of dtype (BW_F16 | BW_BF16); key_meta, value_meta unused
  *   bits 8|4  keys, values int32 [pages][kv_heads][page_size][dim * bits / 32], packed like qweight; key_meta, value_meta float16 pairs
@@ -281,6 +295,15 @@ typedef struct bw_cache {
  * Keys and values that share memory (or their pairs) are refused with BW_EINVAL. */
 int bw_cache_write(const bw_cache* cache, int act_dtype, int64_t T, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                    int64_t v_head, const int64_t* slots, void* stream);
+
+/* Queries, keys and values of heads->tokens tokens on their way into attention, in one launch: queries and keys rotated (and normed) as bw_rotate_heads (axes NULL) or
+ * bw_rotate_axes does, keys and values written into their slots as bw_cache_write does.  The norm's 1 / sqrt(mean(x^2) + eps) is formed in float64 and rounded
+ * once; keys are rounded to act_dtype before they are quantised: without norms queries and cache have the bits that the two calls leave.
+ * heads->k_heads is the cache's kv_heads, heads->dim its dim.  A token whose position lies outside the table gets zeros as queries, and is left out of the cache as one
+ * whose slot lies outside it is.  The slots of one call differ; q, k, v and q_out are no part of the cache.
+ *   q, k, v  act_dtype (the cache's dtype at 16 bits), strided as q of bw_rotate_heads; q_out contiguous */
+int bw_cache_append(const bw_cache* cache, const bw_heads* heads, const bw_axes* axes, int act_dtype, const void* q, int64_t q_row, int64_t q_head,
+                    const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* slots, void* q_out, void* stream);
 
 /* The rows of T slots as k_out, v_out [T][kv_heads][dim] of out_dtype (BW_F16 | BW_BF16; the cache's dtype at 16 bits): scale * (code -
  * zero point) rounded once (a finite value beyond float16's range to its largest).  Zeros for a slot outside the cache. */
