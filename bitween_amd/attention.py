@@ -96,6 +96,18 @@ def _cache_args(keys, values, key_meta, value_meta, bits, group_size):
     return tuple(None if t is None else _hip._plain(t) for t in (keys, values, key_meta, value_meta)) + (int(bits), int(group_size))
 
 
+def _window(what, window, sinks):
+    """window (0: all tokens) and sinks as whole numbers."""
+    for n, name, least in ((window, "window", 1), (sinks, "sinks", 0)):
+        if n is None and name == "window":
+            continue
+        if not isinstance(n, int) or isinstance(n, bool):
+            raise TypeError(f"{what}: {name} must be a whole number, got {type(n).__name__}")
+        if n < least:
+            raise ValueError(f"{what}: {name} must be at least {least}, got {n}")
+    return min(window or 0, 2 ** 62), min(sinks, 2 ** 62)
+
+
 def _taken(what, out):
     if out is None:
         raise _hip.BitweenHipError(f"{what}: these arguments are not taken")
@@ -258,10 +270,11 @@ def read_cache(slots, keys, values, key_meta=None, value_meta=None, bits=16, gro
     return _taken("read_cache", _native("cache_read")(_whole(slots, "slots", torch.int64), *_cache_args(keys, values, key_meta, value_meta, bits, group_size), code))
 
 
-def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_meta=None, bits=16, group_size=64, scale=None):
+def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_meta=None, bits=16, group_size=64, scale=None, window=None,
+                    sinks=0):
     """Attention of one new token of each sequence over a paged cache (see write_cache): q [batch, q_heads, dim] -> [batch, q_heads, dim],
 
-        out = sum_t softmax_t(scale q . k_t) v_t   over t < lengths[b],
+        out = sum_t softmax_t(scale q . k_t) v_t   over t < lengths[b]; with a window over the last `window` of these and the first `sinks`,
 
     token t of sequence b in row t % page_size of page page_table[b, t // page_size] (int32 [batch, pages of a sequence]); lengths int32
     [batch], the new token's own row included where it is written first.  kv_heads divides q_heads; query head h reads head
@@ -270,14 +283,16 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
     A sequence of length 0 (an idle row of a padded batch) gives zeros.  What lies behind a sequence's last token is not looked at - neither the
     rows nor the table's entries.  A score of minus infinity (an infinity among the keys) has weight 0, and a sequence without any other score gives NaN, as
     one of plus infinity or NaN does; an infinity or a NaN among the values leaves nothing finite in its channel, whatever its weight.  A length beyond
-    the table is cut to it; a page number outside the cache is a page without tokens.  Lengths and table are read on the GPU when the kernel runs, so a
+    the table is cut to it; a page number outside the cache is a page without tokens.  Table entries of pages that neither window nor sinks reach are not looked at: such pages
+    may be given back.  Lengths and table are read on the GPU when the kernel runs, so a
     captured call follows them.  No gradients."""
     if scale is None:
         scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
-    out = _native("cache_attention")(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale)
+    what = "cache_attention"
+    width, first = _window(what, window, sinks)
+    out = _native("cache_attention")(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale, width, first)
     if out is not None:
         return out
-    what = "cache_attention"
     dim = _checked_cache(what, keys, values, key_meta, value_meta, bits, group_size)
     _tensor(q, "q", *((keys.dtype,) if bits == 16 else _HALF))
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % keys.shape[1]:
@@ -290,19 +305,7 @@ def cache_attention(q, page_table, lengths, keys, values, key_meta=None, value_m
     _no_grad(what, q, keys, values, key_meta, value_meta)
     _no_tangent(what, q, keys, values, key_meta, value_meta)
     return _taken(what, _native("cache_attention")(_hip._plain(q), _whole(page_table, "page_table", torch.int32), _whole(lengths, "lengths", torch.int32),
-                                                   *_cache_args(keys, values, key_meta, value_meta, bits, group_size), float(scale)))
-
-
-def _window(what, window, sinks):
-    """window (0: all tokens) and sinks as whole numbers."""
-    for n, name, least in ((window, "window", 1), (sinks, "sinks", 0)):
-        if n is None and name == "window":
-            continue
-        if not isinstance(n, int) or isinstance(n, bool):
-            raise TypeError(f"{what}: {name} must be a whole number, got {type(n).__name__}")
-        if n < least:
-            raise ValueError(f"{what}: {name} must be at least {least}, got {n}")
-    return min(window or 0, 2 ** 62), min(sinks, 2 ** 62)
+                                                   *_cache_args(keys, values, key_meta, value_meta, bits, group_size), float(scale), width, first))
 
 
 def prompt_attention(q, k, v, q_starts=None, k_starts=None, window=None, sinks=0, scale=None):
@@ -398,9 +401,9 @@ class PagedCache:
         """read_cache of this cache, in its dtype."""
         return read_cache(slots, self.keys, self.values, self.key_meta, self.value_meta, self.bits, self.group_size, self.dtype)
 
-    def attend(self, q, page_table, lengths, scale=None):
+    def attend(self, q, page_table, lengths, scale=None, window=None, sinks=0):
         """cache_attention over this cache."""
-        return cache_attention(q, page_table, lengths, self.keys, self.values, self.key_meta, self.value_meta, self.bits, self.group_size, scale)
+        return cache_attention(q, page_table, lengths, self.keys, self.values, self.key_meta, self.value_meta, self.bits, self.group_size, scale, window, sinks)
 
     def slots(self, page_table, positions, sequences=None):
         """The slots (int64) of the tokens at `positions` (int64 [tokens]): of the sequences 0, 1, ... one each, or of `sequences` (int64 [tokens]).

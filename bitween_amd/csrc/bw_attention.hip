@@ -85,10 +85,13 @@ int attention_check(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages
 // Workgroups, and whether every segment gets one of its own: nothing to cut, nothing to join.  With room for 512 tokens to a sequence always (128
 // sequences of 12 heads of 64: 15.3 us against 20.0), with room for 1024 where there are segments for half the CUs at least (64 sequences of up to
 // 1000, 8 heads of 128 in 4 bits: 16.6 against 22.4; 4 such sequences: 15.2 against 10.1), beyond never (32 of up to 2000 in 8 bits: 28.7 against 22.0).
+// (With a window there is room for its tiles and the sinks', however long the table.)
 struct Plan { uint32_t grid; bool whole; };
 constexpr int kWholeTokens = 512, kWholeMany = 1024;
-Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
-    const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries), tokens = max_pages * c->page_size;
+struct Window { int64_t tokens, sinks; };                        // tokens 0: all
+Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages, Window w) {
+    const int64_t share = q_heads / c->kv_heads, segments = B * c->kv_heads * ((share + kQueries - 1) / kQueries), room = max_pages * c->page_size;
+    const int64_t seen = w.tokens && w.tokens < room && w.sinks < room ? ((w.tokens + kTile - 1) / kTile + 1 + (w.sinks + kTile - 1) / kTile) * kTile : room, tokens = seen < room ? seen : room;
     const int cus = bw_device_cus();
     Plan p;
     p.whole = tokens <= (2 * segments >= cus ? kWholeMany : kWholeTokens) && segments < (int64_t)1 << 24;          // (2^32 threads of a launch)
@@ -101,28 +104,24 @@ Plan plan_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
 
 }  // namespace
 
-template <class F> static void launch(const AttentionArgs& a, uint32_t grid, hipStream_t stream) {
-    hipLaunchKernelGGL((attention_kernel<F, 1>), dim3(grid), dim3(256), 0, stream, a);
-}
-
-extern "C" size_t bw_cache_attention_workspace_bytes(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
-    if (attention_check(c, B, q_heads, max_pages) != BW_OK || B == 0) return 0;
-    const Plan p = plan_of(c, B, q_heads, max_pages);
+static size_t workspace_bytes_of(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages, Window w) {
+    if (attention_check(c, B, q_heads, max_pages) != BW_OK || B == 0 || w.tokens < 0 || w.sinks < 0) return 0;
+    const Plan p = plan_of(c, B, q_heads, max_pages, w);
     const int share = q_heads / c->kv_heads, queries = share < kQueries ? share : kQueries;
     return p.whole ? 0 : (size_t)p.grid * (sizeof(Joint) + 2 * (2 * kQueries + queries * c->dim) * sizeof(float));
 }
 
-extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head,
-                                  const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, void* out,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
+static int attend(const bw_cache* c, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head, const int32_t* page_table, int64_t max_pages,
+                  int64_t table_row, const int32_t* lengths, float scale, Window w, void* out, void* workspace, size_t workspace_bytes, void* stream) {
     if (int st = attention_check(c, B, q_heads, max_pages)) return st;
+    if (w.tokens < 0 || w.sinks < 0) return BW_EINVAL;
     if ((act_dtype != BW_F16 && act_dtype != BW_BF16) || (c->bits == 16 && act_dtype != c->dtype)) return BW_EUNSUPPORTED;
     if (B == 0) return BW_OK;
     if (!q || !page_table || !lengths || !out) return BW_EINVAL;
     if (table_row < max_pages && B > 1 && table_row != 0) return BW_EINVAL;
     if (!bw_aligned(q, 16) || !bw_aligned(out, 16) || !bw_aligned(page_table, 4) || !bw_aligned(lengths, 4) || (q_row | q_head) % 8) return BW_EALIGN;
-    const Plan plan = plan_of(c, B, q_heads, max_pages);
-    const size_t bytes = bw_cache_attention_workspace_bytes(c, B, q_heads, max_pages);
+    const Plan plan = plan_of(c, B, q_heads, max_pages, w);
+    const size_t bytes = workspace_bytes_of(c, B, q_heads, max_pages, w);
     if (bytes) {
         if (!workspace || workspace_bytes < bytes) return BW_EWORKSPACE;
         if (!bw_aligned(workspace, 16)) return BW_EALIGN;
@@ -143,6 +142,8 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     a.dim = c->dim; a.row_bytes = c->dim * c->bits / 8;
     a.page_shift = bw_log2(c->page_size);
     a.max_tokens = (int)(max_pages * c->page_size);
+    a.window = w.tokens && w.tokens < a.max_tokens ? (int)w.tokens : a.max_tokens;
+    a.sinks = w.sinks < a.max_tokens ? (int)w.sinks : a.max_tokens;
     a.q_bf16 = act_dtype == BW_BF16;
     a.cus = bw_device_cus();
     a.whole = plan.whole;
@@ -151,13 +152,13 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
     if (c->bits == 8) bw_launch_attention_w8(a, c->group, plan.grid, st);
     else if (c->bits == 4) bw_launch_attention_w4(a, c->group, plan.grid, st);
     else if (c->dtype == BW_F16) {
-        if (c->dim <= 64) launch<Format16<BW_F16, 64>>(a, plan.grid, st);
-        else if (c->dim <= 128) launch<Format16<BW_F16, 128>>(a, plan.grid, st);
-        else launch<Format16<BW_F16, 256>>(a, plan.grid, st);
+        if (c->dim <= 64) launch_attention<Format16<BW_F16, 64>, 1>(a, plan.grid, st);
+        else if (c->dim <= 128) launch_attention<Format16<BW_F16, 128>, 1>(a, plan.grid, st);
+        else launch_attention<Format16<BW_F16, 256>, 1>(a, plan.grid, st);
     } else {
-        if (c->dim <= 64) launch<Format16<BW_BF16, 64>>(a, plan.grid, st);
-        else if (c->dim <= 128) launch<Format16<BW_BF16, 128>>(a, plan.grid, st);
-        else launch<Format16<BW_BF16, 256>>(a, plan.grid, st);
+        if (c->dim <= 64) launch_attention<Format16<BW_BF16, 64>, 1>(a, plan.grid, st);
+        else if (c->dim <= 128) launch_attention<Format16<BW_BF16, 128>, 1>(a, plan.grid, st);
+        else launch_attention<Format16<BW_BF16, 256>, 1>(a, plan.grid, st);
     }
     if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     if (!plan.whole) {
@@ -167,4 +168,24 @@ extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* 
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
     return BW_OK;
+}
+
+extern "C" size_t bw_cache_attention_workspace_bytes(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages) {
+    return workspace_bytes_of(c, B, q_heads, max_pages, Window{0, 0});
+}
+
+extern "C" int bw_cache_attention(const bw_cache* c, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head,
+                                  const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, void* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(c, act_dtype, q, B, q_heads, q_row, q_head, page_table, max_pages, table_row, lengths, scale, Window{0, 0}, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t bw_cache_attention_window_workspace_bytes(const bw_cache* c, int64_t B, int q_heads, int64_t max_pages, int64_t window, int64_t sinks) {
+    return workspace_bytes_of(c, B, q_heads, max_pages, Window{window, sinks});
+}
+
+extern "C" int bw_cache_attention_window(const bw_cache* c, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head,
+                                         const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, int64_t window,
+                                         int64_t sinks, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(c, act_dtype, q, B, q_heads, q_row, q_head, page_table, max_pages, table_row, lengths, scale, Window{window, sinks}, out, workspace, workspace_bytes, stream);
 }

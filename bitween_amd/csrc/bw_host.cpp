@@ -49,6 +49,8 @@ struct Library {
     decltype(&bw_cache_read) cache_read = nullptr;
     decltype(&bw_cache_attention) attention = nullptr;
     decltype(&bw_cache_attention_workspace_bytes) attention_ws_bytes = nullptr;
+    decltype(&bw_cache_attention_window) window = nullptr;
+    decltype(&bw_cache_attention_window_workspace_bytes) window_ws_bytes = nullptr;
     decltype(&bw_prompt_attention) prompt = nullptr;
     decltype(&bw_prompt_attention_workspace_bytes) prompt_ws_bytes = nullptr;
     decltype(&bw_prompt_attention_grad) prompt_grad = nullptr;
@@ -561,7 +563,7 @@ bool axes_of(PyObject* sections, PyObject* interleaved, bw_axes& axes) {
 
 bool rotation_of(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& positions, const Tensor& qw, const Tensor& kw,
                  double eps, const bw_axes& axes, Rotation& r) {
-    if (!lib.rotate || !q.is_cuda() || !q.has_storage() || !half_type(q.scalar_type()) || k.scalar_type() != q.scalar_type()) return false;
+    if (!lib.rotate || (axes.count && !lib.rotate_axes) || !q.is_cuda() || !q.has_storage() || !half_type(q.scalar_type()) || k.scalar_type() != q.scalar_type()) return false;
     for (const Tensor* t : {&k, &cos, &sin, &positions})
         if (!on_gpu(*t, q)) return false;
     if (positions.scalar_type() != at::kLong || !positions.is_contiguous() || (axes.count && (positions.dim() < 1 || positions.size(0) != axes.count))) return false;
@@ -919,17 +921,24 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     });
 }
 
-// cache_attention(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale) -> out or None
+// cache_attention(q, page_table, lengths, keys, values, key_meta, value_meta, bits, group_size, scale[, window (0: none), sinks]) -> out or None
 PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return guarded([&]() -> PyObject* {
         Cache h;
-        if (nargs != 10 || !plain(args[0]) || !plain(args[1]) || !plain(args[2]) || !cache_of(args + 3, h)) {
+        if ((nargs != 10 && nargs != 12) || !plain(args[0]) || !plain(args[1]) || !plain(args[2]) || !cache_of(args + 3, h)) {
             if (PyErr_Occurred()) return nullptr;
             return none();
         }
         const Tensor q = unpack(args[0]), table = unpack(args[1]), lengths = unpack(args[2]);
         const double scale = PyFloat_AsDouble(args[9]);
+        int64_t window = 0, sinks = 0;
+        if (nargs == 12) {
+            if (!PyLong_Check(args[10]) || !PyLong_Check(args[11])) return none();
+            window = PyLong_AsLongLong(args[10]);
+            sinks = PyLong_AsLongLong(args[11]);
+        }
         if (PyErr_Occurred()) return nullptr;
+        if (window && !lib.window) return none();
         for (const Tensor* t : {&q, &table, &lengths})
             if (!on_gpu(*t, h.keys)) return none();
         if (!half_type(q.scalar_type()) || (h.c.bits == 16 && q.scalar_type() != h.keys.scalar_type()) || q.dim() != 3 || q.size(2) != h.c.dim ||
@@ -949,13 +958,16 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs)
             out = empty({batch, q.size(1), q.size(2)}, q.scalar_type(), q.device());
             if (batch > 0) {
                 const Rows rq(q, batch);
-                const size_t bytes = lib.attention_ws_bytes(&h.c, batch, (int)q.size(1), table.size(1));
+                const size_t bytes = window ? lib.window_ws_bytes(&h.c, batch, (int)q.size(1), table.size(1), window, sinks)
+                                            : lib.attention_ws_bytes(&h.c, batch, (int)q.size(1), table.size(1));
                 Tensor ws;
                 if (bytes) ws = empty({(int64_t)bytes}, at::kByte, q.device());
-                status = lib.attention(&h.c, dtype_code(q.scalar_type()), rq.data, batch, (int)q.size(1), rq.row, rq.head,
-                                       (const int32_t*)table.const_data_ptr(), table.size(1), batch > 1 ? table.stride(0) : table.size(1),
-                                       (const int32_t*)lengths.const_data_ptr(), (float)scale, out.mutable_data_ptr(), bytes ? ws.mutable_data_ptr() : nullptr,
-                                       bytes, stream_of(q.device().index()));
+                auto attend = [&](auto entry, auto... limits) {
+                    return entry(&h.c, dtype_code(q.scalar_type()), rq.data, batch, (int)q.size(1), rq.row, rq.head, (const int32_t*)table.const_data_ptr(), table.size(1),
+                                 batch > 1 ? table.stride(0) : table.size(1), (const int32_t*)lengths.const_data_ptr(), (float)scale, limits..., out.mutable_data_ptr(),
+                                 bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(q.device().index()));
+                };
+                status = window ? attend(lib.window, window, sinks) : attend(lib.attention);
             }
         }
         return checked(std::move(out), status, "bw_cache_attention");
@@ -1117,19 +1129,23 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     get(l.rotate, "bw_rotate_heads");
     get(l.rotate_grad, "bw_rotate_heads_grad");
     get(l.rotate_grad_ws_bytes, "bw_rotate_heads_grad_workspace_bytes");
-    get(l.rotate_axes, "bw_rotate_axes");
-    get(l.rotate_axes_grad, "bw_rotate_axes_grad");
-    get(l.append, "bw_cache_append");
     get(l.cache_write, "bw_cache_write");
     get(l.cache_read, "bw_cache_read");
     get(l.attention, "bw_cache_attention");
     get(l.attention_ws_bytes, "bw_cache_attention_workspace_bytes");
+    const bool step = ok;                                       // ... or without those of prompts, windows and positions of several axes
+    get(l.rotate_axes, "bw_rotate_axes");
+    get(l.rotate_axes_grad, "bw_rotate_axes_grad");
+    get(l.append, "bw_cache_append");
+    get(l.window, "bw_cache_attention_window");
+    get(l.window_ws_bytes, "bw_cache_attention_window_workspace_bytes");
     get(l.prompt, "bw_prompt_attention");
     get(l.prompt_ws_bytes, "bw_prompt_attention_workspace_bytes");
     get(l.prompt_grad, "bw_prompt_attention_grad");
     get(l.prompt_grad_ws_bytes, "bw_prompt_attention_grad_workspace_bytes");
     if (PyErr_Occurred()) return nullptr;
-    if (!ok) l.rotate = nullptr, l.attention = nullptr, l.prompt = nullptr;
+    if (!step) l.rotate = nullptr, l.attention = nullptr;
+    if (!ok) l.rotate_axes = nullptr, l.append = nullptr, l.window = nullptr, l.prompt = nullptr;
     if (!linears) {
         PyErr_SetString(PyExc_RuntimeError, "bind: an entry point is missing");
         return nullptr;

@@ -25,7 +25,7 @@ ABI_VERSION = 10           # what bw_abi_version() of a matching library returns
 ENTRY_POINTS = ("bw_abi_version", "bw_strerror", "bw_quantize_pack", "bw_quantize_pack_add", "bw_dequantize", "bw_qgemv", "bw_qgemm",
                 "bw_qgemm_ws", "bw_qgemm_static", "bw_qgemm_workspace_bytes", "bw_qgemm_tile_rows", "bw_qgemm_tile_cols", "bw_qlinear", "bw_qlinear_ws", "bw_qlinear_workspace_bytes", "bw_qdgrad", "bw_qdgrad_workspace_bytes", "bw_qdgrad_tile_rows", "bw_qdgrad_rows_slices", "bw_cast_bf16_f16", "bw_qlinear_decode_rows", "bw_qgemv_last_kernel",
                 "bw_rotate_heads", "bw_rotate_heads_grad", "bw_rotate_heads_grad_workspace_bytes", "bw_cache_write", "bw_cache_read", "bw_cache_attention", "bw_cache_attention_workspace_bytes",
-                "bw_rotate_axes", "bw_rotate_axes_grad", "bw_cache_append", "bw_prompt_attention", "bw_prompt_attention_workspace_bytes", "bw_prompt_attention_grad", "bw_prompt_attention_grad_workspace_bytes")
+                "bw_rotate_axes", "bw_rotate_axes_grad", "bw_cache_append", "bw_cache_attention_window", "bw_cache_attention_window_workspace_bytes", "bw_prompt_attention", "bw_prompt_attention_workspace_bytes", "bw_prompt_attention_grad", "bw_prompt_attention_grad_workspace_bytes")
 
 
 class BitweenHipError(RuntimeError):
@@ -121,6 +121,8 @@ def load():
     lib.bw_cache_read.argtypes = [cache, i32, i64, vp, vp, vp, vp]
     lib.bw_cache_attention.argtypes = [cache, i32, vp, i64, i32, i64, i64, vp, i64, i64, vp, ctypes.c_float, vp, vp, size, vp]
     lib.bw_cache_attention_workspace_bytes.argtypes = [cache, i64, i32, i64]
+    lib.bw_cache_attention_window.argtypes = [cache, i32, vp, i64, i32, i64, i64, vp, i64, i64, vp, ctypes.c_float, i64, i64, vp, vp, size, vp]
+    lib.bw_cache_attention_window_workspace_bytes.argtypes = [cache, i64, i32, i64, i64, i64]
     axes, prompt = ctypes.POINTER(Axes), ctypes.POINTER(Prompt)
     lib.bw_rotate_axes.argtypes = [heads, axes] + lib.bw_rotate_heads.argtypes[1:]
     lib.bw_rotate_axes_grad.argtypes = [heads, axes] + lib.bw_rotate_heads_grad.argtypes[1:]
@@ -128,9 +130,11 @@ def load():
     lib.bw_prompt_attention.argtypes = [prompt, i32] + [vp, i64, i64] * 3 + [vp, vp, vp, size, vp]
     lib.bw_prompt_attention_grad.argtypes = [prompt, i32] + [vp, i64, i64] * 4 + [vp] * 6 + [size, vp]
     lib.bw_prompt_attention_workspace_bytes.argtypes = lib.bw_prompt_attention_grad_workspace_bytes.argtypes = [prompt]
-    for name in ("bw_rotate_heads_grad_workspace_bytes", "bw_cache_attention_workspace_bytes", "bw_prompt_attention_workspace_bytes", "bw_prompt_attention_grad_workspace_bytes"):
+    for name in ("bw_rotate_heads_grad_workspace_bytes", "bw_cache_attention_workspace_bytes", "bw_cache_attention_window_workspace_bytes", "bw_prompt_attention_workspace_bytes",
+                 "bw_prompt_attention_grad_workspace_bytes"):
         getattr(lib, name).restype = size
-    for name in ("bw_rotate_heads", "bw_rotate_heads_grad", "bw_rotate_axes", "bw_rotate_axes_grad", "bw_cache_append", "bw_cache_write", "bw_cache_read", "bw_cache_attention", "bw_prompt_attention", "bw_prompt_attention_grad"):
+    for name in ("bw_rotate_heads", "bw_rotate_heads_grad", "bw_rotate_axes", "bw_rotate_axes_grad", "bw_cache_append", "bw_cache_write", "bw_cache_read", "bw_cache_attention",
+                 "bw_cache_attention_window", "bw_prompt_attention", "bw_prompt_attention_grad"):
         getattr(lib, name).restype = i32
     for name in ("bw_quantize_pack", "bw_quantize_pack_add", "bw_dequantize", "bw_qgemv", "bw_qgemm", "bw_qgemm_ws", "bw_qgemm_static", "bw_qlinear"):
         getattr(lib, name).restype = i32

@@ -329,6 +329,14 @@ int bw_cache_attention(const bw_cache* cache, int act_dtype, const void* q, int6
                        const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, void* out,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same over a sliding window: the last `window` of a sequence's tokens count (0: all) and its first `sinks`.  Table entries of pages without a token that counts are not looked
+ * at, so that pages which a window has left may be given back. */
+size_t bw_cache_attention_window_workspace_bytes(const bw_cache* cache, int64_t B, int q_heads, int64_t max_pages, int64_t window, int64_t sinks);
+
+int bw_cache_attention_window(const bw_cache* cache, int act_dtype, const void* q, int64_t B, int q_heads, int64_t q_row, int64_t q_head,
+                              const int32_t* page_table, int64_t max_pages, int64_t table_row, const int32_t* lengths, float scale, int64_t window,
+                              int64_t sinks, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Attention of many tokens of each sequence: prompts, training ----
  *   out = sum_t softmax_t(scale q . k_t) v_t   over the tokens t that a new token sees: those up to its own, of them the last `window` and the first
  *   `sinks` (window 0: all)
