@@ -90,45 +90,38 @@ int splits_of(const bw_prompt* p) {
     return (int)(splits < 1 ? 1 : splits < 64 ? splits : 64);
 }
 
-// Gradients of keys and values from their parts: a thread has 4 values.
-template <int DT>
-__global__ __launch_bounds__(256) void prompt_grad_join_kernel(const float* parts, int splits, int64_t all, int dim, uint16_t* k_grad, uint16_t* v_grad) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;                 // of [keys][2][dim]
-    if (at >= all) return;
-    f4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; s++) x += *reinterpret_cast<const f4*>(parts + s * all + at);
-    const int64_t pair = at / dim;
-    uint16_t* out = pair & 1 ? v_grad : k_grad;
-    if (out) store4<DT>(out + (pair >> 1) * dim + (at - pair * dim), x[0], x[1], x[2], x[3]);
-}
-
-// How the gradients' work is cut, and where their workspace has what.
-constexpr int kGradKeys = 32 * kPromptWaves;
+// How the gradients' work is cut, and where their workspace has what (bytes).
+constexpr int kPiecesPerCu = 4;                  // about, over all heads
 struct GradPlan {
-    int splits, far, sinks;
-    size_t delta, parts, sink_parts;             // bytes
+    int target;                                  // pieces of a head; 0: every tile of keys is one
+    int64_t pieces, parts, joins;                // at most
+    size_t delta, plan, parts_at, all;
 };
 GradPlan grad_plan(const bw_prompt* p) {
-    const PromptArgs a = args_of(p);
-    const int64_t resident = bw_device_cus() * (p->dim > 128 ? 1 : 2), seq_q = p->q_tokens / (p->q_starts ? 1 : p->sequences);
-    const int64_t blocks = p->kv_heads * (p->q_starts ? (p->k_tokens + kGradKeys - 1) / kGradKeys : p->sequences * tiles_of(p, p->k_tokens, 1, kGradKeys));
-    const bool window = a.window < p->k_tokens;
-    // tiles of rows that a tile of keys meets, and all that there are
+    const int64_t share = p->q_heads / p->kv_heads, seq_q = p->q_tokens / (p->q_starts ? 1 : p->sequences);
     const int tile = key_tile(p->dim);
-    const int64_t all = (seq_q * a.share + tile - 1) / tile, near_ = window ? ((int64_t)(a.window + kGradKeys) * a.share + tile - 1) / tile : all;
+    const int64_t row_tiles = (seq_q * share + tile - 1) / tile, sequences = p->q_starts ? p->sequences + 2 : p->sequences;
+    const int64_t key_tiles = p->q_starts ? p->k_tokens / kGradKeys + sequences : p->sequences * tiles_of(p, p->k_tokens, 1, kGradKeys);
     GradPlan g = {};
-    const int64_t most = (near_ < all ? near_ : all) / kPartTiles, want = blocks > 0 ? (resident + blocks - 1) / blocks : 1, splits = want < most ? want : most;
-    g.splits = (int)(splits < 1 ? 1 : splits < 16 ? splits : 16);
-    if (window && a.sinks > 0 && p->q_tokens > 0) {
-        g.sinks = a.sinks;
-        const size_t one = (size_t)p->sequences * p->kv_heads * g.sinks * 2 * p->dim * sizeof(float);
-        int64_t far = (all + near_ - 1) / near_;
-        while (far > 1 && one * far > (size_t)256 << 20) far /= 2;
-        g.far = (int)(far < 64 ? far : 64);
-        g.sink_parts = one * g.far;
+    auto room = [&](size_t bytes) {
+        const size_t at = g.all;
+        g.all += (bytes + 15) / 16 * 16;
+        return at;
+    };
+    g.delta = room((size_t)(p->q_tokens * p->q_heads) * sizeof(float));
+    if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
+        g.target = (int)(((int64_t)bw_device_cus() * kPiecesPerCu + p->kv_heads - 1) / p->kv_heads);
+        // (a tile of n among U tiles of rows is cut into n / size rounded up, size at least U / target and kLeastTiles)
+        g.pieces = key_tiles + g.target;
+        const int64_t most = key_tiles * ((row_tiles + kLeastTiles - 1) / kLeastTiles);
+        g.parts = 2 * (int64_t)g.target < most ? 2 * g.target : most;
+        g.joins = g.parts / 2 < key_tiles ? g.parts / 2 : key_tiles;
+        g.plan = room(sizeof(KeyPlan) + 8);
+        room((size_t)g.pieces * sizeof(Piece));
+        room((size_t)g.joins * sizeof(KeyJoin));
+        room((size_t)sequences * sizeof(int));
+        g.parts_at = room((size_t)g.parts * p->kv_heads * kGradKeys * 2 * p->dim * sizeof(float));
     }
-    g.delta = ((size_t)(p->q_tokens * p->q_heads) + 3) / 4 * 16;
-    if (g.splits > 1) g.parts = (size_t)g.splits * p->k_tokens * p->kv_heads * 2 * p->dim * sizeof(float);
     return g;
 }
 
@@ -178,8 +171,7 @@ extern "C" int bw_prompt_attention(const bw_prompt* p, int act_dtype, const void
 
 extern "C" size_t bw_prompt_attention_grad_workspace_bytes(const bw_prompt* p) {
     if (prompt_check(p, BW_F16) != BW_OK) return 0;
-    const GradPlan plan = grad_plan(p);
-    return plan.delta + plan.parts + plan.sink_parts;
+    return grad_plan(p).all;
 }
 
 extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const void* grad, int64_t grad_row, int64_t grad_head, const void* q, int64_t q_row,
@@ -198,9 +190,8 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     for (auto [row, head] : {std::pair<int64_t, int64_t>{q_row, q_head}, {grad_row, grad_head}})
         if (head < 0 || head >= (int64_t)1 << 30 || (share - 1) * head + 65 * row >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
     const GradPlan plan = grad_plan(p);
-    const size_t bytes = plan.delta + plan.parts + plan.sink_parts;
-    if (bytes) {
-        if (!workspace || workspace_bytes < bytes) return BW_EWORKSPACE;
+    if (plan.all) {
+        if (!workspace || workspace_bytes < plan.all) return BW_EWORKSPACE;
         if (!bw_aligned(workspace, 16)) return BW_EALIGN;
     }
     PromptGradArgs g = {};
@@ -213,9 +204,7 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     g.result = (const uint16_t*)out;
     g.q_grad = (uint16_t*)q_grad; g.k_grad = (uint16_t*)k_grad; g.v_grad = (uint16_t*)v_grad;
     g.delta = (float*)workspace;
-    g.parts = (float*)((char*)workspace + plan.delta);
-    g.sink_parts = (float*)((char*)workspace + plan.delta + plan.parts);
-    g.far = plan.far;
+    a.splits = 1;
     g.plain_scale = p->scale;
     PromptGrids grids = {};
     const bool keys = (k_grad || v_grad) && p->k_tokens > 0;
@@ -226,23 +215,27 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
         grids.row_tiles = (uint32_t)tiles;
     }
     if (keys) {
-        const int64_t tiles = tiles_of(p, p->k_tokens, 1, kGradKeys), grid = tiles * a.combos * plan.splits;
-        const int64_t far_combos = (int64_t)p->sequences * p->kv_heads, far = plan.far ? far_combos * plan.far * ((plan.sinks + kGradKeys - 1) / kGradKeys) : 0;
-        if (grid >= (int64_t)1 << 24 || far >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
-        grids.keys = (uint32_t)grid;
+        const int64_t tiles = tiles_of(p, p->k_tokens, 1, kGradKeys), grid = plan.target ? plan.pieces * p->kv_heads : tiles * a.combos;
+        if (grid >= (int64_t)1 << 23 || plan.joins * p->kv_heads >= (int64_t)1 << 22) return BW_EUNSUPPORTED;
+        grids.keys = (uint32_t)(k_grad && v_grad ? 2 * grid : grid);
         grids.key_tiles = (uint32_t)tiles;
-        grids.key_splits = (uint32_t)plan.splits;
-        grids.far = (uint32_t)far;
-        grids.far_combos = (uint32_t)far_combos;
+        if (plan.target) {
+            grids.joins = (uint32_t)plan.joins;
+            char* at = (char*)workspace + plan.plan;
+            auto next = [&](size_t bytes) {
+                char* here = at;
+                at += (bytes + 15) / 16 * 16;
+                return here;
+            };
+            g.target = plan.target;
+            g.room = (int)plan.pieces; g.parts_room = (int)plan.parts; g.joins_room = (int)plan.joins;
+            g.plan = (KeyPlan*)next(sizeof(KeyPlan) + 8);
+            g.pieces = (Piece*)next((size_t)plan.pieces * sizeof(Piece));
+            g.joins = (KeyJoin*)next((size_t)plan.joins * sizeof(KeyJoin));
+            g.tiles_before = (int*)at;
+            g.parts = (float*)((char*)workspace + plan.parts_at);
+        }
     }
     const hipStream_t st = (hipStream_t)stream;
-    if (int failed = act_dtype == BW_F16 ? bw_launch_prompt_grad_f16(g, grids, st) : bw_launch_prompt_grad_bf16(g, grids, st)) return failed;
-    if (keys && plan.splits > 1) {
-        const int64_t all = p->k_tokens * p->kv_heads * 2 * p->dim;
-        const dim3 grid((unsigned)((all / 4 + 255) / 256));
-        if (act_dtype == BW_F16) hipLaunchKernelGGL(prompt_grad_join_kernel<BW_F16>, grid, dim3(256), 0, st, g.parts, plan.splits, all, p->dim, g.k_grad, g.v_grad);
-        else hipLaunchKernelGGL(prompt_grad_join_kernel<BW_BF16>, grid, dim3(256), 0, st, g.parts, plan.splits, all, p->dim, g.k_grad, g.v_grad);
-        if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
-    }
-    return BW_OK;
+    return act_dtype == BW_F16 ? bw_launch_prompt_grad_f16(g, grids, st) : bw_launch_prompt_grad_bf16(g, grids, st);
 }

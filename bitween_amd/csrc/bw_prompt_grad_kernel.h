@@ -1,7 +1,7 @@
 // bw_prompt_grad_kernel.h - gradients of the attention in bw_prompt_kernel.h.  With P = 2^(S c - lse), the weights of the forward again, and g the output's gradient:
 //   dP = g V^T,  delta = rowsum(g out),  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T g
-// One kernel has the rows and goes over the keys (dQ, and delta on the way), another has the keys and goes over the rows (dK, dV), so that every sum is one
-// workgroup's, in one order, and nothing is added up in memory: seven products where five would do, and the same bits every time.
+// One kernel has the rows and goes over the keys (dQ, and delta on the way), another has the keys and goes over the rows (dK, dV), so that every sum is a
+// workgroup's own, in one order: seven products where five would do with sums in memory, and the same bits every time.
 //
 // P and dS enter their second product as 16-bit numbers, rounded once.  In float16, whose steps end at 2^-24, P goes in 2^12 times as large, and dS times a power of two that
 // is each row's (each key's) own: it starts high and comes down where a product would pass 2^15, and the sums with it.
@@ -14,10 +14,15 @@ struct PromptGradArgs {
     int64_t grad_row, grad_head;
     float* delta;                                // as lse
     uint16_t *q_grad, *k_grad, *v_grad;
-    float* parts;                                // [splits][k_tokens][kv_heads][2][dim], where splits > 1
-    float* sink_parts;                           // [sequences][kv_heads][far][sinks][2][dim]
-    int far;                                     // workgroups that share the rows which see a sequence's sinks and not their window; 0: none
     float plain_scale;
+    // keys: the list of the workgroups' pieces (NULL: a piece for every tile of keys), the parts [part][kv_heads][keys][2][dim] and what is to be joined of them
+    struct KeyPlan* plan;
+    struct Piece* pieces;
+    struct KeyJoin* joins;
+    int* tiles_before;                           // of sequence s: where its tiles of keys begin
+    float* parts;
+    int target;                                  // pieces (of one head) that the rows are cut into, about
+    int room, parts_room, joins_room;            // of the lists (starts that decrease could ask for more: tiles of keys are then left out, or not cut)
 };
 
 constexpr int kFirstReach16 = 80, kReachTop = 12, kReachMost = 15, kWeightShift = 12;
@@ -59,7 +64,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     Span p;
     int head;
     uint32_t split;
-    if (!place_of<kRows, false>(a, p, head, split)) return;
+    if (!place_of<kRows, false>(a, blockIdx.x, p, head, split)) return;
     clear_tiles<H>(smem, 4 * H::kTileBytes, a.dim);
     const int row0 = p.tile * kRows + wave * kWaveRows, rows = p.nq * a.share;
     const Row row(a, p, row0 + (lane & 31));
@@ -170,20 +175,71 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         }
 }
 
-// A tile of rows of a sequence (tokens x the query heads of one key head) on its way to LDS; rows from the last on are the last one again.
+// ---- keys ----
+//
+// A workgroup has 128 keys of one sequence and one key head, 32 to a wave, and the rows come by, kKeys at a time: S and dP with a key to a lane, so that P and dS are the
+// second operands of dV^T += g^T P and dK^T += Q^T dS as they lie.  dV and dK are workgroups of their own, side by side in one launch, though both need S: one wave with
+// both sums does not fit (64 registers of operands and 128 of sums leave too few: 283 TFLOP/s with 250 bytes of a lane in memory), and two waves that share S and P through LDS
+// wait for each other every 32 rows (8192 tokens, 32 and 8 heads of 128: 2068 us).
+//
+// Rows are cut into pieces of equal length, each a workgroup's: a small kernel lists them first (plan_keys_kernel), since a key that is seen by all rows meets many times the
+// rows of the last one.  The parts of keys that several workgroups have are added up in order by prompt_grad_join_kernel.
+constexpr int kGradKeys = 32 * kPromptWaves;
+
+// Tiles from ... to - 1 of rows (kKeys each) for the keys from kGradKeys tile on of a sequence; part: which of the parts they leave, or -1.
+struct Piece { int q0, nq, k0, nk, tile, from, to, part; };
+// Keys whose parts are to be added up.
+struct KeyJoin { int key, keys, part, parts; };
+struct KeyPlan { int pieces, joins; };
+
+// Rows of a sequence that see a key: from ... to - 1.
+BW_DEV void rows_of_key(const PromptArgs& a, int nq, int nk, int key, int& from, int& to) {
+    auto row_at = [&](int64_t position) {
+        const int64_t r = (position - (nk - nq)) * a.share, rows = (int64_t)nq * a.share;
+        return (int)(r < 0 ? 0 : r < rows ? r : rows);
+    };
+    from = row_at(key);
+    to = key < a.sinks ? nq * a.share : row_at((int64_t)key + a.window);
+}
+// Tiles of rows that a tile of keys meets.
+BW_DEV void tiles_of_keys(const PromptArgs& a, int nq, int nk, int tile, int tile_rows, int& from, int& to) {
+    const int first = tile * kGradKeys, last = (first + kGradKeys < nk ? first + kGradKeys : nk) - 1;
+    int begin, end, other;
+    rows_of_key(a, nq, nk, first, begin, end);
+    rows_of_key(a, nq, nk, last, other, other);
+    end = end > other ? end : other;
+    from = begin / tile_rows;
+    to = end > begin ? (end - 1) / tile_rows + 1 : from;
+}
+
+// Tiles of rows of a sequence (tokens x the query heads of one key head) on their way to LDS; rows from the last on are the last one again.  Where a tile is whole tokens, as it is
+// for 1, 2, 4 ... query heads to a key head, a lane's place in it stays the same.
 template <class H> struct PackedLoader {
-    uint32_t chunk[H::kLoads];
+    uint32_t place[H::kLoads], chunk[H::kLoads];
     int first;
-    BW_DEV PackedLoader(int lane, int wave) {
+    bool same;
+    BW_DEV PackedLoader(const PromptArgs& a, int lane, int wave, int64_t row, int64_t head) {
         first = wave * H::kLoads * H::kLoadRows + lane / H::kChunks;
+        same = H::kKeys % a.share == 0 && a.dim == H::kPitch;
 #pragma unroll
-        for (int i = 0; i < H::kLoads; i++) chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(first + i * H::kLoadRows)) * 16;
+        for (int i = 0; i < H::kLoads; i++) {
+            const int r = first + i * H::kLoadRows;
+            chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(r)) * 16;
+            uint32_t j;
+            const uint32_t token = a.by_share.div((uint32_t)r, j);
+            place[i] = token * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i];
+        }
     }
     BW_DEV void operator()(const PromptArgs& a, const uint16_t* base, int64_t row, int64_t head, int from, int rows, uint32_t to, int wave) const {
         to += wave * H::kLoads * 1024;
         uint32_t rest;
         const uint32_t token0 = a.by_share.div((uint32_t)from, rest);
         base += token0 * row;
+        if (same && from + H::kKeys <= rows) {
+#pragma unroll
+            for (int i = 0; i < H::kLoads; i++) load_to_lds(base, place[i], to + i * 1024);
+            return;
+        }
         uint32_t bytes = (uint32_t)a.dim * 2;
         asm("" : "+s"(bytes));
 #pragma unroll
@@ -191,8 +247,7 @@ template <class H> struct PackedLoader {
             const int r = from + first + i * H::kLoadRows;
             uint32_t j;
             const uint32_t token = a.by_share.div((uint32_t)(r < rows ? r : rows - 1), j);
-            const uint32_t at = (token - token0) * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i];
-            if (chunk[i] < bytes) load_to_lds(base, at, to + i * 1024);
+            if (chunk[i] < bytes) load_to_lds(base, (token - token0) * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i], to + i * 1024);
         }
     }
 };
@@ -200,162 +255,112 @@ BW_DEV void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
 }
 
-// FAR: only rows that see the keys as sinks and not in their window, a share of them; otherwise only those that have them in their window (all, without a window).
-template <class H, bool FAR>
-__global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(PromptGradArgs g) {
-    extern __shared__ __align__(1024) char smem[];               // [2][Q, g, lse, delta]
-    constexpr int DT = H::kType, kTileKeys = 32 * kPromptWaves, kStage = 2 * H::kTileBytes + 512, kTileRows = H::kKeys;
+template <class H> constexpr int kKeyStage = 2 * H::kTileBytes + 512;           // Q, g, lse, delta of a tile of rows
+
+// One piece: dK of its keys, or dV.
+template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const Piece& p, int head, char* smem) {
+    constexpr int DT = H::kType, kTileRows = H::kKeys;
     const PromptArgs& a = g.p;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5;
-    Span p;
-    int head, sequence = 0;
-    uint32_t split;
-    if (FAR) {                                                   // a workgroup for a sequence, a tile of its sinks and a share of the rows
-        uint32_t combo, s, h;
-        uint32_t slot = a.by_combos.div(blockIdx.x, combo);
-        split = slot % (uint32_t)g.far;
-        slot /= (uint32_t)g.far;
-        s = a.by_heads.div(combo, h);
-        head = (int)h;
-        sequence = (int)s;
-        if (a.q_starts) {
-            tokens_at(a.q_starts, sequence, a.sequences, a.q_tokens, p.q0, p.nq);
-            tokens_at(a.k_starts, sequence, a.sequences, a.k_tokens, p.k0, p.nk);
-            p.q0 = __builtin_amdgcn_readfirstlane(p.q0);
-            p.nq = __builtin_amdgcn_readfirstlane(p.nq);
-            p.k0 = __builtin_amdgcn_readfirstlane(p.k0);
-            p.nk = __builtin_amdgcn_readfirstlane(p.nk);
-        } else {
-            p = Span{sequence * a.seq_q, a.seq_q, sequence * a.seq_k, a.seq_k, 0};
-        }
-        p.tile = (int)slot;
-    } else {
-        if (!place_of<kTileKeys, true>(a, p, head, split, &sequence)) return;
-    }
-    const int first = p.tile * kTileKeys, keys_all = FAR && a.sinks < p.nk ? a.sinks : p.nk, rows = p.nq * a.share, offset = p.nk - p.nq;
-    if (FAR && first >= keys_all) return;
-    clear_tiles<H>(smem, 2 * kStage, a.dim);
-    const int key = first + wave * 32 + (lane & 31);
-    const bool live = key < keys_all;
+    const int rows = p.nq * a.share, wave_first = p.tile * kGradKeys + wave * 32, key = wave_first + (lane & 31);
+    const bool live = key < p.nk;
     const int64_t token = p.k0 + (live ? key : 0);
-    u4 k[H::kSteps], v[H::kSteps];
+    u4 k[H::kSteps], v[DK ? H::kSteps : 1];
     load_row<H>(k, a.k + token * a.k_row + head * a.k_head, live, a.dim, half);
-    load_row<H>(v, a.v + token * a.v_row + head * a.v_head, live, a.dim, half);
+    if constexpr (DK) load_row<H>(v, a.v + token * a.v_row + head * a.v_head, live, a.dim, half);
 #pragma unroll
     for (int s = 0; s < H::kSteps; s++)
 #pragma unroll
         for (int j = 0; j < 4; j++) k[s][j] ^= a.flip;
 
-    // Rows that count for a key: from ... to - 1 (positions key ... key + window - 1; further ones as a sink).
-    auto row_at = [&](int64_t position) {
-        const int64_t r = (position - offset) * a.share;
-        return (int)(r < 0 ? 0 : r < rows ? r : rows);
-    };
-    auto rows_of = [&](int n, int& from, int& to) {
-        from = row_at(FAR ? (int64_t)n + a.window : n);
-        to = FAR ? rows : row_at((int64_t)n + a.window);
-    };
-    int row_from, row_to, from, to, other;
-    rows_of(key, row_from, row_to);
-    if (!live) row_from = row_to = 0;
-    const int last = (first + kTileKeys < keys_all ? first + kTileKeys : keys_all) - 1;
-    if (last < first) from = to = 0;
-    else {
-        rows_of(first, from, other);
-        rows_of(last, other, to);
+    // Rows that count for the lane's key; for any of the wave's; for all of them.
+    int row_from = 0, row_to = 0, any_from = 0, any_to = 0, all_from = 0, all_to = 0;
+    if (live) rows_of_key(a, p.nq, p.nk, key, row_from, row_to);
+    if (wave_first < p.nk) {
+        const int wave_last = wave_first + 31 < p.nk ? wave_first + 31 : p.nk - 1;
+        int first_to, last_to, ignored;
+        rows_of_key(a, p.nq, p.nk, wave_first, any_from, first_to);
+        rows_of_key(a, p.nq, p.nk, wave_last, all_from, last_to);
+        any_to = first_to > last_to ? first_to : last_to;
+        // (the first key that is no sink leaves its window first)
+        rows_of_key(a, p.nq, p.nk, a.sinks > wave_first && a.sinks <= wave_last ? a.sinks : wave_first, ignored, all_to);
     }
-    // ... for all of the wave's keys, and for any
-    const int wave_first = first + wave * 32, wave_last = wave_first + 31 < last ? wave_first + 31 : last;
-    int any_from = 0, any_to = 0, all_from = 0, all_to = 0;
-    if (wave_first <= wave_last) {
-        rows_of(wave_first, any_from, all_to);
-        rows_of(wave_last, all_from, any_to);
-    }
-    const int tile_from = from / kTileRows, tile_count = to > from ? (to - 1) / kTileRows - tile_from + 1 : 0, pieces = FAR ? g.far : a.splits;
-    const int begin = (int)((int64_t)tile_count * split / pieces), end = (int)((int64_t)tile_count * (split + 1) / pieces);
 
-    const PackedLoader<H> load(lane, wave);
+    const PackedLoader<H> load_q(a, lane, wave, a.q_row, a.q_head), load_g(a, lane, wave, g.grad_row, g.grad_head);
     const TileReader<H> read(lane);
     const uint16_t *queries = a.q + p.q0 * a.q_row + (int64_t)head * a.share * a.q_head, *grads = g.grad + p.q0 * g.grad_row + (int64_t)head * a.share * g.grad_head;
     const int64_t stats = (int64_t)head * a.q_tokens * a.share + (int64_t)p.q0 * a.share;
     const uint32_t lds = lds_address(smem);
     auto fetch = [&](int i) __attribute__((always_inline)) {
-        const int at = (tile_from + i) * kTileRows;
-        const uint32_t into = lds + (i & 1) * kStage;
-        load(a, queries, a.q_row, a.q_head, at, rows, into, wave);
-        load(a, grads, g.grad_row, g.grad_head, at, rows, into + H::kTileBytes, wave);
+        const int at = i * kTileRows;
+        const uint32_t into = lds + (i & 1) * kKeyStage<H>;
+        load_q(a, queries, a.q_row, a.q_head, at, rows, into, wave);
+        load_g(a, grads, g.grad_row, g.grad_head, at, rows, into + H::kTileBytes, wave);
         const int r = at + lane < rows ? lane : rows - 1 - at;
         if (wave == 0) load4_to_lds(a.lse + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes);
-        if (wave == 1) load4_to_lds(g.delta + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes + 256);
+        if (DK && wave == 1) load4_to_lds(g.delta + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes + 256);
     };
 
-    f16v dk[H::kBlocks], dv[H::kBlocks];
+    f16v acc[H::kBlocks];
     int reach = 0;
-    for (int careful = 0;; careful = 1) {
+    for (int careful = 0;; careful = 1) {                        // (see prompt_forward_kernel)
 #pragma unroll
-        for (int m = 0; m < H::kBlocks; m++) dk[m] = dv[m] = f16v{};
+        for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
-        if (begin < end) fetch(begin);
-        for (int i = begin; i < end; i++) {
+        if (p.from < p.to) fetch(p.from);
+        for (int i = p.from; i < p.to; i++) {
             wait_tiles();
-            if (i + 1 < end) fetch(i + 1);
-            char* tile = smem + (i & 1) * kStage;
-            const int at = (tile_from + i) * kTileRows;
+            if (i + 1 < p.to) fetch(i + 1);
+            char* tile = smem + (i & 1) * kKeyStage<H>;
+            const int at = i * kTileRows;
             const bool none = at >= any_to || at + kTileRows <= any_from, all = at >= all_from && at + kTileRows <= all_to;
             if (!careful && none) continue;
 #pragma unroll
             for (int b = 0; b < kTileRows / 32; b++) {
-                u4 pw[2], sw[2];
+                u4 w[2];
                 if (!none) {
                     f16v s = f16v{}, dp = f16v{};
 #pragma unroll
                     for (int n = 0; n < H::kSteps; n++) s = mfma32<DT>(read.rows(tile, b, n), k[n], s);
+                    if constexpr (DK) {
 #pragma unroll
-                    for (int n = 0; n < H::kSteps; n++) dp = mfma32<DT>(read.rows(tile + H::kTileBytes, b, n), v[n], dp);
-                    float w[16], ds[16];
+                        for (int n = 0; n < H::kSteps; n++) dp = mfma32<DT>(read.rows(tile + H::kTileBytes, b, n), v[n], dp);
+                    }
+                    float x[16];
+                    const char* stat = tile + 2 * H::kTileBytes + (32 * b + 4 * half) * 4;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const f4 lse = *reinterpret_cast<const f4*>(tile + 2 * H::kTileBytes + (32 * b + 8 * j + 4 * half) * 4);
-                        const f4 delta = *reinterpret_cast<const f4*>(tile + 2 * H::kTileBytes + 256 + (32 * b + 8 * j + 4 * half) * 4);
+                        const f4 lse = *reinterpret_cast<const f4*>(stat + 32 * j);
 #pragma unroll
-                        for (int n = 0; n < 4; n++) {
-                            w[4 * j + n] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + n], a.scale, (DT == BW_F16 ? (float)kWeightShift : 0.f) - lse[n]));
-                            ds[4 * j + n] = w[4 * j + n] * (dp[4 * j + n] - delta[n]);
+                        for (int n = 0; n < 4; n++) x[4 * j + n] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + n], a.scale, (DT == BW_F16 ? (float)kWeightShift : 0.f) - lse[n]));
+                        if constexpr (DK) {
+                            const f4 delta = *reinterpret_cast<const f4*>(stat + 256 + 32 * j);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) x[4 * j + n] *= dp[4 * j + n] - delta[n];
                         }
                     }
                     if (!all) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
                             const int r = at + 32 * b + 8 * (j / 4) + 4 * half + j % 4;
-                            const bool counts = r >= row_from && r < row_to;
-                            w[j] = counts ? w[j] : 0.f;
-                            ds[j] = counts ? ds[j] : 0.f;
+                            x[j] = r >= row_from && r < row_to ? x[j] : 0.f;
                         }
                     }
-                    if constexpr (DT == BW_F16) fit_reach<16, H::kBlocks>(ds, reach, dk);
-                    pack16<DT>(w, pw);
-                    pack16<DT>(ds, sw);
+                    if constexpr (DK && DT == BW_F16) fit_reach<16, H::kBlocks>(x, reach, acc);
+                    pack16<DT>(x, w);
                 }
+                char* from = tile + (DK ? 0 : H::kTileBytes);
                 if (careful) {
-                    char *qs = tile + b * 32 * H::kPitch * 2, *gs = qs + H::kTileBytes;
+                    char* block = from + b * 32 * H::kPitch * 2;
                     __syncthreads();
-                    if (!none) {
-                        auto counts = [&](int n) { return at + 32 * b + n >= row_from && at + 32 * b + n < row_to; };
-                        add_nonfinite<H>(qs, 32, lane, dk, counts);
-                        add_nonfinite<H>(gs, 32, lane, dv, counts);
-                    }
-                    keep_finite<H>(qs, 32 * H::kPitch * 2);
-                    keep_finite<H>(gs, 32 * H::kPitch * 2);
+                    if (!none) add_nonfinite<H>(block, 32, lane, acc, [&](int n) { return at + 32 * b + n >= row_from && at + 32 * b + n < row_to; });
+                    keep_finite<H>(block, 32 * H::kPitch * 2);
                 }
                 if (!none) {
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
-                        for (int m = 0; m < H::kBlocks; m++) dv[m] = mfma32<DT>(read.columns(tile + H::kTileBytes, 2 * b + t, m), pw[t], dv[m]);
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int m = 0; m < H::kBlocks; m++) dk[m] = mfma32<DT>(read.columns(tile, 2 * b + t, m), sw[t], dk[m]);
+                        for (int m = 0; m < H::kBlocks; m++) acc[m] = mfma32<DT>(read.columns(from, 2 * b + t, m), w[t], acc[m]);
                 }
             }
         }
@@ -364,36 +369,174 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(Prom
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) check = __builtin_fmaf(dv[m][j], 0.f, __builtin_fmaf(dk[m][j], 0.f, check));
+            for (int j = 0; j < 16; j++) check = __builtin_fmaf(acc[m][j], 0.f, check);
         if (!any_thread(smem, wave, live && check != 0.f)) break;
     }
     if (!live) return;
-    const float k_by = g.plain_scale * (DT == BW_F16 ? __builtin_ldexpf(1.f, -reach - kWeightShift) : 1.f), v_by = DT == BW_F16 ? __builtin_ldexpf(1.f, -kWeightShift) : 1.f;
-    const int64_t sink_at = ((int64_t)(sequence * a.kv_heads + head) * g.far * a.sinks + key) * 2 * a.dim;
-    float* part = FAR ? g.sink_parts + sink_at + (int64_t)split * a.sinks * 2 * a.dim
-                      : a.splits > 1 ? g.parts + (((int64_t)split * a.k_tokens + token) * a.kv_heads + head) * 2 * a.dim : nullptr;
-    const bool sinks = !FAR && g.far && split == 0 && key < a.sinks && sequence < a.sequences;
+    const float by = (DK ? g.plain_scale : 1.f) * (DT == BW_F16 ? __builtin_ldexpf(1.f, -kWeightShift - (DK ? reach : 0)) : 1.f);
+    float* part = p.part < 0 ? nullptr : g.parts + ((((int64_t)p.part * a.kv_heads + head) * kGradKeys + key - p.tile * kGradKeys) * 2 + DK) * a.dim;
+    uint16_t* out = (DK ? g.k_grad : g.v_grad) + (token * a.kv_heads + head) * a.dim;
 #pragma unroll
     for (int m = 0; m < H::kBlocks; m++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             const int d = 32 * m + 8 * b + 4 * half;
+            const f4 x = f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]} * by;
             if (d >= a.dim) continue;
-            f4 x = f4{dk[m][4 * b], dk[m][4 * b + 1], dk[m][4 * b + 2], dk[m][4 * b + 3]} * k_by, y = f4{dv[m][4 * b], dv[m][4 * b + 1], dv[m][4 * b + 2], dv[m][4 * b + 3]} * v_by;
-            if (sinks) {
-                for (int n = 0; n < g.far; n++) {
-                    const float* from = g.sink_parts + sink_at + (int64_t)n * a.sinks * 2 * a.dim + d;
-                    x += *reinterpret_cast<const f4*>(from);
-                    y += *reinterpret_cast<const f4*>(from + a.dim);
-                }
-            }
-            if (part) {
-                *reinterpret_cast<f4*>(part + d) = x;
-                *reinterpret_cast<f4*>(part + a.dim + d) = y;
-            } else {
-                const int64_t to_at = (token * a.kv_heads + head) * a.dim + d;
-                if (g.k_grad) store4<DT>(g.k_grad + to_at, x[0], x[1], x[2], x[3]);
-                if (g.v_grad) store4<DT>(g.v_grad + to_at, y[0], y[1], y[2], y[3]);
-            }
+            if (part) *reinterpret_cast<f4*>(part + d) = x;
+            else store4<DT>(out + d, x[0], x[1], x[2], x[3]);
         }
+}
+
+template <class H>
+__global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(PromptGradArgs g) {
+    extern __shared__ __align__(1024) char smem[];               // [2][Q, g, lse, delta]
+    const PromptArgs& a = g.p;
+    // dK and dV in turn, where both are wanted
+    const bool both = g.k_grad && g.v_grad, dk = both ? !(blockIdx.x & 1) : g.k_grad != nullptr;
+    const uint32_t block = both ? blockIdx.x >> 1 : blockIdx.x;
+    uint32_t head;
+    Piece p;
+    if (g.plan) {
+        const uint32_t at = a.by_heads.div(block, head);
+        if ((int)at >= g.plan->pieces) return;
+        p = g.pieces[at];
+        if (p.nk == 0) return;
+    } else {
+        Span s;
+        int h;
+        uint32_t none;
+        if (!place_of<kGradKeys, true>(a, block, s, h, none)) return;
+        head = (uint32_t)h;
+        p = Piece{s.q0, s.nq, s.k0, s.nk, s.tile, 0, 0, -1};
+        tiles_of_keys(a, p.nq, p.nk, p.tile, H::kKeys, p.from, p.to);
+    }
+    clear_tiles<H>(smem, 2 * kKeyStage<H>, a.dim);
+    if (dk) key_grad<H, true>(g, p, (int)head, smem);
+    else key_grad<H, false>(g, p, (int)head, smem);
+}
+
+// ---- the list of pieces ----
+
+constexpr int kPlanThreads = 1024;
+// Sum of the threads' numbers before this one's, and of all.
+BW_DEV int sum_before(int* lds, int mine, int& all) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int other = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += other;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    int before = sum - mine;
+    all = 0;
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+        if (w < wave) before += lds[w];
+        all += lds[w];
+    }
+    return before;
+}
+
+// Every tile of keys in pieces of at most so many tiles of rows that there are about g.target pieces; one workgroup.
+static __global__ __launch_bounds__(kPlanThreads) void plan_keys_kernel(PromptGradArgs g, int tile_rows, int least) {
+    __shared__ int lds[kPlanThreads / 64];
+    __shared__ unsigned long long units;
+    const PromptArgs& a = g.p;
+    const int sequences = a.q_starts ? a.sequences + 2 : a.sequences, thread = (int)threadIdx.x;
+    auto tokens = [&](int s, Piece& p) {
+        if (a.q_starts) {
+            tokens_at(a.q_starts, s, a.sequences, a.q_tokens, p.q0, p.nq);
+            tokens_at(a.k_starts, s, a.sequences, a.k_tokens, p.k0, p.nk);
+            if (s >= a.sequences) p.nq = 0;
+        } else {
+            p.q0 = s * a.seq_q; p.nq = a.seq_q; p.k0 = s * a.seq_k; p.nk = a.seq_k;
+        }
+    };
+    int tiles = 0;
+    for (int base = 0; base < sequences; base += kPlanThreads) {
+        const int s = base + thread;
+        Piece p = {};
+        if (s < sequences) tokens(s, p);
+        int all;
+        const int before = tiles + sum_before(lds, (p.nk + kGradKeys - 1) / kGradKeys, all);
+        if (s < sequences) g.tiles_before[s] = before;
+        tiles += all;
+    }
+    if (thread == 0) units = 0;
+    __syncthreads();                                             // (and its fence: tiles_before is read below)
+    auto piece_of = [&](int n) {                                 // the n-th tile of keys
+        int lo = 0, hi = sequences;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (g.tiles_before[mid] <= n) lo = mid;
+            else hi = mid;
+        }
+        Piece p = {};
+        tokens(lo, p);
+        p.tile = n - g.tiles_before[lo];
+        tiles_of_keys(a, p.nq, p.nk, p.tile, tile_rows, p.from, p.to);
+        return p;
+    };
+    unsigned long long mine = 0;
+    for (int n = thread; n < tiles; n += kPlanThreads) {
+        const Piece p = piece_of(n);
+        mine += (unsigned)(p.to - p.from);
+    }
+    atomicAdd(&units, mine);                                     // (whole numbers: any order gives the same)
+    __syncthreads();
+    const unsigned long long each = (units + g.target - 1) / g.target;
+    const int size = each > (unsigned)least ? (int)each : least;
+    int pieces = 0, parts = 0, joins = 0;
+    for (int base = 0; base < tiles; base += kPlanThreads) {
+        const int n = base + thread;
+        Piece p = {};
+        int cuts = 0;
+        if (n < tiles) {
+            p = piece_of(n);
+            cuts = (p.to - p.from + size - 1) / size;
+            if (cuts < 1) cuts = 1;
+        }
+        int all_pieces, all_parts, all_joins;
+        const int piece = pieces + sum_before(lds, cuts, all_pieces), part = parts + sum_before(lds, cuts > 1 ? cuts : 0, all_parts), join = joins + sum_before(lds, cuts > 1, all_joins);
+        const bool whole = cuts > 1 && (part + cuts > g.parts_room || join >= g.joins_room);
+        for (int c = 0; c < cuts && piece + c < g.room; c++) {
+            Piece one = p;
+            if (!whole) {
+                one.from = p.from + (int)((int64_t)(p.to - p.from) * c / cuts);
+                one.to = p.from + (int)((int64_t)(p.to - p.from) * (c + 1) / cuts);
+            } else if (c) {
+                one.nk = 0;                                      // nothing
+                one.to = one.from;
+            }
+            one.part = cuts > 1 && !whole ? part + c : -1;
+            g.pieces[piece + c] = one;
+        }
+        if (cuts > 1 && join < g.joins_room) g.joins[join] = whole ? KeyJoin{0, 0, 0, 0} : KeyJoin{p.k0 + p.tile * kGradKeys, p.nk - p.tile * kGradKeys < kGradKeys ? p.nk - p.tile * kGradKeys : kGradKeys, part, cuts};
+        pieces += all_pieces;
+        parts += all_parts;
+        joins += all_joins;
+    }
+    if (thread == 0) *g.plan = KeyPlan{pieces < g.room ? pieces : g.room, joins < g.joins_room ? joins : g.joins_room};
+}
+
+// Gradients of the keys that lie in several parts: a workgroup has 1024 values of one join and head, [keys][2][dim].
+template <int DT>
+__global__ __launch_bounds__(256) void prompt_grad_join_kernel(PromptGradArgs g, int chunks) {
+    const PromptArgs& a = g.p;
+    uint32_t head;
+    const uint32_t rest = a.by_heads.div(blockIdx.x, head);
+    const int join = (int)(rest / (uint32_t)chunks), at = (int)((rest - join * chunks) * 1024 + threadIdx.x * 4);
+    if (join >= g.plan->joins) return;
+    const KeyJoin j = g.joins[join];
+    if (at >= j.keys * 2 * a.dim) return;
+    const int64_t pitch = (int64_t)a.kv_heads * kGradKeys * 2 * a.dim;
+    const float* from = g.parts + ((int64_t)j.part * a.kv_heads + head) * kGradKeys * 2 * a.dim + at;
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < j.parts; n++) x += *reinterpret_cast<const f4*>(from + n * pitch);
+    const int key = at / (2 * a.dim), d = at - key * 2 * a.dim, other = d >= a.dim;
+    uint16_t* out = other ? g.k_grad : g.v_grad;
+    if (out) store4<DT>(out + ((int64_t)(j.key + key) * a.kv_heads + head) * a.dim + d - other * a.dim, x[0], x[1], x[2], x[3]);
 }

@@ -133,20 +133,22 @@ template <class H> struct TileReader {
 template <int DT> constexpr uint32_t kExponent = DT == BW_F16 ? 0x7C00u : 0x7F80u;
 template <int DT> BW_DEV bool finite16(uint32_t v) { return (v & kExponent<DT>) != kExponent<DT>; }
 // Whether it is true for any thread of the workgroup; through LDS that nothing else is in any more.
-BW_DEV bool any_thread(char* smem, int wave, bool is) {
+template <int WAVES = kPromptWaves> BW_DEV bool any_thread(char* smem, int wave, bool is) {
     const uint64_t hit = __builtin_amdgcn_ballot_w64(is);
     __syncthreads();
     reinterpret_cast<volatile uint32_t*>(smem)[wave] = hit != 0;
     __syncthreads();
-    const u4 all = *reinterpret_cast<const u4*>(smem);
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) any |= reinterpret_cast<const uint32_t*>(smem)[i];
     __syncthreads();
-    return __builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]);
+    return __builtin_amdgcn_readfirstlane(any);
 }
 // Infinities and NaN of a tile made 0, by the whole workgroup.
-template <class H> BW_DEV void keep_finite(char* tile, int bytes) {
+template <class H, int THREADS = 256> BW_DEV void keep_finite(char* tile, int bytes) {
     __syncthreads();
 #pragma unroll 1
-    for (int at = (int)threadIdx.x * 4; at < bytes; at += 256 * 4) {
+    for (int at = (int)threadIdx.x * 4; at < bytes; at += THREADS * 4) {
         const uint32_t w = *reinterpret_cast<uint32_t*>(tile + at);
         *reinterpret_cast<uint32_t*>(tile + at) = (finite16<H::kType>(w) ? w & 0xFFFFu : 0u) | (finite16<H::kType>(w >> 16) ? w & 0xFFFF0000u : 0u);
     }
@@ -197,7 +199,7 @@ BW_DEV void tokens_at(const int32_t* starts, int s, int sequences, int all, int&
 }
 // The slot'th tile over all sequences, TILE rows or keys each; false: there are fewer.  The last tile of a sequence, which sees the most, goes first (rows), or
 // the first, which most see (keys).
-template <int TILE, bool KEYS> BW_DEV bool find_tile(const PromptArgs& a, uint32_t slot, Span& p, int* sequence) {
+template <int TILE, bool KEYS> BW_DEV bool find_tile(const PromptArgs& a, uint32_t slot, Span& p) {
     const int lane = (int)threadIdx.x & 63;
     uint32_t before = 0;
     for (int base = 0; base < a.sequences + 2; base += 64) {
@@ -224,7 +226,6 @@ template <int TILE, bool KEYS> BW_DEV bool find_tile(const PromptArgs& a, uint32
             tokens_at(a.q_starts, found, a.sequences, a.q_tokens, p.q0, p.nq);
             tokens_at(a.k_starts, found, a.sequences, a.k_tokens, p.k0, p.nk);
             if (found >= a.sequences) (KEYS ? p.nq : p.nk) = 0;
-            if (sequence) *sequence = found;
             p.q0 = __builtin_amdgcn_readfirstlane(p.q0);
             p.nq = __builtin_amdgcn_readfirstlane(p.nq);
             p.k0 = __builtin_amdgcn_readfirstlane(p.k0);
@@ -238,19 +239,18 @@ template <int TILE, bool KEYS> BW_DEV bool find_tile(const PromptArgs& a, uint32
 
 // What this workgroup has: a tile of one sequence and one key-value head.  Neighbouring workgroups have different heads (and go to different dies), so that the
 // tiles of a head, which read the same keys, share a die's cache wherever 8 divides the number of heads.
-template <int TILE, bool KEYS> BW_DEV bool place_of(const PromptArgs& a, Span& p, int& head, uint32_t& split, int* sequence = nullptr) {
+template <int TILE, bool KEYS> BW_DEV bool place_of(const PromptArgs& a, uint32_t block, Span& p, int& head, uint32_t& split) {
     uint32_t combo;
-    uint32_t slot = a.by_combos.div(blockIdx.x, combo);
+    uint32_t slot = a.by_combos.div(block, combo);
     split = slot / a.tiles;
     slot -= split * a.tiles;
     if (a.q_starts) {
         head = (int)combo;
-        return find_tile<TILE, KEYS>(a, slot, p, sequence);
+        return find_tile<TILE, KEYS>(a, slot, p);
     }
     uint32_t h;
     const uint32_t s = a.by_heads.div(combo, h);
     head = (int)h;
-    if (sequence) *sequence = (int)s;
     p = Span{(int)s * a.seq_q, a.seq_q, (int)s * a.seq_k, a.seq_k, (int)(KEYS ? slot : a.tiles - 1 - slot)};
     return true;
 }
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     Span p;
     int head;
     uint32_t split;
-    if (!place_of<kRows, false>(a, p, head, split)) return;
+    if (!place_of<kRows, false>(a, blockIdx.x, p, head, split)) return;
     clear_tiles<H>(smem, 4 * H::kTileBytes, a.dim);
     const int row0 = p.tile * kRows + wave * kWaveRows, rows = p.nq * a.share;
     const Row row(a, p, row0 + (lane & 31));
