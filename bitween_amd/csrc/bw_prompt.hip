@@ -42,7 +42,7 @@ int prompt_check(const bw_prompt* p, int act_dtype) {
     if (!p->q_starts && (p->q_tokens % p->sequences || p->k_tokens % p->sequences)) return BW_EINVAL;
     if (act_dtype != BW_F16 && act_dtype != BW_BF16) return BW_EUNSUPPORTED;
     if (p->dim % 8 || p->dim > 256 || p->q_heads > 65535 || p->sequences > 1 << 20) return BW_EUNSUPPORTED;
-    if (p->q_tokens >= (int64_t)1 << 31 || p->k_tokens >= (int64_t)1 << 31 || p->q_tokens + p->k_tokens >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    if (p->q_tokens >= (int64_t)1 << 31 || p->k_tokens >= (int64_t)1 << 31 || p->q_tokens + p->k_tokens >= ((int64_t)1 << 31) - 1024) return BW_EUNSUPPORTED;
     if (p->q_tokens * p->q_heads >= (int64_t)1 << 31 || (p->k_tokens + p->q_tokens) * p->kv_heads >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
     if (!bw_aligned(p->q_starts, 4) || !bw_aligned(p->k_starts, 4)) return BW_EALIGN;
     return BW_OK;

@@ -98,29 +98,30 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
     const RowLoader<H> load_k(lane, wave, a.k_row), load_v(lane, wave, a.v_row);
     const TileReader<H> read(lane);
-    const uint16_t *keys = a.k + p.k0 * a.k_row + head * a.k_head, *values = a.v + p.k0 * a.v_row + head * a.v_head;
+    const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);
     const uint32_t lds = lds_address(smem);
-    auto fetch = [&](int i) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)tiles[i] * H::kKeys;
-        const int n = p.nk - (int)at;
-        const uint32_t to = lds + (i & 1) * 2 * H::kTileBytes;
-        load_k(keys + at * a.k_row, n, to, wave, a.dim);
-        load_v(values + at * a.v_row, n, to + H::kTileBytes, wave, a.dim);
+    auto fetch = [&](const KeyWalk<H>& next) __attribute__((always_inline)) {
+        const uint32_t to = lds + (next.i & 1) * 2 * H::kTileBytes;
+        load_k(next.k, p.nk - next.at, to, wave, a.dim);
+        load_v(next.v, p.nk - next.at, to + H::kTileBytes, wave, a.dim);
     };
 
     f16v acc[H::kBlocks];
     int reach = 0;
-    for (int careful = 0;; careful = 1) {                        // (see prompt_forward_kernel)
+    auto pass = [&](auto is_careful) __attribute__((always_inline)) {       // (see prompt_forward_kernel)
+        constexpr bool careful = decltype(is_careful)::value;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
-        if (tiles.count) fetch(0);
+        KeyWalk<H> next(a, p, head, tiles, 0);
+        if (tiles.count) fetch(next);
         for (int i = 0; i < tiles.count; i++) {
+            const int at = next.at;
+            next.step(a);
             wait_tiles();
-            if (i + 1 < tiles.count) fetch(i + 1);
+            if (next.i < tiles.count) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
-            const int at = tiles[i] * H::kKeys;
-            const Seen which = row0 < rows ? seen_of(a, wave_low, wave_high, at, H::kKeys) : kNone;
+            const Seen which = seen(at);
             if (!careful && which == kNone) continue;
 #pragma unroll
             for (int b = 0; b < H::kKeyBlocks; b++) {
@@ -131,6 +132,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
                     for (int k = 0; k < H::kSteps; k++) s = mfma32<DT>(read.rows(tile, b, k), q[k], s);
 #pragma unroll
                     for (int k = 0; k < H::kSteps; k++) dp = mfma32<DT>(read.rows(tile + H::kTileBytes, b, k), grad[k], dp);
+                    reads_ahead<2 * H::kSteps, 1, 4>();
                     float ds[16];
 #pragma unroll
                     for (int j = 0; j < 16; j++) ds[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale, -lse)) * (dp[j] - delta);
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
                     if constexpr (DT == BW_F16) fit_reach<16, H::kBlocks>(ds, reach, acc);
                     pack16<DT>(ds, w);
                 }
-                if (careful) {
+                if constexpr (careful) {
                     __syncthreads();
                     if (which != kNone) add_nonfinite<H>(tile + b * 32 * H::kPitch * 2, 32, lane, acc, [&](int n) { return sees(a, row.position, at + 32 * b + n); });
                     keep_finite<H>(tile + b * 32 * H::kPitch * 2, 32 * H::kPitch * 2);
@@ -154,14 +156,9 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
                 }
             }
         }
-        if (careful) break;
-        float check = 0.f;
-#pragma unroll
-        for (int m = 0; m < H::kBlocks; m++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) check = __builtin_fmaf(acc[m][j], 0.f, check);
-        if (!any_thread(smem, wave, row.live && check != 0.f)) break;
-    }
+    };
+    pass(std::false_type{});
+    if (any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc))) pass(std::true_type{});
     if (!row.live) return;
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
@@ -212,34 +209,40 @@ BW_DEV void tiles_of_keys(const PromptArgs& a, int nq, int nk, int tile, int til
     to = end > begin ? (end - 1) / tile_rows + 1 : from;
 }
 
-// Tiles of rows of a sequence (tokens x the query heads of one key head) on their way to LDS; rows from the last on are the last one again.  Where a tile is whole tokens, as it is
-// for 1, 2, 4 ... query heads to a key head, a lane's place in it stays the same.
+// Tiles of rows of a sequence (tokens x the query heads of one key head) on their way to LDS, one after the other; rows from the last on are the last one again.  Where a tile is
+// whole tokens, as it is for 1, 2, 4 ... query heads to a key head, a lane's place in it stays the same.
 template <class H> struct PackedLoader {
     uint32_t place[H::kLoads], chunk[H::kLoads];
-    int first;
-    bool same;
-    BW_DEV PackedLoader(const PromptArgs& a, int lane, int wave, int64_t row, int64_t head) {
+    int first, same_to;                          // row of the lane in the first load; tiles that begin before it are whole ones of such tokens
+    int64_t step;
+    const uint16_t *base, *next;
+    BW_DEV PackedLoader(const PromptArgs& a, int lane, int wave, const uint16_t* from, int64_t row, int64_t head, int rows, int at) {
         first = wave * H::kLoads * H::kLoadRows + lane / H::kChunks;
-        same = H::kKeys % a.share == 0 && a.dim == H::kPitch;
+        uint32_t j;
+        const int tokens = (int)a.by_share.div((uint32_t)H::kKeys, j);
+        same_to = j == 0 && a.dim == H::kPitch ? rows - H::kKeys + 1 : 0;
+        step = tokens * row;
+        base = from;
+        next = from + a.by_share.div((uint32_t)at, j) * row;
 #pragma unroll
         for (int i = 0; i < H::kLoads; i++) {
             const int r = first + i * H::kLoadRows;
             chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(r)) * 16;
-            uint32_t j;
             const uint32_t token = a.by_share.div((uint32_t)r, j);
             place[i] = token * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i];
         }
     }
-    BW_DEV void operator()(const PromptArgs& a, const uint16_t* base, int64_t row, int64_t head, int from, int rows, uint32_t to, int wave) const {
+    BW_DEV void operator()(const PromptArgs& a, int64_t row, int64_t head, int from, int rows, uint32_t to, int wave) {
         to += wave * H::kLoads * 1024;
-        uint32_t rest;
-        const uint32_t token0 = a.by_share.div((uint32_t)from, rest);
-        base += token0 * row;
-        if (same && from + H::kKeys <= rows) {
+        if (from < same_to) {
 #pragma unroll
-            for (int i = 0; i < H::kLoads; i++) load_to_lds(base, place[i], to + i * 1024);
+            for (int i = 0; i < H::kLoads; i++) load_to_lds(next, place[i], to + i * 1024);
+            next += step;
             return;
         }
+        uint32_t rest;
+        const uint32_t token0 = a.by_share.div((uint32_t)from, rest);
+        const uint16_t* here = base + token0 * row;
         uint32_t bytes = (uint32_t)a.dim * 2;
         asm("" : "+s"(bytes));
 #pragma unroll
@@ -247,12 +250,12 @@ template <class H> struct PackedLoader {
             const int r = from + first + i * H::kLoadRows;
             uint32_t j;
             const uint32_t token = a.by_share.div((uint32_t)(r < rows ? r : rows - 1), j);
-            if (chunk[i] < bytes) load_to_lds(base, (token - token0) * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i], to + i * 1024);
+            if (chunk[i] < bytes) load_to_lds(here, (token - token0) * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i], to + i * 1024);
         }
     }
 };
 BW_DEV void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory");
 }
 
 template <class H> constexpr int kKeyStage = 2 * H::kTileBytes + 512;           // Q, g, lse, delta of a tile of rows
@@ -286,16 +289,15 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
         rows_of_key(a, p.nq, p.nk, a.sinks > wave_first && a.sinks <= wave_last ? a.sinks : wave_first, ignored, all_to);
     }
 
-    const PackedLoader<H> load_q(a, lane, wave, a.q_row, a.q_head), load_g(a, lane, wave, g.grad_row, g.grad_head);
     const TileReader<H> read(lane);
     const uint16_t *queries = a.q + p.q0 * a.q_row + (int64_t)head * a.share * a.q_head, *grads = g.grad + p.q0 * g.grad_row + (int64_t)head * a.share * g.grad_head;
     const int64_t stats = (int64_t)head * a.q_tokens * a.share + (int64_t)p.q0 * a.share;
     const uint32_t lds = lds_address(smem);
-    auto fetch = [&](int i) __attribute__((always_inline)) {
+    auto fetch = [&](PackedLoader<H>& load_q, PackedLoader<H>& load_g, int i) __attribute__((always_inline)) {
         const int at = i * kTileRows;
         const uint32_t into = lds + (i & 1) * kKeyStage<H>;
-        load_q(a, queries, a.q_row, a.q_head, at, rows, into, wave);
-        load_g(a, grads, g.grad_row, g.grad_head, at, rows, into + H::kTileBytes, wave);
+        load_q(a, a.q_row, a.q_head, at, rows, into, wave);
+        load_g(a, g.grad_row, g.grad_head, at, rows, into + H::kTileBytes, wave);
         const int r = at + lane < rows ? lane : rows - 1 - at;
         if (wave == 0) load4_to_lds(a.lse + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes);
         if (DK && wave == 1) load4_to_lds(g.delta + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes + 256);
@@ -303,14 +305,16 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
 
     f16v acc[H::kBlocks];
     int reach = 0;
-    for (int careful = 0;; careful = 1) {                        // (see prompt_forward_kernel)
+    auto pass = [&](auto is_careful) __attribute__((always_inline)) {       // (see prompt_forward_kernel)
+        constexpr bool careful = decltype(is_careful)::value;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
-        if (p.from < p.to) fetch(p.from);
+        PackedLoader<H> load_q(a, lane, wave, queries, a.q_row, a.q_head, rows, p.from * kTileRows), load_g(a, lane, wave, grads, g.grad_row, g.grad_head, rows, p.from * kTileRows);
+        if (p.from < p.to) fetch(load_q, load_g, p.from);
         for (int i = p.from; i < p.to; i++) {
             wait_tiles();
-            if (i + 1 < p.to) fetch(i + 1);
+            if (i + 1 < p.to) fetch(load_q, load_g, i + 1);
             char* tile = smem + (i & 1) * kKeyStage<H>;
             const int at = i * kTileRows;
             const bool none = at >= any_to || at + kTileRows <= any_from, all = at >= all_from && at + kTileRows <= all_to;
@@ -326,6 +330,7 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
 #pragma unroll
                         for (int n = 0; n < H::kSteps; n++) dp = mfma32<DT>(read.rows(tile + H::kTileBytes, b, n), v[n], dp);
                     }
+                    reads_ahead<(DK ? 2 : 1) * H::kSteps, 1, 4>();
                     float x[16];
                     const char* stat = tile + 2 * H::kTileBytes + (32 * b + 4 * half) * 4;
 #pragma unroll
@@ -350,7 +355,7 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
                     pack16<DT>(x, w);
                 }
                 char* from = tile + (DK ? 0 : H::kTileBytes);
-                if (careful) {
+                if constexpr (careful) {
                     char* block = from + b * 32 * H::kPitch * 2;
                     __syncthreads();
                     if (!none) add_nonfinite<H>(block, 32, lane, acc, [&](int n) { return at + 32 * b + n >= row_from && at + 32 * b + n < row_to; });
@@ -364,14 +369,9 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
                 }
             }
         }
-        if (careful) break;
-        float check = 0.f;
-#pragma unroll
-        for (int m = 0; m < H::kBlocks; m++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) check = __builtin_fmaf(acc[m][j], 0.f, check);
-        if (!any_thread(smem, wave, live && check != 0.f)) break;
-    }
+    };
+    pass(std::false_type{});
+    if (any_thread(smem, wave, live && not_finite<H::kBlocks>(acc))) pass(std::true_type{});
     if (!live) return;
     const float by = (DK ? g.plain_scale : 1.f) * (DT == BW_F16 ? __builtin_ldexpf(1.f, -kWeightShift - (DK ? reach : 0)) : 1.f);
     float* part = p.part < 0 ? nullptr : g.parts + ((((int64_t)p.part * a.kv_heads + head) * kGradKeys + key - p.tile * kGradKeys) * 2 + DK) * a.dim;

@@ -64,8 +64,22 @@ BW_DEV uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const 
 // 16 bytes of every lane from base + offset to LDS at `to` + 16 lane.  Assembly, because the compiler would wait for it before any read of LDS; the
 // waits and barriers are placed by the callers (wait_tiles).  (Wait states: M0 and a scalar that a vector instruction may have written.)
 BW_DEV void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory");
 }
+// The order of a region's instructions, N of a kind at a time: the compiler reads an operand from LDS right before the product that takes it, and waits for it there.
+template <int N> BW_DEV void then_reads() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
+template <int N> BW_DEV void then_products() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
+template <int N> BW_DEV void then_vector() { __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
+template <int N> BW_DEV void then_exponentials() { __builtin_amdgcn_sched_group_barrier(0x400, N, 0); }
+// N products with PER reads each, AHEAD products' worth of them before the first.
+template <int N, int PER, int AHEAD> BW_DEV void reads_ahead() {
+    then_reads<PER * (AHEAD < N ? AHEAD : N)>();
+    static_for<0, N>([&](auto i) {
+        then_products<1>();
+        if constexpr (decltype(i)::value + AHEAD < N) then_reads<PER>();
+    });
+}
+
 // What was asked for has arrived, for all waves.
 BW_DEV void wait_tiles() {
     asm volatile("" ::: "memory");
@@ -260,7 +274,7 @@ struct KeyTiles {
     int sinks, first, count;
     BW_DEV KeyTiles(const PromptArgs& a, int low, int high, int nk, int tile) {
         if (high < 0 || nk <= 0) { sinks = first = count = 0; return; }
-        const int from = low - a.window + 1;                       // (low - 2^31 + 2 fits)
+        const int from = low - a.window + 1;
         first = from > 0 ? from / tile : 0;
         const int s = a.sinks < nk ? a.sinks : nk;
         sinks = (s + tile - 1) / tile;
@@ -270,13 +284,43 @@ struct KeyTiles {
     }
     BW_DEV int operator[](int i) const { return i < sinks ? i : i - sinks + first; }
 };
+// Keys and values of the tiles one after the other: what the next one's rows begin at.
+template <class H> struct KeyWalk {
+    const uint16_t *k, *v;
+    int at, i, jump_at, jump;
+    BW_DEV KeyWalk(const PromptArgs& a, const Span& p, int head, const KeyTiles& tiles, int begin) {
+        i = begin;
+        at = tiles[begin] * H::kKeys;
+        jump_at = tiles.sinks;
+        jump = (tiles.first - tiles.sinks) * H::kKeys;
+        k = a.k + (int64_t)(p.k0 + at) * a.k_row + head * a.k_head;
+        v = a.v + (int64_t)(p.k0 + at) * a.v_row + head * a.v_head;
+    }
+    BW_DEV void step(const PromptArgs& a) {
+        int by = H::kKeys;
+        if (++i == jump_at) by += jump;
+        at += by;
+        k += by * a.k_row;
+        v += by * a.v_row;
+    }
+};
 
-// Which keys rows at positions low ... high see of the n keys from `at` on: none, some, or all.
+// Which keys rows at positions low ... high see of N from `at` on: none, some, or all.
 enum Seen { kNone, kSome, kAll };
-BW_DEV Seen seen_of(const PromptArgs& a, int low, int high, int at, int n) {
-    if (at > high || (at + n <= low - a.window + 1 && at >= a.sinks)) return kNone;
-    return at + n - 1 <= low && (at > high - a.window || at + n <= a.sinks) ? kAll : kSome;
-}
+template <int N> struct SeenOf {
+    int none_above, all_to, window_from, sinks, all_from;
+    BW_DEV SeenOf(const PromptArgs& a, int low, int high, bool any) {
+        none_above = any ? high : -1;                            // (no rows: nothing is seen)
+        all_to = low - N + 1;
+        window_from = low - a.window + 1 - N;
+        sinks = a.sinks;
+        all_from = high - a.window + 1;
+    }
+    BW_DEV Seen operator()(int at) const {
+        if (at > none_above || (at <= window_from && at >= sinks)) return kNone;
+        return at <= all_to && (at >= all_from || at + N <= sinks) ? kAll : kSome;
+    }
+};
 BW_DEV bool sees(const PromptArgs& a, int position, int key) { return key <= position && (key > position - a.window || key < a.sinks); }
 
 // 16 bytes of a row for every step of 16 values of the head, zeros where there is nothing: an operand of the wave's rows.
@@ -286,6 +330,13 @@ template <class H> BW_DEV void load_row(u4* out, const uint16_t* row, bool live,
         const int d = 16 * s + 8 * half;
         out[s] = live && d < dim ? *reinterpret_cast<const u4*>(row + d) : u4{0, 0, 0, 0};
     }
+}
+
+// sum + the two 16-bit values of a word
+template <int DT> BW_DEV float add_pair(uint32_t w, float sum) {
+    typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+    if constexpr (DT == BW_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2v, w), __builtin_bit_cast(b2v, 0x3F803F80u), sum, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), __builtin_bit_cast(h2, 0x3C003C00u), sum, false);
 }
 
 // The rows of a wave: lane l (and l + 32) has row first + l of the sequence.
@@ -310,6 +361,16 @@ BW_DEV void positions_of(const PromptArgs& a, const Span& p, int from, int to, i
 
 // Four values d ... d + 3 of an output row.
 template <int DT> BW_DEV void store4(uint16_t* p, float x, float y, float z, float w) { *reinterpret_cast<u2*>(p) = u2{narrow_pair<DT>(x, y), narrow_pair<DT>(z, w)}; }
+
+// Whether a sum of the lane is an infinity or a NaN.
+template <int BLOCKS> BW_DEV bool not_finite(const f16v* acc) {
+    float check = 0.f;
+#pragma unroll
+    for (int m = 0; m < BLOCKS; m++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) check = __builtin_fmaf(acc[m][j], 0.f, check);
+    return check != 0.f;
+}
 
 template <class H> BW_DEV void clear_tiles(char* smem, int bytes, int dim) {
     if (dim == H::kPitch) return;                                // (values behind the head's end are not loaded)
@@ -345,33 +406,34 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
 
     const RowLoader<H> load_k(lane, wave, a.k_row), load_v(lane, wave, a.v_row);
     const TileReader<H> read(lane);
-    const uint16_t *keys = a.k + p.k0 * a.k_row + head * a.k_head, *values = a.v + p.k0 * a.v_row + head * a.v_head;
+    const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);
     const uint32_t lds = lds_address(smem);
-    auto fetch = [&](int i) __attribute__((always_inline)) {
-        const int64_t at = (int64_t)tiles[i] * H::kKeys;
-        const int n = p.nk - (int)at;
-        const uint32_t to = lds + (i & 1) * 2 * H::kTileBytes;
-        load_k(keys + at * a.k_row, n, to, wave, a.dim);
-        load_v(values + at * a.v_row, n, to + H::kTileBytes, wave, a.dim);
+    auto fetch = [&](const KeyWalk<H>& next) __attribute__((always_inline)) {
+        const uint32_t to = lds + (next.i & 1) * 2 * H::kTileBytes;
+        load_k(next.k, p.nk - next.at, to, wave, a.dim);
+        load_v(next.v, p.nk - next.at, to + H::kTileBytes, wave, a.dim);
     };
 
     f16v acc[H::kBlocks];
     float r, l;
     // An infinity or a NaN among the values leaves nothing finite in 0 times it, also where the mask hides its token.  Where a result is not finite, the tile
-    // is done again, carefully: the products take finite values only, the others are added to the rows that see them.
-    for (int careful = 0;; careful = 1) {
+    // is done again, carefully: the products take finite values only, the others are added to the rows that see them.  (A loop of its own: what it needs is not there in the other.)
+    auto pass = [&](auto is_careful) __attribute__((always_inline)) {
+        constexpr bool careful = decltype(is_careful)::value;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         r = kLowestScore;
         l = 0.f;
-        if (begin < end) fetch(begin);
+        KeyWalk<H> next(a, p, head, tiles, begin);
+        if (begin < end) fetch(next);
         for (int i = begin; i < end; i++) {
+            const int at = next.at;
+            next.step(a);
             wait_tiles();
-            if (i + 1 < end) fetch(i + 1);
+            if (next.i < end) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
-            const int at = tiles[i] * H::kKeys;
-            const Seen which = row0 < rows ? seen_of(a, wave_low, wave_high, at, H::kKeys) : kNone;
-            if (careful) {
+            const Seen which = seen(at);
+            if constexpr (careful) {
                 if (which != kNone) add_nonfinite<H>(tile + H::kTileBytes, H::kKeys, lane, acc, [&](int n) { return sees(a, row.position, at + n); });
                 keep_finite<H>(tile + H::kTileBytes, H::kTileBytes);
             }
@@ -383,6 +445,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
 #pragma unroll
                 for (int k = 0; k < H::kSteps; k++) s[b] = mfma32<DT>(read.rows(tile, b, k), q[k], s[b]);
             }
+            reads_ahead<H::kKeyBlocks * H::kSteps, 1, 4>();
             if (which == kSome) {
 #pragma unroll
                 for (int b = 0; b < H::kKeyBlocks; b++)
@@ -412,23 +475,34 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + 2 * j], a.scale, -r)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + 2 * j + 1], a.scale, -r));
-                        l += x + y;
                         w[j] = narrow_pair<DT>(x, y);
                     }
+                    // (the sum of the weights as they are multiplied, two at a time: what their rounding adds to the values it takes off again)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) l = add_pair<DT>(w[j], l);
 #pragma unroll
                     for (int m = 0; m < H::kBlocks; m++) {
                         acc[m] = mfma32<DT>(read.columns(tile + H::kTileBytes, 2 * b + t, m), w, acc[m]);
                     }
                 }
+            // the weights of 16 keys while the products of the 16 before them are under way
+            then_reads<2 * H::kBlocks>();
+            then_vector<8>();
+            then_exponentials<8>();
+            then_vector<8>();
+            static_for<1, 2 * H::kKeyBlocks>([&](auto) {
+                static_for<0, H::kBlocks>([&](auto) {
+                    then_products<1>();
+                    then_reads<2>();
+                    then_vector<(16 + H::kBlocks - 1) / H::kBlocks>();
+                    then_exponentials<(8 + H::kBlocks - 1) / H::kBlocks>();
+                });
+            });
+            then_products<H::kBlocks>();
         }
-        if (careful) break;
-        float check = 0.f;
-#pragma unroll
-        for (int m = 0; m < H::kBlocks; m++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) check = __builtin_fmaf(acc[m][j], 0.f, check);
-        if (!any_thread(smem, wave, row.live && check != 0.f)) break;
-    }
+    };
+    pass(std::false_type{});
+    if (any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc))) pass(std::true_type{});
 
     l += __shfl_xor(l, 32, 64);
     if (!row.live) return;
