@@ -5,6 +5,11 @@
 //
 // P and dS enter their second product as 16-bit numbers, rounded once.  In float16, whose steps end at 2^-24, P goes in 2^12 times as large, and dS times a power of two that
 // is each row's (each key's) own: it starts high and comes down where a product would pass 2^15, and the sums with it.
+//
+// A row's dS add up to zero, but for what dS and the output (in delta) were rounded by: a remainder e, which puts e times the mean of the keys into dQ.  Keys are projected with
+// channels far from zero, so that this was the larger part of dQ's error (8192 tokens, bfloat16, channels at 2 to 6 of keys that spread by 1: 0.0045 of dQ, 0.0023 without it).
+// dQ = scale dS (K - c) for any c: e is summed as the product takes it, and e c taken off, c the mean of 32 keys that all of a
+// wave's rows see, nearer to zero where these are fewer (one key says little of the mean).
 #pragma once
 #include "bw_prompt_kernel.h"
 
@@ -28,7 +33,7 @@ struct PromptGradArgs {
 constexpr int kFirstReach16 = 80, kReachTop = 12, kReachMost = 15, kWeightShift = 12;
 
 // The power of two (of each lane) that its values `x`, times 2^reach, go into a product with, which brings down the sums in `acc` where it comes down.
-template <int N, int BLOCKS> BW_DEV void fit_reach(float* x, int& reach, f16v* acc) {
+template <int N, int BLOCKS> BW_DEV void fit_reach(float* x, int& reach, f16v* acc, float& sum) {
     float most = 0.f;
 #pragma unroll
     for (int j = 0; j < N; j++) most = fmaxf(most, __builtin_fabsf(x[j]));
@@ -41,6 +46,7 @@ template <int N, int BLOCKS> BW_DEV void fit_reach(float* x, int& reach, f16v* a
         reach = now;
 #pragma unroll
         for (int m = 0; m < BLOCKS; m++) acc[m] *= by;
+        sum *= by;
     }
     const float with = __builtin_ldexpf(1.f, reach);
 #pragma unroll
@@ -108,11 +114,13 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
 
     f16v acc[H::kBlocks];
     int reach = 0;
+    float rest = 0.f;                                            // sum of the dS, as rounded
     auto pass = [&](auto is_careful) __attribute__((always_inline)) {       // (see prompt_forward_kernel)
         constexpr bool careful = decltype(is_careful)::value;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
+        rest = 0.f;
         KeyWalk<H> next(a, p, head, tiles, 0);
         if (tiles.count) fetch(next);
         for (int i = 0; i < tiles.count; i++) {
@@ -140,8 +148,10 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
 #pragma unroll
                         for (int j = 0; j < 16; j++) ds[j] = sees(a, row.position, at + 32 * b + 8 * (j / 4) + 4 * half + j % 4) ? ds[j] : 0.f;
                     }
-                    if constexpr (DT == BW_F16) fit_reach<16, H::kBlocks>(ds, reach, acc);
+                    if constexpr (DT == BW_F16) fit_reach<16, H::kBlocks>(ds, reach, acc, rest);
                     pack16<DT>(ds, w);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) rest = add_pair<DT>(w[j / 4][j % 4], rest);
                 }
                 if constexpr (careful) {
                     __syncthreads();
@@ -159,7 +169,35 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     };
     pass(std::false_type{});
     if (any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc))) pass(std::true_type{});
+    char* mean = smem + wave * H::kPitch * 4;                    // (any_thread's barrier: the tiles are done with)
+    {
+        const int to = wave_low + 1, lowest = wave_low - 31 > wave_high - a.window + 1 ? wave_low - 31 : wave_high - a.window + 1, from = lowest > 0 ? lowest : 0;
+        const int d = lane % H::kChunks * 8;
+        float c[8] = {};
+        if (d < a.dim) {
+            const uint16_t* key = a.k + (int64_t)p.k0 * a.k_row + head * a.k_head + d;
+#pragma unroll 4
+            for (int n = from + lane / H::kChunks; n < to; n += H::kLoadRows) {
+                const u4 w = *reinterpret_cast<const u4*>(key + n * a.k_row);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    c[2 * j] = __builtin_fmaf(widen16<DT>((uint16_t)w[j]), 1.f / 32.f, c[2 * j]);
+                    c[2 * j + 1] = __builtin_fmaf(widen16<DT>((uint16_t)(w[j] >> 16)), 1.f / 32.f, c[2 * j + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = H::kChunks; o < 64; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < 8; j++) c[j] += __shfl_xor(c[j], o, 64);
+        if (lane < H::kChunks) {
+            *reinterpret_cast<f4*>(mean + d * 4) = f4{c[0], c[1], c[2], c[3]};
+            *reinterpret_cast<f4*>(mean + d * 4 + 16) = f4{c[4], c[5], c[6], c[7]};
+        }
+    }
+    __syncthreads();
     if (!row.live) return;
+    rest += __shfl_xor(rest, 32, 64);
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
 #pragma unroll
@@ -167,7 +205,8 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             const int d = 32 * m + 8 * b + 4 * half;
-            const f4 x = f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]} * back * g.plain_scale;
+            const f4 c = *reinterpret_cast<const f4*>(mean + d * 4);
+            const f4 x = (f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]} - rest * c) * back * g.plain_scale;
             if (d < a.dim) store4<DT>(out + d, x[0], x[1], x[2], x[3]);
         }
 }
@@ -351,7 +390,10 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
                             x[j] = r >= row_from && r < row_to ? x[j] : 0.f;
                         }
                     }
-                    if constexpr (DK && DT == BW_F16) fit_reach<16, H::kBlocks>(x, reach, acc);
+                    if constexpr (DK && DT == BW_F16) {
+                        float none = 0.f;
+                        fit_reach<16, H::kBlocks>(x, reach, acc, none);
+                    }
                     pack16<DT>(x, w);
                 }
                 char* from = tile + (DK ? 0 : H::kTileBytes);

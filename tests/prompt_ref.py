@@ -46,7 +46,11 @@ def head(q, k, v, seen, scale, grad=None):
     # (float16: a step of dS's type below the largest of its row or column, 2^12 at least)
     row, column = small * ds.abs().amax(-1, keepdim=True), small * ds.abs().amax(0, keepdim=True)
     dq, dk = scale * (ds @ k), scale * (ds.t() @ q)
-    dq_off = abs(scale) * ((ds_off + row * seen) @ k.abs())
+    # dQ = scale dS (K - c), c a mean of keys that the row sees (no value of it is larger than the largest of theirs): in 64 bits sum(dS) c is nothing, as a row's dS add up to
+    # zero; what they are off by adds up to sum(dS's bounds) at most, and meets c in dQ.
+    wrong = (ds_off + row) * seen
+    largest = torch.stack([torch.where(s[:, None], k.abs(), 0.0).amax(0) for s in seen]) if n else torch.zeros_like(q)
+    dq_off = abs(scale) * (wrong @ k.abs() + wrong.sum(-1, keepdim=True) * largest)
     dk_off = abs(scale) * ((ds_off + column * seen).t() @ q.abs())
     rows = [(out, off)]
     for want, o in ((dq, dq_off), (dk, dk_off), (dv, dv_off)):
