@@ -6,24 +6,42 @@
 
 namespace {
 
-// out = the parts of a row put together; a row's part: reference, sum, two unused, sums of the values [dim].  A thread has 4 values of a row.
+// out = the parts of a row put together: [row][part] reference and sum, then [row][part][dim] sums of the values.  A thread has 4 values of a row, and 8 parts under way at a
+// time (one at a time: 28.6 us for 2016 rows of 128 in 32 parts).
 template <int DT>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, int threads, uint32_t rows) {
     const uint32_t i = blockIdx.x * (256 / threads) + threadIdx.x / threads;
     const int d = (int)(threadIdx.x % threads) * 4;
     if (threadIdx.x / threads >= 256 / threads || i >= rows) return;
-    const int64_t pitch = a.dim + 4;
-    const float* part = a.partial + (int64_t)i * a.splits * pitch;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; s++) top = fmaxf(top, part[s * pitch]);
-    float sum = 0.f;
+    const u2* stats = reinterpret_cast<const u2*>(a.partial) + (int64_t)i * a.splits;
+    const float* part = a.partial + (int64_t)rows * a.splits * 2 + (int64_t)i * a.splits * a.dim + d;
+    float top = -INFINITY, sum = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; s++) {
-        const float r = part[s * pitch];
-        if (r == -INFINITY) continue;                              // no key of this part is seen
-        const float f = __builtin_amdgcn_exp2f(r - top);
-        sum += f * part[s * pitch + 1];
-        o += f * *reinterpret_cast<const f4*>(part + s * pitch + 4 + d);
+    for (int s = 0; s < a.splits; s += 8) {
+        f4 x[8];
+        float r[8], l[8], high = top;
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            const int at = s + n < a.splits ? s + n : s;
+            const u2 w = stats[at];
+            const uint32_t first = w[0], second = w[1];
+            r[n] = s + n < a.splits ? __builtin_bit_cast(float, first) : -INFINITY;
+            l[n] = __builtin_bit_cast(float, second);
+            x[n] = *reinterpret_cast<const f4*>(part + (int64_t)at * a.dim);
+            high = fmaxf(high, r[n]);
+        }
+        if (high == -INFINITY) continue;                           // no key of these parts is seen
+        const float keep = __builtin_amdgcn_exp2f(top - high);
+        top = high;
+        sum *= keep;
+        o *= keep;
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            if (r[n] == -INFINITY) continue;                       // (nothing was summed)
+            const float f = __builtin_amdgcn_exp2f(r[n] - top);
+            sum += f * l[n];
+            o += f * x[n];
+        }
     }
     const bool empty = top == -INFINITY;
     o *= empty ? 0.f : 1.f / sum;
@@ -77,17 +95,34 @@ PromptArgs args_of(const bw_prompt* p) {
 
 int key_tile(int dim) { return dim > 128 ? 32 : 64; }
 
-// Parts that the keys of a tile of rows are cut into: where there are fewer tiles of rows than workgroups that the chip holds.
-constexpr int kPartTiles = 4;
+// Parts that the keys of a tile of rows are cut into: the number for which the longest workgroup (or, in several rounds, the mean of all), the second launch and the parts' way
+// through memory take the least together.  In microseconds, as measured: a tile of keys takes a workgroup 0.9 (heads of 64), 1.5 (128) and 2 (256, of half the keys), 1.4 times that
+// where two share a CU; the join 5, and its parts, written and read, go at 4 TB/s.  512 tokens of 8192, 32 and 8 heads of 128: 1 part 193 us, 2 110, 3 100, 4 88; 63 of 32063: 8 parts 106 us,
+// 16 63, 32 59, 48 70; 1024 tokens alone: 1 part 31 us, 2 41; 256 of 4096, heads of 64: 1 part 62 us, 4 25, 8 20, 16 26.
 int splits_of(const bw_prompt* p) {
-    const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), resident = bw_device_cus() * (p->dim > 128 ? 1 : 2);
-    const int64_t blocks = p->kv_heads * (p->q_starts ? (p->q_tokens * share + kRows - 1) / kRows : p->sequences * tiles_of(p, p->q_tokens, share, kRows));
-    int64_t keys = p->k_tokens / (p->q_starts ? 1 : p->sequences);
+    const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), cus = bw_device_cus(), resident = cus * (p->dim > 128 ? 1 : 2);
+    const int64_t of = p->q_starts ? p->sequences : 1, tiles = (p->q_tokens * share + kRows - 1) / kRows;
+    const int64_t row_tiles = p->q_starts ? (tiles > p->sequences ? tiles : p->sequences < p->q_tokens ? p->sequences : p->q_tokens) : p->sequences * tiles_of(p, p->q_tokens, share, kRows);
+    const double blocks = (double)p->kv_heads * row_tiles;
+    // (of packed sequences, whose lengths are not known here, twice the mean)
+    int64_t keys = p->q_starts ? (p->k_tokens * 2 + of - 1) / of : p->k_tokens / p->sequences, rows = p->q_tokens / p->sequences;
+    if (keys > p->k_tokens) keys = p->k_tokens;
     const int64_t reach = p->window ? p->window + p->sinks + kRows / share + 2 : keys;
-    if (reach < keys) keys = reach;
-    const int64_t most = (keys + tile - 1) / tile / kPartTiles, want = blocks > 0 ? resident / blocks : 1;
-    const int64_t splits = want < most ? want : most;
-    return (int)(splits < 1 ? 1 : splits < 64 ? splits : 64);
+    const bool all = reach >= keys;
+    if (!all) keys = reach;
+    const double longest = (double)((keys + tile - 1) / tile), mean = all && keys > 0 ? longest * (1. - 0.5 * (rows < keys ? rows : keys) / keys) : longest;
+    const double one = p->dim > 128 ? 2.0 : 0.3 + p->dim * 0.0094;
+    int best = 1;
+    double least = 0.;
+    for (int s = 1; s <= 64 && (s == 1 || s * 2 <= longest); s++) {
+        const double rounds = blocks * s / resident, tiles_each = rounds > 1. && mean * rounds > longest ? mean * rounds : longest;
+        const double time = tiles_each / s * one * (blocks * s > cus && resident > cus ? 1.4 : 1.) + (s > 1 ? 5. + (double)p->q_tokens * p->q_heads * p->dim * 8. * s / 4e6 : 0.);
+        if (s == 1 || time < least) {
+            best = s;
+            least = time;
+        }
+    }
+    return best;
 }
 
 // How the gradients' work is cut, and where their workspace has what (bytes).
@@ -130,7 +165,7 @@ GradPlan grad_plan(const bw_prompt* p) {
 extern "C" size_t bw_prompt_attention_workspace_bytes(const bw_prompt* p) {
     if (prompt_check(p, BW_F16) != BW_OK || p->q_tokens == 0) return 0;
     const int splits = splits_of(p);
-    return splits > 1 ? (size_t)(p->q_tokens * p->q_heads) * splits * (p->dim + 4) * sizeof(float) : 0;
+    return splits > 1 ? (size_t)(p->q_tokens * p->q_heads) * splits * (p->dim + 2) * sizeof(float) : 0;
 }
 
 extern "C" int bw_prompt_attention(const bw_prompt* p, int act_dtype, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,

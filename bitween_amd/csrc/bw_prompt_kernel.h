@@ -507,15 +507,16 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     l += __shfl_xor(l, 32, 64);
     if (!row.live) return;
     const int64_t index = (int64_t)head * a.q_tokens * a.share + token * a.share + row.head;       // of the row among all
-    if (a.splits > 1) {                                           // reference, sum, sums of the values [dim]
-        float* part = a.partial + (index * a.splits + split) * (a.dim + 4);
-        if (half == 0) *reinterpret_cast<u2*>(part) = u2{__builtin_bit_cast(uint32_t, begin < end ? r : -INFINITY), __builtin_bit_cast(uint32_t, l)};
+    if (a.splits > 1) {                                           // (see prompt_join_kernel)
+        const int64_t parts = (int64_t)a.q_tokens * a.q_heads * a.splits, at = index * a.splits + split;
+        if (half == 0) reinterpret_cast<u2*>(a.partial)[at] = u2{__builtin_bit_cast(uint32_t, begin < end ? r : -INFINITY), __builtin_bit_cast(uint32_t, l)};
+        float* part = a.partial + parts * 2 + at * a.dim;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++)
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 const int d = 32 * m + 8 * b + 4 * half;
-                if (d < a.dim) *reinterpret_cast<f4*>(part + 4 + d) = f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]};
+                if (d < a.dim) *reinterpret_cast<f4*>(part + d) = f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]};
             }
         return;
     }
