@@ -42,113 +42,129 @@ BW_DEV double rsqrt_wide(double x) {
     return y;
 }
 
+// A thread has its place in some of a token's heads, a.slices apart: the queries', the keys' and the values', and their angles once.
 template <int DT, int CH, bool AXES, int BITS>
 __global__ __launch_bounds__(256) void append_kernel(RotateArgs a, AppendArgs c) {
     __shared__ __align__(16) uint32_t extrema[BITS == 16 ? 4 : 512];
     const uint32_t units = (uint32_t)(a.q_heads + 2 * c.kv_heads), item = (blockIdx.x * 256 + threadIdx.x) >> a.lane_shift;
     const int lane = (int)threadIdx.x & ((1 << a.lane_shift) - 1);
-    const bool there = item < (uint32_t)a.T * units, live = there && lane < a.lanes;
+    const bool there = item < (uint32_t)a.T * a.slices, live = there && lane < a.lanes;
     const uint32_t it = there ? item : 0;                        // (lanes that fill a head up are of its kind)
-    const int token = (int)(it / units);
-    int head = (int)(it - (uint32_t)token * units);
-    const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + c.kv_heads, is_k = !is_q && !is_v;
-    head -= is_q ? 0 : is_v ? a.q_heads + c.kv_heads : a.q_heads;
+    const int token = (int)(it / a.slices);
     int first, second;
     bool turns;
     chunks_of<CH>(a, live ? lane : 0, first, second, turns);
-    const uint16_t* src = is_q ? a.q + token * a.q_row + head * a.q_head : is_v ? c.v + token * c.v_row + head * c.v_head : a.k + token * a.k_row + head * a.k_head;
-    const Raw<CH> raw[2] = {load_raw<CH>(src + first), load_raw<CH>(src + second)};
+    auto source = [&](int unit) {
+        return unit < a.q_heads ? a.q + token * a.q_row + unit * a.q_head : unit < a.q_heads + c.kv_heads ? a.k + token * a.k_row + (unit - a.q_heads) * a.k_head
+                                                                          : c.v + token * c.v_row + (unit - a.q_heads - c.kv_heads) * c.v_head;
+    };
+    uint32_t unit = it - (uint32_t)token * a.slices;
+    const uint16_t* src = source((int)unit);
+    Raw<CH> raw[2] = {load_raw<CH>(src + first), load_raw<CH>(src + second)};
     const int64_t slot = c.slots[token];
     const Position<AXES> pos(a, token);
-    uint32_t w[2][CH / 2];                                       // the chunks as they are stored
-#pragma unroll
-    for (int j = 0; j < CH / 2; j++) { w[0][j] = raw[0][j]; w[1][j] = raw[1][j]; }
-    if (!is_v) {
-        Angle<CH> angle;
-        if (pos.kept && turns) angle.load(a, pos, first);
-        float x[CH], y[CH];
-        widen_raw<DT, CH>(raw[0], x);
-        widen_raw<DT, CH>(raw[1], y);
-        const void* weight = is_k ? a.k_weight : a.q_weight;
-        if (weight) {
-            double ss = 0.;
-            if (live) {
-#pragma unroll
-                for (int j = 0; j < CH; j++) ss = __builtin_fma((double)x[j], (double)x[j], __builtin_fma((double)y[j], (double)y[j], ss));
-            }
-            const float r = (float)rsqrt_wide(wide_sum<DT>(ss, a.lane_shift) / a.dim + (double)a.eps);
-            float g[CH];
-            load_weight<DT, CH>(weight, a.weight_f32, first, g);
-#pragma unroll
-            for (int j = 0; j < CH; j++) x[j] = x[j] * r * g[j];
-            load_weight<DT, CH>(weight, a.weight_f32, second, g);
-#pragma unroll
-            for (int j = 0; j < CH; j++) y[j] = y[j] * r * g[j];
-        }
-        if (pos.kept && turns) angle.template turn<1>(x, y);
-#pragma unroll
-        for (int j = 0; j < CH / 2; j++) {
-            w[0][j] = narrow_pair<DT>(x[2 * j], x[2 * j + 1]);
-            w[1][j] = narrow_pair<DT>(y[2 * j], y[2 * j + 1]);
-        }
-    }
+    Angle<CH> angle;
+    if (pos.kept && turns && unit < (uint32_t)(a.q_heads + c.kv_heads)) angle.load(a, pos, first);
+    const bool kept = live && pos.kept && slot >= 0 && slot < c.rows;
+    const int64_t page = slot >> c.page_shift, in_page = slot & ((1 << c.page_shift) - 1);
     auto store = [](void* p, const uint32_t* w) {
         if constexpr (CH == 8) *reinterpret_cast<u4*>(p) = u4{w[0], w[1], w[2], w[3]};
         else *reinterpret_cast<u2*>(p) = u2{w[0], w[1]};
     };
-    if (is_q) {
-        if (live) {
-            uint16_t* out = a.q_out + ((int64_t)token * a.q_heads + head) * a.dim;
-            if (!pos.kept) {
+    for (;;) {
+        const uint32_t next = unit + a.slices;
+        const bool more = next < units, is_q = unit < (uint32_t)a.q_heads, is_v = unit >= (uint32_t)(a.q_heads + c.kv_heads), is_k = !is_q && !is_v;
+        const int head = (int)unit - (is_q ? 0 : is_v ? a.q_heads + c.kv_heads : a.q_heads);
+        src = source((int)(more ? next : unit));
+        const Raw<CH> after[2] = {load_raw<CH>(src + first), load_raw<CH>(src + second)};
+        uint32_t w[2][CH / 2];                                   // the chunks as they are stored
 #pragma unroll
-                for (int j = 0; j < CH / 2; j++) w[0][j] = w[1][j] = 0;
-            }
-            store(out + first, w[0]);
-            store(out + second, w[1]);
-        }
-        return;
-    }
-    const bool kept = live && pos.kept && slot >= 0 && slot < c.rows;
-    const int64_t page = slot >> c.page_shift, in_page = slot & ((1 << c.page_shift) - 1), row = ((page * c.kv_heads + head) << c.page_shift) + in_page;
-    uint8_t* out = is_v ? c.values : c.keys;
-    if constexpr (BITS == 16) {
-        if (kept) {
-            store(out + (row * a.dim + first) * 2, w[0]);
-            store(out + (row * a.dim + second) * 2, w[1]);
-        }
-    } else {
-        // (a wave's lanes of keys and values are all here; those of queries have nothing in LDS)
-        uint32_t* mine = extrema + ((threadIdx.x >> 6) * 128 + ((threadIdx.x & 63) >> a.lane_shift << (a.lane_shift + 1)));
-        if (lane < a.lanes) {
-            mine[first / CH] = extrema_of<CH / 2>(w[0]);
-            mine[second / CH] = extrema_of<CH / 2>(w[1]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        uint32_t* meta = is_v ? c.value_meta : c.key_meta;
+        for (int j = 0; j < CH / 2; j++) { w[0][j] = raw[0][j]; w[1][j] = raw[1][j]; }
+        if (!is_v) {
+            float x[CH], y[CH];
+            widen_raw<DT, CH>(raw[0], x);
+            widen_raw<DT, CH>(raw[1], y);
+            const void* weight = is_k ? a.k_weight : a.q_weight;
+            if (weight) {
+                double ss = 0.;
+                if (live) {
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-            const int at = n ? second : first, chunk = at / CH, group = chunk / c.group_chunks;
-            const u4* from = reinterpret_cast<const u4*>(mine + group * c.group_chunks);
-            uint32_t both = 0;
-            if (lane < a.lanes) {
-                for (int i = 0; i < c.group_chunks / 4; i++) {
-                    const u4 t = from[i];
-                    both = max16(both, max16(max16(t[0], t[1]), max16(t[2], t[3])));
+                    for (int j = 0; j < CH; j++) ss = __builtin_fma((double)x[j], (double)x[j], __builtin_fma((double)y[j], (double)y[j], ss));
                 }
-            }
-            const GroupCoder<DT, BITS> coder(both);
-            uint32_t q[CH];
+                const float r = (float)rsqrt_wide(wide_sum<DT>(ss, a.lane_shift) / a.dim + (double)a.eps);
+                float g[CH];
+                load_weight<DT, CH>(weight, a.weight_f32, first, g);
 #pragma unroll
-            for (int j = 0; j < CH; j++) q[j] = coder.code(widen16<DT>((uint16_t)(w[n][j / 2] >> (16 * (j & 1)))));
-            if (!kept) continue;
-            uint8_t* dst = out + row * (a.dim * BITS / 8) + at * BITS / 8;
-            if constexpr (BITS == 8 && CH == 8) *reinterpret_cast<u2*>(dst) = u2{bytes_of(q[0], q[1], q[2], q[3]), bytes_of(q[4], q[5], q[6], q[7])};
-            else if constexpr (BITS == 8) *reinterpret_cast<uint32_t*>(dst) = bytes_of(q[0], q[1], q[2], q[3]);
-            else if constexpr (CH == 8) *reinterpret_cast<uint32_t*>(dst) = bytes_of(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4);
-            else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)bytes_of(q[0] | q[1] << 4, q[2] | q[3] << 4, 0, 0);
-            if (chunk % c.group_chunks == 0) meta[(((page * c.kv_heads + head) * c.groups + group) << c.page_shift) + in_page] = coder.pair;
+                for (int j = 0; j < CH; j++) x[j] = x[j] * r * g[j];
+                load_weight<DT, CH>(weight, a.weight_f32, second, g);
+#pragma unroll
+                for (int j = 0; j < CH; j++) y[j] = y[j] * r * g[j];
+            }
+            if (pos.kept && turns) angle.template turn<1>(x, y);
+#pragma unroll
+            for (int j = 0; j < CH / 2; j++) {
+                w[0][j] = narrow_pair<DT>(x[2 * j], x[2 * j + 1]);
+                w[1][j] = narrow_pair<DT>(y[2 * j], y[2 * j + 1]);
+            }
         }
+        const int64_t row = ((page * c.kv_heads + head) << c.page_shift) + in_page;
+        uint8_t* out = is_v ? c.values : c.keys;
+        if (is_q) {
+            if (live) {
+                uint16_t* to = a.q_out + ((int64_t)token * a.q_heads + head) * a.dim;
+                if (!pos.kept) {
+#pragma unroll
+                    for (int j = 0; j < CH / 2; j++) w[0][j] = w[1][j] = 0;
+                }
+                store(to + first, w[0]);
+                store(to + second, w[1]);
+            }
+        } else if constexpr (BITS == 16) {
+            if (kept) {
+                store(out + (row * a.dim + first) * 2, w[0]);
+                store(out + (row * a.dim + second) * 2, w[1]);
+            }
+        } else {
+            // (a head's lanes are all here; those of queries leave nothing in LDS)
+            uint32_t* mine = extrema + ((threadIdx.x >> 6) * 128 + ((threadIdx.x & 63) >> a.lane_shift << (a.lane_shift + 1)));
+            if (lane < a.lanes) {
+                mine[first / CH] = extrema_of<CH / 2>(w[0]);
+                mine[second / CH] = extrema_of<CH / 2>(w[1]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            uint32_t* meta = is_v ? c.value_meta : c.key_meta;
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const int at = n ? second : first, chunk = at / CH, group = chunk / c.group_chunks;
+                const u4* from = reinterpret_cast<const u4*>(mine + group * c.group_chunks);
+                uint32_t both = 0;
+                if (lane < a.lanes) {
+                    for (int i = 0; i < c.group_chunks / 4; i++) {
+                        const u4 t = from[i];
+                        both = max16(both, max16(max16(t[0], t[1]), max16(t[2], t[3])));
+                    }
+                }
+                const GroupCoder<DT, BITS> coder(both);
+                uint32_t q[CH];
+#pragma unroll
+                for (int j = 0; j < CH; j++) q[j] = coder.code(widen16<DT>((uint16_t)(w[n][j / 2] >> (16 * (j & 1)))));
+                if (!kept) continue;
+                uint8_t* dst = out + row * (a.dim * BITS / 8) + at * BITS / 8;
+                if constexpr (BITS == 8 && CH == 8) *reinterpret_cast<u2*>(dst) = u2{bytes_of(q[0], q[1], q[2], q[3]), bytes_of(q[4], q[5], q[6], q[7])};
+                else if constexpr (BITS == 8) *reinterpret_cast<uint32_t*>(dst) = bytes_of(q[0], q[1], q[2], q[3]);
+                else if constexpr (CH == 8) *reinterpret_cast<uint32_t*>(dst) = bytes_of(q[0] | q[1] << 4, q[2] | q[3] << 4, q[4] | q[5] << 4, q[6] | q[7] << 4);
+                else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)bytes_of(q[0] | q[1] << 4, q[2] | q[3] << 4, 0, 0);
+                if (chunk % c.group_chunks == 0) meta[(((page * c.kv_heads + head) * c.groups + group) << c.page_shift) + in_page] = coder.pair;
+            }
+            // (the next head's extrema go where these are read)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (!more) return;
+        unit = next;
+        raw[0] = after[0];
+        raw[1] = after[1];
     }
 }
 
@@ -201,7 +217,8 @@ extern "C" int bw_cache_append(const bw_cache* cache, const bw_heads* h, const b
     const int64_t per_block = 256 >> a.lane_shift, most = (((int64_t)1 << 32) - 256) / (units << a.lane_shift);
     for (int64_t at = 0; at < h->tokens; at += most) {
         a.T = (int)(h->tokens - at < most ? h->tokens - at : most);
-        const dim3 grid((unsigned)((a.T * units + per_block - 1) / per_block));
+        a.slices = (uint32_t)slices_of(a, (int)units);
+        const dim3 grid((unsigned)(((int64_t)a.T * a.slices + per_block - 1) / per_block));
 #define BW_APPEND(DT, CH) \
     if (act_dtype == DT && chunk == CH && axes) launch_append<DT, CH, true>(a, c, cache->bits, grid, (hipStream_t)stream); \
     else if (act_dtype == DT && chunk == CH) launch_append<DT, CH, false>(a, c, cache->bits, grid, (hipStream_t)stream);

@@ -544,19 +544,19 @@ struct Rotation {
     Tensor weights[2];                                          // the queries' and the keys', as the kernels read them
 };
 
-// sections (None or a tuple of up to four numbers) and interleaved; count 0: one position for each token.
+// sections (None or a tuple or list of up to four numbers) and interleaved; count 0: one position for each token.
 bool axes_of(PyObject* sections, PyObject* interleaved, bw_axes& axes) {
     axes = {};
     if (sections == Py_None) return interleaved == Py_False;
-    if (!PyTuple_Check(sections) || PyTuple_GET_SIZE(sections) < 1 || PyTuple_GET_SIZE(sections) > 4 || !PyBool_Check(interleaved)) return false;
-    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sections); i++) {
-        PyObject* n = PyTuple_GET_ITEM(sections, i);
+    if ((!PyTuple_Check(sections) && !PyList_Check(sections)) || PySequence_Fast_GET_SIZE(sections) < 1 || PySequence_Fast_GET_SIZE(sections) > 4 || !PyBool_Check(interleaved)) return false;
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(sections); i++) {
+        PyObject* n = PySequence_Fast_GET_ITEM(sections, i);
         if (!PyLong_CheckExact(n)) return false;
         const long v = PyLong_AsLong(n);
         if (PyErr_Occurred() || v < 0 || v > 65535) return false;
         axes.sections[i] = (int)v;
     }
-    axes.count = (int)PyTuple_GET_SIZE(sections);
+    axes.count = (int)PySequence_Fast_GET_SIZE(sections);
     axes.interleaved = interleaved == Py_True;
     return true;
 }

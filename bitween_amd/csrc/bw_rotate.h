@@ -23,6 +23,7 @@ struct RotateArgs {
     int axes;                                    // positions of a token: [axes][position_pitch]
     int64_t position_pitch;
     uint32_t axis[8];                            // of each pair, two bits
+    uint32_t slices, k_slices;                   // threads (of a head's place) for each token: see slices_of; gradient: the queries' and the keys'
 };
 
 // CH 16-bit values as they come from memory, and as float32.
@@ -181,6 +182,14 @@ static inline RotateArgs rotate_args(const bw_heads* h, const bw_axes* x = nullp
         }
     }
     return a;
+}
+
+// Threads (of one place in a head) for each token, of which each has as many of its `heads` as leave the chip about 1024 workgroups, 8 at most, and their angles once: 16384 tokens
+// of 32 and 8 heads of 128 and three axes 111 us with one head each, 73 so.
+static inline int slices_of(const RotateArgs& a, int heads) {
+    const int64_t rounds = ((int64_t)a.T * heads << a.lane_shift) / (256 * 1024);
+    const int each = (int)(rounds < 1 ? 1 : rounds < 8 ? rounds : 8);
+    return (heads + each - 1) / each;
 }
 
 // The axes fit the pairs: they take all of them, and interleaved ones find theirs.

@@ -14,27 +14,14 @@
 
 namespace {
 
-template <int DT, int CH, bool AXES>
-__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
-    const uint32_t heads = (uint32_t)(a.q_heads + a.k_heads), item = (blockIdx.x * 256 + threadIdx.x) >> a.lane_shift;
-    const int lane = (int)threadIdx.x & ((1 << a.lane_shift) - 1);
-    const bool live = item < (uint32_t)a.T * heads && lane < a.lanes;
-    const uint32_t it = live ? item : 0;
-    const int token = (int)(it / heads);
-    int head = (int)(it - (uint32_t)token * heads);
+// One head of a thread: loaded, normed, turned, stored.
+template <int DT, int CH> BW_DEV void rotate_head(const RotateArgs& a, const Raw<CH>& raw1, const Raw<CH>& raw2, const Angle<CH>& angle, int token, int head, bool live, bool kept, bool turns,
+                                                  int first, int second) {
     const bool is_k = head >= a.q_heads;
     if (is_k) head -= a.q_heads;
-    int first, second;
-    bool turns;
-    chunks_of<CH>(a, live ? lane : 0, first, second, turns);
-    const uint16_t* src = is_k ? a.k + token * a.k_row + head * a.k_head : a.q + token * a.q_row + head * a.q_head;
-    const Position<AXES> pos(a, token);
     float x[CH], y[CH];
-    widen_raw<DT, CH>(load_raw<CH>(src + first), x);
-    widen_raw<DT, CH>(load_raw<CH>(src + second), y);
-    const bool kept = pos.kept;
-    Angle<CH> angle;
-    if (kept && turns) angle.load(a, pos, first);
+    widen_raw<DT, CH>(raw1, x);
+    widen_raw<DT, CH>(raw2, y);
     if (a.q_weight || a.k_weight) {
         const void* weight = is_k ? a.k_weight : a.q_weight;
         float ss = 0.f;
@@ -66,12 +53,62 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     store_chunk<DT, CH>(dst + second, y);
 }
 
+template <int DT, int CH>
+__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
+    const uint32_t heads = (uint32_t)(a.q_heads + a.k_heads), item = (blockIdx.x * 256 + threadIdx.x) >> a.lane_shift;
+    const int lane = (int)threadIdx.x & ((1 << a.lane_shift) - 1);
+    const bool live = item < (uint32_t)a.T * heads && lane < a.lanes;
+    const uint32_t it = live ? item : 0;
+    const int token = (int)(it / heads), head = (int)(it - (uint32_t)token * heads);
+    int first, second;
+    bool turns;
+    chunks_of<CH>(a, live ? lane : 0, first, second, turns);
+    const uint16_t* src = head >= a.q_heads ? a.k + token * a.k_row + (head - a.q_heads) * a.k_head : a.q + token * a.q_row + head * a.q_head;
+    const Position<false> pos(a, token);
+    const Raw<CH> raw1 = load_raw<CH>(src + first), raw2 = load_raw<CH>(src + second);
+    Angle<CH> angle;
+    if (pos.kept && turns) angle.load(a, pos, first);
+    rotate_head<DT, CH>(a, raw1, raw2, angle, token, head, live, pos.kept, turns, first, second);
+}
+
+// Positions of several axes: the angles come from as many rows of the tables as there are axes, so that a thread keeps them for a.each heads of its token, `slices` apart
+// (4095 tokens of 32 and 8 heads of 128 with norms, three interleaved axes: 26.6 us with one head).
+template <int DT, int CH>
+__global__ __launch_bounds__(256) void rotate_axes_kernel(RotateArgs a) {
+    const uint32_t heads = (uint32_t)(a.q_heads + a.k_heads), item = (blockIdx.x * 256 + threadIdx.x) >> a.lane_shift;
+    const int lane = (int)threadIdx.x & ((1 << a.lane_shift) - 1);
+    const bool live = item < (uint32_t)a.T * a.slices && lane < a.lanes;
+    const uint32_t it = live ? item : 0;
+    const int token = (int)(it / a.slices);
+    int first, second;
+    bool turns;
+    chunks_of<CH>(a, live ? lane : 0, first, second, turns);
+    const Position<true> pos(a, token);
+    auto source = [&](uint32_t head) { return (int)head >= a.q_heads ? a.k + token * a.k_row + ((int)head - a.q_heads) * a.k_head : a.q + token * a.q_row + (int)head * a.q_head; };
+    uint32_t head = it - (uint32_t)token * a.slices;
+    const uint16_t* src = source(head);
+    Raw<CH> raw1 = load_raw<CH>(src + first), raw2 = load_raw<CH>(src + second);
+    Angle<CH> angle;
+    if (pos.kept && turns) angle.load(a, pos, first);
+    for (;;) {
+        const uint32_t next = head + a.slices;
+        const bool more = next < heads;
+        src = source(more ? next : head);
+        const Raw<CH> next1 = load_raw<CH>(src + first), next2 = load_raw<CH>(src + second);
+        rotate_head<DT, CH>(a, raw1, raw2, angle, token, (int)head, live, pos.kept, turns, first, second);
+        if (!more) return;
+        head = next;
+        raw1 = next1;
+        raw2 = next2;
+    }
+}
+
 // One block serves the queries' heads or the keys', 256 >> lane_shift at a time.
 template <int DT, int CH, bool AXES>
 __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
     __shared__ float sums[256 * 2 * CH];
     const bool is_k = (int)blockIdx.x >= a.q_blocks;
-    const uint32_t heads = (uint32_t)(is_k ? a.k_heads : a.q_heads), per_block = 256u >> a.lane_shift, items = (uint32_t)a.T * heads;
+    const uint32_t heads = (uint32_t)(is_k ? a.k_heads : a.q_heads), per_block = 256u >> a.lane_shift, items = (uint32_t)a.T * (AXES ? (is_k ? a.k_slices : a.slices) : heads);
     const uint32_t block = is_k ? blockIdx.x - a.q_blocks : blockIdx.x, blocks = is_k ? gridDim.x - a.q_blocks : a.q_blocks;
     const int lane = (int)threadIdx.x & ((1 << a.lane_shift) - 1);
     int first, second;
@@ -88,14 +125,26 @@ __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
         load_weight<DT, CH>(weight, a.weight_f32, first, w1);
         load_weight<DT, CH>(weight, a.weight_f32, second, w2);
     }
-    // (the same number of rounds for every thread of the block: all of them take part in the sums)
-    for (uint32_t base = block * per_block; base < items; base += blocks * per_block) {
+    Angle<CH> angle;
+    bool kept = false;
+    // (the same number of rounds for every thread of the block: all of them take part in the sums; positions of several axes: a.each heads of a token one after the other, which
+    // share their angles)
+    for (uint32_t base = block * per_block, turn = 0; base < items;) {
         const uint32_t item = base + (threadIdx.x >> a.lane_shift);
-        const bool live = item < items && lane < a.lanes;
-        const uint32_t it = live ? item : 0;
-        const int token = (int)(it / heads), head = (int)(it - (uint32_t)token * heads);
-        const Position<AXES> pos(a, token);
-        const bool kept = pos.kept;
+        const uint32_t per_token = AXES ? (is_k ? a.k_slices : a.slices) : heads, it0 = item < items && lane < a.lanes ? item : 0;
+        const int token = (int)(it0 / per_token), head0 = (int)(it0 - (uint32_t)token * per_token + turn * per_token);
+        const bool live = item < items && lane < a.lanes && (!AXES || head0 < (int)heads);
+        const int head = live ? head0 : 0;
+        if (!AXES || turn == 0) {
+            const Position<AXES> pos(a, token);
+            kept = pos.kept;
+            if (kept && turns) angle.load(a, pos, first);
+        }
+        if (AXES && (turn + 1) * per_token < heads) turn++;
+        else {
+            turn = 0;
+            base += blocks * per_block;
+        }
         const uint16_t* g = gs + token * g_row + head * g_head;
         const uint16_t* in = xs + token * x_row + head * x_head;
         const Raw<CH> g1 = load_raw<CH>(g + first), g2 = load_raw<CH>(g + second);
@@ -104,8 +153,6 @@ __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
             x1 = load_raw<CH>(in + first);
             x2 = load_raw<CH>(in + second);
         }
-        Angle<CH> angle;
-        if (kept && turns) angle.load(a, pos, first);
         float x[CH], y[CH];
         widen_raw<DT, CH>(g1, x);
         widen_raw<DT, CH>(g2, y);
@@ -224,10 +271,11 @@ int rotate(const bw_heads* h, const bw_axes* x, int act_dtype, const void* q, in
     const int64_t heads = h->q_heads + h->k_heads, per_block = 256 >> a.lane_shift, most = (((int64_t)1 << 32) - 256) / (heads << a.lane_shift);
     for (int64_t at = 0; at < h->tokens; at += most) {
         a.T = (int)(h->tokens - at < most ? h->tokens - at : most);
-        const dim3 grid((unsigned)((a.T * heads + per_block - 1) / per_block)), block(256);
+        a.slices = x ? (uint32_t)slices_of(a, (int)heads) : (uint32_t)heads;
+        const dim3 grid((unsigned)(((int64_t)a.T * a.slices + per_block - 1) / per_block)), block(256);
 #define BW_ROTATE(DT, CH) \
-    if (act_dtype == DT && chunk_of(h) == CH && x) hipLaunchKernelGGL((rotate_kernel<DT, CH, true>), grid, block, 0, (hipStream_t)stream, a); \
-    else if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_kernel<DT, CH, false>), grid, block, 0, (hipStream_t)stream, a);
+    if (act_dtype == DT && chunk_of(h) == CH && x) hipLaunchKernelGGL((rotate_axes_kernel<DT, CH>), grid, block, 0, (hipStream_t)stream, a); \
+    else if (act_dtype == DT && chunk_of(h) == CH) hipLaunchKernelGGL((rotate_kernel<DT, CH>), grid, block, 0, (hipStream_t)stream, a);
         BW_ROTATE(BW_F16, 8) BW_ROTATE(BW_F16, 4) BW_ROTATE(BW_BF16, 8) BW_ROTATE(BW_BF16, 4)
 #undef BW_ROTATE
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
@@ -263,6 +311,16 @@ int rotate_grad(const bw_heads* h, const bw_axes* x, int act_dtype, const void* 
     a.q_out = (uint16_t*)q_grad; a.k_out = (uint16_t*)k_grad;
     a.q_blocks = h->tokens ? grad_blocks(h, h->q_heads) : 0;
     const int blocks = h->tokens ? a.q_blocks + grad_blocks(h, h->k_heads) : 0;
+    if (x) {
+        // (as many heads to a thread as there would be rounds: each block has about one)
+        auto slices = [&](int heads, int of) {
+            const int64_t rounds = h->tokens ? ((h->tokens * heads << a.lane_shift) + 256 * (int64_t)of - 1) / (256 * (int64_t)of) : 1;
+            const int each = (int)(rounds < 8 ? rounds : 8);
+            return (uint32_t)((heads + each - 1) / each);
+        };
+        a.slices = slices(h->q_heads, a.q_blocks);
+        a.k_slices = slices(h->k_heads, blocks - a.q_blocks);
+    }
     const bool sums = q_weight_grad || k_weight_grad;
     if (sums && blocks) {
         if (!workspace || workspace_bytes < grad_workspace(h)) return BW_EWORKSPACE;
