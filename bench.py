@@ -710,7 +710,7 @@ def extras_llama7b_decoder_graph(torch, hip, QuantizedLinear, layers):
 def extras_llama7b_decoder_paged(torch, hip, QuantizedLinear, layers):
     """The decoder of llama7b_decoder_graph (sibling launches fused, HIP glue) with the library's rotation, paged cache and attention
     of one token in place of the glue's: 512-token prompt and 256 tokens, and the same step again with 3584 tokens cached before it (the glue takes 4096), where the
-    cache is what is read most.  Only on request (--only llama7b_decoder_paged)."""
+    cache is what is read most; also with a window of 1024 tokens and 4 sinks.  Only on request (--only llama7b_decoder_paged)."""
     import bitween_amd
     import bench_decoder as bd
     nlayers, prompt, new_tokens, cached = 32, 512, 256, 3584
@@ -724,11 +724,11 @@ def extras_llama7b_decoder_paged(torch, hip, QuantizedLinear, layers):
     qmodel.alloc_state()
     bitween_amd.fuse_sibling_linears(qmodel)
     res = {}
-    for label, bits, glue in (("glue_attention", None, True), ("paged_16_bits", 16, True), ("paged_8_bits", 8, True), ("paged_4_bits", 4, True),
-                              ("paged_16_bits_torch_glue", 16, False)):
+    for label, bits, glue, window in (("glue_attention", None, True, None), ("paged_16_bits", 16, True, None), ("paged_8_bits", 8, True, None), ("paged_4_bits", 4, True, None),
+                                      ("paged_16_bits_torch_glue", 16, False, None), ("paged_16_bits_window_1024", 16, True, 1024), ("paged_8_bits_window_1024", 8, True, 1024)):
         qmodel.paged = qmodel.glue = None
         if bits is not None:
-            qmodel.use_paged_cache(bits, 64)
+            qmodel.use_paged_cache(bits, 64, window=window, sinks=4 if window else 0)
         if glue:
             qmodel.use_hip_glue(splits=16)
         res[label] = {}

@@ -17,7 +17,8 @@ With use_hip_glue() the decode step runs the same arithmetic through five small 
 of about seventeen torch kernels per layer; the prompt always goes through the torch ops.
 
 With use_paged_cache(bits) queries and keys are rotated, cached and attended to by the library's own operators (bitween_amd.rotate_heads and a
-PagedCache of 16, 8 or 4 bits per layer), with or without the glue kernels around them.
+PagedCache of 16, 8 or 4 bits per layer), with or without the glue kernels around them; with a window, every token sees that many of the last tokens and the first
+`sinks`, and the prompt goes through bitween_amd.prompt_attention.
 
 Random weights N(0, 0.02) from a seed (no checkpoint can be fetched); the numbers say how fast the path runs,
 not what it generates.
@@ -158,10 +159,11 @@ class Decoder(nn.Module):
         """Run step() through the HIP glue kernels (head dimension 128, float16 parameters; call after alloc_state)."""
         self.glue = HipGlue(self, splits)
 
-    def use_paged_cache(self, bits=16, group_size=64, page_size=64):
+    def use_paged_cache(self, bits=16, group_size=64, page_size=64, window=None, sinks=0):
         """Keep keys and values in a PagedCache per layer instead of self.kv (call after alloc_state; self.paged = None goes back).  The cache
-        lies in pages in an order of its own, the rotary table is float32."""
+        lies in pages in an order of its own, the rotary table is float32.  window, sinks: what a token sees (None: all before it)."""
         from bitween_amd import PagedCache
+        self.window, self.sinks = window, sinks
         dev = self.lm_head.weight.device
         pages = -(-self.max_len // page_size)
         self.paged = [PagedCache(pages, self.heads, self.head_dim, page_size, bits, group_size, device=dev) for _ in self.layers]
@@ -207,9 +209,10 @@ class Decoder(nn.Module):
         return q, k, v
 
     def _attend_paged(self, q, k, v, i):
-        """The attention of a decode step: rotation, cache write and attention, [1, hidden]."""
-        q, _, _ = self._rotate_and_cache(i, q, k, v, self.pos)
-        return self.paged[i].attend(q, self.page_table, self._lengths).view(1, self.hidden)
+        """The attention of a decode step: rotation with the cache write, and attention, [1, hidden]."""
+        q, k, v = (x.view(1, self.heads, self.head_dim) for x in (q, k, v))
+        q = self.paged[i].append(q, k, v, self.cos32, self.sin32, self.pos, self._slots)
+        return self.paged[i].attend(q, self.page_table, self._lengths, window=self.window, sinks=self.sinks).view(1, self.hidden)
 
     def _rope(self, qk):
         """qk [T, 2 * heads, head_dim] float16 -> the same with pairs (x_i, x_{i + d/2}) rotated by the angle of the
@@ -255,8 +258,10 @@ class Decoder(nn.Module):
             o = torch.bmm(torch.softmax(scores, dim=-1, dtype=torch.float32).to(torch.float16), vc[0]).transpose(0, 1)
         return self._mlp(layer, x + att.o_proj(o.reshape(t, self.hidden)))
 
-    @staticmethod
-    def _attend_prompt(q, k, v):
+    def _attend_prompt(self, q, k, v):
+        if self.paged is not None and self.window is not None:
+            from bitween_amd import prompt_attention
+            return prompt_attention(q, k, v, window=self.window, sinks=self.sinks)
         return F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None],
                                               is_causal=True)[0].transpose(0, 1)
 
