@@ -224,6 +224,8 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     // (a row's place in a tile of rows of a key head's query heads is 32 bits of bytes)
     for (auto [row, head] : {std::pair<int64_t, int64_t>{q_row, q_head}, {grad_row, grad_head}})
         if (head < 0 || head >= (int64_t)1 << 30 || (share - 1) * head + 65 * row >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
+    const bool keys = (k_grad || v_grad) && p->k_tokens > 0;
+    if (p->q_tokens == 0 && !keys) return BW_OK;
     const GradPlan plan = grad_plan(p);
     if (plan.all) {
         if (!workspace || workspace_bytes < plan.all) return BW_EWORKSPACE;
@@ -242,7 +244,6 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     a.splits = 1;
     g.plain_scale = p->scale;
     PromptGrids grids = {};
-    const bool keys = (k_grad || v_grad) && p->k_tokens > 0;
     if (p->q_tokens > 0) {
         const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos;
         if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
