@@ -98,8 +98,8 @@ int key_tile(int dim) { return dim > 128 ? 32 : 64; }
 // Parts that the keys of a tile of rows are cut into: the number for which the longest workgroup (or, in several rounds, the mean of all), the second launch and the parts' way
 // through memory take the least together.  In microseconds, as measured: a tile of keys takes a workgroup 0.9 (heads of 64), 1.5 (128) and 2 (256, of half the keys), 1.4 times that
 // where two share a CU; the join 5, and its parts, written and read, go at 4 TB/s.  512 tokens of 8192, 32 and 8 heads of 128: 1 part 193 us, 2 110, 3 100, 4 88; 63 of 32063: 8 parts 106 us,
-// 16 63, 32 59, 48 70; 1024 tokens alone: 1 part 31 us, 2 41; 256 of 4096, heads of 64: 1 part 62 us, 4 25, 8 20, 16 26.
-int splits_of(const bw_prompt* p) {
+// 16 63, 32 59, 48 70; 1024 tokens alone: 1 part 31 us, 2 41; 256 of 4096, heads of 64: 1 part 62 us, 4 25, 8 20, 16 26.  `times`: a tile of the queries' gradient takes 1.25 times as long.
+int splits_of(const bw_prompt* p, double times = 1.) {
     const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), cus = bw_device_cus(), resident = cus * (p->dim > 128 ? 1 : 2);
     const int64_t of = p->q_starts ? p->sequences : 1, tiles = (p->q_tokens * share + kRows - 1) / kRows;
     const int64_t row_tiles = p->q_starts ? (tiles > p->sequences ? tiles : p->sequences < p->q_tokens ? p->sequences : p->q_tokens) : p->sequences * tiles_of(p, p->q_tokens, share, kRows);
@@ -111,7 +111,7 @@ int splits_of(const bw_prompt* p) {
     const bool all = reach >= keys;
     if (!all) keys = reach;
     const double longest = (double)((keys + tile - 1) / tile), mean = all && keys > 0 ? longest * (1. - 0.5 * (rows < keys ? rows : keys) / keys) : longest;
-    const double one = p->dim > 128 ? 2.0 : 0.3 + p->dim * 0.0094;
+    const double one = times * (p->dim > 128 ? 2.0 : 0.3 + p->dim * 0.0094);
     int best = 1;
     double least = 0.;
     for (int s = 1; s <= 64 && (s == 1 || s * 2 <= longest); s++) {
@@ -119,7 +119,7 @@ int splits_of(const bw_prompt* p) {
         const double time = tiles_each / s * one * (blocks * s > cus && resident > cus ? 1.4 : 1.) + (s > 1 ? 5. + (double)p->q_tokens * p->q_heads * p->dim * 8. * s / 4e6 : 0.);
         if (s == 1 || time < least) {
             best = s;
-            least = time;
+            least = s == 1 ? 0.9 * time : time;                      // (parts where they gain a tenth at least)
         }
     }
     return best;
@@ -130,7 +130,8 @@ constexpr int kPiecesPerCu = 4;                  // about, over all heads
 struct GradPlan {
     int target;                                  // pieces of a head; 0: every tile of keys is one
     int64_t pieces, parts, joins;                // at most
-    size_t delta, plan, parts_at, all;
+    int q_splits;                                // parts of a row's keys, for the queries' gradient
+    size_t delta, plan, parts_at, q_parts, all;
 };
 GradPlan grad_plan(const bw_prompt* p) {
     const int64_t share = p->q_heads / p->kv_heads, seq_q = p->q_tokens / (p->q_starts ? 1 : p->sequences);
@@ -144,6 +145,8 @@ GradPlan grad_plan(const bw_prompt* p) {
         return at;
     };
     g.delta = room((size_t)(p->q_tokens * p->q_heads) * sizeof(float));
+    g.q_splits = p->q_tokens > 0 ? splits_of(p, 1.25) : 1;
+    if (g.q_splits > 1) g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
     if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
         g.target = (int)(((int64_t)bw_device_cus() * kPiecesPerCu + p->kv_heads - 1) / p->kv_heads);
         // (a tile of n among U tiles of rows is cut into n / size rounded up, size at least U / target and kLeastTiles)
@@ -241,11 +244,12 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     g.result = (const uint16_t*)out;
     g.q_grad = (uint16_t*)q_grad; g.k_grad = (uint16_t*)k_grad; g.v_grad = (uint16_t*)v_grad;
     g.delta = (float*)workspace;
-    a.splits = 1;
+    a.splits = q_grad ? plan.q_splits : 1;
+    g.q_parts = a.splits > 1 ? (float*)((char*)workspace + plan.q_parts) : nullptr;
     g.plain_scale = p->scale;
     PromptGrids grids = {};
     if (p->q_tokens > 0) {
-        const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos;
+        const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos * a.splits;
         if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
         grids.rows = (uint32_t)grid;
         grids.row_tiles = (uint32_t)tiles;

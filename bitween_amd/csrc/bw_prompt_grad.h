@@ -21,6 +21,13 @@ template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptG
         g.p.tiles = grids.row_tiles;
         hipLaunchKernelGGL(prompt_query_grad_kernel<H>, dim3(grids.rows), dim3(256), 4 * H::kTileBytes, stream, g);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
+        if (g.p.splits > 1) {
+            const int threads = g.p.dim / 4;
+            const uint32_t rows = (uint32_t)(g.p.q_tokens * g.p.q_heads), per = 256 / threads;
+            hipLaunchKernelGGL(prompt_query_join_kernel<H::kType>, dim3((rows + per - 1) / per), dim3(256), 0, stream, g, threads, rows);
+            if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
+            g.p.splits = 1;
+        }
     }
     if (!grids.keys) return BW_OK;
     if (g.plan) {

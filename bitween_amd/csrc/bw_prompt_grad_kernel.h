@@ -19,6 +19,7 @@ struct PromptGradArgs {
     int64_t grad_row, grad_head;
     float* delta;                                // as lse
     uint16_t *q_grad, *k_grad, *v_grad;
+    float* q_parts;                              // where a row's keys are cut into p.splits parts: [row][part][dim]
     float plain_scale;
     // keys: the list of the workgroups' pieces (NULL: a piece for every tile of keys), the parts [part][kv_heads][keys][2][dim] and what is to be joined of them
     struct KeyPlan* plan;
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         }
         delta += __shfl_xor(delta, 32, 64);
     }
-    if (row.live && half == 0) g.delta[index] = delta;
+    if (row.live && half == 0 && split == 0) g.delta[index] = delta;
     if (!g.q_grad) return;
     const float lse = row.live ? a.lse[index] : INFINITY;
 
@@ -102,6 +103,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     positions_of(a, p, p.tile * kRows, (p.tile + 1) * kRows, low, high);
     positions_of(a, p, row0 < rows ? row0 : p.tile * kRows, row0 + kWaveRows, wave_low, wave_high);
     const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
+    const int begin = (int)((int64_t)tiles.count * split / a.splits), end = (int)((int64_t)tiles.count * (split + 1) / a.splits);
     const RowLoader<H> load_k(lane, wave, a.k_row), load_v(lane, wave, a.v_row);
     const TileReader<H> read(lane);
     const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);
@@ -121,13 +123,13 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
         rest = 0.f;
-        KeyWalk<H> next(a, p, head, tiles, 0);
-        if (tiles.count) fetch(next);
-        for (int i = 0; i < tiles.count; i++) {
+        KeyWalk<H> next(a, p, head, tiles, begin);
+        if (begin < end) fetch(next);
+        for (int i = begin; i < end; i++) {
             const int at = next.at;
             next.step(a);
             wait_tiles();
-            if (next.i < tiles.count) fetch(next);
+            if (next.i < end) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
             const Seen which = seen(at);
             if (!careful && which == kNone) continue;
@@ -200,6 +202,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     rest += __shfl_xor(rest, 32, 64);
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
+    float* part = a.splits > 1 ? g.q_parts + (index * a.splits + split) * a.dim : nullptr;
 #pragma unroll
     for (int m = 0; m < H::kBlocks; m++)
 #pragma unroll
@@ -207,8 +210,32 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
             const int d = 32 * m + 8 * b + 4 * half;
             const f4 c = *reinterpret_cast<const f4*>(mean + d * 4);
             const f4 x = (f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]} - rest * c) * back * g.plain_scale;
-            if (d < a.dim) store4<DT>(out + d, x[0], x[1], x[2], x[3]);
+            if (d >= a.dim) continue;
+            if (part) *reinterpret_cast<f4*>(part + d) = x;
+            else store4<DT>(out + d, x[0], x[1], x[2], x[3]);
         }
+}
+
+// dQ = the parts of a row added up in order; a thread has 4 values of a row, and 8 parts under way.
+template <int DT>
+__global__ __launch_bounds__(256) void prompt_query_join_kernel(PromptGradArgs g, int threads, uint32_t rows) {
+    const PromptArgs& a = g.p;
+    const uint32_t i = blockIdx.x * (256 / threads) + threadIdx.x / threads;
+    const int d = (int)(threadIdx.x % threads) * 4;
+    if (threadIdx.x / threads >= 256 / threads || i >= rows) return;
+    const float* part = g.q_parts + (int64_t)i * a.splits * a.dim + d;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; s += 8) {
+        f4 x[8];
+#pragma unroll
+        for (int n = 0; n < 8; n++) x[n] = *reinterpret_cast<const f4*>(part + (int64_t)(s + n < a.splits ? s + n : s) * a.dim);
+#pragma unroll
+        for (int n = 0; n < 8; n++)
+            if (s + n < a.splits) o += x[n];
+    }
+    uint32_t j;
+    const uint32_t token_head = a.by_share.div(i, j), head = token_head / (uint32_t)a.q_tokens, token = token_head - head * a.q_tokens;
+    store4<DT>(g.q_grad + ((int64_t)token * a.q_heads + head * a.share + j) * a.dim + d, o[0], o[1], o[2], o[3]);
 }
 
 // ---- keys ----
