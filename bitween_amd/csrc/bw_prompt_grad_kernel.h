@@ -17,7 +17,7 @@ struct PromptGradArgs {
     PromptArgs p;
     const uint16_t *grad, *result;               // of the output; result [tokens][q_heads][dim]
     int64_t grad_row, grad_head;
-    float* delta;                                // as lse
+    float* delta;                                // its negative, as lse
     uint16_t *q_grad, *k_grad, *v_grad;
     float* q_parts;                              // where a row's keys are cut into p.splits parts: [row][part][dim]
     float plain_scale;
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         }
         delta += __shfl_xor(delta, 32, 64);
     }
-    if (row.live && half == 0 && split == 0) g.delta[index] = delta;
+    if (row.live && half == 0 && split == 0) g.delta[index] = -delta;
     if (!g.q_grad) return;
     const float lse = row.live ? a.lse[index] : INFINITY;
 
@@ -104,14 +104,16 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     positions_of(a, p, row0 < rows ? row0 : p.tile * kRows, row0 + kWaveRows, wave_low, wave_high);
     const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
     const int begin = (int)((int64_t)tiles.count * split / a.splits), end = (int)((int64_t)tiles.count * (split + 1) / a.splits);
-    const RowLoader<H> load_k(lane, wave, a.k_row), load_v(lane, wave, a.v_row);
+    const RowLoader<H> load_k(a, lane, wave, a.k_row), load_v(a, lane, wave, a.v_row);
     const TileReader<H> read(lane);
     const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);
-    const uint32_t lds = lds_address(smem);
+    const uint32_t lds = own(lds_address(smem));
+    const int keys = own(p.nk);
+    const float scale = own(a.scale);
     auto fetch = [&](const KeyWalk<H>& next) __attribute__((always_inline)) {
         const uint32_t to = lds + (next.i & 1) * 2 * H::kTileBytes;
-        load_k(next.k, p.nk - next.at, to, wave, a.dim);
-        load_v(next.v, p.nk - next.at, to + H::kTileBytes, wave, a.dim);
+        load_k(next.k, keys - next.at, to, wave);
+        load_v(next.v, keys - next.at, to + H::kTileBytes, wave);
     };
 
     f16v acc[H::kBlocks];
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         if (begin < end) fetch(next);
         for (int i = begin; i < end; i++) {
             const int at = next.at;
-            next.step(a);
+            next.step();
             wait_tiles();
             if (next.i < end) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
                     reads_ahead<2 * H::kSteps, 1, 4>();
                     float ds[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) ds[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale, -lse)) * (dp[j] - delta);
+                    for (int j = 0; j < 16; j++) ds[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], scale, -lse)) * (dp[j] - delta);
                     if (which == kSome) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) ds[j] = sees(a, row.position, at + 32 * b + 8 * (j / 4) + 4 * half + j % 4) ? ds[j] : 0.f;
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
                     if (which != kNone) add_nonfinite<H>(tile + b * 32 * H::kPitch * 2, 32, lane, acc, [&](int n) { return sees(a, row.position, at + 32 * b + n); });
                     keep_finite<H>(tile + b * 32 * H::kPitch * 2, 32 * H::kPitch * 2);
                 }
-                if (which != kNone) {
+                if (which != kNone) {                            // (with the first of these operands read before the weights, as for the keys below: no gain with heads of 128, a tenth lost with 64 and 256)
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -324,6 +326,24 @@ BW_DEV void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory");
 }
 
+// sums += the transposed product of 32 rows of a tile with the 16 + 16 values of a lane: the second 16's operands are read while the first products are under way.  `first`: the first
+// 16's, read by then.
+template <class H> BW_DEV void first_columns(const TileReader<H>& read, const char* tile, int block, u4* first) {
+#pragma unroll
+    for (int m = 0; m < H::kBlocks; m++) first[m] = read.columns(tile, 2 * block, m);
+}
+template <class H> BW_DEV void add_columns(const TileReader<H>& read, const char* tile, int block, const u4* first, const u4* w, f16v* acc) {
+    in_order();
+    u4 second[H::kBlocks];
+#pragma unroll
+    for (int m = 0; m < H::kBlocks; m++) second[m] = read.columns(tile, 2 * block + 1, m);
+#pragma unroll
+    for (int m = 0; m < H::kBlocks; m++) acc[m] = mfma32<H::kType>(first[m], w[0], acc[m]);
+    in_order();
+#pragma unroll
+    for (int m = 0; m < H::kBlocks; m++) acc[m] = mfma32<H::kType>(second[m], w[1], acc[m]);
+}
+
 template <class H> constexpr int kKeyStage = 2 * H::kTileBytes + 512;           // Q, g, lse, delta of a tile of rows
 
 // One piece: dK of its keys, or dV.
@@ -357,6 +377,11 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
 
     const TileReader<H> read(lane);
     const uint16_t *queries = a.q + p.q0 * a.q_row + (int64_t)head * a.share * a.q_head, *grads = g.grad + p.q0 * g.grad_row + (int64_t)head * a.share * g.grad_head;
+    any_from = own(any_from);
+    any_to = own(any_to);
+    all_from = own(all_from);
+    all_to = own(all_to);
+    const float scale = own(a.scale);
     const int64_t stats = (int64_t)head * a.q_tokens * a.share + (int64_t)p.q0 * a.share;
     const uint32_t lds = lds_address(smem);
     auto fetch = [&](PackedLoader<H>& load_q, PackedLoader<H>& load_g, int i) __attribute__((always_inline)) {
@@ -387,9 +412,21 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
             if (!careful && none) continue;
 #pragma unroll
             for (int b = 0; b < kTileRows / 32; b++) {
-                u4 w[2];
+                u4 w[2], first[H::kBlocks];
+                char* from = tile + (DK ? 0 : H::kTileBytes);
                 if (!none) {
+                    const char* stat = tile + 2 * H::kTileBytes + (32 * b + 4 * half) * 4;
                     f16v s = f16v{}, dp = f16v{};
+                    in_order();
+                    if constexpr (DK) {                            // dP - delta: the sums begin at -delta
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const f4 delta = *reinterpret_cast<const f4*>(stat + 256 + 32 * j);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) dp[4 * j + n] = delta[n];
+                        }
+                        in_order();
+                    }
 #pragma unroll
                     for (int n = 0; n < H::kSteps; n++) s = mfma32<DT>(read.rows(tile, b, n), k[n], s);
                     if constexpr (DK) {
@@ -397,17 +434,18 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
                         for (int n = 0; n < H::kSteps; n++) dp = mfma32<DT>(read.rows(tile + H::kTileBytes, b, n), v[n], dp);
                     }
                     reads_ahead<(DK ? 2 : 1) * H::kSteps, 1, 4>();
+                    in_order();
+                    f4 lses[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) lses[j] = *reinterpret_cast<const f4*>(stat + 32 * j);
+                    if constexpr (!careful) first_columns<H>(read, from, b, first);
                     float x[16];
-                    const char* stat = tile + 2 * H::kTileBytes + (32 * b + 4 * half) * 4;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const f4 lse = *reinterpret_cast<const f4*>(stat + 32 * j);
 #pragma unroll
-                        for (int n = 0; n < 4; n++) x[4 * j + n] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + n], a.scale, (DT == BW_F16 ? (float)kWeightShift : 0.f) - lse[n]));
-                        if constexpr (DK) {
-                            const f4 delta = *reinterpret_cast<const f4*>(stat + 256 + 32 * j);
-#pragma unroll
-                            for (int n = 0; n < 4; n++) x[4 * j + n] *= dp[4 * j + n] - delta[n];
+                        for (int n = 0; n < 4; n++) {
+                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * j + n], scale, (DT == BW_F16 ? (float)kWeightShift : 0.f) - lses[j][n]));
+                            x[4 * j + n] = DK ? p * dp[4 * j + n] : p;
                         }
                     }
                     if (!all) {
@@ -423,19 +461,14 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
                     }
                     pack16<DT>(x, w);
                 }
-                char* from = tile + (DK ? 0 : H::kTileBytes);
                 if constexpr (careful) {
                     char* block = from + b * 32 * H::kPitch * 2;
                     __syncthreads();
                     if (!none) add_nonfinite<H>(block, 32, lane, acc, [&](int n) { return at + 32 * b + n >= row_from && at + 32 * b + n < row_to; });
                     keep_finite<H>(block, 32 * H::kPitch * 2);
+                    if (!none) first_columns<H>(read, from, b, first);
                 }
-                if (!none) {
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int m = 0; m < H::kBlocks; m++) acc[m] = mfma32<DT>(read.columns(from, 2 * b + t, m), w[t], acc[m]);
-                }
+                if (!none) add_columns<H>(read, from, b, first, w, acc);
             }
         }
     };

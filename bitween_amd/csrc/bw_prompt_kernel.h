@@ -71,6 +71,8 @@ template <int N> BW_DEV void then_reads() { __builtin_amdgcn_sched_group_barrier
 template <int N> BW_DEV void then_products() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
 template <int N> BW_DEV void then_vector() { __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
 template <int N> BW_DEV void then_exponentials() { __builtin_amdgcn_sched_group_barrier(0x400, N, 0); }
+// Nothing is moved past it.
+BW_DEV void in_order() { __builtin_amdgcn_sched_barrier(0); }
 // N products with PER reads each, AHEAD products' worth of them before the first.
 template <int N, int PER, int AHEAD> BW_DEV void reads_ahead() {
     then_reads<PER * (AHEAD < N ? AHEAD : N)>();
@@ -78,6 +80,12 @@ template <int N, int PER, int AHEAD> BW_DEV void reads_ahead() {
         then_products<1>();
         if constexpr (decltype(i)::value + AHEAD < N) then_reads<PER>();
     });
+}
+
+// A scalar register of its own for a number that a loop needs: an argument lies in a block of 16, which is read back from a vector register as a whole where there are not enough.
+template <class T> BW_DEV T own(T x) {
+    asm("" : "+s"(x));
+    return x;
 }
 
 // What was asked for has arrived, for all waves.
@@ -91,27 +99,29 @@ BW_DEV void wait_tiles() {
 // A tile of rows of one head on its way to LDS.  Rows from `rows` on are those of the last one again (the mask hides them); values behind the head's end are not
 // loaded.
 template <class H> struct RowLoader {
-    uint32_t row_bytes, chunk[H::kLoads];
-    int first;                                   // row of the lane in the first load
-    BW_DEV RowLoader(int lane, int wave, int64_t row) {
-        row_bytes = (uint32_t)(row * 2);
+    uint32_t row_bytes, bytes, chunk[H::kLoads], at;
+    int first, whole;                            // row of the lane in the first load; tiles with that many rows are whole ones
+    BW_DEV RowLoader(const PromptArgs& a, int lane, int wave, int64_t row) {
+        row_bytes = own((uint32_t)(row * 2));
+        bytes = own((uint32_t)a.dim * 2);
+        whole = own(a.dim == H::kPitch ? H::kKeys : 0x7fffffff);
         first = wave * H::kLoads * H::kLoadRows + lane / H::kChunks;
+        at = (uint32_t)first * row_bytes;
 #pragma unroll
         for (int i = 0; i < H::kLoads; i++) chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(first + i * H::kLoadRows)) * 16;
     }
-    BW_DEV void operator()(const uint16_t* base, int rows, uint32_t to, int wave, int dim) const {
+    BW_DEV void operator()(const void* base, int rows, uint32_t to, int wave) const {
         to += wave * H::kLoads * 1024;
-        if (rows >= H::kKeys && dim == H::kPitch) {
-            const uint32_t at = (uint32_t)first * row_bytes;
+        if (rows >= whole) {
 #pragma unroll
             for (int i = 0; i < H::kLoads; i++) load_to_lds(base, at + i * H::kLoadRows * row_bytes + chunk[i], to + i * 1024);
         } else {
-            uint32_t bytes = (uint32_t)dim * 2;
-            asm("" : "+s"(bytes));                               // (the comparisons below are not kept in registers over the loop)
+            uint32_t some = bytes;
+            asm("" : "+s"(some));                                // (the comparisons below are not kept in registers over the loop)
 #pragma unroll
             for (int i = 0; i < H::kLoads; i++) {
                 const int r = first + i * H::kLoadRows;
-                if (chunk[i] < bytes) load_to_lds(base, (uint32_t)(r < rows ? r : rows - 1) * row_bytes + chunk[i], to + i * 1024);
+                if (chunk[i] < some) load_to_lds(base, (uint32_t)(r < rows ? r : rows - 1) * row_bytes + chunk[i], to + i * 1024);
             }
         }
     }
@@ -286,22 +296,24 @@ struct KeyTiles {
 };
 // Keys and values of the tiles one after the other: what the next one's rows begin at.
 template <class H> struct KeyWalk {
-    const uint16_t *k, *v;
+    const char *k, *v;
+    uint32_t k_step, v_step;
     int at, i, jump_at, jump;
     BW_DEV KeyWalk(const PromptArgs& a, const Span& p, int head, const KeyTiles& tiles, int begin) {
         i = begin;
         at = tiles[begin] * H::kKeys;
-        jump_at = tiles.sinks;
-        jump = (tiles.first - tiles.sinks) * H::kKeys;
-        k = a.k + (int64_t)(p.k0 + at) * a.k_row + head * a.k_head;
-        v = a.v + (int64_t)(p.k0 + at) * a.v_row + head * a.v_head;
+        jump_at = own(tiles.sinks);
+        jump = own(tiles.first - tiles.sinks + 1);
+        k_step = own((uint32_t)(H::kKeys * 2 * a.k_row));        // (rows are 2^24 - 1 apart at most)
+        v_step = own((uint32_t)(H::kKeys * 2 * a.v_row));
+        k = own((const char*)(a.k + (int64_t)(p.k0 + at) * a.k_row + head * a.k_head));
+        v = own((const char*)(a.v + (int64_t)(p.k0 + at) * a.v_row + head * a.v_head));
     }
-    BW_DEV void step(const PromptArgs& a) {
-        int by = H::kKeys;
-        if (++i == jump_at) by += jump;
-        at += by;
-        k += by * a.k_row;
-        v += by * a.v_row;
+    BW_DEV void step() {
+        const int by = ++i == jump_at ? jump : 1;
+        at += by * H::kKeys;
+        k += (uint64_t)k_step * (uint32_t)by;
+        v += (uint64_t)v_step * (uint32_t)by;
     }
 };
 
@@ -310,11 +322,11 @@ enum Seen { kNone, kSome, kAll };
 template <int N> struct SeenOf {
     int none_above, all_to, window_from, sinks, all_from;
     BW_DEV SeenOf(const PromptArgs& a, int low, int high, bool any) {
-        none_above = any ? high : -1;                            // (no rows: nothing is seen)
-        all_to = low - N + 1;
-        window_from = low - a.window + 1 - N;
-        sinks = a.sinks;
-        all_from = high - a.window + 1;
+        none_above = own(any ? high : -1);                       // (no rows: nothing is seen)
+        all_to = own(low - N + 1);
+        window_from = own(low - a.window + 1 - N);
+        sinks = own(a.sinks);
+        all_from = own(high - a.window + 1);
     }
     BW_DEV Seen operator()(int at) const {
         if (at > none_above || (at <= window_from && at >= sinks)) return kNone;
@@ -404,14 +416,16 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
     const int begin = (int)((int64_t)tiles.count * split / a.splits), end = (int)((int64_t)tiles.count * (split + 1) / a.splits);
 
-    const RowLoader<H> load_k(lane, wave, a.k_row), load_v(lane, wave, a.v_row);
+    const RowLoader<H> load_k(a, lane, wave, a.k_row), load_v(a, lane, wave, a.v_row);
     const TileReader<H> read(lane);
     const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);
-    const uint32_t lds = lds_address(smem);
+    const uint32_t lds = own(lds_address(smem));
+    const int keys = own(p.nk);
+    const float scale = own(a.scale);
     auto fetch = [&](const KeyWalk<H>& next) __attribute__((always_inline)) {
         const uint32_t to = lds + (next.i & 1) * 2 * H::kTileBytes;
-        load_k(next.k, p.nk - next.at, to, wave, a.dim);
-        load_v(next.v, p.nk - next.at, to + H::kTileBytes, wave, a.dim);
+        load_k(next.k, keys - next.at, to, wave);
+        load_v(next.v, keys - next.at, to + H::kTileBytes, wave);
     };
 
     f16v acc[H::kBlocks];
@@ -428,7 +442,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
         if (begin < end) fetch(next);
         for (int i = begin; i < end; i++) {
             const int at = next.at;
-            next.step(a);
+            next.step();
             wait_tiles();
             if (next.i < end) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
@@ -446,6 +460,10 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
                 for (int k = 0; k < H::kSteps; k++) s[b] = mfma32<DT>(read.rows(tile, b, k), q[k], s[b]);
             }
             reads_ahead<H::kKeyBlocks * H::kSteps, 1, 4>();
+            in_order();
+            u4 v[H::kBlocks];
+#pragma unroll
+            for (int m = 0; m < H::kBlocks; m++) v[m] = read.columns(tile + H::kTileBytes, 0, m);
             if (which == kSome) {
 #pragma unroll
                 for (int b = 0; b < H::kKeyBlocks; b++)
@@ -457,7 +475,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
             for (int b = 0; b < H::kKeyBlocks; b++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) top = fmaxf(top, s[b][j]);
-            top *= a.scale;
+            top *= scale;
             if (__builtin_amdgcn_ballot_w64(top > r + kWeightMost<DT>)) {
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 // (of those rows only that need it: a row's result does not hang on its neighbours)
@@ -467,38 +485,44 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
 #pragma unroll
                 for (int m = 0; m < H::kBlocks; m++) acc[m] *= keep;
             }
+            // 16 keys at a time: their values and weights are got ready while the products of the 16 before them are under way
+            auto weights = [&](int step) __attribute__((always_inline)) {
+                u4 w;
 #pragma unroll
-            for (int b = 0; b < H::kKeyBlocks; b++)
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    u4 w;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + 2 * j], a.scale, -r)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + 2 * j + 1], a.scale, -r));
-                        w[j] = narrow_pair<DT>(x, y);
-                    }
-                    // (the sum of the weights as they are multiplied, two at a time: what their rounding adds to the values it takes off again)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) l = add_pair<DT>(w[j], l);
-#pragma unroll
-                    for (int m = 0; m < H::kBlocks; m++) {
-                        acc[m] = mfma32<DT>(read.columns(tile + H::kTileBytes, 2 * b + t, m), w, acc[m]);
-                    }
+                for (int j = 0; j < 4; j++) {
+                    const int n = 8 * (step & 1) + 2 * j;
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][n], scale, -r)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][n + 1], scale, -r));
+                    w[j] = narrow_pair<DT>(x, y);
                 }
-            // the weights of 16 keys while the products of the 16 before them are under way
-            then_reads<2 * H::kBlocks>();
-            then_vector<8>();
-            then_exponentials<8>();
-            then_vector<8>();
-            static_for<1, 2 * H::kKeyBlocks>([&](auto) {
-                static_for<0, H::kBlocks>([&](auto) {
-                    then_products<1>();
-                    then_reads<2>();
-                    then_vector<(16 + H::kBlocks - 1) / H::kBlocks>();
-                    then_exponentials<(8 + H::kBlocks - 1) / H::kBlocks>();
-                });
-            });
-            then_products<H::kBlocks>();
+                return w;
+            };
+            u4 w = weights(0);
+#pragma unroll
+            for (int step = 0; step < 2 * H::kKeyBlocks; step++) {
+                u4 next_v[H::kBlocks], next_w;
+                if (step + 1 < 2 * H::kKeyBlocks) {
+#pragma unroll
+                    for (int m = 0; m < H::kBlocks; m++) next_v[m] = read.columns(tile + H::kTileBytes, step + 1, m);
+                    next_w = weights(step + 1);
+                }
+                // (the sum of the weights as they are multiplied, two at a time: what their rounding adds to the values it takes off again)
+#pragma unroll
+                for (int j = 0; j < 4; j++) l = add_pair<DT>(w[j], l);
+#pragma unroll
+                for (int m = 0; m < H::kBlocks; m++) acc[m] = mfma32<DT>(v[m], w, acc[m]);
+                if (step + 1 < 2 * H::kKeyBlocks) {
+                    then_reads<2 * H::kBlocks>();
+                    static_for<0, H::kBlocks>([&](auto) {
+                        then_products<1>();
+                        then_vector<(16 + H::kBlocks - 1) / H::kBlocks>();
+                        then_exponentials<(8 + H::kBlocks - 1) / H::kBlocks>();
+                    });
+                    w = next_w;
+#pragma unroll
+                    for (int m = 0; m < H::kBlocks; m++) v[m] = next_v[m];
+                }
+                in_order();
+            }
         }
     };
     pass(std::false_type{});
