@@ -185,10 +185,10 @@ extern "C" int bw_prompt_attention(const bw_prompt* p, int act_dtype, const void
     a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
     a.out = (uint16_t*)out;
     a.lse = lse;
-    a.splits = splits_of(p);
+    a.set_splits(splits_of(p));
     const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos * a.splits;
     if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
-    a.tiles = (uint32_t)tiles;
+    a.set_tiles((uint32_t)tiles);
     const size_t bytes = bw_prompt_attention_workspace_bytes(p);
     if (bytes) {
         if (!workspace || workspace_bytes < bytes) return BW_EWORKSPACE;
@@ -244,7 +244,7 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     g.result = (const uint16_t*)out;
     g.q_grad = (uint16_t*)q_grad; g.k_grad = (uint16_t*)k_grad; g.v_grad = (uint16_t*)v_grad;
     g.delta = (float*)workspace;
-    a.splits = q_grad ? plan.q_splits : 1;
+    a.set_splits(q_grad ? plan.q_splits : 1);
     g.q_parts = a.splits > 1 ? (float*)((char*)workspace + plan.q_parts) : nullptr;
     g.plain_scale = p->scale;
     PromptGrids grids = {};

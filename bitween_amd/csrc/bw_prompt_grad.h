@@ -18,7 +18,7 @@ template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptG
     for (int i = 0; i < 2; i++)
         if (!bw_allow_big_lds(kernels[i], done[i])) return BW_ELAUNCH;
     if (grids.rows) {
-        g.p.tiles = grids.row_tiles;
+        g.p.set_tiles(grids.row_tiles);
         hipLaunchKernelGGL(prompt_query_grad_kernel<H>, dim3(grids.rows), dim3(256), 4 * H::kTileBytes, stream, g);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
         if (g.p.splits > 1) {
@@ -26,7 +26,7 @@ template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptG
             const uint32_t rows = (uint32_t)(g.p.q_tokens * g.p.q_heads), per = 256 / threads;
             hipLaunchKernelGGL(prompt_query_join_kernel<H::kType>, dim3((rows + per - 1) / per), dim3(256), 0, stream, g, threads, rows);
             if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
-            g.p.splits = 1;
+            g.p.set_splits(1);
         }
     }
     if (!grids.keys) return BW_OK;
@@ -34,7 +34,7 @@ template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptG
         hipLaunchKernelGGL(plan_keys_kernel, dim3(1), dim3(kPlanThreads), 0, stream, g, H::kKeys, kLeastTiles);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     }
-    g.p.tiles = grids.key_tiles;
+    g.p.set_tiles(grids.key_tiles);
     hipLaunchKernelGGL(prompt_key_grad_kernel<H>, dim3(grids.keys), dim3(256), 2 * kKeyStage<H>, stream, g);
     if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
     if (grids.joins) {

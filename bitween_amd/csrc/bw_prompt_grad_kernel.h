@@ -103,7 +103,8 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     positions_of(a, p, p.tile * kRows, (p.tile + 1) * kRows, low, high);
     positions_of(a, p, row0 < rows ? row0 : p.tile * kRows, row0 + kWaveRows, wave_low, wave_high);
     const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
-    const int begin = (int)((int64_t)tiles.count * split / a.splits), end = (int)((int64_t)tiles.count * (split + 1) / a.splits);
+    int begin, end;
+    tiles.part(a, split, begin, end);
     const RowLoader<H> load_k(a, lane, wave, a.k_row), load_v(a, lane, wave, a.v_row);
     const TileReader<H> read(lane);
     const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);

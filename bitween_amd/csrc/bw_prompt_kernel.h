@@ -38,9 +38,17 @@ struct PromptArgs {
     int q_heads, kv_heads, share, dim;
     int window, sinks, splits;
     uint32_t combos, tiles;                      // workgroups: `combos` x (row or key tiles of a sequence, or slots) x splits
-    FastDiv by_share, by_combos, by_heads;
+    FastDiv by_share, by_combos, by_heads, by_tiles, by_splits;
     float scale;                                 // times log2 e, positive
     uint32_t flip;                               // sign bits that turn the queries for a negative scale
+    void set_tiles(uint32_t n) {
+        tiles = n;
+        by_tiles = FastDiv(n ? n : 1);
+    }
+    void set_splits(int n) {
+        splits = n;
+        by_splits = FastDiv((uint32_t)n);
+    }
 };
 
 // kDim: the head dimension filled up to whole MFMAs; kPitch: values of a row in LDS, a power of two.
@@ -266,8 +274,7 @@ template <int TILE, bool KEYS> BW_DEV bool find_tile(const PromptArgs& a, uint32
 template <int TILE, bool KEYS> BW_DEV bool place_of(const PromptArgs& a, uint32_t block, Span& p, int& head, uint32_t& split) {
     uint32_t combo;
     uint32_t slot = a.by_combos.div(block, combo);
-    split = slot / a.tiles;
-    slot -= split * a.tiles;
+    split = a.by_tiles.div(slot, slot);
     if (a.q_starts) {
         head = (int)combo;
         return find_tile<TILE, KEYS>(a, slot, p);
@@ -293,6 +300,13 @@ struct KeyTiles {
         count = sinks + last - first + 1;
     }
     BW_DEV int operator[](int i) const { return i < sinks ? i : i - sinks + first; }
+    // The split'th of a.splits parts.
+    BW_DEV void part(const PromptArgs& a, uint32_t split, int& from, int& to) const {
+        uint32_t rest;
+        const int each = (int)a.by_splits.div((uint32_t)(count + a.splits - 1), rest);
+        from = (int)split * each < count ? (int)split * each : count;
+        to = from + each < count ? from + each : count;
+    }
 };
 // Keys and values of the tiles one after the other: what the next one's rows begin at.
 template <class H> struct KeyWalk {
@@ -414,7 +428,8 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     positions_of(a, p, p.tile * kRows, (p.tile + 1) * kRows, low, high);
     positions_of(a, p, row0 < rows ? row0 : p.tile * kRows, row0 + kWaveRows, wave_low, wave_high);
     const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
-    const int begin = (int)((int64_t)tiles.count * split / a.splits), end = (int)((int64_t)tiles.count * (split + 1) / a.splits);
+    int begin, end;
+    tiles.part(a, split, begin, end);
 
     const RowLoader<H> load_k(a, lane, wave, a.k_row), load_v(a, lane, wave, a.v_row);
     const TileReader<H> read(lane);
