@@ -126,7 +126,9 @@ int splits_of(const bw_prompt* p, double times = 1.) {
 }
 
 // How the gradients' work is cut, and where their workspace has what (bytes).
-constexpr int kPiecesPerCu = 4;                  // about, over all heads
+// About, over all heads (8192 tokens, 32 and 8 heads of 128, gradients of keys and values: 1 1549 us, 2 1479, 3 1495, 4 1513; with a window of 1024 451, 444, 512, 483; 2048 tokens 149, 153,
+// 162, 160).  Of heads up to 64 a CU holds more workgroups at once (16 and 4 heads of 64: 2 480 us, 4 438).
+constexpr int pieces_per_cu(int dim) { return dim <= 64 ? 4 : 2; }
 struct GradPlan {
     int target;                                  // pieces of a head; 0: every tile of keys is one
     int64_t pieces, parts, joins;                // at most
@@ -148,7 +150,7 @@ GradPlan grad_plan(const bw_prompt* p) {
     g.q_splits = p->q_tokens > 0 ? splits_of(p, 1.25) : 1;
     if (g.q_splits > 1) g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
     if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
-        g.target = (int)(((int64_t)bw_device_cus() * kPiecesPerCu + p->kv_heads - 1) / p->kv_heads);
+        g.target = (int)(((int64_t)bw_device_cus() * pieces_per_cu(p->dim) + p->kv_heads - 1) / p->kv_heads);
         // (a tile of n among U tiles of rows is cut into n / size rounded up, size at least U / target and kLeastTiles)
         g.pieces = key_tiles + g.target;
         const int64_t most = key_tiles * ((row_tiles + kLeastTiles - 1) / kLeastTiles);

@@ -9,9 +9,6 @@ struct PromptGrids { uint32_t rows, row_tiles, keys, key_tiles, joins; };
 int bw_launch_prompt_grad_f16(const PromptGradArgs& g, const PromptGrids& grids, hipStream_t stream);
 int bw_launch_prompt_grad_bf16(const PromptGradArgs& g, const PromptGrids& grids, hipStream_t stream);
 
-// A piece of keys has at least so many tiles of rows.
-constexpr int kLeastTiles = 4;
-
 template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptGrids& grids, hipStream_t stream) {
     static uint64_t done[2] = {};
     const void* kernels[2] = {(const void*)prompt_query_grad_kernel<H>, (const void*)prompt_key_grad_kernel<H>};
@@ -19,7 +16,7 @@ template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptG
         if (!bw_allow_big_lds(kernels[i], done[i])) return BW_ELAUNCH;
     if (grids.rows) {
         g.p.set_tiles(grids.row_tiles);
-        hipLaunchKernelGGL(prompt_query_grad_kernel<H>, dim3(grids.rows), dim3(256), 4 * H::kTileBytes, stream, g);
+        hipLaunchKernelGGL(prompt_query_grad_kernel<H>, dim3(grids.rows + (g.plan ? 1 : 0)), dim3(256), 4 * H::kTileBytes, stream, g);
         if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
         if (g.p.splits > 1) {
             const int threads = g.p.dim / 4;
@@ -30,10 +27,6 @@ template <class H> static int launch_prompt_grad(PromptGradArgs g, const PromptG
         }
     }
     if (!grids.keys) return BW_OK;
-    if (g.plan) {
-        hipLaunchKernelGGL(plan_keys_kernel, dim3(1), dim3(kPlanThreads), 0, stream, g, H::kKeys, kLeastTiles);
-        if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;
-    }
     g.p.set_tiles(grids.key_tiles);
     hipLaunchKernelGGL(prompt_key_grad_kernel<H>, dim3(grids.keys), dim3(256), 2 * kKeyStage<H>, stream, g);
     if (hipGetLastError() != hipSuccess) return BW_ELAUNCH;

@@ -62,6 +62,147 @@ template <int DT> BW_DEV void pack16(const float* x, u4* w) {
         for (int j = 0; j < 4; j++) w[t][j] = narrow_pair<DT>(x[8 * t + 2 * j], x[8 * t + 2 * j + 1]);
 }
 
+// ---- the list of pieces of the keys' gradients (see key_grad) ----
+
+// A piece has at least so many tiles of rows.
+constexpr int kLeastTiles = 4;
+
+
+constexpr int kGradKeys = 32 * kPromptWaves;
+
+// Tiles from ... to - 1 of rows (kKeys each) for the keys from kGradKeys tile on of a sequence; part: which of the parts they leave, or -1.
+struct Piece { int q0, nq, k0, nk, tile, from, to, part; };
+// Keys whose parts are to be added up.
+struct KeyJoin { int key, keys, part, parts; };
+struct KeyPlan { int pieces, joins; };
+
+// Rows of a sequence that see a key: from ... to - 1.
+BW_DEV void rows_of_key(const PromptArgs& a, int nq, int nk, int key, int& from, int& to) {
+    auto row_at = [&](int64_t position) {
+        const int64_t r = (position - (nk - nq)) * a.share, rows = (int64_t)nq * a.share;
+        return (int)(r < 0 ? 0 : r < rows ? r : rows);
+    };
+    from = row_at(key);
+    to = key < a.sinks ? nq * a.share : row_at((int64_t)key + a.window);
+}
+// Tiles of rows that a tile of keys meets.
+BW_DEV void tiles_of_keys(const PromptArgs& a, int nq, int nk, int tile, int tile_rows, int& from, int& to) {
+    const int first = tile * kGradKeys, last = (first + kGradKeys < nk ? first + kGradKeys : nk) - 1;
+    int begin, end, other;
+    rows_of_key(a, nq, nk, first, begin, end);
+    rows_of_key(a, nq, nk, last, other, other);
+    end = end > other ? end : other;
+    from = begin / tile_rows;
+    to = end > begin ? (end - 1) / tile_rows + 1 : from;
+}
+
+constexpr int kPlanThreads = 256;
+// Sum of the threads' numbers before this one's, and of all.
+BW_DEV int sum_before(int* lds, int mine, int& all) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int other = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += other;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = sum;
+    __syncthreads();
+    int before = sum - mine;
+    all = 0;
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+        if (w < wave) before += lds[w];
+        all += lds[w];
+    }
+    return before;
+}
+
+// Every tile of keys in pieces of at most so many tiles of rows that there are about g.target pieces; by one workgroup.
+BW_DEV void plan_keys(const PromptGradArgs& g, char* smem, int tile_rows) {
+    int* lds = reinterpret_cast<int*>(smem);
+    unsigned long long& units = *reinterpret_cast<unsigned long long*>(smem + 64);
+    const int least = kLeastTiles;
+    const PromptArgs& a = g.p;
+    const int sequences = a.q_starts ? a.sequences + 2 : a.sequences, thread = (int)threadIdx.x;
+    auto tokens = [&](int s, Piece& p) {
+        if (a.q_starts) {
+            tokens_at(a.q_starts, s, a.sequences, a.q_tokens, p.q0, p.nq);
+            tokens_at(a.k_starts, s, a.sequences, a.k_tokens, p.k0, p.nk);
+            if (s >= a.sequences) p.nq = 0;
+        } else {
+            p.q0 = s * a.seq_q; p.nq = a.seq_q; p.k0 = s * a.seq_k; p.nk = a.seq_k;
+        }
+    };
+    int tiles = 0;
+    for (int base = 0; base < sequences; base += kPlanThreads) {
+        const int s = base + thread;
+        Piece p = {};
+        if (s < sequences) tokens(s, p);
+        int all;
+        const int before = tiles + sum_before(lds, (p.nk + kGradKeys - 1) / kGradKeys, all);
+        if (s < sequences) g.tiles_before[s] = before;
+        tiles += all;
+    }
+    if (thread == 0) units = 0;
+    __syncthreads();                                             // (and its fence: tiles_before is read below)
+    auto piece_of = [&](int n) {                                 // the n-th tile of keys
+        int lo = 0, hi = sequences;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (g.tiles_before[mid] <= n) lo = mid;
+            else hi = mid;
+        }
+        Piece p = {};
+        tokens(lo, p);
+        p.tile = n - g.tiles_before[lo];
+        tiles_of_keys(a, p.nq, p.nk, p.tile, tile_rows, p.from, p.to);
+        return p;
+    };
+    unsigned long long mine = 0;
+    for (int n = thread; n < tiles; n += kPlanThreads) {
+        const Piece p = piece_of(n);
+        mine += (unsigned)(p.to - p.from);
+    }
+    atomicAdd(&units, mine);                                     // (whole numbers: any order gives the same)
+    __syncthreads();
+    const unsigned long long each = (units + g.target - 1) / g.target;
+    const int size = each > (unsigned)least ? (int)each : least;
+    int pieces = 0, parts = 0, joins = 0;
+    for (int base = 0; base < tiles; base += kPlanThreads) {
+        const int n = base + thread;
+        Piece p = {};
+        int cuts = 0;
+        if (n < tiles) {
+            p = piece_of(n);
+            const int tiles_of_rows = p.to - p.from;
+            cuts = (tiles_of_rows - tiles_of_rows / 4 + size - 1) / size;        // (a third longer rather than cut: parts cost a way through memory)
+            if (cuts < 1) cuts = 1;
+        }
+        int all_pieces, all_parts, all_joins;
+        const int piece = pieces + sum_before(lds, cuts, all_pieces), part = parts + sum_before(lds, cuts > 1 ? cuts : 0, all_parts), join = joins + sum_before(lds, cuts > 1, all_joins);
+        const bool whole = cuts > 1 && (part + cuts > g.parts_room || join >= g.joins_room);
+        for (int c = 0; c < cuts && piece + c < g.room; c++) {
+            Piece one = p;
+            if (!whole) {
+                one.from = p.from + (int)((int64_t)(p.to - p.from) * c / cuts);
+                one.to = p.from + (int)((int64_t)(p.to - p.from) * (c + 1) / cuts);
+            } else if (c) {
+                one.nk = 0;                                      // nothing
+                one.to = one.from;
+            }
+            one.part = cuts > 1 && !whole ? part + c : -1;
+            g.pieces[piece + c] = one;
+        }
+        if (cuts > 1 && join < g.joins_room) g.joins[join] = whole ? KeyJoin{0, 0, 0, 0} : KeyJoin{p.k0 + p.tile * kGradKeys, p.nk - p.tile * kGradKeys < kGradKeys ? p.nk - p.tile * kGradKeys : kGradKeys, part, cuts};
+        pieces += all_pieces;
+        parts += all_parts;
+        joins += all_joins;
+    }
+    if (thread == 0) *g.plan = KeyPlan{pieces < g.room ? pieces : g.room, joins < g.joins_room ? joins : g.joins_room};
+}
+
+// Beside the queries' gradient, whose workgroups it is hidden among, the first workgroup lists the pieces of the keys' (on its own, in between: 14 us).
 template <class H>
 __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(PromptGradArgs g) {
     extern __shared__ __align__(1024) char smem[];               // [2][K, V]
@@ -71,7 +212,11 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     Span p;
     int head;
     uint32_t split;
-    if (!place_of<kRows, false>(a, blockIdx.x, p, head, split)) return;
+    if (g.plan && blockIdx.x == 0) {
+        plan_keys(g, smem, H::kKeys);
+        return;
+    }
+    if (!place_of<kRows, false>(a, g.plan ? blockIdx.x - 1 : blockIdx.x, p, head, split)) return;
     clear_tiles<H>(smem, 4 * H::kTileBytes, a.dim);
     const int row0 = p.tile * kRows + wave * kWaveRows, rows = p.nq * a.share;
     const Row row(a, p, row0 + (lane & 31));
@@ -248,36 +393,8 @@ __global__ __launch_bounds__(256) void prompt_query_join_kernel(PromptGradArgs g
 // both sums does not fit (64 registers of operands and 128 of sums leave too few: 283 TFLOP/s with 250 bytes of a lane in memory), and two waves that share S and P through LDS
 // wait for each other every 32 rows (8192 tokens, 32 and 8 heads of 128: 2068 us).
 //
-// Rows are cut into pieces of equal length, each a workgroup's: a small kernel lists them first (plan_keys_kernel), since a key that is seen by all rows meets many times the
+// Rows are cut into pieces of equal length, each a workgroup's: a workgroup lists them first (plan_keys), since a key that is seen by all rows meets many times the
 // rows of the last one.  The parts of keys that several workgroups have are added up in order by prompt_grad_join_kernel.
-constexpr int kGradKeys = 32 * kPromptWaves;
-
-// Tiles from ... to - 1 of rows (kKeys each) for the keys from kGradKeys tile on of a sequence; part: which of the parts they leave, or -1.
-struct Piece { int q0, nq, k0, nk, tile, from, to, part; };
-// Keys whose parts are to be added up.
-struct KeyJoin { int key, keys, part, parts; };
-struct KeyPlan { int pieces, joins; };
-
-// Rows of a sequence that see a key: from ... to - 1.
-BW_DEV void rows_of_key(const PromptArgs& a, int nq, int nk, int key, int& from, int& to) {
-    auto row_at = [&](int64_t position) {
-        const int64_t r = (position - (nk - nq)) * a.share, rows = (int64_t)nq * a.share;
-        return (int)(r < 0 ? 0 : r < rows ? r : rows);
-    };
-    from = row_at(key);
-    to = key < a.sinks ? nq * a.share : row_at((int64_t)key + a.window);
-}
-// Tiles of rows that a tile of keys meets.
-BW_DEV void tiles_of_keys(const PromptArgs& a, int nq, int nk, int tile, int tile_rows, int& from, int& to) {
-    const int first = tile * kGradKeys, last = (first + kGradKeys < nk ? first + kGradKeys : nk) - 1;
-    int begin, end, other;
-    rows_of_key(a, nq, nk, first, begin, end);
-    rows_of_key(a, nq, nk, last, other, other);
-    end = end > other ? end : other;
-    from = begin / tile_rows;
-    to = end > begin ? (end - 1) / tile_rows + 1 : from;
-}
-
 // Tiles of rows of a sequence (tokens x the query heads of one key head) on their way to LDS, one after the other; rows from the last on are the last one again.  Where a tile is
 // whole tokens, as it is for 1, 2, 4 ... query heads to a key head, a lane's place in it stays the same.
 template <class H> struct PackedLoader {
@@ -517,112 +634,6 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(Prom
     clear_tiles<H>(smem, 2 * kKeyStage<H>, a.dim);
     if (dk) key_grad<H, true>(g, p, (int)head, smem);
     else key_grad<H, false>(g, p, (int)head, smem);
-}
-
-// ---- the list of pieces ----
-
-constexpr int kPlanThreads = 1024;
-// Sum of the threads' numbers before this one's, and of all.
-BW_DEV int sum_before(int* lds, int mine, int& all) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int other = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += other;
-    }
-    __syncthreads();
-    if (lane == 63) lds[wave] = sum;
-    __syncthreads();
-    int before = sum - mine;
-    all = 0;
-    for (int w = 0; w < kPlanThreads / 64; w++) {
-        if (w < wave) before += lds[w];
-        all += lds[w];
-    }
-    return before;
-}
-
-// Every tile of keys in pieces of at most so many tiles of rows that there are about g.target pieces; one workgroup.
-static __global__ __launch_bounds__(kPlanThreads) void plan_keys_kernel(PromptGradArgs g, int tile_rows, int least) {
-    __shared__ int lds[kPlanThreads / 64];
-    __shared__ unsigned long long units;
-    const PromptArgs& a = g.p;
-    const int sequences = a.q_starts ? a.sequences + 2 : a.sequences, thread = (int)threadIdx.x;
-    auto tokens = [&](int s, Piece& p) {
-        if (a.q_starts) {
-            tokens_at(a.q_starts, s, a.sequences, a.q_tokens, p.q0, p.nq);
-            tokens_at(a.k_starts, s, a.sequences, a.k_tokens, p.k0, p.nk);
-            if (s >= a.sequences) p.nq = 0;
-        } else {
-            p.q0 = s * a.seq_q; p.nq = a.seq_q; p.k0 = s * a.seq_k; p.nk = a.seq_k;
-        }
-    };
-    int tiles = 0;
-    for (int base = 0; base < sequences; base += kPlanThreads) {
-        const int s = base + thread;
-        Piece p = {};
-        if (s < sequences) tokens(s, p);
-        int all;
-        const int before = tiles + sum_before(lds, (p.nk + kGradKeys - 1) / kGradKeys, all);
-        if (s < sequences) g.tiles_before[s] = before;
-        tiles += all;
-    }
-    if (thread == 0) units = 0;
-    __syncthreads();                                             // (and its fence: tiles_before is read below)
-    auto piece_of = [&](int n) {                                 // the n-th tile of keys
-        int lo = 0, hi = sequences;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (g.tiles_before[mid] <= n) lo = mid;
-            else hi = mid;
-        }
-        Piece p = {};
-        tokens(lo, p);
-        p.tile = n - g.tiles_before[lo];
-        tiles_of_keys(a, p.nq, p.nk, p.tile, tile_rows, p.from, p.to);
-        return p;
-    };
-    unsigned long long mine = 0;
-    for (int n = thread; n < tiles; n += kPlanThreads) {
-        const Piece p = piece_of(n);
-        mine += (unsigned)(p.to - p.from);
-    }
-    atomicAdd(&units, mine);                                     // (whole numbers: any order gives the same)
-    __syncthreads();
-    const unsigned long long each = (units + g.target - 1) / g.target;
-    const int size = each > (unsigned)least ? (int)each : least;
-    int pieces = 0, parts = 0, joins = 0;
-    for (int base = 0; base < tiles; base += kPlanThreads) {
-        const int n = base + thread;
-        Piece p = {};
-        int cuts = 0;
-        if (n < tiles) {
-            p = piece_of(n);
-            cuts = (p.to - p.from + size - 1) / size;
-            if (cuts < 1) cuts = 1;
-        }
-        int all_pieces, all_parts, all_joins;
-        const int piece = pieces + sum_before(lds, cuts, all_pieces), part = parts + sum_before(lds, cuts > 1 ? cuts : 0, all_parts), join = joins + sum_before(lds, cuts > 1, all_joins);
-        const bool whole = cuts > 1 && (part + cuts > g.parts_room || join >= g.joins_room);
-        for (int c = 0; c < cuts && piece + c < g.room; c++) {
-            Piece one = p;
-            if (!whole) {
-                one.from = p.from + (int)((int64_t)(p.to - p.from) * c / cuts);
-                one.to = p.from + (int)((int64_t)(p.to - p.from) * (c + 1) / cuts);
-            } else if (c) {
-                one.nk = 0;                                      // nothing
-                one.to = one.from;
-            }
-            one.part = cuts > 1 && !whole ? part + c : -1;
-            g.pieces[piece + c] = one;
-        }
-        if (cuts > 1 && join < g.joins_room) g.joins[join] = whole ? KeyJoin{0, 0, 0, 0} : KeyJoin{p.k0 + p.tile * kGradKeys, p.nk - p.tile * kGradKeys < kGradKeys ? p.nk - p.tile * kGradKeys : kGradKeys, part, cuts};
-        pieces += all_pieces;
-        parts += all_parts;
-        joins += all_joins;
-    }
-    if (thread == 0) *g.plan = KeyPlan{pieces < g.room ? pieces : g.room, joins < g.joins_room ? joins : g.joins_room};
 }
 
 // Gradients of the keys that lie in several parts: a workgroup has 1024 values of one join and head, [keys][2][dim].
