@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
             wait_tiles();
             if (next.i < end) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
-            const Seen which = seen(at);
+            const int which = seen(at);
             if (!careful && which == kNone) continue;
 #pragma unroll
             for (int b = 0; b < H::kKeyBlocks; b++) {
@@ -294,10 +294,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
                     float ds[16];
 #pragma unroll
                     for (int j = 0; j < 16; j++) ds[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], scale, -lse)) * (dp[j] - delta);
-                    if (which == kSome) {
-#pragma unroll
-                        for (int j = 0; j < 16; j++) ds[j] = sees(a, row.position, at + 32 * b + 8 * (j / 4) + 4 * half + j % 4) ? ds[j] : 0.f;
-                    }
+                    if (which != kAll) hide<16>(which, a, row.position, at + 32 * b + 4 * half, 0.f, ds);
                     if constexpr (DT == BW_F16) fit_reach<16, H::kBlocks>(ds, reach, acc, rest);
                     pack16<DT>(ds, w);
 #pragma unroll

@@ -331,8 +331,8 @@ template <class H> struct KeyWalk {
     }
 };
 
-// Which keys rows at positions low ... high see of N from `at` on: none, some, or all.
-enum Seen { kNone, kSome, kAll };
+// Which keys rows at positions low ... high see of N from `at` on: none, all, or without those that are later than some row, or that some row's window has left.
+enum Seen { kNone = -1, kAll = 0, kLater = 1, kLeft = 2 };
 template <int N> struct SeenOf {
     int none_above, all_to, window_from, sinks, all_from;
     BW_DEV SeenOf(const PromptArgs& a, int low, int high, bool any) {
@@ -342,11 +342,24 @@ template <int N> struct SeenOf {
         sinks = own(a.sinks);
         all_from = own(high - a.window + 1);
     }
-    BW_DEV Seen operator()(int at) const {
+    BW_DEV int operator()(int at) const {
         if (at > none_above || (at <= window_from && at >= sinks)) return kNone;
-        return at <= all_to && (at >= all_from || at + N <= sinks) ? kAll : kSome;
+        return (at > all_to ? kLater : 0) | (at < all_from && at + N > sinks ? kLeft : 0);
     }
 };
+// Values of a lane, for keys from + 8 (j / 4) + j % 4 and a row at `position`: `hidden` in place of those that the row does not see.
+template <int N> BW_DEV void hide(int which, const PromptArgs& a, int position, int from, float hidden, float* x) {
+    if (which & kLater) {
+        const int last = position - from;
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = 8 * (j / 4) + j % 4 <= last ? x[j] : hidden;
+    }
+    if (which & kLeft) {
+        const int left = position - a.window - from, sinks = a.sinks - from;
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = 8 * (j / 4) + j % 4 > left || 8 * (j / 4) + j % 4 < sinks ? x[j] : hidden;
+    }
+}
 BW_DEV bool sees(const PromptArgs& a, int position, int key) { return key <= position && (key > position - a.window || key < a.sinks); }
 
 // 16 bytes of a row for every step of 16 values of the head, zeros where there is nothing: an operand of the wave's rows.
@@ -461,7 +474,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
             wait_tiles();
             if (next.i < end) fetch(next);
             char* tile = smem + (i & 1) * 2 * H::kTileBytes;
-            const Seen which = seen(at);
+            const int which = seen(at);
             if constexpr (careful) {
                 if (which != kNone) add_nonfinite<H>(tile + H::kTileBytes, H::kKeys, lane, acc, [&](int n) { return sees(a, row.position, at + n); });
                 keep_finite<H>(tile + H::kTileBytes, H::kTileBytes);
@@ -469,27 +482,26 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
             if (which == kNone) continue;
             f16v s[H::kKeyBlocks];
 #pragma unroll
-            for (int b = 0; b < H::kKeyBlocks; b++) {
-                s[b] = f16v{};
+            for (int b = 0; b < H::kKeyBlocks; b++) s[b] = f16v{};
 #pragma unroll
-                for (int k = 0; k < H::kSteps; k++) s[b] = mfma32<DT>(read.rows(tile, b, k), q[k], s[b]);
-            }
+            for (int k = 0; k < H::kSteps; k++)
+#pragma unroll
+                for (int b = 0; b < H::kKeyBlocks; b++) s[b] = mfma32<DT>(read.rows(tile, b, k), q[k], s[b]);
             reads_ahead<H::kKeyBlocks * H::kSteps, 1, 4>();
             in_order();
             u4 v[H::kBlocks];
 #pragma unroll
             for (int m = 0; m < H::kBlocks; m++) v[m] = read.columns(tile + H::kTileBytes, 0, m);
-            if (which == kSome) {
+            if (which != kAll) {
 #pragma unroll
-                for (int b = 0; b < H::kKeyBlocks; b++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) s[b][j] = sees(a, row.position, at + 32 * b + 8 * (j / 4) + 4 * half + j % 4) ? s[b][j] : -INFINITY;
+                for (int b = 0; b < H::kKeyBlocks; b++) hide<16>(which, a, row.position, at + 32 * b + 4 * half, -INFINITY, reinterpret_cast<float*>(&s[b]));
             }
-            float top = s[0][0];
+            float tops[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
             for (int b = 0; b < H::kKeyBlocks; b++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) top = fmaxf(top, s[b][j]);
+                for (int j = b ? 0 : 4; j < 16; j++) tops[j / 4] = fmaxf(tops[j / 4], s[b][j]);
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top *= scale;
             if (__builtin_amdgcn_ballot_w64(top > r + kWeightMost<DT>)) {
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
