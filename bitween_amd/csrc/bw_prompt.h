@@ -2,8 +2,8 @@
 #pragma once
 #include "bw_prompt_kernel.h"
 
-int bw_launch_prompt_f16(const PromptArgs& a, uint32_t grid, hipStream_t stream);
-int bw_launch_prompt_bf16(const PromptArgs& a, uint32_t grid, hipStream_t stream);
+int bw_launch_prompt_f16(const PromptArgs& a, uint32_t grid, int groups, hipStream_t stream);
+int bw_launch_prompt_bf16(const PromptArgs& a, uint32_t grid, int groups, hipStream_t stream);
 
 // f(Head) for the smallest head that holds `dim` values.
 template <int DT, class F> static int with_head(int dim, F&& f) {
@@ -13,9 +13,9 @@ template <int DT, class F> static int with_head(int dim, F&& f) {
     return f(Head<DT, 256>{});
 }
 
-template <class H> static int launch_prompt(const PromptArgs& a, uint32_t grid, hipStream_t stream) {
+template <class H, int GROUPS> static int launch_prompt(const PromptArgs& a, uint32_t grid, hipStream_t stream) {
     static uint64_t done = 0;
-    if (!bw_allow_big_lds((const void*)prompt_forward_kernel<H>, done)) return BW_ELAUNCH;
-    hipLaunchKernelGGL(prompt_forward_kernel<H>, dim3(grid), dim3(256), 4 * H::kTileBytes, stream, a);
+    if (!bw_allow_big_lds((const void*)prompt_forward_kernel<H, GROUPS>, done)) return BW_ELAUNCH;
+    hipLaunchKernelGGL((prompt_forward_kernel<H, GROUPS>), dim3(grid), dim3(256), 4 * H::kTileBytes * GROUPS, stream, a);
     return hipGetLastError() == hipSuccess ? BW_OK : BW_ELAUNCH;
 }

@@ -95,12 +95,16 @@ PromptArgs args_of(const bw_prompt* p) {
 
 int key_tile(int dim) { return dim > 128 ? 32 : 64; }
 
-// Parts that the keys of a tile of rows are cut into: the number for which the longest workgroup (or, in several rounds, the mean of all), the second launch and the parts' way
-// through memory take the least together.  In microseconds, as measured: a tile of keys takes a workgroup 0.9 (heads of 64), 1.5 (128) and 2 (256, of half the keys), 1.4 times that
-// where two share a CU; the join 5, and its parts, written and read, go at 4 TB/s.  512 tokens of 8192, 32 and 8 heads of 128: 1 part 193 us, 2 110, 3 100, 4 88; 63 of 32063: 8 parts 106 us,
-// 16 63, 32 59, 48 70; 1024 tokens alone: 1 part 31 us, 2 41; 256 of 4096, heads of 64: 1 part 62 us, 4 25, 8 20, 16 26.  `times`: a tile of the queries' gradient takes 1.25 times as long.
-int splits_of(const bw_prompt* p, double times = 1.) {
-    const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), cus = bw_device_cus(), resident = cus * (p->dim > 128 ? 1 : 2);
+// Parts that the keys of a tile of rows are cut into, and waves' groups of a workgroup (see prompt_forward_kernel): what takes the least by this count, in microseconds, as measured.
+// A tile of keys takes a workgroup 0.9 (heads of 64), 1.5 (128) or 1.7 (256, of half the keys); where two share a CU, each a little more, both together 1.4 of that.  The workgroups'
+// longest, or the work of all, whichever is more; what they begin and end with; for parts the join, 5, and their way to memory and back at 4 TB/s.
+//   1 part, 1 group | 1 part, 2 groups | best parts, groups, us: 256 tokens, 32 heads of 128: 12.3, 9.7; 512: 17.9, 13.0; 1024 (8 key heads): 28.3, 25.7; 1536: 41.2, 48.1; 2048: 54.8, 71.6;
+//   128 of 2048: 48.5, 29.8, (4, 2) 20.2; 512 of 8192: 175, 107, (4, 1) 82.6; 63 of 32063: (8, 1) 95, (16, 1) 58, (32, 1) 56, (48, 1) 66; 256 of 4096, heads of 64: 59.9, 36.5, (4, 2) 18.1.
+// `times`: a tile of the queries' gradient, which has no groups, takes 1.25 times as long.
+struct Parts { int splits, groups; };
+Parts parts_of(const bw_prompt* p, double times = 1., bool may_group = true) {
+    const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), cus = bw_device_cus();
+    const bool two = p->dim <= 128;                                 // workgroups of one group to a CU
     const int64_t of = p->q_starts ? p->sequences : 1, tiles = (p->q_tokens * share + kRows - 1) / kRows;
     const int64_t row_tiles = p->q_starts ? (tiles > p->sequences ? tiles : p->sequences < p->q_tokens ? p->sequences : p->q_tokens) : p->sequences * tiles_of(p, p->q_tokens, share, kRows);
     const double blocks = (double)p->kv_heads * row_tiles;
@@ -111,17 +115,22 @@ int splits_of(const bw_prompt* p, double times = 1.) {
     const bool all = reach >= keys;
     if (!all) keys = reach;
     const double longest = (double)((keys + tile - 1) / tile), mean = all && keys > 0 ? longest * (1. - 0.5 * (rows < keys ? rows : keys) / keys) : longest;
-    const double one = times * (p->dim > 128 ? 2.0 : 0.3 + p->dim * 0.0094);
-    int best = 1;
+    const double one = times * (two ? 0.3 + p->dim * 0.0094 : 1.7);
+    Parts best = {1, 1};
     double least = 0.;
-    for (int s = 1; s <= 64 && (s == 1 || s * 2 <= longest); s++) {
-        const double rounds = blocks * s / resident, tiles_each = rounds > 1. && mean * rounds > longest ? mean * rounds : longest;
-        const double time = tiles_each / s * one * (blocks * s > cus && resident > cus ? 1.4 : 1.) + (s > 1 ? 5. + (double)p->q_tokens * p->q_heads * p->dim * 8. * s / 4e6 : 0.);
-        if (s == 1 || time < least) {
-            best = s;
-            least = s == 1 ? 0.9 * time : time;                      // (parts where they gain a tenth at least)
+    for (int groups = 1; groups <= (may_group ? 2 : 1); groups++)
+        for (int s = 1; s <= 64 && (s == 1 || s * 2 * groups <= longest); s *= 2) {
+            const bool share_cu = groups == 1 && two && blocks * s > cus;
+            const double rounds = groups * blocks * s / (cus * (groups == 1 && two ? 2 : 1));
+            const double last = longest / (s * groups) * one * (share_cu ? 1.05 : 1.), work = mean * blocks / cus * one * (share_cu ? 0.7 : 1.);
+            double time = (last > work ? last : work) + (groups == 1 ? 4. + (rounds > 1. ? rounds : 1.) : 2.5 + 4.5 * (rounds > 1. ? rounds : 1.));
+            if (s > 1) time += 5. + (double)p->q_tokens * p->q_heads * p->dim * 8. * s / 4e6;
+            const bool plain = s == 1 && groups == 1;
+            if (plain || time < least) {
+                best = Parts{s, groups};
+                least = plain ? 0.95 * time : time;                  // (anything else where it gains something)
+            }
         }
-    }
     return best;
 }
 
@@ -147,7 +156,7 @@ GradPlan grad_plan(const bw_prompt* p) {
         return at;
     };
     g.delta = room((size_t)(p->q_tokens * p->q_heads) * sizeof(float));
-    g.q_splits = p->q_tokens > 0 ? splits_of(p, 1.25) : 1;
+    g.q_splits = p->q_tokens > 0 ? parts_of(p, 1.25, false).splits : 1;
     if (g.q_splits > 1) g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
     if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
         g.target = (int)(((int64_t)bw_device_cus() * pieces_per_cu(p->dim) + p->kv_heads - 1) / p->kv_heads);
@@ -169,7 +178,7 @@ GradPlan grad_plan(const bw_prompt* p) {
 
 extern "C" size_t bw_prompt_attention_workspace_bytes(const bw_prompt* p) {
     if (prompt_check(p, BW_F16) != BW_OK || p->q_tokens == 0) return 0;
-    const int splits = splits_of(p);
+    const int splits = parts_of(p).splits;
     return splits > 1 ? (size_t)(p->q_tokens * p->q_heads) * splits * (p->dim + 2) * sizeof(float) : 0;
 }
 
@@ -187,8 +196,9 @@ extern "C" int bw_prompt_attention(const bw_prompt* p, int act_dtype, const void
     a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
     a.out = (uint16_t*)out;
     a.lse = lse;
-    a.set_splits(splits_of(p));
-    const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos * a.splits;
+    const Parts parts = parts_of(p);
+    a.set_splits(parts.splits);
+    const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows / parts.groups), grid = tiles * a.combos * a.splits;
     if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
     a.set_tiles((uint32_t)tiles);
     const size_t bytes = bw_prompt_attention_workspace_bytes(p);
@@ -198,7 +208,7 @@ extern "C" int bw_prompt_attention(const bw_prompt* p, int act_dtype, const void
         a.partial = (float*)workspace;
     }
     const hipStream_t st = (hipStream_t)stream;
-    if (int failed = act_dtype == BW_F16 ? bw_launch_prompt_f16(a, (uint32_t)grid, st) : bw_launch_prompt_bf16(a, (uint32_t)grid, st)) return failed;
+    if (int failed = act_dtype == BW_F16 ? bw_launch_prompt_f16(a, (uint32_t)grid, parts.groups, st) : bw_launch_prompt_bf16(a, (uint32_t)grid, parts.groups, st)) return failed;
     if (a.splits > 1) {
         const int threads = p->dim / 4;
         const uint32_t rows = (uint32_t)(p->q_tokens * p->q_heads), per = 256 / threads;

@@ -104,30 +104,31 @@ BW_DEV void wait_tiles() {
     asm volatile("" ::: "memory");
 }
 
-// A tile of rows of one head on its way to LDS.  Rows from `rows` on are those of the last one again (the mask hides them); values behind the head's end are not
+// TILES tiles of rows of one head on their way to LDS.  Rows from `rows` on are those of the last one again (the mask hides them); values behind the head's end are not
 // loaded.
-template <class H> struct RowLoader {
-    uint32_t row_bytes, bytes, chunk[H::kLoads], at;
+template <class H, int TILES = 1> struct RowLoader {
+    static constexpr int kLoads = H::kLoads * TILES, kKeys = H::kKeys * TILES;
+    uint32_t row_bytes, bytes, chunk[kLoads], at;
     int first, whole;                            // row of the lane in the first load; tiles with that many rows are whole ones
     BW_DEV RowLoader(const PromptArgs& a, int lane, int wave, int64_t row) {
         row_bytes = own((uint32_t)(row * 2));
         bytes = own((uint32_t)a.dim * 2);
-        whole = own(a.dim == H::kPitch ? H::kKeys : 0x7fffffff);
-        first = wave * H::kLoads * H::kLoadRows + lane / H::kChunks;
+        whole = own(a.dim == H::kPitch ? kKeys : 0x7fffffff);
+        first = wave * kLoads * H::kLoadRows + lane / H::kChunks;
         at = (uint32_t)first * row_bytes;
 #pragma unroll
-        for (int i = 0; i < H::kLoads; i++) chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(first + i * H::kLoadRows)) * 16;
+        for (int i = 0; i < kLoads; i++) chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(first + i * H::kLoadRows)) * 16;
     }
     BW_DEV void operator()(const void* base, int rows, uint32_t to, int wave) const {
-        to += wave * H::kLoads * 1024;
+        to += wave * kLoads * 1024;
         if (rows >= whole) {
 #pragma unroll
-            for (int i = 0; i < H::kLoads; i++) load_to_lds(base, at + i * H::kLoadRows * row_bytes + chunk[i], to + i * 1024);
+            for (int i = 0; i < kLoads; i++) load_to_lds(base, at + i * H::kLoadRows * row_bytes + chunk[i], to + i * 1024);
         } else {
             uint32_t some = bytes;
             asm("" : "+s"(some));                                // (the comparisons below are not kept in registers over the loop)
 #pragma unroll
-            for (int i = 0; i < H::kLoads; i++) {
+            for (int i = 0; i < kLoads; i++) {
                 const int r = first + i * H::kLoadRows;
                 if (chunk[i] < some) load_to_lds(base, (uint32_t)(r < rows ? r : rows - 1) * row_bytes + chunk[i], to + i * 1024);
             }
@@ -309,23 +310,24 @@ struct KeyTiles {
     }
 };
 // Keys and values of the tiles one after the other: what the next one's rows begin at.
-template <class H> struct KeyWalk {
+template <class H, int TILES = 1> struct KeyWalk {
+    static constexpr int kKeys = H::kKeys * TILES;
     const char *k, *v;
     uint32_t k_step, v_step;
     int at, i, jump_at, jump;
     BW_DEV KeyWalk(const PromptArgs& a, const Span& p, int head, const KeyTiles& tiles, int begin) {
         i = begin;
-        at = tiles[begin] * H::kKeys;
+        at = tiles[begin] * kKeys;
         jump_at = own(tiles.sinks);
         jump = own(tiles.first - tiles.sinks + 1);
-        k_step = own((uint32_t)(H::kKeys * 2 * a.k_row));        // (rows are 2^24 - 1 apart at most)
-        v_step = own((uint32_t)(H::kKeys * 2 * a.v_row));
+        k_step = own((uint32_t)(kKeys * 2 * a.k_row));        // (rows are 2^24 - 1 apart at most)
+        v_step = own((uint32_t)(kKeys * 2 * a.v_row));
         k = own((const char*)(a.k + (int64_t)(p.k0 + at) * a.k_row + head * a.k_head));
         v = own((const char*)(a.v + (int64_t)(p.k0 + at) * a.v_row + head * a.v_head));
     }
     BW_DEV void step() {
         const int by = ++i == jump_at ? jump : 1;
-        at += by * H::kKeys;
+        at += by * kKeys;
         k += (uint64_t)k_step * (uint32_t)by;
         v += (uint64_t)v_step * (uint32_t)by;
     }
@@ -417,17 +419,20 @@ template <class H> BW_DEV void clear_tiles(char* smem, int bytes, int dim) {
     __syncthreads();
 }
 
-template <class H>
+// GROUPS 2: half the rows to a workgroup, and two tiles of keys at a time, of which two waves have one each; what they sum for a row is added up at the end, through LDS.  Half the steps,
+// where there are few workgroups and their steps, one after the other, are what it takes (512 tokens, 32 heads of 128: 17.9 us, 13.0 so; with many workgroups the steps overlap without: 2048 tokens, 32 and 8 heads, 54.8, 71.6 so).
+template <class H, int GROUPS>
 __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(PromptArgs a) {
     extern __shared__ __align__(1024) char smem[];               // [2][K, V]
+    constexpr int kTileRows = kRows / GROUPS, kBytes = H::kTileBytes * GROUPS;
     constexpr int DT = H::kType;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5;
     Span p;
     int head;
     uint32_t split;
-    if (!place_of<kRows, false>(a, blockIdx.x, p, head, split)) return;
-    clear_tiles<H>(smem, 4 * H::kTileBytes, a.dim);
-    const int row0 = p.tile * kRows + wave * kWaveRows, rows = p.nq * a.share;
+    if (!place_of<kTileRows, false>(a, blockIdx.x, p, head, split)) return;
+    clear_tiles<H>(smem, 4 * kBytes, a.dim);
+    const int group = wave / (kPromptWaves / GROUPS), row0 = p.tile * kTileRows + wave % (kPromptWaves / GROUPS) * kWaveRows, rows = p.nq * a.share;
     const Row row(a, p, row0 + (lane & 31));
     const int64_t token = p.q0 + row.token;
     u4 q[H::kSteps];
@@ -438,22 +443,22 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
         for (int j = 0; j < 4; j++) q[s][j] ^= a.flip;
 
     int low, high, wave_low, wave_high;
-    positions_of(a, p, p.tile * kRows, (p.tile + 1) * kRows, low, high);
-    positions_of(a, p, row0 < rows ? row0 : p.tile * kRows, row0 + kWaveRows, wave_low, wave_high);
-    const KeyTiles tiles(a, low, high, p.nk, H::kKeys);
+    positions_of(a, p, p.tile * kTileRows, (p.tile + 1) * kTileRows, low, high);
+    positions_of(a, p, row0 < rows ? row0 : p.tile * kTileRows, row0 + kWaveRows, wave_low, wave_high);
+    const KeyTiles tiles(a, low, high, p.nk, H::kKeys * GROUPS);
     int begin, end;
     tiles.part(a, split, begin, end);
 
-    const RowLoader<H> load_k(a, lane, wave, a.k_row), load_v(a, lane, wave, a.v_row);
+    const RowLoader<H, GROUPS> load_k(a, lane, wave, a.k_row), load_v(a, lane, wave, a.v_row);
     const TileReader<H> read(lane);
     const SeenOf<H::kKeys> seen(a, wave_low, wave_high, row0 < rows);
     const uint32_t lds = own(lds_address(smem));
     const int keys = own(p.nk);
     const float scale = own(a.scale);
-    auto fetch = [&](const KeyWalk<H>& next) __attribute__((always_inline)) {
-        const uint32_t to = lds + (next.i & 1) * 2 * H::kTileBytes;
+    auto fetch = [&](const KeyWalk<H, GROUPS>& next) __attribute__((always_inline)) {
+        const uint32_t to = lds + (next.i & 1) * 2 * kBytes;
         load_k(next.k, keys - next.at, to, wave);
-        load_v(next.v, keys - next.at, to + H::kTileBytes, wave);
+        load_v(next.v, keys - next.at, to + kBytes, wave);
     };
 
     f16v acc[H::kBlocks];
@@ -466,18 +471,18 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         r = kLowestScore;
         l = 0.f;
-        KeyWalk<H> next(a, p, head, tiles, begin);
+        KeyWalk<H, GROUPS> next(a, p, head, tiles, begin);
         if (begin < end) fetch(next);
         for (int i = begin; i < end; i++) {
-            const int at = next.at;
+            const int at = next.at + group * H::kKeys;
             next.step();
             wait_tiles();
             if (next.i < end) fetch(next);
-            char* tile = smem + (i & 1) * 2 * H::kTileBytes;
+            char *stage = smem + (i & 1) * 2 * kBytes, *tile = stage + group * H::kTileBytes, *values = tile + kBytes;
             const int which = seen(at);
             if constexpr (careful) {
-                if (which != kNone) add_nonfinite<H>(tile + H::kTileBytes, H::kKeys, lane, acc, [&](int n) { return sees(a, row.position, at + n); });
-                keep_finite<H>(tile + H::kTileBytes, H::kTileBytes);
+                if (which != kNone) add_nonfinite<H>(values, H::kKeys, lane, acc, [&](int n) { return sees(a, row.position, at + n); });
+                keep_finite<H>(stage + kBytes, kBytes);
             }
             if (which == kNone) continue;
             f16v s[H::kKeyBlocks];
@@ -491,7 +496,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
             in_order();
             u4 v[H::kBlocks];
 #pragma unroll
-            for (int m = 0; m < H::kBlocks; m++) v[m] = read.columns(tile + H::kTileBytes, 0, m);
+            for (int m = 0; m < H::kBlocks; m++) v[m] = read.columns(values, 0, m);
             if (which != kAll) {
 #pragma unroll
                 for (int b = 0; b < H::kKeyBlocks; b++) hide<16>(which, a, row.position, at + 32 * b + 4 * half, -INFINITY, reinterpret_cast<float*>(&s[b]));
@@ -529,7 +534,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
                 u4 next_v[H::kBlocks], next_w;
                 if (step + 1 < 2 * H::kKeyBlocks) {
 #pragma unroll
-                    for (int m = 0; m < H::kBlocks; m++) next_v[m] = read.columns(tile + H::kTileBytes, step + 1, m);
+                    for (int m = 0; m < H::kBlocks; m++) next_v[m] = read.columns(values, step + 1, m);
                     next_w = weights(step + 1);
                 }
                 // (the sum of the weights as they are multiplied, two at a time: what their rounding adds to the values it takes off again)
@@ -556,6 +561,33 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     if (any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc))) pass(std::true_type{});
 
     l += __shfl_xor(l, 32, 64);
+    if constexpr (GROUPS > 1) {
+        static_assert(GROUPS == 2, "two");
+        char* other = smem + wave % 2 * (H::kBlocks * 4096 + 512);
+        __syncthreads();
+        if (group) {
+#pragma unroll
+            for (int m = 0; m < H::kBlocks; m++)
+#pragma unroll
+                for (int b = 0; b < 4; b++) *reinterpret_cast<f4*>(other + ((4 * m + b) * 64 + lane) * 16) = f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]};
+            reinterpret_cast<float*>(other + H::kBlocks * 4096)[lane] = r;
+            reinterpret_cast<float*>(other + H::kBlocks * 4096)[64 + lane] = l;
+        }
+        __syncthreads();
+        if (group) return;
+        const float r2 = reinterpret_cast<float*>(other + H::kBlocks * 4096)[lane], l2 = reinterpret_cast<float*>(other + H::kBlocks * 4096)[64 + lane];
+        const float top = fmaxf(r, r2), f1 = __builtin_amdgcn_exp2f(r - top), f2 = __builtin_amdgcn_exp2f(r2 - top);
+        r = top;
+        l = l * f1 + l2 * f2;
+#pragma unroll
+        for (int m = 0; m < H::kBlocks; m++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const f4 x = *reinterpret_cast<const f4*>(other + ((4 * m + b) * 64 + lane) * 16);
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[m][4 * b + i] = acc[m][4 * b + i] * f1 + x[i] * f2;
+            }
+    }
     if (!row.live) return;
     const int64_t index = (int64_t)head * a.q_tokens * a.share + token * a.share + row.head;       // of the row among all
     if (a.splits > 1) {                                           // (see prompt_join_kernel)

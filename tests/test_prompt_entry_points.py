@@ -186,7 +186,7 @@ def test_prompt_and_window_kernels_keep_their_values_in_registers():
     kernels = list(_kernel_metadata(hip_loader.library_path()))
     rows = [k for k in kernels if "prompt_forward" in k[".name"]]
     grads = [k for k in kernels if "prompt_query_grad" in k[".name"] or "prompt_key_grad" in k[".name"]]
-    assert len(rows) == 8 and len(grads) == 16                   # by type, and heads up to 64, 96, 128, 256
+    assert len(rows) == 16 and len(grads) == 16                  # by type, and heads up to 64, 96, 128, 256; one group of waves, or two
     assert not any(k[".private_segment_fixed_size"] for k in rows)
     for k in grads:
         assert k[".private_segment_fixed_size"] <= (256 if "Li256E" in k[".name"] else 32), k[".name"]
