@@ -100,7 +100,7 @@ int key_tile(int dim) { return dim > 128 ? 32 : 64; }
 // longest, or the work of all, whichever is more; what they begin and end with; for parts the join, 5, and their way to memory and back at 4 TB/s.
 //   1 part, 1 group | 1 part, 2 groups | best parts, groups, us: 256 tokens, 32 heads of 128: 12.3, 9.7; 512: 17.9, 13.0; 1024 (8 key heads): 28.3, 25.7; 1536: 41.2, 48.1; 2048: 54.8, 71.6;
 //   128 of 2048: 48.5, 29.8, (4, 2) 20.2; 512 of 8192: 175, 107, (4, 1) 82.6; 63 of 32063: (8, 1) 95, (16, 1) 58, (32, 1) 56, (48, 1) 66; 256 of 4096, heads of 64: 59.9, 36.5, (4, 2) 18.1.
-// `times`: a tile of the queries' gradient, which has no groups, takes 1.25 times as long.
+// `times`: a tile of the queries' gradient, which has no groups, takes 1.5 times as long.
 struct Parts { int splits, groups; };
 Parts parts_of(const bw_prompt* p, double times = 1., bool may_group = true) {
     const int share = p->q_heads / p->kv_heads, tile = key_tile(p->dim), cus = bw_device_cus();
@@ -156,7 +156,7 @@ GradPlan grad_plan(const bw_prompt* p) {
         return at;
     };
     g.delta = room((size_t)(p->q_tokens * p->q_heads) * sizeof(float));
-    g.q_splits = p->q_tokens > 0 ? parts_of(p, 1.25, false).splits : 1;
+    g.q_splits = p->q_tokens > 0 ? parts_of(p, 1.5, false).splits : 1;
     if (g.q_splits > 1) g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
     if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
         g.target = (int)(((int64_t)bw_device_cus() * pieces_per_cu(p->dim) + p->kv_heads - 1) / p->kv_heads);

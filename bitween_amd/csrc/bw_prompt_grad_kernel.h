@@ -7,9 +7,8 @@
 // is each row's (each key's) own: it starts high and comes down where a product would pass 2^15, and the sums with it.
 //
 // A row's dS add up to zero, but for what dS and the output (in delta) were rounded by: a remainder e, which puts e times the mean of the keys into dQ.  Keys are projected with
-// channels far from zero, so that this was the larger part of dQ's error (8192 tokens, bfloat16, channels at 2 to 6 of keys that spread by 1: 0.0045 of dQ, 0.0023 without it).
-// dQ = scale dS (K - c) for any c: e is summed as the product takes it, and e c taken off, c the mean of 32 keys that all of a
-// wave's rows see, nearer to zero where these are fewer (one key says little of the mean).
+// channels far from zero, so that this was the larger part of dQ's error (8192 tokens, bfloat16, channels at 2 to 6 of keys that spread by 1: 0.0045 of dQ, 0.0024 without it; 2 tokens: 0.0060 and 0.0025).
+// dQ = scale dS (K - c) for any c: e is summed as the product takes it, and e c taken off, c the mean of the last 32 keys that a row sees.
 #pragma once
 #include "bw_prompt_kernel.h"
 
@@ -315,50 +314,71 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         }
     };
     pass(std::false_type{});
-    if (any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc))) pass(std::true_type{});
-    char* mean = smem + wave * H::kPitch * 4;                    // (any_thread's barrier: the tiles are done with)
-    {
-        const int to = wave_low + 1, lowest = wave_low - 31 > wave_high - a.window + 1 ? wave_low - 31 : wave_high - a.window + 1, from = lowest > 0 ? lowest : 0;
-        const int d = lane % H::kChunks * 8;
-        float c[8] = {};
-        if (d < a.dim) {
-            const uint16_t* key = a.k + (int64_t)p.k0 * a.k_row + head * a.k_head + d;
-#pragma unroll 4
-            for (int n = from + lane / H::kChunks; n < to; n += H::kLoadRows) {
-                const u4 w = *reinterpret_cast<const u4*>(key + n * a.k_row);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    c[2 * j] = __builtin_fmaf(widen16<DT>((uint16_t)w[j]), 1.f / 32.f, c[2 * j]);
-                    c[2 * j + 1] = __builtin_fmaf(widen16<DT>((uint16_t)(w[j] >> 16)), 1.f / 32.f, c[2 * j + 1]);
-                }
-            }
-        }
-#pragma unroll
-        for (int o = H::kChunks; o < 64; o <<= 1)
-#pragma unroll
-            for (int j = 0; j < 8; j++) c[j] += __shfl_xor(c[j], o, 64);
-        if (lane < H::kChunks) {
-            *reinterpret_cast<f4*>(mean + d * 4) = f4{c[0], c[1], c[2], c[3]};
-            *reinterpret_cast<f4*>(mean + d * 4 + 16) = f4{c[4], c[5], c[6], c[7]};
-        }
-    }
-    __syncthreads();
-    if (!row.live) return;
+    const bool some = any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc));
+    if (some) pass(std::true_type{});
     rest += __shfl_xor(rest, 32, 64);
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
     float* part = a.splits > 1 ? g.q_parts + (index * a.splits + split) * a.dim : nullptr;
+    // c: of each row the mean of the last 32 keys at most that it sees, by a product with weights of 1 / 32; of the up to 63 keys of a wave's rows in two steps.  Infinities and NaN
+    // are left out, where there are any: each of these keys is seen by a row of the wave, and a row that sees one has no finite result.
+    __syncthreads();
+    char* mine = smem + wave * 32 * H::kPitch * 2;
+    const int last = row.position, windowed = last - a.window + 1, from = windowed > last - 31 ? windowed > 0 ? windowed : 0 : last > 31 ? last - 31 : 0;
+    const int lowest = wave_low - (a.window < 32 ? a.window : 32) + 1, first_key = lowest > 0 ? lowest : 0, chunk = lane % H::kChunks;
+    const float one = last >= from ? 1.f / (float)(last - from + 1) : 0.f;
+    constexpr int kAtOnce = H::kBlocks < 4 ? H::kBlocks : 4;
 #pragma unroll
-    for (int m = 0; m < H::kBlocks; m++)
+    for (int m0 = 0; m0 < H::kBlocks; m0 += kAtOnce) {
+        f16v mean[kAtOnce];
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            const int d = 32 * m + 8 * b + 4 * half;
-            const f4 c = *reinterpret_cast<const f4*>(mean + d * 4);
-            const f4 x = (f4{acc[m][4 * b], acc[m][4 * b + 1], acc[m][4 * b + 2], acc[m][4 * b + 3]} - rest * c) * back * g.plain_scale;
-            if (d >= a.dim) continue;
-            if (part) *reinterpret_cast<f4*>(part + d) = x;
-            else store4<DT>(out + d, x[0], x[1], x[2], x[3]);
+        for (int m = 0; m < kAtOnce; m++) mean[m] = f16v{};
+#pragma unroll 1
+        for (int base = first_key; base <= first_key + 32; base += 32) {
+#pragma unroll
+            for (int i = 0; i < 32 / H::kLoadRows; i++) {
+                const int n = i * H::kLoadRows + lane / H::kChunks;
+                u4 v = {0, 0, 0, 0};
+                if (base + n <= wave_high && chunk * 8 < a.dim) v = *reinterpret_cast<const u4*>(a.k + (int64_t)(p.k0 + base + n) * a.k_row + head * a.k_head + chunk * 8);
+                if (some) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t w = v[j];
+                        v[j] = (finite16<DT>(w) ? w & 0xFFFFu : 0u) | (finite16<DT>(w >> 16) ? w & 0xFFFF0000u : 0u);
+                    }
+                }
+                *reinterpret_cast<u4*>(mine + n * H::kPitch * 2 + (chunk ^ swizzle<H::kPitch>(n)) * 16) = v;
+            }
+            __syncthreads();
+            float x[16];
+            u4 w[2];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int key = base + 8 * (j / 4) + 4 * half + j % 4;
+                x[j] = key >= from && key <= last ? one : 0.f;
+            }
+            pack16<DT>(x, w);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int m = 0; m < kAtOnce; m++) mean[m] = mfma32<DT>(read.columns(mine, t, m0 + m), w[t], mean[m]);
+            __syncthreads();
         }
+        if (row.live) {
+#pragma unroll
+            for (int m = 0; m < kAtOnce; m++)
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const int d = 32 * (m0 + m) + 8 * b + 4 * half;
+                    f4 x;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = (acc[m0 + m][4 * b + i] - rest * mean[m][4 * b + i]) * back * g.plain_scale;
+                    if (d >= a.dim) continue;
+                    if (part) *reinterpret_cast<f4*>(part + d) = x;
+                    else store4<DT>(out + d, x[0], x[1], x[2], x[3]);
+                }
+        }
+    }
 }
 
 // dQ = the parts of a row added up in order; a thread has 4 values of a row, and 8 parts under way.
