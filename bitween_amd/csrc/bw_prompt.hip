@@ -96,7 +96,7 @@ PromptArgs args_of(const bw_prompt* p) {
 int key_tile(int dim) { return dim > 128 ? 32 : 64; }
 
 // Parts that the keys of a tile of rows are cut into, and waves' groups of a workgroup (see prompt_forward_kernel): what takes the least by this count, in microseconds, as measured.
-// A tile of keys takes a workgroup 0.9 (heads of 64), 1.5 (128) or 1.7 (256, of half the keys); where two share a CU, each a little more, both together 1.4 of that.  The workgroups'
+// A tile of keys takes a workgroup 0.9 (heads of 64), 1.36 (96), 1.5 (128) or 1.7 (256, of half the keys); where two share a CU, each a little more, both together 1.4 of that.  The workgroups'
 // longest, or the work of all, whichever is more; what they begin and end with; for parts the join, 5, and their way to memory and back at 4 TB/s.
 //   1 part, 1 group | 1 part, 2 groups | best parts, groups, us: 256 tokens, 32 heads of 128: 12.3, 9.7; 512: 17.9, 13.0; 1024 (8 key heads): 28.3, 25.7; 1536: 41.2, 48.1; 2048: 54.8, 71.6;
 //   128 of 2048: 48.5, 29.8, (4, 2) 20.2; 512 of 8192: 175, 107, (4, 1) 82.6; 63 of 32063: (8, 1) 95, (16, 1) 58, (32, 1) 56, (48, 1) 66; 256 of 4096, heads of 64: 59.9, 36.5, (4, 2) 18.1.
@@ -115,7 +115,7 @@ Parts parts_of(const bw_prompt* p, double times = 1., bool may_group = true) {
     const bool all = reach >= keys;
     if (!all) keys = reach;
     const double longest = (double)((keys + tile - 1) / tile), mean = all && keys > 0 ? longest * (1. - 0.5 * (rows < keys ? rows : keys) / keys) : longest;
-    const double one = times * (two ? 0.3 + p->dim * 0.0094 : 1.7);
+    const double one = times * (p->dim <= 64 ? 0.9 : p->dim <= 96 ? 1.36 : two ? 1.5 : 1.7);
     Parts best = {1, 1};
     double least = 0.;
     for (int groups = 1; groups <= (may_group ? 2 : 1); groups++)
