@@ -1,14 +1,17 @@
-"""What stands between the quantized linears of a decoder layer: rotation of queries and keys (with the norm of each head), a paged
-key-value cache that may hold 8- or 4-bit codes, and the attention of one new token over it.
+"""What stands between the quantized linears of a decoder layer: rotation of queries and keys (with the norm of each head, by one position of a token or by several), a paged
+key-value cache that may hold 8- or 4-bit codes, the attention of one new token over it, and that of many (prompts, training); attention over all tokens or a sliding window and sinks.
 
-    q, k = rotate_heads(q, k, cos, sin, positions)
+    q, k = rotate_heads(q, k, cos, sin, positions)                 # prompts, training
+    out = prompt_attention(q, k, v, starts, window=1024, sinks=4)
     cache.write(k, v, slots)
-    out = cache.attend(q, page_table, lengths)
+
+    q = cache.append(q, k, v, cos, sin, positions, slots)          # a decode step: rotation and cache write in one
+    out = cache.attend(q, page_table, lengths, window=1024, sinks=4)
 
 Each is one HIP kernel of libbitween_hip.so (the attention is joined by a second one where a sequence is cut, and so are the gradients of norm
-weights); they run on torch's current stream, allocate their outputs and workspaces from its allocator, and can be captured in HIP
-graphs.  Cache and attention have no derivatives: under grad mode a tensor that asks for gradients raises, a forward-mode tangent always (for the
-rotation too).  There is no CPU path: CPU tensors raise.  The reference has no counterpart; its models bring these as eager torch operations.
+weights; the gradients of prompt_attention are two, or three); they run on torch's current stream, allocate their outputs and workspaces from its allocator, and can be captured in HIP
+graphs.  rotate_heads and prompt_attention have gradients and no second derivatives; the cache and its attention have none: under grad mode a tensor that asks for gradients raises, a
+forward-mode tangent always (for all of them).  There is no CPU path: CPU tensors raise.  The reference has no counterpart; its models bring these as eager torch operations.
 """
 import operator
 

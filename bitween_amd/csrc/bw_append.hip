@@ -5,6 +5,9 @@
 // thread leaves its chunks' extrema in LDS, where a head's chunks lie in order, and reads those of its groups; a head never leaves its wave, so that nothing
 // waits but the wave.
 //
+// One pass over memory: launch-bound up to a few hundred tokens (one token 2.4 us; 64 with norms into 8 bits 4.7), HBM beyond: 8191 tokens of 32 and 8 heads of 128 by three axes into 4 bits
+// 38 us (177 MB, 4.7 TB/s; 59 with one head to a thread, which loads its angles from three rows of the tables for each).
+//
 // The codes hang on the rotated key's last bit next to a border, so what goes into it is kept reproducible: the sum of squares and its root are float64
 // (whose order no longer shows), the rest are single float32 operations.  64-bit operations cost what 32-bit ones do here, twice over, and memory is waited for either way.
 #include "bw_rotate.h"

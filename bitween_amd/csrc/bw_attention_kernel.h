@@ -36,6 +36,10 @@
 // divided by it at the end.  P itself stays float32, and so do r and l.  (With one reference for all groups of a token a group 2^-10 of the largest
 // erred by 2^-10.  The reach and its vote for each group cost 1 ... 4 % with heads of 128, 9 % with 16 queries over groups of 32 in 8 bits, 18 % with four groups
 // of 64 to a head.)
+//
+// Over a window (window_kernel, the same body): a segment's tiles are those of its sinks and those from the window's first token on, and only where a tile's tokens do not all count is each looked at.
+// One sequence of 131072 tokens that sees 4096 and 4 sinks, 32 and 8 heads of 128, 16 bits: 9.9 us and 3.4 for the join (17 MB, 3.3 us: latency); 48 sequences that see 2000 in 8 bits: 38 and 4.7 us
+// (185 MB, 4.9 TB/s); 128 that see 500, 12 heads of 64 in 4 bits: 24 us (48 MB: the issue of instructions, as without a window).
 #pragma once
 #include "bw_cache.h"
 

@@ -9,6 +9,9 @@
 // A row's dS add up to zero, but for what dS and the output (in delta) were rounded by: a remainder e, which puts e times the mean of the keys into dQ.  Keys are projected with
 // channels far from zero, so that this was the larger part of dQ's error (8192 tokens, bfloat16, channels at 2 to 6 of keys that spread by 1: 0.0045 of dQ, 0.0024 without it; 2 tokens: 0.0060 and 0.0025).
 // dQ = scale dS (K - c) for any c: e is summed as the product takes it, and e c taken off, c the mean of the last 32 keys that a row sees.
+//
+// What bounds them is what bounds the forward; matrix cores busy 51 % (dQ) and 45 % (dK, dV), vector unit 41 and 35 %.  8192 tokens, 32 and 8 heads of 128, bfloat16: dQ 767 us (1075 TFLOP/s of its three
+// products), dK and dV 1370 (1000 of their five), 2140 in all.
 #pragma once
 #include "bw_prompt_kernel.h"
 

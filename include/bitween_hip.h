@@ -371,7 +371,7 @@ int bw_prompt_attention(const bw_prompt* prompt, int act_dtype, const void* q, i
  * q, k, v, out and lse as the forward had and left them.  With P the weights: dV = P^T grad, dS = P (grad V^T - rowsum(grad out)), dQ = scale dS K, dK = scale dS^T Q; all sums
  * float32, each in one order (the same inputs give the same bits); P and dS enter their second products rounded once to act_dtype (in float16 as a power of two times that of
  * their row or key, so that small gradients keep their bits).  Rows of k and v that belong to no sequence get zeros; what an infinity or a NaN of one token touches is what
- * sees it, or what it sees.
+ * sees it, or what it sees.  A row's dS add up to zero but for roundings: what theirs add up to is taken off with the mean of the last 32 keys at most that the row sees.
  * Beside the forward's: rows of q and grad 0 ... 2^24 - 1 elements apart, a key head's query heads and 65 rows within 2^31 elements; a workspace of
  * bw_prompt_attention_grad_workspace_bytes(...) bytes (16-byte aligned). */
 size_t bw_prompt_attention_grad_workspace_bytes(const bw_prompt* prompt);
