@@ -30,7 +30,7 @@ struct PromptGradArgs {
     int* tiles_before;                           // of sequence s: where its tiles of keys begin
     float* parts;
     int target;                                  // pieces (of one head) that the rows are cut into, about
-    int room, parts_room, joins_room;            // of the lists (starts that decrease could ask for more: tiles of keys are then left out, or not cut)
+    int room, parts_room, joins_room;            // of the lists
 };
 
 constexpr int kFirstReach16 = 80, kReachTop = 12, kReachMost = 15, kWeightShift = 12;
@@ -136,18 +136,25 @@ BW_DEV void plan_keys(const PromptGradArgs& g, char* smem, int tile_rows) {
             p.q0 = s * a.seq_q; p.nq = a.seq_q; p.k0 = s * a.seq_k; p.nk = a.seq_k;
         }
     };
+    int& decreases = *reinterpret_cast<int*>(smem + 72);
+    if (thread == 0) {
+        units = 0;
+        decreases = 0;
+    }
+    __syncthreads();
     int tiles = 0;
     for (int base = 0; base < sequences; base += kPlanThreads) {
         const int s = base + thread;
         Piece p = {};
         if (s < sequences) tokens(s, p);
+        if (a.q_starts && s < a.sequences && start_at(a.k_starts, s + 1, a.k_tokens) < start_at(a.k_starts, s, a.k_tokens)) decreases = 1;
         int all;
         const int before = tiles + sum_before(lds, (p.nk + kGradKeys - 1) / kGradKeys, all);
         if (s < sequences) g.tiles_before[s] = before;
         tiles += all;
     }
-    if (thread == 0) units = 0;
     __syncthreads();                                             // (and its fence: tiles_before is read below)
+    if (decreases) tiles = 0;                                    // (the same tokens over and over, more than can be counted: no gradients then)
     auto piece_of = [&](int n) {                                 // the n-th tile of keys
         int lo = 0, hi = sequences;
         while (hi - lo > 1) {
