@@ -257,6 +257,7 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     g.q_grad = (uint16_t*)q_grad; g.k_grad = (uint16_t*)k_grad; g.v_grad = (uint16_t*)v_grad;
     g.delta = (float*)workspace;
     a.set_splits(q_grad ? plan.q_splits : 1);
+    g.exact = plan.q_splits == 1 && (q_grad || k_grad);             // (the same for dK, whichever other gradients are wanted)
     g.q_parts = a.splits > 1 ? (float*)((char*)workspace + plan.q_parts) : nullptr;
     g.plain_scale = p->scale;
     PromptGrids grids = {};

@@ -9,6 +9,8 @@
 // A row's dS add up to zero, but for what dS and the output (in delta) were rounded by: a remainder e, which puts e times the mean of the keys into dQ.  Keys are projected with
 // channels far from zero, so that this was the larger part of dQ's error (8192 tokens, bfloat16, channels at 2 to 6 of keys that spread by 1: 0.0045 of dQ, 0.0024 without it; 2 tokens: 0.0060 and 0.0025).
 // dQ = scale dS (K - c) for any c: e is summed as the product takes it, and e c taken off, c the mean of the last 32 keys that a row sees.
+// What the dS add up to before they are rounded is what the rounded output is off by in delta (the weights of a row add up to 1): the rows' kernel sees all keys, where they are not cut into
+// parts, and hands delta on to dK without it (dK's error, 2 tokens: 0.0039 with it, 0.0024 without).
 //
 // What bounds them is what bounds the forward; matrix cores busy 51 % (dQ) and 45 % (dK, dV), vector unit 41 and 35 %.  8192 tokens, 32 and 8 heads of 128, bfloat16: dQ 767 us (1075 TFLOP/s of its three
 // products), dK and dV 1370 (1000 of their five), 2140 in all.
@@ -20,6 +22,7 @@ struct PromptGradArgs {
     const uint16_t *grad, *result;               // of the output; result [tokens][q_heads][dim]
     int64_t grad_row, grad_head;
     float* delta;                                // its negative, as lse
+    int exact;                                   // delta is that of the weights, not of the rounded result (see below)
     uint16_t *q_grad, *k_grad, *v_grad;
     float* q_parts;                              // where a row's keys are cut into p.splits parts: [row][part][dim]
     float plain_scale;
@@ -213,7 +216,7 @@ BW_DEV void plan_keys(const PromptGradArgs& g, char* smem, int tile_rows) {
 
 // Beside the queries' gradient, whose workgroups it is hidden among, the first workgroup lists the pieces of the keys' (on its own, in between: 14 us).
 template <class H>
-__global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(PromptGradArgs g) {
+__global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void prompt_query_grad_kernel(PromptGradArgs g) {
     extern __shared__ __align__(1024) char smem[];               // [2][K, V]
     constexpr int DT = H::kType;
     const PromptArgs& a = g.p;
@@ -249,8 +252,8 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
         }
         delta += __shfl_xor(delta, 32, 64);
     }
-    if (row.live && half == 0 && split == 0) g.delta[index] = -delta;
-    if (!g.q_grad) return;
+    if (!g.exact && row.live && half == 0 && split == 0) g.delta[index] = -delta;
+    if (!g.q_grad && !g.exact) return;
     const float lse = row.live ? a.lse[index] : INFINITY;
 
     int low, high, wave_low, wave_high;
@@ -273,13 +276,13 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
 
     f16v acc[H::kBlocks];
     int reach = 0;
-    float rest = 0.f;                                            // sum of the dS, as rounded
+    float rest = 0.f, left = 0.f;                                // sums of the dS, as rounded and before
     auto pass = [&](auto is_careful) __attribute__((always_inline)) {       // (see prompt_forward_kernel)
         constexpr bool careful = decltype(is_careful)::value;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
-        rest = 0.f;
+        rest = left = 0.f;
         KeyWalk<H> next(a, p, head, tiles, begin);
         if (begin < end) fetch(next);
         for (int i = begin; i < end; i++) {
@@ -304,6 +307,8 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
 #pragma unroll
                     for (int j = 0; j < 16; j++) ds[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], scale, -lse)) * (dp[j] - delta);
                     if (which != kAll) hide<16>(which, a, row.position, at + 32 * b + 4 * half, 0.f, ds);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) left += ds[j];
                     if constexpr (DT == BW_F16) fit_reach<16, H::kBlocks>(ds, reach, acc, rest);
                     pack16<DT>(ds, w);
 #pragma unroll
@@ -327,6 +332,11 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_query_grad_kernel(Pr
     const bool some = any_thread(smem, wave, row.live && not_finite<H::kBlocks>(acc));
     if (some) pass(std::true_type{});
     rest += __shfl_xor(rest, 32, 64);
+    left += __shfl_xor(left, 32, 64);
+    if (g.exact) {
+        if (row.live && half == 0) g.delta[index] = -(delta + left);
+        if (!g.q_grad) return;
+    }
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
     float* part = a.splits > 1 ? g.q_parts + (index * a.splits + split) * a.dim : nullptr;
