@@ -432,48 +432,57 @@ __global__ __launch_bounds__(256) void prompt_query_join_kernel(PromptGradArgs g
 //
 // Rows are cut into pieces of equal length, each a workgroup's: a workgroup lists them first (plan_keys), since a key that is seen by all rows meets many times the
 // rows of the last one.  The parts of keys that several workgroups have are added up in order by prompt_grad_join_kernel.
-// Tiles of rows of a sequence (tokens x the query heads of one key head) on their way to LDS, one after the other; rows from the last on are the last one again.  Where a tile is
+// Tiles of rows of a sequence (tokens x the query heads of one key head) on their way to LDS; rows from the last on are the last one again.  Where a tile is
 // whole tokens, as it is for 1, 2, 4 ... query heads to a key head, a lane's place in it stays the same.
 template <class H> struct PackedLoader {
     uint32_t place[H::kLoads], chunk[H::kLoads];
     int first, same_to;                          // row of the lane in the first load; tiles that begin before it are whole ones of such tokens
-    int64_t step;
-    const uint16_t *base, *next;
-    BW_DEV PackedLoader(const PromptArgs& a, int lane, int wave, const uint16_t* from, int64_t row, int64_t head, int rows, int at) {
+    uint32_t step, row_bytes, head_bytes, bytes;
+    const char* base;
+    BW_DEV PackedLoader(const PromptArgs& a, int lane, int wave, const uint16_t* from, int64_t row, int64_t head, int rows) {
         first = wave * H::kLoads * H::kLoadRows + lane / H::kChunks;
         uint32_t j;
         const int tokens = (int)a.by_share.div((uint32_t)H::kKeys, j);
-        same_to = j == 0 && a.dim == H::kPitch ? rows - H::kKeys + 1 : 0;
-        step = tokens * row;
-        base = from;
-        next = from + a.by_share.div((uint32_t)at, j) * row;
+        same_to = own(j == 0 ? rows - H::kKeys + 1 : 0);
+        step = own((uint32_t)(2 * tokens * row));                // (rows are 2^24 - 1 apart at most, and a key head's query heads 2^31)
+        row_bytes = own((uint32_t)(2 * row));
+        head_bytes = own((uint32_t)(2 * head));
+        bytes = own((uint32_t)a.dim * 2);
+        base = own((const char*)from);
 #pragma unroll
         for (int i = 0; i < H::kLoads; i++) {
             const int r = first + i * H::kLoadRows;
             chunk[i] = (uint32_t)((lane % H::kChunks) ^ swizzle<H::kPitch>(r)) * 16;
             const uint32_t token = a.by_share.div((uint32_t)r, j);
-            place[i] = token * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i];
+            place[i] = token * row_bytes + j * head_bytes + chunk[i];
         }
     }
-    BW_DEV void operator()(const PromptArgs& a, int64_t row, int64_t head, int from, int rows, uint32_t to, int wave) {
+    BW_DEV void operator()(const PromptArgs& a, int tile, int rows, uint32_t to, int wave) const {
+        const int from = tile * H::kKeys;
         to += wave * H::kLoads * 1024;
+        uint32_t some = bytes;
+        asm("" : "+s"(some));                                    // (the comparisons below are not kept in registers over the loop)
         if (from < same_to) {
+            const char* here = base + (uint64_t)step * (uint32_t)tile;
+            if (some == H::kPitch * 2) {
 #pragma unroll
-            for (int i = 0; i < H::kLoads; i++) load_to_lds(next, place[i], to + i * 1024);
-            next += step;
+                for (int i = 0; i < H::kLoads; i++) load_to_lds(here, place[i], to + i * 1024);
+            } else {
+#pragma unroll
+                for (int i = 0; i < H::kLoads; i++)
+                    if (chunk[i] < some) load_to_lds(here, place[i], to + i * 1024);
+            }
             return;
         }
         uint32_t rest;
         const uint32_t token0 = a.by_share.div((uint32_t)from, rest);
-        const uint16_t* here = base + token0 * row;
-        uint32_t bytes = (uint32_t)a.dim * 2;
-        asm("" : "+s"(bytes));
+        const char* here = base + (uint64_t)row_bytes * token0;
 #pragma unroll
         for (int i = 0; i < H::kLoads; i++) {
             const int r = from + first + i * H::kLoadRows;
             uint32_t j;
             const uint32_t token = a.by_share.div((uint32_t)(r < rows ? r : rows - 1), j);
-            if (chunk[i] < bytes) load_to_lds(here, (token - token0) * (uint32_t)(2 * row) + j * (uint32_t)(2 * head) + chunk[i], to + i * 1024);
+            if (chunk[i] < some) load_to_lds(here, (token - token0) * row_bytes + j * head_bytes + chunk[i], to + i * 1024);
         }
     }
 };
@@ -537,13 +546,15 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
     all_from = own(all_from);
     all_to = own(all_to);
     const float scale = own(a.scale);
+    const int begin = own(p.from), end = own(p.to);
     const int64_t stats = (int64_t)head * a.q_tokens * a.share + (int64_t)p.q0 * a.share;
     const uint32_t lds = lds_address(smem);
-    auto fetch = [&](PackedLoader<H>& load_q, PackedLoader<H>& load_g, int i) __attribute__((always_inline)) {
+    const PackedLoader<H> load_q(a, lane, wave, queries, a.q_row, a.q_head, rows), load_g(a, lane, wave, grads, g.grad_row, g.grad_head, rows);
+    auto fetch = [&](int i) __attribute__((always_inline)) {
         const int at = i * kTileRows;
         const uint32_t into = lds + (i & 1) * kKeyStage<H>;
-        load_q(a, a.q_row, a.q_head, at, rows, into, wave);
-        load_g(a, g.grad_row, g.grad_head, at, rows, into + H::kTileBytes, wave);
+        load_q(a, i, rows, into, wave);
+        load_g(a, i, rows, into + H::kTileBytes, wave);
         const int r = at + lane < rows ? lane : rows - 1 - at;
         if (wave == 0) load4_to_lds(a.lse + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes);
         if (DK && wave == 1) load4_to_lds(g.delta + stats + at, (uint32_t)r * 4, into + 2 * H::kTileBytes + 256);
@@ -556,11 +567,10 @@ template <class H, bool DK> BW_DEV void key_grad(const PromptGradArgs& g, const 
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++) acc[m] = f16v{};
         reach = kFirstReach16;
-        PackedLoader<H> load_q(a, lane, wave, queries, a.q_row, a.q_head, rows, p.from * kTileRows), load_g(a, lane, wave, grads, g.grad_row, g.grad_head, rows, p.from * kTileRows);
-        if (p.from < p.to) fetch(load_q, load_g, p.from);
-        for (int i = p.from; i < p.to; i++) {
+        if (begin < end) fetch(begin);
+        for (int i = begin; i < end; i++) {
             wait_tiles();
-            if (i + 1 < p.to) fetch(load_q, load_g, i + 1);
+            if (i + 1 < end) fetch(i + 1);
             char* tile = smem + (i & 1) * kKeyStage<H>;
             const int at = i * kTileRows;
             const bool none = at >= any_to || at + kTileRows <= any_from, all = at >= all_from && at + kTileRows <= all_to;
@@ -649,13 +659,15 @@ template <class H>
 __global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(PromptGradArgs g) {
     extern __shared__ __align__(1024) char smem[];               // [2][Q, g, lse, delta]
     const PromptArgs& a = g.p;
-    // dK and dV in turn, where both are wanted
-    const bool both = g.k_grad && g.v_grad, dk = both ? !(blockIdx.x & 1) : g.k_grad != nullptr;
-    const uint32_t block = both ? blockIdx.x >> 1 : blockIdx.x;
-    uint32_t head;
+    // Neighbouring workgroups, which go to different dies, have different heads: those of a die go over the same rows.  dK and dV of a piece, where both are wanted, are workgroups of the
+    // same head, and which comes first changes from piece to piece, so that every die gets as many of the longer (8192 tokens, 32 and 8 heads of 128: 1496 us with dK on the dies of even
+    // numbers, 1300 ... 1350 so).
+    const bool both = g.k_grad && g.v_grad;
+    uint32_t head, at = (g.plan ? a.by_heads : a.by_combos).div(blockIdx.x, head);
+    const bool dk = both ? !(__builtin_popcount(at) & 1) : g.k_grad != nullptr;
+    if (both) at >>= 1;
     Piece p;
     if (g.plan) {
-        const uint32_t at = a.by_heads.div(block, head);
         if ((int)at >= g.plan->pieces) return;
         p = g.pieces[at];
         if (p.nk == 0) return;
@@ -663,7 +675,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(Prom
         Span s;
         int h;
         uint32_t none;
-        if (!place_of<kGradKeys, true>(a, block, s, h, none)) return;
+        if (!place_of<kGradKeys, true>(a, at * a.combos + head, s, h, none)) return;
         head = (uint32_t)h;
         p = Piece{s.q0, s.nq, s.k0, s.nk, s.tile, 0, 0, -1};
         tiles_of_keys(a, p.nq, p.nk, p.tile, H::kKeys, p.from, p.to);
