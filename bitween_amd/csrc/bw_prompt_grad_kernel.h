@@ -1,7 +1,7 @@
 // bw_prompt_grad_kernel.h - gradients of the attention in bw_prompt_kernel.h.  With P = 2^(S c - lse), the weights of the forward again, and g the output's gradient:
 //   dP = g V^T,  delta = rowsum(g out),  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T g
 // One kernel has the rows and goes over the keys (dQ, and delta on the way), another has the keys and goes over the rows (dK, dV), so that every sum is a
-// workgroup's own, in one order: seven products where five would do with sums in memory, and the same bits every time.
+// workgroup's own, in one order: eight products where five would do with sums in memory, and the same bits every time.
 //
 // P and dS enter their second product as 16-bit numbers, rounded once.  In float16, whose steps end at 2^-24, P goes in 2^12 times as large, and dS times a power of two that
 // is each row's (each key's) own: it starts high and comes down where a product would pass 2^15, and the sums with it.
@@ -12,8 +12,8 @@
 // What the dS add up to before they are rounded is what the rounded output is off by in delta (the weights of a row add up to 1): the rows' kernel sees all keys, where they are not cut into
 // parts, and hands delta on to dK without it (dK's error, 2 tokens: 0.0039 with it, 0.0024 without).
 //
-// What bounds them is what bounds the forward; matrix cores busy 51 % (dQ) and 45 % (dK, dV), vector unit 41 and 35 %.  8192 tokens, 32 and 8 heads of 128, bfloat16: dQ 767 us (1075 TFLOP/s of its three
-// products), dK and dV 1370 (1000 of their five), 2140 in all.
+// What bounds them is what bounds the forward; matrix cores busy 49 ... 51 % (dQ) and 46 % (dK, dV), vector unit 42 and 36 %.  8192 tokens, 32 and 8 heads of 128, bfloat16: dQ 770 ... 840 us (1075 ... 980 TFLOP/s
+// of its three products, as the clocks of cards differ), dK and dV 1300 ... 1420 (1060 ... 970 of their five), 2075 ... 2260 in all.
 #pragma once
 #include "bw_prompt_kernel.h"
 

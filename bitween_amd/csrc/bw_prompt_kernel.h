@@ -14,8 +14,8 @@
 // rows at four neighbouring ones (V^T).
 //
 // What bounds it: the matrix cores and the vector unit of a SIMD, which its two waves share: 32 MFMAs of 32 cycles for a tile of 64 keys and heads of 128, 32 exponentials of 16 cycles and about 130
-// other vector instructions of 4; busy 51 % and 46 % of the time, at the clock that the part holds under such load (about 2.1 GHz).  8192 tokens, 32 query and 8 key heads of 128, bfloat16: 514 ... 530 us,
-// 1040 ... 1071 TFLOP/s (the library's product of 8192^3: 1327); 601 us before operands were read ahead of their products, the loop for values that are not finite had become another, and the
+// other vector instructions of 4; busy 51 % and 46 % of the time, at the clock that the part holds under such load (about 2.1 GHz).  8192 tokens, 32 query and 8 key heads of 128, bfloat16: 510 ... 563 us as
+// the clocks of cards differ, 1079 ... 977 TFLOP/s (the library's product of 8192^3: 1327); 601 us before operands were read ahead of their products, the loop for values that are not finite had become another, and the
 // scalars of the loop registers of their own (64 a tile came from spilled vector registers).  Heads of 64: 860 TFLOP/s (the same exponentials for half the products).  Not taken: 32 keys at a time with
 // the next scores under the weights (623 us for 564), higher wave priority in either product (nothing), four waves a SIMD with heads of 64 (nine registers in memory, nothing gained).
 #pragma once
