@@ -111,7 +111,8 @@ Parts parts_of(const bw_prompt* p, double times = 1., bool may_group = true) {
     // (of packed sequences, whose lengths are not known here, twice the mean)
     int64_t keys = p->q_starts ? (p->k_tokens * 2 + of - 1) / of : p->k_tokens / p->sequences, rows = p->q_tokens / p->sequences;
     if (keys > p->k_tokens) keys = p->k_tokens;
-    const int64_t reach = p->window ? p->window + p->sinks + kRows / share + 2 : keys;
+    auto few = [&](int64_t n) { return n < p->k_tokens ? n : p->k_tokens; };
+    const int64_t reach = p->window ? few(p->window) + few(p->sinks) + kRows / share + 2 : keys;
     const bool all = reach >= keys;
     if (!all) keys = reach;
     const double longest = (double)((keys + tile - 1) / tile), mean = all && keys > 0 ? longest * (1. - 0.5 * (rows < keys ? rows : keys) / keys) : longest;

@@ -161,7 +161,9 @@ def test_workspaces_of_prompts():
         row = p.q_tokens * p.q_heads * (p.dim + 2) * 4
         assert size % row == 0 and size <= 64 * row              # a reference, a sum and the values of each part
         assert lib.bw_prompt_attention_workspace_bytes(_prompt(**fields, window=16)) <= size
-        assert lib.bw_prompt_attention_workspace_bytes(_prompt(**fields, window=(1 << 63) - 1, sinks=(1 << 63) - 1)) >= 0
+        for large in (p.k_tokens, 1 << 40, 1 << 62, (1 << 63) - 1):
+            for sinks in (0, large):
+                assert lib.bw_prompt_attention_workspace_bytes(_prompt(**fields, window=large, sinks=sinks)) == size         # a window of everything is none
         assert lib.bw_prompt_attention_grad_workspace_bytes(p) >= p.q_tokens * p.q_heads * 4
 
 
