@@ -72,3 +72,25 @@ def test_a_captured_step_follows_its_inputs(dtype):
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
         torch.cuda.synchronize()
         del eager
+
+
+def _layouts(batch, tokens, heads, dim, dtype, gen):
+    def rand(*shape):
+        return torch.randn(*shape, device="cuda", generator=gen).to(dtype)
+    return {"heads outside": rand(batch, heads, tokens, dim).transpose(1, 2), "one head for all": rand(batch, tokens, 1, dim).expand(batch, tokens, heads, dim),
+            "one sequence for all": rand(1, tokens, heads, dim).expand(batch, tokens, heads, dim), "one token for all": rand(batch, 1, heads, dim).expand(batch, tokens, heads, dim),
+            "every second token": rand(batch, 2 * tokens, heads, dim)[:, ::2], "every second value": rand(batch, tokens, heads, 2 * dim)[..., ::2],
+            "off 16 bytes": rand(batch * tokens * heads * dim + 1)[1:].view(batch, tokens, heads, dim)}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["heads outside", "one head for all", "one sequence for all", "one token for all", "every second token", "every second value", "off 16 bytes"])
+def test_layouts_have_the_bits_of_their_copies(layout, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q, k, v, grad = (_layouts(3, 130, heads, 64, dtype, gen)[layout] for heads in (4, 2, 2, 4))
+    got, want = [], []
+    for to, change in ((got, lambda t: t), (want, lambda t: t.contiguous().clone())):
+        leaves = [change(t).detach().requires_grad_(True) for t in (q, k, v)]
+        out = bw.prompt_attention(*leaves, window=50, sinks=1)
+        to += [out.detach(), *torch.autograd.grad(out, leaves, change(grad))]
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, want))
