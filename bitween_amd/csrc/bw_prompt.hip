@@ -135,10 +135,11 @@ Parts parts_of(const bw_prompt* p, double times = 1., bool may_group = true) {
     return best;
 }
 
-// How the gradients' work is cut, and where their workspace has what (bytes).
-// About, over all heads (8192 tokens, 32 and 8 heads of 128, gradients of keys and values: 1 1549 us, 2 1479, 3 1495, 4 1513; with a window of 1024 451, 444, 512, 483; 2048 tokens 149, 153,
-// 162, 160).  Of heads up to 64 a CU holds more workgroups at once (16 and 4 heads of 64: 2 480 us, 4 438).
+// Pieces of the keys' and values' gradients for each CU, about, over all heads.  All gradients of 8192 tokens, 32 and 8 heads of 128: 1 2182 us, 2 2134, 3 2205, 4 2199; with a window of 1024
+// 625, 622, 668, 659.  Of heads up to 64 a CU holds more workgroups at once (8192 tokens, 16 and 4 heads of 64: 1 766 us, 2 701, 3 658, 4 648, 6 640; of 1000 tokens 63, 55, 56, 38, 38).
 constexpr int pieces_per_cu(int dim) { return dim <= 64 ? 4 : 2; }
+
+// How the gradients' work is cut, and where their workspace has what (bytes).
 struct GradPlan {
     int target;                                  // pieces of a head; 0: every tile of keys is one
     int64_t pieces, parts, joins;                // at most
@@ -161,7 +162,7 @@ GradPlan grad_plan(const bw_prompt* p) {
     if (g.q_splits > 1) g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
     if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
         g.target = (int)(((int64_t)bw_device_cus() * pieces_per_cu(p->dim) + p->kv_heads - 1) / p->kv_heads);
-        // (a tile of n among U tiles of rows is cut into n / size rounded up, size at least U / target and kLeastTiles)
+        // (a tile of keys with n of all U tiles of rows is cut into at most n / size, rounded up; size is at least U / target and kLeastTiles.  One that is up to a third longer stays whole)
         g.pieces = key_tiles + g.target;
         const int64_t most = key_tiles * ((row_tiles + kLeastTiles - 1) / kLeastTiles);
         g.parts = 2 * (int64_t)g.target < most ? 2 * g.target : most;
