@@ -598,7 +598,9 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     const int64_t index = (int64_t)head * a.q_tokens * a.share + token * a.share + row.head;       // of the row among all
     if (a.splits > 1) {                                           // (see prompt_join_kernel)
         const int64_t parts = (int64_t)a.q_tokens * a.q_heads * a.splits, at = index * a.splits + split;
-        if (half == 0) reinterpret_cast<u2*>(a.partial)[at] = u2{__builtin_bit_cast(uint32_t, begin < end ? r : -INFINITY), __builtin_bit_cast(uint32_t, l)};
+        // (a row that sees no key has none in this part either, also where other rows of its tile do: it is empty, not a row whose scores are all minus infinity)
+        const float reference = begin < end && row.position >= 0 ? r : -INFINITY;
+        if (half == 0) reinterpret_cast<u2*>(a.partial)[at] = u2{__builtin_bit_cast(uint32_t, reference), __builtin_bit_cast(uint32_t, l)};
         float* part = a.partial + parts * 2 + at * a.dim;
 #pragma unroll
         for (int m = 0; m < H::kBlocks; m++)
