@@ -340,8 +340,10 @@ __global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void promp
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
     float* part = a.splits > 1 ? g.q_parts + (index * a.splits + split) * a.dim : nullptr;
-    // c: of each row the mean of the last 32 keys at most that it sees, by a product with weights of 1 / 32; of the up to 63 keys of a wave's rows in two steps.  Infinities and NaN
-    // are left out, where there are any: each of these keys is seen by a row of the wave, and a row that sees one has no finite result.
+    // c: of each row the mean of the last 32 keys at most that it sees, by a product with weights of 1 / n (rounded to the type: any c will do); of the up to 63 keys of a wave's rows in two
+    // steps.  Infinities and NaN are left out, where there may be any: each of these keys is seen by a row of the wave, and where one workgroup goes over all keys a row that sees one has
+    // no finite sum.  Where they are cut into parts the key lies in another's, which puts it into that row's dQ; here it would reach the rows before it.
+    const bool finite_only = some || a.splits > 1;
     __syncthreads();
     char* mine = smem + wave * 32 * H::kPitch * 2;
     const int last = row.position, windowed = last - a.window + 1, from = windowed > last - 31 ? windowed > 0 ? windowed : 0 : last > 31 ? last - 31 : 0;
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void promp
                 const int n = i * H::kLoadRows + lane / H::kChunks;
                 u4 v = {0, 0, 0, 0};
                 if (base + n <= wave_high && chunk * 8 < a.dim) v = *reinterpret_cast<const u4*>(a.k + (int64_t)(p.k0 + base + n) * a.k_row + head * a.k_head + chunk * 8);
-                if (some) {
+                if (finite_only) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const uint32_t w = v[j];

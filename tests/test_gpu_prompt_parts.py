@@ -4,6 +4,7 @@ import torch
 
 import bitween_amd as bw
 from bitween_amd.kernels import hip_loader
+from prompt_ref import visible
 from test_gpu_prompt import _check, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +45,38 @@ def test_a_row_without_a_finite_score_is_not_an_empty_one():
     k[0, 0, 0] = float("-inf")
     out = bw.prompt_attention(q, k, v)
     assert not out[:100].any() and torch.isnan(out[100]).all() and torch.isfinite(out[101:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nk,heads,kv,dim,window,sinks", [(512, 512, 4, 2, 128, None, 0), (1024, 1024, 8, 2, 128, None, 0), (63, 2063, 4, 1, 128, None, 0), (600, 512, 2, 1, 256, None, 0),
+                                                             (130, 1500, 2, 1, 96, None, 0), (200, 8000, 2, 1, 64, 4000, 3)])
+def test_infinities_and_nan_touch_what_sees_them(nq, nk, heads, kv, dim, window, sinks, dtype):
+    """One value of q, k, v or the gradient is an infinity or a NaN: what does not see its token (or is not seen by it) has the bits that it has without."""
+    base = [t.contiguous() for t in _inputs(nq, nk, heads, kv, dim, dtype, seed=4)]
+
+    def run(q, k, v, grad):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        out = bw.prompt_attention(*leaves, window=window, sinks=sinks)
+        return [out.detach(), *torch.autograd.grad(out, leaves, grad)]
+
+    clean = run(*base)
+    seen = visible(nq, nk, window, sinks)
+    for which in range(4):
+        n = base[which].shape[0]
+        for token, value in ((n - 1, float("inf")), (n - 7, float("nan")), (n - 20, float("-inf")), (n - 45, float("inf")), (n // 2, float("nan")), (3, float("-inf"))):
+            t = [x.clone() for x in base]
+            t[which][token, -1, 5] = value
+            got = run(*t)
+            if which in (1, 2):
+                rows = seen[:, token]
+                keys = seen[rows].any(0)
+            else:
+                rows = torch.zeros(nq, dtype=torch.bool, device="cuda")
+                rows[token] = True
+                keys = seen[token]
+            for name, g, c, touched in zip(("out", "dq", "dk", "dv"), got, clean, (rows, rows, keys, keys)):
+                assert torch.equal(g[~touched], c[~touched]), (name, which, token, value)
+            if which == 2:
+                assert not torch.isfinite(got[0][rows][:, -1, 5]).any()
+            if which == 1:
+                assert not torch.isfinite(got[1][rows][:, -1, 5]).any()
