@@ -243,7 +243,19 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
         if (head < 0 || head >= (int64_t)1 << 30 || (share - 1) * head + 65 * row >= (int64_t)1 << 31) return BW_EUNSUPPORTED;
     const bool keys = (k_grad || v_grad) && p->k_tokens > 0;
     if (p->q_tokens == 0 && !keys) return BW_OK;
+    // (without rows a key's gradients are zeros, whichever sequence it is of: those of one sequence)
+    bw_prompt one = *p;
+    if (p->q_tokens == 0) {
+        one.sequences = 1;
+        one.q_starts = one.k_starts = nullptr;
+        p = &one;
+    }
     const GradPlan plan = grad_plan(p);
+    // Workgroups are counted with 31 bits: more than twice as many as any call has that the forward takes, which has fewer than 2^24, a tile of each sequence and key head at least.
+    const int64_t combos = p->kv_heads * (int64_t)(p->q_starts ? 1 : p->sequences), key_tiles = tiles_of(p, p->k_tokens, 1, kGradKeys);
+    const int64_t row_tiles = p->q_tokens > 0 ? tiles_of(p, p->q_tokens, (int)share, kRows) : 0;
+    const int64_t row_grid = row_tiles * combos * (q_grad ? plan.q_splits : 1), key_grid = !keys ? 0 : plan.target ? plan.pieces * p->kv_heads : key_tiles * combos;
+    if (row_grid >= (int64_t)1 << 30 || key_grid >= (int64_t)1 << 30) return BW_EUNSUPPORTED;
     if (plan.all) {
         if (!workspace || workspace_bytes < plan.all) return BW_EWORKSPACE;
         if (!bw_aligned(workspace, 16)) return BW_EALIGN;
@@ -263,17 +275,11 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     g.q_parts = a.splits > 1 ? (float*)((char*)workspace + plan.q_parts) : nullptr;
     g.plain_scale = p->scale;
     PromptGrids grids = {};
-    if (p->q_tokens > 0) {
-        const int64_t tiles = tiles_of(p, p->q_tokens, a.share, kRows), grid = tiles * a.combos * a.splits;
-        if (grid >= (int64_t)1 << 24) return BW_EUNSUPPORTED;
-        grids.rows = (uint32_t)grid;
-        grids.row_tiles = (uint32_t)tiles;
-    }
+    grids.rows = (uint32_t)row_grid;
+    grids.row_tiles = (uint32_t)row_tiles;
     if (keys) {
-        const int64_t tiles = tiles_of(p, p->k_tokens, 1, kGradKeys), grid = plan.target ? plan.pieces * p->kv_heads : tiles * a.combos;
-        if (grid >= (int64_t)1 << 23 || plan.joins * p->kv_heads >= (int64_t)1 << 22) return BW_EUNSUPPORTED;
-        grids.keys = (uint32_t)(k_grad && v_grad ? 2 * grid : grid);
-        grids.key_tiles = (uint32_t)tiles;
+        grids.keys = (uint32_t)(k_grad && v_grad ? 2 * key_grid : key_grid);
+        grids.key_tiles = (uint32_t)key_tiles;
         if (plan.target) {
             grids.joins = (uint32_t)plan.joins;
             char* at = (char*)workspace + plan.plan;

@@ -34,6 +34,7 @@ struct PromptGradArgs {
     float* parts;
     int target;                                  // pieces (of one head) that the rows are cut into, about
     int room, parts_room, joins_room;            // of the lists
+    uint32_t before;                             // workgroups in the launches before this one (see in_launches)
 };
 
 constexpr int kFirstReach16 = 80, kReachTop = 12, kReachMost = 15, kWeightShift = 12;
@@ -224,11 +225,12 @@ __global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void promp
     Span p;
     int head;
     uint32_t split;
-    if (g.plan && blockIdx.x == 0) {
+    const uint32_t block = g.before + blockIdx.x;
+    if (g.plan && block == 0) {
         plan_keys(g, smem, H::kKeys);
         return;
     }
-    if (!place_of<kRows, false>(a, g.plan ? blockIdx.x - 1 : blockIdx.x, p, head, split)) return;
+    if (!place_of<kRows, false>(a, g.plan ? block - 1 : block, p, head, split)) return;
     clear_tiles<H>(smem, 4 * H::kTileBytes, a.dim);
     const int row0 = p.tile * kRows + wave * kWaveRows, rows = p.nq * a.share;
     const Row row(a, p, row0 + (lane & 31));
@@ -665,7 +667,7 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_key_grad_kernel(Prom
     // same head, and which comes first changes from piece to piece, so that every die gets as many of the longer (8192 tokens, 32 and 8 heads of 128: 1496 us with dK on the dies of even
     // numbers, 1300 ... 1350 so).
     const bool both = g.k_grad && g.v_grad;
-    uint32_t head, at = (g.plan ? a.by_heads : a.by_combos).div(blockIdx.x, head);
+    uint32_t head, at = (g.plan ? a.by_heads : a.by_combos).div(g.before + blockIdx.x, head);
     const bool dk = both ? !(__builtin_popcount(at) & 1) : g.k_grad != nullptr;
     if (both) at >>= 1;
     Piece p;

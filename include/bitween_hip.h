@@ -350,7 +350,9 @@ int bw_cache_attention_window(const bw_cache* cache, int act_dtype, const void* 
  * Scores, the softmax and all sums are float32; a weight meets its value rounded once to act_dtype (in float16 scaled so that the largest of a row is near its upper end).
  * A score of minus infinity has weight 0, and a row without any other score gives NaN, as one of plus infinity or NaN does; an infinity or a NaN among the values leaves
  * nothing finite in its channel of the rows that see it, whatever its weight, and touches no others.
- * dim a multiple of 8 up to 256, pointers, rows and heads aligned to 16 bytes, rows of k and v 0 ... 2^24 - 1 elements apart; fewer than 2^31 tokens and heads of tokens.
+ * dim a multiple of 8 up to 256, pointers, rows and heads aligned to 16 bytes, rows of k and v 0 ... 2^24 - 1 elements apart; fewer than 2^31 tokens and heads of tokens, 2^20 sequences at
+ * most, and fewer than 2^24 workgroups: tiles of 128 rows (new tokens x query heads of a key head; of 64 where there are few), each sequence's own, of every key head.  The gradients take what
+ * the forward takes.
  *   lse   float32 [q_tokens * q_heads] or NULL: what the gradients need of the forward
  * Where there are few rows their keys are cut into parts, joined in a fixed order through a workspace of bw_prompt_attention_workspace_bytes(...) bytes (16-byte aligned; 0 =
  * none needed). */
