@@ -144,7 +144,7 @@ struct GradPlan {
     int target;                                  // pieces of a head; 0: every tile of keys is one
     int64_t pieces, parts, joins;                // at most
     int q_splits;                                // parts of a row's keys, for the queries' gradient
-    size_t delta, plan, parts_at, q_parts, all;
+    size_t delta, plan, parts_at, q_parts, q_left, all;
 };
 GradPlan grad_plan(const bw_prompt* p) {
     const int64_t share = p->q_heads / p->kv_heads, seq_q = p->q_tokens / (p->q_starts ? 1 : p->sequences);
@@ -159,7 +159,10 @@ GradPlan grad_plan(const bw_prompt* p) {
     };
     g.delta = room((size_t)(p->q_tokens * p->q_heads) * sizeof(float));
     g.q_splits = p->q_tokens > 0 ? parts_of(p, 1.5, false).splits : 1;
-    if (g.q_splits > 1) g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
+    if (g.q_splits > 1) {
+        g.q_parts = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * p->dim * sizeof(float));
+        g.q_left = room((size_t)(p->q_tokens * p->q_heads) * g.q_splits * sizeof(float));
+    }
     if (row_tiles > 2 * kLeastTiles && p->k_tokens > 0) {
         g.target = (int)(((int64_t)bw_device_cus() * pieces_per_cu(p->dim) + p->kv_heads - 1) / p->kv_heads);
         // (a tile of keys with n of all U tiles of rows is cut into at most n / size, rounded up; size is at least U / target and kLeastTiles.  One that is up to a third longer stays whole)
@@ -254,7 +257,8 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     // Workgroups are counted with 31 bits: more than twice as many as any call has that the forward takes, which has fewer than 2^24, a tile of each sequence and key head at least.
     const int64_t combos = p->kv_heads * (int64_t)(p->q_starts ? 1 : p->sequences), key_tiles = tiles_of(p, p->k_tokens, 1, kGradKeys);
     const int64_t row_tiles = p->q_tokens > 0 ? tiles_of(p, p->q_tokens, (int)share, kRows) : 0;
-    const int64_t row_grid = row_tiles * combos * (q_grad ? plan.q_splits : 1), key_grid = !keys ? 0 : plan.target ? plan.pieces * p->kv_heads : key_tiles * combos;
+    const int q_splits = q_grad || k_grad ? plan.q_splits : 1;      // (dV alone needs neither dQ nor delta)
+    const int64_t row_grid = row_tiles * combos * q_splits, key_grid = !keys ? 0 : plan.target ? plan.pieces * p->kv_heads : key_tiles * combos;
     if (row_grid >= (int64_t)1 << 30 || key_grid >= (int64_t)1 << 30) return BW_EUNSUPPORTED;
     if (plan.all) {
         if (!workspace || workspace_bytes < plan.all) return BW_EWORKSPACE;
@@ -270,9 +274,10 @@ extern "C" int bw_prompt_attention_grad(const bw_prompt* p, int act_dtype, const
     g.result = (const uint16_t*)out;
     g.q_grad = (uint16_t*)q_grad; g.k_grad = (uint16_t*)k_grad; g.v_grad = (uint16_t*)v_grad;
     g.delta = (float*)workspace;
-    a.set_splits(q_grad ? plan.q_splits : 1);
-    g.exact = plan.q_splits == 1 && (q_grad || k_grad);             // (the same for dK, whichever other gradients are wanted)
+    a.set_splits(q_splits);
+    g.exact = q_grad || k_grad;                                     // (the same for dK, whichever other gradients are wanted)
     g.q_parts = a.splits > 1 ? (float*)((char*)workspace + plan.q_parts) : nullptr;
+    g.q_left = a.splits > 1 ? (float*)((char*)workspace + plan.q_left) : nullptr;
     g.plain_scale = p->scale;
     PromptGrids grids = {};
     grids.rows = (uint32_t)row_grid;

@@ -9,8 +9,8 @@
 // A row's dS add up to zero, but for what dS and the output (in delta) were rounded by: a remainder e, which puts e times the mean of the keys into dQ.  Keys are projected with
 // channels far from zero, so that this was the larger part of dQ's error (8192 tokens, bfloat16, channels at 2 to 6 of keys that spread by 1: 0.0045 of dQ, 0.0024 without it; 2 tokens: 0.0060 and 0.0025).
 // dQ = scale dS (K - c) for any c: e is summed as the product takes it, and e c taken off, c the mean of the last 32 keys that a row sees.
-// What the dS add up to before they are rounded is what the rounded output is off by in delta (the weights of a row add up to 1): the rows' kernel sees all keys, where they are not cut into
-// parts, and hands delta on to dK without it (dK's error, 2 tokens: 0.0039 with it, 0.0024 without).
+// What the dS add up to before they are rounded is what the rounded output is off by in delta (the weights of a row add up to 1): the rows' kernel, which sees all keys, hands delta on to dK
+// without it (dK's error, 2 tokens: 0.0039 with it, 0.0024 without); where keys are in parts each leaves its sum, and the join takes them off.
 //
 // What bounds them is what bounds the forward; matrix cores busy 49 ... 51 % (dQ) and 46 % (dK, dV), vector unit 42 and 36 %.  8192 tokens, 32 and 8 heads of 128, bfloat16: dQ 770 ... 840 us (1075 ... 980 TFLOP/s
 // of its three products, as the clocks of cards differ), dK and dV 1300 ... 1420 (1060 ... 970 of their five), 2075 ... 2260 in all.
@@ -22,9 +22,9 @@ struct PromptGradArgs {
     const uint16_t *grad, *result;               // of the output; result [tokens][q_heads][dim]
     int64_t grad_row, grad_head;
     float* delta;                                // its negative, as lse
-    int exact;                                   // delta is that of the weights, not of the rounded result (see below)
+    int exact;                                   // delta is wanted that is that of the weights, not of the rounded result (see above)
     uint16_t *q_grad, *k_grad, *v_grad;
-    float* q_parts;                              // where a row's keys are cut into p.splits parts: [row][part][dim]
+    float *q_parts, *q_left;                     // where a row's keys are cut into p.splits parts: [row][part][dim], and sums of their dS [row][part]
     float plain_scale;
     // keys: the list of the workgroups' pieces (NULL: a piece for every tile of keys), the parts [part][kv_heads][keys][2][dim] and what is to be joined of them
     struct KeyPlan* plan;
@@ -254,8 +254,8 @@ __global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void promp
         }
         delta += __shfl_xor(delta, 32, 64);
     }
-    if (!g.exact && row.live && half == 0 && split == 0) g.delta[index] = -delta;
-    if (!g.q_grad && !g.exact) return;
+    if ((!g.exact || a.splits > 1) && row.live && half == 0 && split == 0) g.delta[index] = -delta;
+    if (!g.exact) return;
     const float lse = row.live ? a.lse[index] : INFINITY;
 
     int low, high, wave_low, wave_high;
@@ -335,10 +335,11 @@ __global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void promp
     if (some) pass(std::true_type{});
     rest += __shfl_xor(rest, 32, 64);
     left += __shfl_xor(left, 32, 64);
-    if (g.exact) {
-        if (row.live && half == 0) g.delta[index] = -(delta + left);
-        if (!g.q_grad) return;
+    if (row.live && half == 0) {
+        if (a.splits > 1) g.q_left[index * a.splits + split] = left;
+        else g.delta[index] = -(delta + left);
     }
+    if (!g.q_grad) return;
     const float back = DT == BW_F16 ? __builtin_ldexpf(1.f, -reach) : 1.f;
     uint16_t* out = g.q_grad + (token * a.q_heads + head * a.share + row.head) * a.dim;
     float* part = a.splits > 1 ? g.q_parts + (index * a.splits + split) * a.dim : nullptr;
@@ -405,23 +406,34 @@ __global__ __launch_bounds__(256, H::kPitch == 64 ? 3 : H::kResident) void promp
     }
 }
 
-// dQ = the parts of a row added up in order; a thread has 4 values of a row, and 8 parts under way.
+// dQ = the parts of a row added up in order, and delta without what their dS add up to; a thread has 4 values of a row, and 8 parts under way.
 template <int DT>
 __global__ __launch_bounds__(256) void prompt_query_join_kernel(PromptGradArgs g, int threads, uint32_t rows) {
     const PromptArgs& a = g.p;
     const uint32_t i = blockIdx.x * (256 / threads) + threadIdx.x / threads;
     const int d = (int)(threadIdx.x % threads) * 4;
     if (threadIdx.x / threads >= 256 / threads || i >= rows) return;
-    const float* part = g.q_parts + (int64_t)i * a.splits * a.dim + d;
+    const float *part = g.q_parts + (int64_t)i * a.splits * a.dim + d, *lefts = g.q_left + (int64_t)i * a.splits;
     f4 o = {0.f, 0.f, 0.f, 0.f};
+    float left = 0.f;
     for (int s = 0; s < a.splits; s += 8) {
         f4 x[8];
+        float y[8];
 #pragma unroll
-        for (int n = 0; n < 8; n++) x[n] = *reinterpret_cast<const f4*>(part + (int64_t)(s + n < a.splits ? s + n : s) * a.dim);
+        for (int n = 0; n < 8; n++) {
+            const int at = s + n < a.splits ? s + n : s;
+            y[n] = lefts[at];
+            if (g.q_grad) x[n] = *reinterpret_cast<const f4*>(part + (int64_t)at * a.dim);
+        }
 #pragma unroll
-        for (int n = 0; n < 8; n++)
-            if (s + n < a.splits) o += x[n];
+        for (int n = 0; n < 8; n++) {
+            if (s + n >= a.splits) continue;
+            left += y[n];
+            if (g.q_grad) o += x[n];
+        }
     }
+    if (d == 0) g.delta[i] -= left;
+    if (!g.q_grad) return;
     uint32_t j;
     const uint32_t token_head = a.by_share.div(i, j), head = token_head / (uint32_t)a.q_tokens, token = token_head - head * a.q_tokens;
     store4<DT>(g.q_grad + ((int64_t)token * a.q_heads + head * a.share + j) * a.dim + d, o[0], o[1], o[2], o[3]);

@@ -1,10 +1,11 @@
-"""prompt_attention where the keys of a row are cut into parts that a second kernel joins."""
+"""prompt_attention where the keys of a row are cut into parts that a second kernel joins: tokens with nothing to see, infinities and NaN, the keys' gradient."""
 import pytest
 import torch
 
 import bitween_amd as bw
 from bitween_amd.kernels import hip_loader
-from prompt_ref import visible
+from attention_ref import half_step
+from prompt_ref import close, visible
 from test_gpu_prompt import _check, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +81,49 @@ def test_infinities_and_nan_touch_what_sees_them(nq, nk, heads, kv, dim, window,
                 assert not torch.isfinite(got[0][rows][:, -1, 5]).any()
             if which == 1:
                 assert not torch.isfinite(got[1][rows][:, -1, 5]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nk,dim", [(1, 700, 128), (4, 1500, 64), (63, 2063, 128), (9, 2000, 256)])
+def test_the_outputs_rounding_is_not_in_the_keys_gradient(nq, nk, dim, dtype):
+    """Values of multiples of 1/16 within 2 of 8 (exact in both types), so that the output and its rounding are large beside what the keys' gradient is made of.  Bounds of every value, h
+    being half a step:
+
+    dS = P (dP - delta), of which the products take h of itself; P errs by loose = 2 (dim + 16) 2^-24 of the scores' magnitudes + 2 n 2^-24; dP by (dim + 2) 2^-23 of |g| |v|; delta in float32 by
+    dim 2^-23 of |g out| and n 2^-23 of sum |dS|, and with what the output errs by (`off`: h |out| + (h + loose) P |v|) only by that part of it by which the weights do not add up to 1, h + loose.
+    dK = scale sum dS q: these, n 2^-23 of |dS| |q|, and its own rounding."""
+    h, small, scale = half_step(dtype), 2.0 ** -37 if dtype == torch.float16 else 0.0, dim ** -0.5
+    gen = torch.Generator(device="cuda").manual_seed(nk + dim)
+    q, g = (torch.randn(nq, 2, dim, device="cuda", generator=gen).to(dtype) for _ in range(2))
+    k = torch.randn(nk, 2, dim, device="cuda", generator=gen).to(dtype)
+    v = (8 + torch.randint(-32, 33, (nk, 2, dim), device="cuda", generator=gen) / 16).to(dtype)
+    assert _is_cut(q, k)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dk = torch.autograd.grad(bw.prompt_attention(*leaves), leaves, g)[1]
+    seen = visible(nq, nk, None, 0)
+    for n in range(2):
+        x, y, z, up = (t.detach()[:, n].double() for t in (q, k, v, g))
+        p = (x @ y.t() * scale).masked_fill(~seen, float("-inf")).softmax(-1)
+        out, dp = p @ z, up @ z.t()
+        delta = (up * out).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        loose = 2 * (dim + 16) * 2.0 ** -24 * (x.abs() @ y.abs().t() * scale * seen).amax(-1, keepdim=True) + 2 * nk * 2.0 ** -24
+        off = h * out.abs() + (h + loose) * (p @ z.abs()) + small * (seen.double() @ z.abs()) + 2.0 ** -25
+        of_delta = (up.abs() * off).sum(-1, keepdim=True)
+        wrong = h * ds.abs() + p * (loose * (dp - delta).abs() + (dim + 2) * 2.0 ** -23 * (up.abs() @ z.abs().t()) + dim * 2.0 ** -23 * (up * out).abs().sum(-1, keepdim=True)
+                                    + (h + loose) * of_delta + nk * 2.0 ** -23 * ds.abs().sum(-1, keepdim=True)) + small * ds.abs().amax(0, keepdim=True)
+        want = scale * (ds.t() @ x)
+        bound = scale * ((wrong * seen).t() @ x.abs() + nk * 2.0 ** -23 * (ds.abs().t() @ x.abs())) + h * want.abs() + 2.0 ** -25
+        close(dk[:, n], want, bound, "dk")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [(63, 2063, 4, 1, 128), (512, 512, 4, 2, 128), (9, 2000, 2, 2, 256)])
+def test_each_gradient_alone(nq, nk, heads, kv, dim, dtype):
+    q, k, v, grad = _inputs(nq, nk, heads, kv, dim, dtype, seed=5)
+    full = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(bw.prompt_attention(*full), full, grad)
+    for wanted in ((0,), (1,), (2,), (0, 1), (1, 2), (0, 2)):
+        some = [t.detach().clone().requires_grad_(i in wanted) for i, t in enumerate((q, k, v))]
+        got = torch.autograd.grad(bw.prompt_attention(*some), [some[i] for i in wanted], grad)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, wanted)), wanted
