@@ -78,7 +78,7 @@ BW_DEV uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const 
 // 16 bytes of every lane from base + offset to LDS at `to` + 16 lane.  Assembly, because the compiler would wait for it before any read of LDS; the
 // waits and barriers are placed by the callers (wait_tiles).  (Wait states: M0 and a scalar that a vector instruction may have written.)
 BW_DEV void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
 }
 // The order of a region's instructions, N of a kind at a time: the compiler reads an operand from LDS right before the product that takes it, and waits for it there.
 template <int N> BW_DEV void then_reads() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
