@@ -37,12 +37,13 @@ template <int DT> BW_DEV double wide_sum(double v, int shift) {
     if (shift > 4) add([](float x) { return __shfl_xor(x, 16, 64); });
     return v;
 }
-// 1 / sqrt(x), to within a few units of a float64's last place: two steps from the instruction's 2^-14 or better.
+// 1 / sqrt(x), to within a few units of a float64's last place: two steps from the instruction's 2^-14 or better.  Of an infinity 0, which the steps would make NaN: what is
+// finite in such a head is 0 then.
 BW_DEV double rsqrt_wide(double x) {
     double y = __builtin_amdgcn_rsq(x);
 #pragma unroll
     for (int i = 0; i < 2; i++) y = __builtin_fma(y, 0.5 * __builtin_fma(-x * y, y, 1.0), y);
-    return y;
+    return x == __builtin_inf() ? 0.0 : y;
 }
 
 // A thread has its place in some of a token's heads, a.slices apart: the queries', the keys' and the values', and their angles once.
