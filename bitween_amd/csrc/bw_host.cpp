@@ -552,8 +552,9 @@ bool axes_of(PyObject* sections, PyObject* interleaved, bw_axes& axes) {
     for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(sections); i++) {
         PyObject* n = PySequence_Fast_GET_ITEM(sections, i);
         if (!PyLong_CheckExact(n)) return false;
-        const long v = PyLong_AsLong(n);
-        if (PyErr_Occurred() || v < 0 || v > 65535) return false;
+        int beyond = 0;                                          // (a number of any size is Python's to refuse)
+        const long v = PyLong_AsLongAndOverflow(n, &beyond);
+        if (beyond || v < 0 || v > 65535) return false;
         axes.sections[i] = (int)v;
     }
     axes.count = (int)PySequence_Fast_GET_SIZE(sections);
