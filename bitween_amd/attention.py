@@ -21,6 +21,7 @@ from torch.autograd import forward_ad
 from .kernels import hip_loader as _hip
 
 _HALF = (torch.float16, torch.bfloat16)
+_FAR = 2 ** 62                                                # beyond every cache and tensor
 
 
 def _native(name):
@@ -101,6 +102,8 @@ def _cache_args(keys, values, key_meta, value_meta, bits, group_size):
 
 def _window(what, window, sinks):
     """window (0: all tokens) and sinks as whole numbers."""
+    if type(sinks) is int and 0 <= sinks <= _FAR and (window is None or (type(window) is int and 1 <= window <= _FAR)):      # (nearly every call, before which the GPU waits)
+        return window or 0, sinks
     for n, name, least in ((window, "window", 1), (sinks, "sinks", 0)):
         if n is None and name == "window":
             continue
@@ -108,7 +111,7 @@ def _window(what, window, sinks):
             raise TypeError(f"{what}: {name} must be a whole number, got {type(n).__name__}")
         if n < least:
             raise ValueError(f"{what}: {name} must be at least {least}, got {n}")
-    return min(window or 0, 2 ** 62), min(sinks, 2 ** 62)
+    return min(window or 0, _FAR), min(sinks, _FAR)
 
 
 def _taken(what, out):
