@@ -502,9 +502,6 @@ template <class H> struct PackedLoader {
         }
     }
 };
-BW_DEV void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
-}
 
 // sums += the transposed product of 32 rows of a tile with the 16 + 16 values of a lane: the second 16's operands are read while the first products are under way.  `first`: the first
 // 16's, read by then.

@@ -75,11 +75,18 @@ template <int DT> BW_DEV f16v mfma32(u4 a, u4 b, f16v c) {
 typedef __attribute__((address_space(3))) char lds_char;
 BW_DEV uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
 
-// 16 bytes of every lane from base + offset to LDS at `to` + 16 lane.  Assembly, because the compiler would wait for it before any read of LDS; the
-// waits and barriers are placed by the callers (wait_tiles).  (Wait states: M0 and a scalar that a vector instruction may have written.)
+// 16 bytes (4) of every lane from base + offset to LDS at `to` + 16 (4) lane.  Assembly, because the compiler would wait for it before any read of LDS; the
+// waits and barriers are placed by the callers (wait_tiles).  (Wait states: M0 and a scalar that a vector instruction may have written.  M0 is one of the registers that the compiler never
+// hands out, which its warning about the list says; naming it keeps its own settings of M0, were there any, from being carried over the statement.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 BW_DEV void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
 }
+BW_DEV void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 // The order of a region's instructions, N of a kind at a time: the compiler reads an operand from LDS right before the product that takes it, and waits for it there.
 template <int N> BW_DEV void then_reads() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
 template <int N> BW_DEV void then_products() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
