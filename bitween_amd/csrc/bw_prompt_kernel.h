@@ -603,10 +603,11 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
     }
     if (!row.live) return;
     const int64_t index = (int64_t)head * a.q_tokens * a.share + token * a.share + row.head;       // of the row among all
+    const bool empty = row.position < 0 || p.nk == 0;             // no key is seen: zeros
     if (a.splits > 1) {                                           // (see prompt_join_kernel)
         const int64_t parts = (int64_t)a.q_tokens * a.q_heads * a.splits, at = index * a.splits + split;
         // (a row that sees no key has none in this part either, also where other rows of its tile do: it is empty, not a row whose scores are all minus infinity)
-        const float reference = begin < end && row.position >= 0 ? r : -INFINITY;
+        const float reference = begin < end && !empty ? r : -INFINITY;
         if (half == 0) reinterpret_cast<u2*>(a.partial)[at] = u2{__builtin_bit_cast(uint32_t, reference), __builtin_bit_cast(uint32_t, l)};
         float* part = a.partial + parts * 2 + at * a.dim;
 #pragma unroll
@@ -618,7 +619,6 @@ __global__ __launch_bounds__(256, H::kResident) void prompt_forward_kernel(Promp
             }
         return;
     }
-    const bool empty = row.position < 0 || p.nk == 0;             // no key is seen: zeros
     const float inv = empty ? 0.f : 1.f / l;
     if (a.lse && half == 0) a.lse[index] = empty ? INFINITY : r + __builtin_amdgcn_logf(l);
     uint16_t* out = a.out + (token * a.q_heads + head * a.share + row.head) * a.dim;
