@@ -87,9 +87,9 @@ PromptArgs args_of(const bw_prompt* p) {
     a.by_combos = FastDiv(a.combos);
     a.by_heads = FastDiv((uint32_t)p->kv_heads);
     a.flip = p->scale < 0.f ? 0x80008000u : 0u;
-    // (scale 0: all scores that are numbers weigh the same, and hidden ones, minus infinity, stay hidden)
+    // (scale 0: all scores that are numbers weigh the same, and hidden ones, minus infinity, stay hidden: the smallest number, which makes 2^-21 of the largest score)
     const float scale = __builtin_fabsf(p->scale) * 1.44269504088896340736f;
-    a.scale = scale < 1e-38f ? 1e-38f : scale;
+    a.scale = scale == 0.f ? __FLT_DENORM_MIN__ : scale;
     return a;
 }
 
