@@ -3,7 +3,9 @@
 // One kernel has the rows and goes over the keys (dQ, and delta on the way), another has the keys and goes over the rows (dK, dV), so that every sum is a
 // workgroup's own, in one order: eight products where five would do with sums in memory, and the same bits every time.
 //
-// P and dS enter their second product as 16-bit numbers, rounded once.  In float16, whose steps end at 2^-24, P goes in 2^12 times as large, and dS times a power of two that
+// P and dS enter their second product as 16-bit numbers, rounded once (as in the forward, at the same price of a second product for each).  lse is that of the forward's rounded weights, so that a
+// row's P add up to 1 but for half a step at most (of a few keys; where there are many the roundings cancel); a float32 sum beside it would cost the forward 5 % (heads of 64 9 %), one here some 15
+// registers, which go to memory.  In float16, whose steps end at 2^-24, P goes in 2^12 times as large, and dS times a power of two that
 // is each row's (each key's) own: it starts high and comes down where a product would pass 2^15, and the sums with it.
 //
 // A row's dS add up to zero, but for what dS and the output (in delta) were rounded by: a remainder e, which puts e times the mean of the keys into dQ.  Keys are projected with
@@ -443,7 +445,8 @@ __global__ __launch_bounds__(256) void prompt_query_join_kernel(PromptGradArgs g
 //
 // A workgroup has 128 keys of one sequence and one key head, 32 to a wave, and the rows come by, kKeys at a time: S and dP with a key to a lane, so that P and dS are the
 // second operands of dV^T += g^T P and dK^T += Q^T dS as they lie.  dV and dK are workgroups of their own, side by side in one launch, though both need S: one wave with
-// both sums does not fit (64 registers of operands and 128 of sums leave too few: 283 TFLOP/s with 250 bytes of a lane in memory), and two waves that share S and P through LDS
+// both sums does not fit two workgroups to a CU (of 256 registers, 64 of operands and 128 of sums leave too few: 283 TFLOP/s with 250 bytes of a lane in memory; one workgroup, with 512, has not been
+// tried), and two waves that share S and P through LDS
 // wait for each other every 32 rows (8192 tokens, 32 and 8 heads of 128: 2068 us).
 //
 // Rows are cut into pieces of equal length, each a workgroup's: a workgroup lists them first (plan_keys), since a key that is seen by all rows meets many times the

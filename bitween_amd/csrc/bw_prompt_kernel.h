@@ -14,8 +14,8 @@
 // rows at four neighbouring ones (V^T).
 //
 // What bounds it: the matrix cores and the vector unit of a SIMD, which its two waves share: 32 MFMAs of 32 cycles for a tile of 64 keys and heads of 128, 32 exponentials of 16 cycles and about 130
-// other vector instructions of 4; busy 51 % and 46 % of the time, at the clock that the part holds under such load (about 2.1 GHz).  8192 tokens, 32 query and 8 key heads of 128, bfloat16: 510 ... 563 us as
-// the clocks of cards differ, 1079 ... 977 TFLOP/s (the library's product of 8192^3: 1327); 601 us before operands were read ahead of their products, the loop for values that are not finite had become another, and the
+// other vector instructions of 4; busy 51 % and 46 % of the time, at the clock that the part holds under such load (about 2.1 GHz).  8192 tokens, 32 query and 8 key heads of 128, bfloat16: 510 ... 595 us as
+// the clocks of cards differ, and with what ran before, 1079 ... 924 TFLOP/s (the library's product of 8192^3: 1327); 601 us before operands were read ahead of their products, the loop for values that are not finite had become another, and the
 // scalars of the loop registers of their own (64 a tile came from spilled vector registers).  Heads of 64: 860 TFLOP/s (the same exponentials for half the products).  Not taken: 32 keys at a time with
 // the next scores under the weights (623 us for 564), higher wave priority in either product (nothing), four waves a SIMD with heads of 64 (nine registers in memory, nothing gained).
 #pragma once
@@ -27,8 +27,9 @@ typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 128, kWaveRows = 32, kPromptWaves = 4;
 // Where weights lie in their 16-bit type: in float16, whose steps end at 2^-24, the largest at 2^12 and more when its reference is set, up to 2^15 until the
-// reference is raised; in bfloat16 never above 1, so that no product is larger than its value.  One rounding to the type, at most 2^-12 (2^-9) of a weight: the
-// result's own rounding is as large.
+// reference is raised; in bfloat16 never above 1, so that no product is larger than its value.  One rounding to the type, at most half a step of a weight (2^-11 of it, 2^-8 in
+// bfloat16), as large as the result's own: 1500 tokens with heads of 128 in bfloat16 err by 0.0020 of the result, 0.0016 of which its rounding makes.  A second number for what the rounding
+// leaves, and a second product, would take that to 0.0016, and 8192 tokens from 534 to 716 us (heads of 64 162 to 230).
 template <int DT> constexpr float kWeightTop = DT == BW_F16 ? 12.f : -8.f;
 template <int DT> constexpr float kWeightMost = DT == BW_F16 ? 15.f : 0.f;
 constexpr float kLowestScore = -3.4028235e38f;

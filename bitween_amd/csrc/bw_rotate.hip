@@ -9,7 +9,8 @@
 //
 // One pass over memory, a dozen float32 operations a value: launch-bound up to a few hundred tokens (one token 2.3 us as a graph), HBM and, as every head
 // loads its token's cosines and sines, the L2 beyond: 2048 tokens of 32 and 8 heads of 128 in bfloat16 with both norms take 11 us (42 MB, 3.8 TB/s),
-// their gradients 17 (63 MB) and 4 for the sum; torch copies 21 MB in 7 us.  By three axes: 1024 tokens without norms 8 us, 4095 with norms 19 (84 MB, 4.4 TB/s), their gradients 37 (126 MB, 3.4 TB/s)
+// their gradients 17 (63 MB) and 4 for the sum; torch copies 21 MB in 7 us.  By three axes: 1024 tokens without norms 8 us, 4095 with norms 19 (84 MB, 4.4 TB/s), their gradients 37 (126 MB, 3.4 TB/s:
+// the forward asks for the next head's values while it has one, they ask for a head's when they need them)
 // and 4, 16384 without 73 (335 MB, 4.6 TB/s).
 #include "bw_rotate.h"
 
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     rotate_head<DT, CH>(a, raw1, raw2, angle, token, head, live, pos.kept, turns, first, second);
 }
 
-// Positions of several axes: the angles come from as many rows of the tables as there are axes, so that a thread keeps them for a.each heads of its token, `slices` apart
+// Positions of several axes: the angles come from as many rows of the tables as there are axes, so that a thread keeps them for several heads of its token, a.slices apart
 // (4095 tokens of 32 and 8 heads of 128 with norms, three interleaved axes: 26.6 us with one head).
 template <int DT, int CH>
 __global__ __launch_bounds__(256) void rotate_axes_kernel(RotateArgs a) {
@@ -128,8 +129,8 @@ __global__ __launch_bounds__(256) void rotate_grad_kernel(RotateArgs a) {
     }
     Angle<CH> angle;
     bool kept = false;
-    // (the same number of rounds for every thread of the block: all of them take part in the sums; positions of several axes: a.each heads of a token one after the other, which
-    // share their angles)
+    // (the same number of rounds for every thread of the block: all of them take part in the sums; positions of several axes: heads of a token, a.slices or a.k_slices apart, one after the
+    // other, which share their angles)
     for (uint32_t base = block * per_block, turn = 0; base < items;) {
         const uint32_t item = base + (threadIdx.x >> a.lane_shift);
         const uint32_t per_token = AXES ? (is_k ? a.k_slices : a.slices) : heads, it0 = item < items && lane < a.lanes ? item : 0;
